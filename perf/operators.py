@@ -306,7 +306,8 @@ def _exact8(x):
     C = x.shape[1]
     groups = torch.nn.functional.pad(x, (0, -C % 32)).unflatten(1, (-1, 32))
     exponent = torch.frexp(torch.linalg.vector_norm(groups, ord=math.inf, dim=2, keepdim=True))[1] - 7
-    step = torch.ldexp(torch.ones_like(groups[..., :1]), exponent.clamp(min=-126))
+    # (the power of two by its bits: torch.ldexp goes through pow, which is not exact)
+    step = ((exponent.clamp(min=-126).long() + 1023) << 52).view(torch.float64)
     return (torch.round(groups / step).clamp(-127, 127) * step).flatten(1)[:, :C]
 
 
