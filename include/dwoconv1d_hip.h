@@ -312,6 +312,52 @@ int dwo_linear_norm_planes(const void *x, const float *gamma_in, const float *be
                            const void *bias, const float *gamma, const float *beta, float eps, void *out, int images, int HW,
                            int N, int K, int dtype, void *stream);
 
+/*
+ * Operators around wide layers, for training and evaluation; no counterpart in the reference's extension.  Tensors are dense, of one type
+ * `dtype` (DWO_F32, DWO_BF16, DWO_F16), parameters' gradients are written as grad_dtype.  rows is below 2^31, channels are at most 65536;
+ * inputs, outputs that a kernel reads again, and workspaces are 16-byte aligned.  Sums, exponentials and statistics are fp32.  ws holds at least
+ * the bytes that the matching function gives (0: sizes that are not accepted); nothing in it has to survive a call, and calls that
+ * overlap in time take one each.
+ *
+ * dwo_pack8:   8-bit checkpoints: x [rows,C] -> codes [rows,C] (signed bytes q) and exps [rows,ceil(C/32)] (bytes), standing for q * 2^(exp -
+ *              127): groups of 32 neighbours along a row, scale 2^(floor(log2(largest magnitude)) - 6), at least 2^-126, q rounded to even
+ *              and at most 127; exp 0: zeros, 255: a group with an infinity or NaN, all NaN.  Where y is not null also y = act(x).
+ * dwo_unpack8: out [rows,C] = the values held, or where dy is not null dy * act'(value held).
+ * dwo_layer8:  y [rows,D] = x [rows,C] w^T + bias for w [D,C] (bias may be null), and where codes is not null x's checkpoint.
+ *              _backward: dx = dy w, dw = dy^T (values held), db = sum over rows of dy; each may be null, db only goes with dw.
+ * dwo_gated:   a = x w_in^T + b_in for w_in [2H,C], y = (act(a[:, :H]) * a[:, H:]) w_out^T + b_out for w_out [D,H]; b_in and b_out may be
+ *              null.  keep (or null): 2 * rows * H' floats, H' the next multiple of eight, for the backward pass, which takes either x and
+ *              keep, or x's checkpoint in their place and computes at the values held.  Its outputs may be null; a bias gradient
+ *              only goes with its weight's.
+ * dwo_head:    softmax cross entropy of logits l = x w^T + bias for w [V,C], V at most 2^24, and 64-bit targets: loss = log sum exp l -
+ *              (1 - smoothing) l[target] - smoothing * mean(l); 0 where target is `ignore`, NaN where it is no class.  count null: loss
+ *              [rows]; else loss[0] is the mean over the rows not ignored and count[0] receives their number.  lse [rows] and count are
+ *              what the backward pass takes, up [rows], or up[0] for a mean, the gradient of the loss.
+ */
+#define DWO_GELU 0 /* g Phi(g) */
+#define DWO_SILU 1 /* g / (1 + exp(-g)) */
+int dwo_pack8(const void *x, void *y, void *codes, void *exps, size_t rows, int C, int act, int dtype, void *stream);
+int dwo_unpack8(const void *codes, const void *exps, const void *dy, void *out, size_t rows, int C, int act, int dtype,
+                void *stream);
+size_t dwo_layer8_workspace_bytes(size_t rows, int C, int D, int backward, int dtype);
+int dwo_layer8(const void *x, const void *w, const void *bias, void *y, void *codes, void *exps, void *ws, size_t ws_bytes,
+               size_t rows, int C, int D, int dtype, void *stream);
+int dwo_layer8_backward(const void *dy, const void *codes, const void *exps, const void *w, void *dx, void *dw, void *db, void *ws,
+                        size_t ws_bytes, size_t rows, int C, int D, int dtype, int grad_dtype, void *stream);
+size_t dwo_gated_workspace_bytes(size_t rows, int C, int H, int D, int backward, int held8, int dtype);
+int dwo_gated_forward(const void *x, const void *w_in, const void *b_in, const void *w_out, const void *b_out, void *y, float *keep,
+                      void *ws, size_t ws_bytes, size_t rows, int C, int H, int D, int act, int dtype, void *stream);
+int dwo_gated_backward(const void *dy, const void *x, const void *codes, const void *exps, const float *keep, const void *w_in,
+                       const void *b_in, const void *w_out, void *dx, void *dw_in, void *db_in, void *dw_out, void *db_out, void *ws,
+                       size_t ws_bytes, size_t rows, int C, int H, int D, int act, int dtype, int grad_dtype, void *stream);
+size_t dwo_head_workspace_bytes(size_t rows, int C, int V, int backward, int dtype);
+int dwo_head_forward(const void *x, const void *w, const void *bias, const void *targets, long long ignore, float smoothing,
+                     float *lse, float *loss, float *count, void *ws, size_t ws_bytes, size_t rows, int C, int V, int dtype,
+                     void *stream);
+int dwo_head_backward(const float *up, const void *x, const void *w, const void *bias, const void *targets, long long ignore,
+                      float smoothing, const float *lse, const float *count, void *dx, void *dw, void *db, void *ws,
+                      size_t ws_bytes, size_t rows, int C, int V, int dtype, int grad_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

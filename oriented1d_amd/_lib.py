@@ -50,6 +50,17 @@ SIGNATURES = {
     "dwo_block_mlp": (_i, [_vp] * 8 + [_i] * 4 + [_vp]),
     "dwo_linear_norm_planes": (_i, [_vp] * 3 + [ctypes.c_float] + [_vp] * 4 + [ctypes.c_float, _vp] + [_i] * 5 + [_vp]),
     "dwo_linear_wgrad": (_i, [_vp] * 5 + [_sz, _sz] + [_i] * 4 + [_vp]),
+    "dwo_pack8": (_i, [_vp] * 4 + [_sz] + [_i] * 3 + [_vp]),
+    "dwo_unpack8": (_i, [_vp] * 4 + [_sz] + [_i] * 3 + [_vp]),
+    "dwo_layer8_workspace_bytes": (_sz, [_sz] + [_i] * 4),
+    "dwo_layer8": (_i, [_vp] * 7 + [_sz, _sz] + [_i] * 3 + [_vp]),
+    "dwo_layer8_backward": (_i, [_vp] * 8 + [_sz, _sz] + [_i] * 4 + [_vp]),
+    "dwo_gated_workspace_bytes": (_sz, [_sz] + [_i] * 6),
+    "dwo_gated_forward": (_i, [_vp] * 8 + [_sz, _sz] + [_i] * 5 + [_vp]),
+    "dwo_gated_backward": (_i, [_vp] * 14 + [_sz, _sz] + [_i] * 6 + [_vp]),
+    "dwo_head_workspace_bytes": (_sz, [_sz] + [_i] * 4),
+    "dwo_head_forward": (_i, [_vp] * 4 + [ctypes.c_longlong, ctypes.c_float] + [_vp] * 4 + [_sz, _sz] + [_i] * 3 + [_vp]),
+    "dwo_head_backward": (_i, [_vp] * 5 + [ctypes.c_longlong, ctypes.c_float] + [_vp] * 6 + [_sz, _sz] + [_i] * 4 + [_vp]),
 }
 
 _lib = None

@@ -15,7 +15,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import fused
+from . import checkpoint8 as held, fused, losses
+from .feedforward import GatedMLP
 from .dwoconv1d import DepthwiseOrientedConv1d
 
 # (block kernel sizes, stem kernel size) per variant -- models/convnext.py:485-492
@@ -157,6 +158,11 @@ class Stem1D(nn.Module):
         return F.gelu(norm(x)) if y is None else y
 
 
+def gated_hidden(dim):
+    """Hidden units of a gated block with as many weights as two pointwise layers of 4 * dim: 8/3 dim, up to a multiple of eight."""
+    return 8 * -(-dim // 3)
+
+
 def _operator(conv):
     """The operator in a block's slot: what a wrapper without hooks calls."""
     return conv.conv if fused.plain(conv, ConvWrapper) else conv
@@ -164,14 +170,27 @@ def _operator(conv):
 
 class Block(nn.Module):
     """ConvNeXt-1D block (one oriented conv, models/convnext.py:255-319) or 1D++ block (a second
-    oriented conv with a residual tap on the 4*dim hidden tensor in NHWC, :322-399)."""
+    oriented conv with a residual tap on the 4*dim hidden tensor in NHWC, :322-399).
+
+    ``mlp="gated"`` has a ``GatedMLP`` of as many weights (``.mlp``) in place of the pointwise layers and GELU of a 1D block;
+    ``checkpoint8`` keeps the inputs of the pointwise layers and of GELU, or of the gated block, in 8 bits while training (their
+    results stay as they are, gradients are taken at the values held).  The reference has neither."""
 
     def __init__(self, dim, kernel_sizes, plus_plus, drop_path=0.0, layer_scale_init_value=1e-6,
-                 layer_offset=0.0, n_dir=8, arbitrary_size=False, wrapped=False):
+                 layer_offset=0.0, n_dir=8, arbitrary_size=False, wrapped=False, mlp="plain", checkpoint8=False):
         super().__init__()
+        if mlp not in ("plain", "gated"):
+            raise ValueError("mlp must be 'plain' or 'gated'")
+        if mlp == "gated" and plus_plus:
+            raise ValueError("a 1D++ block has an operator between its pointwise layers: its mlp cannot be gated")
+        self.checkpoint8 = bool(checkpoint8)
         self.norm = nn.LayerNorm(dim, eps=1e-6)
-        self.pwconv1 = fused.Linear(dim, 4 * dim)
-        self.pwconv2 = fused.Linear(4 * dim, dim)
+        if mlp == "gated":
+            self.mlp = GatedMLP(dim, gated_hidden(dim), checkpoint8=checkpoint8)
+        else:
+            self.mlp = None
+            self.pwconv1 = fused.Linear(dim, 4 * dim)
+            self.pwconv2 = fused.Linear(4 * dim, dim)
         self.gamma = (nn.Parameter(layer_scale_init_value * torch.ones(dim))
                       if layer_scale_init_value > 0 else None)
         self.drop_path = StochasticDepth(drop_path) if drop_path > 0.0 else nn.Identity()
@@ -197,18 +216,30 @@ class Block(nn.Module):
         if fuse:  # permute + LayerNorm as one pass
             y = fused.nchw_layernorm_nhwc(y, self.norm.weight, self.norm.bias, self.norm.eps)
         else:  # (recorded by autograd: one pass each way as well)
-            z = fused.tile_norm(y, self.norm, self.pwconv1) if fused.plain(self.norm, nn.LayerNorm) else None
+            first = self.pwconv1 if self.mlp is None else self.mlp
+            z = fused.tile_norm(y, self.norm, first) if fused.plain(self.norm, nn.LayerNorm) else None
             y = self.norm(y.permute(0, 2, 3, 1).contiguous()) if z is None else z
+        if self.mlp is not None:
+            y = self.mlp(y)
+            return fused.nhwc_scale_add_nchw(y, self.gamma, x) if fuse else self._join(x, y)
         if fuse and not self.plus_plus:
             out = fused.block_mlp(y, self.pwconv1, self.pwconv2, self.gamma, x)
             if out is not None:
                 return out
-        y = fused.linear_gelu(y, self.pwconv1)
+        lean = (self.checkpoint8 and torch.is_grad_enabled() and fused.plain(self.pwconv1, fused.Linear)
+                and fused.plain(self.pwconv2, fused.Linear))
+        if lean:
+            y = held.act8(held.linear8(y, self.pwconv1.weight, self.pwconv1.bias))
+        else:
+            y = fused.linear_gelu(y, self.pwconv1)
         if self.plus_plus:
             y = self.dwconv2(y)
         if fuse:  # layer scale + permute + residual behind the layer (no stochastic depth in eval)
             return fused.linear_tail(y, self.pwconv2, self.gamma, x)
-        y = self.pwconv2(y)
+        return self._join(x, held.linear8(y, self.pwconv2.weight, self.pwconv2.bias) if lean else self.pwconv2(y))
+
+    def _join(self, x, y):
+        """The residual branch's end: layer scale, planes and the sum with the block's input."""
         if self.gamma is not None:
             if self._keeps_all():
                 out = fused.block_tail(y, self.gamma, x)
@@ -230,11 +261,11 @@ class ConvNeXt1D(nn.Module):
     semantic_segmentation/backbone/convnext.py:395-399,433-443).  ``backbone=True`` is that
     backbone in full: stage outputs, kernel sizes cropped per stage (:316-327), any input size,
     and the operators held in wrappers (parameter names ``...dwconv.conv.weight``), so that
-    checkpoints converted by ``backbone_weights.convert_to_backbone_state_dict`` load."""
+    checkpoints converted by ``backbone_weights.convert_to_backbone_state_dict`` load.  ``mlp`` and ``checkpoint8`` are the blocks'."""
 
     def __init__(self, in_chans=3, num_classes=1000, depths=(3, 3, 9, 3), dims=(96, 192, 384, 768),
                  drop_path_rate=0.0, layer_scale_init_value=1e-6, head_init_scale=1.0, variant="1d",
-                 N=8, stem_dim1=64, arbitrary_size=False, out_stages=False, backbone=False):
+                 N=8, stem_dim1=64, arbitrary_size=False, out_stages=False, backbone=False, mlp="plain", checkpoint8=False):
         super().__init__()
         if variant not in _VARIANTS:
             raise ValueError("variant must be '1d' or '1dpp'")
@@ -254,7 +285,7 @@ class ConvNeXt1D(nn.Module):
             self.stages.append(nn.Sequential(*[
                 Block(dims[i], stage_ks[i], variant == "1dpp", rates[done + j],
                       layer_scale_init_value, _odd_layer_offset(j), N, arbitrary_size,
-                      wrapped=backbone) for j in range(depth)]))
+                      wrapped=backbone, mlp=mlp, checkpoint8=checkpoint8) for j in range(depth)]))
             done += depth
         if out_stages:
             for i in range(4):
@@ -286,7 +317,8 @@ class ConvNeXt1D(nn.Module):
                 return y
         return layer(x)
 
-    def forward(self, x):
+    def forward_features(self, x):
+        """The four stage outputs (``out_stages``), or what the classifier reads."""
         outs = []
         for i in range(4):
             x = self.stages[i](self._downsample(i, x))
@@ -294,7 +326,22 @@ class ConvNeXt1D(nn.Module):
                 outs.append(getattr(self, "norm%d" % i)(x))
         if self.out_stages:
             return outs
-        return self.head(self.norm(x.mean((-2, -1))))
+        return self.norm(x.mean((-2, -1)))
+
+    def forward(self, x):
+        x = self.forward_features(x)
+        return x if self.out_stages else self.head(x)
+
+    def loss(self, x, target, label_smoothing=0.0, ignore_index=-100):
+        """Mean softmax cross entropy of the images x against int64 classes, as fp32: ``F.cross_entropy(self(x), target, ...)`` without
+        its logits in memory."""
+        if self.out_stages:
+            raise ValueError("a network of stage outputs has no classes")
+        features = self.forward_features(x)
+        if not fused.plain(self.head, nn.Linear):
+            return F.cross_entropy(self.head(features).float(), target, ignore_index=ignore_index, label_smoothing=label_smoothing)
+        return losses.linear_cross_entropy(features, self.head.weight, self.head.bias, target, ignore_index=ignore_index,
+                                           label_smoothing=label_smoothing)
 
 
 def convnext_tiny_1d(variant="1d", **kw):

@@ -1,0 +1,316 @@
+// Softmax cross entropy of a linear layer over many classes, without keeping its logits:
+//   l = x w^T + b,  lse = log sum_v exp l_v,  loss = lse - (1 - eps) l_t - eps mean_v l_v
+//   G = up (exp(l - lse) - (1 - eps) [v = t] - eps / V),  dx = G w,  dw = G^T x,  db = sum over rows of G
+//
+// Forward: one product over all classes whose epilogue leaves, for a row and a wave's classes, their largest logit and the sum of
+// exponentials below it; a second kernel joins them.  Backward, in pieces of the classes: the product again, its sums turned into G, which
+// alone goes through memory, rounded to the activations' type for the two products that read it.  Eight products of rows x
+// classes x channels in place of the six of a pass that keeps its logits; what would be kept is two or more bytes a row and class.
+#include "dwo_product.h"
+
+namespace dwo {
+
+struct Targets {
+    const long long *t;
+    long long ignore;
+    long V;
+    // the class of row m, -1 where the row is ignored, -2 where it has no class there is
+    __device__ __forceinline__ long of(long m) const {
+        const long long v = t[m];
+        return v == ignore ? -1L : v >= 0 && v < V ? (long)v : -2L;
+    }
+};
+
+struct StatsEpi {
+    static constexpr bool kSums = false;
+    Values bias;
+    Targets targets;
+    float2 *part;  // [classes / width][M]: largest, sum of exponentials
+    float *sum;    // the same of sums of logits, or null
+    float *at;     // [M]: the target's logit
+    int width;     // classes of a wave, eight to a lane
+    struct Lane {
+        float bias[8];
+    };
+    __device__ __forceinline__ Lane begin(const Product &p, long n) const {
+        Lane l;
+#pragma unroll
+        for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
+        return l;
+    }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
+        const long t = m < p.M ? targets.of(m) : -1;
+        float most = -INFINITY, s = 0.f, all = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool real = n + e < p.N;
+            v[e] = real ? v[e] + l.bias[e] : -INFINITY;
+            most = fmaxf(most, v[e]);
+            if (real) all += v[e];
+            if (n + e == t) at[m] = v[e];
+        }
+        for (int off = 1; off < width / 8; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        // (all -infinity: no exponential; NaN is in no maximum and in the sum)
+        const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s += prod_exp(v[e] - base);
+        for (int off = 1; off < width / 8; off <<= 1) {
+            s += __shfl_xor(s, off, 64);
+            if (sum != nullptr) all += __shfl_xor(all, off, 64);
+        }
+        if (n % width == 0 && n < p.N && m < p.M) {
+            const size_t to = (size_t)(n / width) * p.M + m;
+            part[to] = make_float2(most, s);
+            if (sum != nullptr) sum[to] = all;
+        }
+    }
+};
+
+// Sixteen rows per workgroup, sixteen threads a row.
+__global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict__ part, const float *__restrict__ sum,
+                                                        const float *__restrict__ at, Targets targets, float *__restrict__ lse,
+                                                        float *__restrict__ loss, float2 *__restrict__ block, long M, int parts,
+                                                        float eps) {
+    __shared__ float most_of[16][17], sum_of[16][17], all_of[16][17];
+    __shared__ float2 rows[16];
+    const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const long m = (long)blockIdx.x * 16 + r;
+    float most = -INFINITY, s = 0.f, all = 0.f;
+    if (m < M)
+        for (int p = k; p < parts; p += 16) {
+            const float2 v = part[(size_t)p * M + m];
+            const float next = fmaxf(most, v.x), base = next == -INFINITY ? 0.f : next;
+            s = s * prod_exp(most - base) + v.y * prod_exp(v.x - base);
+            most = next;
+            if (sum != nullptr) all += sum[(size_t)p * M + m];
+        }
+    most_of[k][r] = most, sum_of[k][r] = s, all_of[k][r] = all;
+    __syncthreads();
+    if (k == 0) {
+        for (int i = 1; i < 16; i++) most = fmaxf(most, most_of[i][r]);
+        const float base = most == -INFINITY ? 0.f : most;
+        s = 0.f, all = 0.f;
+        for (int i = 0; i < 16; i++) s += sum_of[i][r] * prod_exp(most_of[i][r] - base), all += all_of[i][r];
+        float value = 0.f, count = 0.f;
+        if (m < M) {
+            const float l = base + logf(s);
+            lse[m] = l;
+            const long t = targets.of(m);
+            if (t == -2) value = NAN;
+            else if (t >= 0) value = (l - at[m]) * (1.f - eps);
+            if (t >= 0 && sum != nullptr) value += eps * (l - all / (float)targets.V);
+            count = t != -1 ? 1.f : 0.f;
+            if (loss != nullptr) loss[m] = value;
+        }
+        rows[r] = make_float2(value, count);
+    }
+    __syncthreads();
+    if (block != nullptr && threadIdx.x == 0) {
+        float2 t = make_float2(0.f, 0.f);
+        for (int i = 0; i < 16; i++) t.x += rows[i].x, t.y += rows[i].y;
+        block[blockIdx.x] = t;
+    }
+}
+
+// loss[0] = the mean over the rows that count, count[0] how many do; one workgroup, fixed order, in 64 bits (many rows)
+__global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restrict__ block, int blocks, float *__restrict__ loss,
+                                                         float *__restrict__ count) {
+    __shared__ double value[1024], number[1024];
+    double a = 0.0, b = 0.0;
+    for (int i = threadIdx.x; i < blocks; i += 1024) a += block[i].x, b += block[i].y;
+    value[threadIdx.x] = a, number[threadIdx.x] = b;
+    __syncthreads();
+    for (int half = 512; half > 0; half >>= 1) {
+        if ((int)threadIdx.x < half)
+            value[threadIdx.x] += value[threadIdx.x + half], number[threadIdx.x] += number[threadIdx.x + half];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) loss[0] = (float)(value[0] / number[0]), count[0] = (float)number[0];
+}
+
+// What G is multiplied with so that fp16 holds it, a power of two that brings the largest |up| to 2^13 .. 2^14 (G is at most |up|), and
+// its inverse: probabilities below 6e-8 would be lost otherwise.
+__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, const float *__restrict__ count, long M,
+                                                          float *__restrict__ scale) {
+    __shared__ unsigned most[1024];
+    unsigned v = 0;
+    const long n = count != nullptr ? 1 : M;
+    for (long i = threadIdx.x; i < n; i += 1024) v = max(v, __float_as_uint(count != nullptr ? up[i] / count[0] : up[i]) & 0x7fffffffu);
+    most[threadIdx.x] = v;
+    __syncthreads();
+    for (int half = 512; half > 0; half >>= 1) {
+        if ((int)threadIdx.x < half) most[threadIdx.x] = max(most[threadIdx.x], most[threadIdx.x + half]);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const int e = (int)(most[0] >> 23);  // biased exponent; the scale's is 254 + 13 - e
+        const int k = e == 0 || e == 255 ? 127 : min(max(267 - e, 1), 253);
+        scale[0] = __uint_as_float((unsigned)k << 23), scale[1] = __uint_as_float((unsigned)(254 - k) << 23);
+    }
+}
+
+struct GradEpi {
+    static constexpr bool kSums = false;
+    Values bias;      // of the piece
+    Targets targets;  // V: all classes
+    long from;        // the piece's first class
+    const float *lse, *up, *count, *scale;  // count: a mean's (up has one value), or null; scale may be null
+    float eps;
+    Out g;            // [M][pitch]
+    struct Lane {
+        float bias[8], extra, flat;
+    };
+    __device__ __forceinline__ Lane begin(const Product &p, long n) const {
+        Lane l;
+        l.extra = (scale != nullptr ? scale[0] : 1.f) * (count != nullptr ? up[0] / count[0] : 1.f), l.flat = eps / (float)targets.V;
+#pragma unroll
+        for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
+        return l;
+    }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
+        if (m >= p.M || n >= g.pitch) return;
+        const long t = targets.of(m);
+        const float total = lse[m], f = t == -2 ? NAN : count != nullptr ? l.extra : up[m] * l.extra;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float hit = from + n + e == t ? 1.f - eps : 0.f;
+            v[e] = t == -1 || n + e >= p.N ? 0.f : (prod_exp(v[e] + l.bias[e] - total) - hit - l.flat) * f;
+        }
+        out_octet(g, true, m, n, g.pitch, v);
+    }
+};
+
+struct HeadSizes {
+    long rows, C, V;
+    int dtype;
+    HeadSizes(size_t r, int c, int v, int t) : rows((long)r), C(c), V(v), dtype(t) {}
+    bool ok() const { return rows >= 1 && rows < 1L << 31 && C >= 1 && C <= 65536 && V >= 1 && V <= 1 << 24 && known(dtype); }
+    // classes of a piece: G of a piece has about 2^27 values, 256 MB in 16 bits, what the last cache before memory holds
+    long piece() const {
+        const long most = (1L << 27) / rows / 256 * 256;
+        return V <= most ? V : most < 1024 ? 1024 : most;
+    }
+};
+
+static int head_forward(const HeadSizes &s, const void *x, const void *w, const void *b, Targets targets, float eps, float *lse,
+                        float *loss, float *count, bool mean, Arena &ws, hipStream_t st) {
+    Operand ox, ow;
+    int e;
+    if ((e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st)) || (e = stage_operand(ow, w, s.V, s.C, s.dtype, ws, st))) return e;
+    const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
+    const int width = wave_columns(s.rows, s.V);
+    const int parts = (int)((s.V + width - 1) / width), blocks = (int)((s.rows + 15) / 16);
+    float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
+    float *sum = eps > 0.f ? (float *)ws.take((size_t)parts * s.rows * sizeof(float)) : nullptr;
+    float *at = (float *)ws.take((size_t)s.rows * sizeof(float));
+    float2 *block = mean ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
+    if (ws.dry()) return 0;
+    const StatsEpi epi{{b, s.dtype}, targets, part, sum, at, width};
+    if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
+    head_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss, block, s.rows, parts,
+                                                                  eps);
+    if (mean) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
+    return status();
+}
+
+static int head_backward(const HeadSizes &s, const float *up, const void *x, const void *w, const void *b, Targets targets, float eps,
+                         const float *lse, const float *count, void *dx, void *dw, void *db, int grad, Arena &ws, hipStream_t st) {
+    Operand ox, ow;
+    int e;
+    if ((e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st)) || (e = stage_operand(ow, w, s.V, s.C, s.dtype, ws, st))) return e;
+    const long piece = s.piece();
+    const Operand g = take_operand(ws, s.rows, up8(piece), s.dtype);
+    // dx is summed over the pieces in fp32
+    const bool many = piece < s.V;
+    float *sum = many && dx != nullptr && s.dtype != DWO_F32 ? (float *)ws.take((size_t)s.rows * s.C * sizeof(float)) : (float *)dx;
+    float *scale = s.dtype == DWO_F16 ? (float *)ws.take(2 * sizeof(float)) : nullptr;
+    if (scale != nullptr && !ws.dry()) {
+        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, count, s.rows, scale);
+        if ((e = status())) return e;
+    }
+    const size_t size = size_of(s.dtype), grad_size = size_of(grad);
+    const float *alpha = scale != nullptr ? scale + 1 : nullptr;
+    const size_t held = ws.used;
+    size_t peak = held;
+    for (long from = 0; from < s.V; from += piece) {
+        const long n = s.V - from < piece ? s.V - from : piece;
+        ws.used = held;  // (the pieces' partial sums take the same place)
+        Operand wp = ow;
+        wp.p = (const char *)ow.p + (size_t)from * ow.pitch * 2;
+        Operand gp = g;
+        gp.pitch = up8(n), gp.plane = s.rows * gp.pitch;
+        if (!ws.dry()) {
+            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, up, count, scale, eps,
+                              out_of(gp, s.dtype)};
+            if ((e = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st))) return e;
+        }
+        if (dx != nullptr) {
+            const bool last = from + n == s.V;
+            PlainEpi epi = plain_epilogue({last ? dx : (void *)sum, s.C, 0, last ? s.dtype : (int)OUT_F32});
+            epi.alpha = alpha, epi.before = from > 0 ? sum : nullptr;
+            if ((e = plain_product(gp, false, wp, true, s.rows, s.C, n, s.dtype, epi, ws, st))) return e;
+        }
+        if (dw != nullptr) {
+            PlainEpi epi = plain_epilogue({(char *)dw + (size_t)from * s.C * grad_size, s.C, 0, grad});
+            epi.sums = {db != nullptr ? (char *)db + from * grad_size : nullptr, 0, 0, grad};
+            epi.alpha = alpha;
+            if ((e = plain_product(gp, true, ox, true, n, s.C, s.rows, s.dtype, epi, ws, st))) return e;
+        }
+        if (ws.used > peak) peak = ws.used;
+    }
+    ws.used = peak;
+    return 0;
+}
+
+}  // namespace dwo
+
+using namespace dwo;
+
+extern "C" {
+
+size_t dwo_head_workspace_bytes(size_t rows, int C, int V, int backward, int dtype) {
+    const HeadSizes s(rows, C, V, dtype);
+    if (!s.ok()) return 0;
+    Arena ws{nullptr, 0};
+    void *const any = (void *)256;  // (nothing is launched)
+    const Targets t{(const long long *)any, 0, V};
+    if (backward)
+        head_backward(s, (const float *)any, any, any, any, t, 0.1f, (const float *)any, (const float *)any, any, any, any, DWO_F32, ws,
+                      nullptr);
+    else
+        head_forward(s, any, any, any, t, 0.1f, (float *)any, (float *)any, (float *)any, true, ws, nullptr);
+    return ws.used + 256;
+}
+
+int dwo_head_forward(const void *x, const void *w, const void *bias, const void *targets, long long ignore, float smoothing, float *lse,
+                     float *loss, float *count, void *ws, size_t ws_bytes, size_t rows, int C, int V, int dtype, void *stream) {
+    if (!x || !w || !targets || !lse || !loss || !ws) return DWO_ERR_NULL_POINTER;
+    const HeadSizes s(rows, C, V, dtype);
+    if (!known(dtype)) return DWO_ERR_BAD_DTYPE;
+    if (!s.ok() || !(smoothing >= 0.f && smoothing <= 1.f) || ((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) % 16 != 0 ||
+        (uintptr_t)targets % 8 != 0)
+        return DWO_ERR_BAD_SHAPE;
+    if (ws_bytes < dwo_head_workspace_bytes(rows, C, V, 0, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
+    (void)hipGetLastError();
+    Arena a{(char *)ws, 0};
+    return head_forward(s, x, w, bias, {(const long long *)targets, ignore, s.V}, smoothing, lse, loss, count, count != nullptr, a,
+                        (hipStream_t)stream);
+}
+
+int dwo_head_backward(const float *up, const void *x, const void *w, const void *bias, const void *targets, long long ignore,
+                      float smoothing, const float *lse, const float *count, void *dx, void *dw, void *db, void *ws, size_t ws_bytes,
+                      size_t rows, int C, int V, int dtype, int grad_dtype, void *stream) {
+    if (!up || !x || !w || !targets || !lse || !ws) return DWO_ERR_NULL_POINTER;
+    const HeadSizes s(rows, C, V, dtype);
+    if (!known(dtype) || !known(grad_dtype)) return DWO_ERR_BAD_DTYPE;
+    if (!s.ok() || !(smoothing >= 0.f && smoothing <= 1.f) || ((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) % 16 != 0 ||
+        (uintptr_t)targets % 8 != 0 || (db && !dw))
+        return DWO_ERR_BAD_SHAPE;
+    if (ws_bytes < dwo_head_workspace_bytes(rows, C, V, 1, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
+    (void)hipGetLastError();
+    Arena a{(char *)ws, 0};
+    return head_backward(s, up, x, w, bias, {(const long long *)targets, ignore, s.V}, smoothing, lse, count, dx, dw, db, grad_dtype, a,
+                         (hipStream_t)stream);
+}
+
+}  // extern "C"

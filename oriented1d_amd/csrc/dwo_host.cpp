@@ -16,6 +16,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 
 #include "dwoconv1d_hip.h"
 
@@ -53,6 +54,17 @@ struct Library {
     decltype(&::dwo_linear_rows) linear_rows;
     decltype(&::dwo_linear_planes) linear_planes;
     decltype(&::dwo_linear_norm_planes) linear_norm_planes;
+    decltype(&::dwo_pack8) pack8;
+    decltype(&::dwo_unpack8) unpack8;
+    decltype(&::dwo_layer8_workspace_bytes) layer8_workspace_bytes;
+    decltype(&::dwo_layer8) layer8;
+    decltype(&::dwo_layer8_backward) layer8_backward;
+    decltype(&::dwo_gated_workspace_bytes) gated_workspace_bytes;
+    decltype(&::dwo_gated_forward) gated_forward;
+    decltype(&::dwo_gated_backward) gated_backward;
+    decltype(&::dwo_head_workspace_bytes) head_workspace_bytes;
+    decltype(&::dwo_head_forward) head_forward;
+    decltype(&::dwo_head_backward) head_backward;
 } lib;
 
 [[noreturn]] void fail(const std::string &msg) { throw std::runtime_error(msg); }
@@ -91,6 +103,17 @@ void bind_library(const std::string &path) {
     find(lib.linear_rows, "dwo_linear_rows");
     find(lib.linear_planes, "dwo_linear_planes");
     find(lib.linear_norm_planes, "dwo_linear_norm_planes");
+    find(lib.pack8, "dwo_pack8");
+    find(lib.unpack8, "dwo_unpack8");
+    find(lib.layer8_workspace_bytes, "dwo_layer8_workspace_bytes");
+    find(lib.layer8, "dwo_layer8");
+    find(lib.layer8_backward, "dwo_layer8_backward");
+    find(lib.gated_workspace_bytes, "dwo_gated_workspace_bytes");
+    find(lib.gated_forward, "dwo_gated_forward");
+    find(lib.gated_backward, "dwo_gated_backward");
+    find(lib.head_workspace_bytes, "dwo_head_workspace_bytes");
+    find(lib.head_forward, "dwo_head_forward");
+    find(lib.head_backward, "dwo_head_backward");
 }
 
 void check(int status, const char *what) {
@@ -714,6 +737,8 @@ Tensor conv_norm(const Tensor &x, const Tensor &w, const OptTensor &bias, const 
     return pieces ? std::get<0>(ln_tile(y, g, b, eps, false, y.scalar_type(), false)) : nchw_layernorm_nhwc(y, g, b, eps);
 }
 
+#include "dwo_host_wide.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -733,6 +758,12 @@ PYBIND11_MODULE(_host, m) {
     m.def("linear_rows", &linear_rows);
     m.def("linear_planes", &linear_planes);
     m.def("linear_norm_planes", &linear_norm_planes);
+    m.def("pack8", &pack8_entry);
+    m.def("unpack8", &unpack8_entry);
+    m.def("act8", &act8);
+    m.def("linear8", &linear8);
+    m.def("gated", &gated);
+    m.def("head", &head);
     m.def("ln_rows", &ln_rows);
     m.def("ln_rows_backward", &ln_rows_backward);
     m.def("ln_tile", &ln_tile);

@@ -306,8 +306,8 @@ struct LinearArgs {
 // 401408 x 96 120 / 113, 100352 x 192 108.5 / 105; the first one 401408 x 384 x 96 173 / 167, 25088 x 1536 x 384 60 / 57.
 // gelu_rounded, whose tail is exact to the result's rounding, has no place here: a separate layer's rounding of u, which the
 // tail magnifies by u^2, is gone, and was worth five to nine times the difference.  Infinities and NaN give what u * (1 + erf) gives.
-__device__ __forceinline__ float lin_gelu(float u) {
-    const float t = __builtin_fabsf(u);
+// 1/2 - Phi(-t), t >= 0
+__device__ __forceinline__ float lin_half_erf(float t) {
     float p = __builtin_fmaf(t, -2.09645073e-06f, 3.15079535e-05f);
     p = __builtin_fmaf(t, p, -0.000153187882f);
     p = __builtin_fmaf(t, p, -0.000206634976f);
@@ -316,7 +316,11 @@ __device__ __forceinline__ float lin_gelu(float u) {
     p = __builtin_fmaf(t, p, -0.459194624f);
     p = __builtin_fmaf(t, p, -1.15110672f);
     p = __builtin_fmaf(t, p, -0.999999963f);
-    return __builtin_fmaf(t, 0.5f - __builtin_amdgcn_exp2f(p), 0.5f * u);
+    return 0.5f - __builtin_amdgcn_exp2f(p);
+}
+__device__ __forceinline__ float lin_gelu(float u) {
+    const float t = __builtin_fabsf(u);
+    return __builtin_fmaf(t, lin_half_erf(t), 0.5f * u);
 }
 
 typedef unsigned mma_u2 __attribute__((ext_vector_type(2)));

@@ -1,0 +1,512 @@
+// Matrix products of the operators around wide layers: the gated feed-forward block (dwo_gated.hip), the cross entropy of many classes
+// (dwo_head.hip) and layers with 8-bit checkpoints (dwo_check8.hip).
+//
+//   D[m][n] = sum_k A[m][k] * B[n][k]   with an epilogue on the sums while they are in registers.
+//
+// Either operand lies in memory with k fast (A [M][K]) or with k slow (A [K][M], what the product of a gradient reads), so that no
+// tensor is transposed.  Values are 16 bits wide, sums 32.  fp32 operands come as three planes of bf16 whose sum they are (8 + 8 + 8
+// bits of mantissa, stage_kernel), and their product is six of the nine products of planes, small ones first: what is left out is below
+// 2^-24 of the whole.  417 TFLOP/s at best, where the fp32 matrix instructions give 157, at the accuracy of sums in fp32.
+#pragma once
+
+#include "dwo_linear.h"
+
+namespace dwo {
+
+struct Operand {  // rows of `pitch` values (a multiple of eight), 16-byte aligned; `plane` values from one plane to the next
+    const void *p;
+    long pitch, plane;
+    int planes;  // 1 or 3
+};
+struct Product {
+    Operand a, b;
+    long M, N, K;
+    long gap;  // gated weights: values from the row of a gate to that of what it multiplies (0: rows as they come)
+    int pairs;
+    unsigned codes_a, codes_b;  // the planes of each pair, two bits a pair
+    int mtiles, ntiles, splits;
+    int per, steps;  // steps of 64 per split, in all
+};
+
+// (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); where one operand has a single plane, the other's planes
+inline void product_pairs(Product &p) {
+    const bool a = p.a.planes == 3, b = p.b.planes == 3;
+    p.pairs = a && b ? 6 : a || b ? 3 : 1;
+    p.codes_a = a && b ? 0x052 : a ? 0x006 : 0;
+    p.codes_b = a && b ? 0x118 : b ? 0x006 : 0;
+}
+
+// ------------------------------------------------------------------------------------------------- stages in LDS
+constexpr int kProdK = 64;  // summed indices of a stage
+
+// R rows (k fast) or columns (k slow) of an operand, 64 summed indices, straight to LDS: sixteen bytes per lane and load, zeros beyond
+// the operand's ends.  k fast: rows of 128 bytes whose 16-byte pieces are permuted by the row (lin_fragment).  k slow: 64 rows of R
+// values whose 32-byte units are permuted by the row, so that the eight rows of a transposing read lie on different banks.
+// HALF > 0: rows come in runs of HALF gates and the HALF rows that these multiply.
+__device__ __forceinline__ int prod_key(int row, int R) {
+    return R >= 128 ? (row & 3) | (row >> 1 & 4) : (row >> 1 & 1) | (row >> 2 & 2);
+}
+template <int R, int THREADS, bool SLOW, int HALF>
+struct Stage {
+    static constexpr int U = R * 8 / THREADS;
+    static_assert(R * 8 % THREADS == 0 && THREADS % 64 == 0, "whole loads");
+    const char *base;
+    long left, pitch, plane, gap;  // bytes; left: rows (k fast) or bytes (k slow) from base to the operand's end
+    unsigned off[U];
+    __device__ __forceinline__ void init(const Operand &o, long rows, long r0, long K, long skip) {
+        pitch = o.pitch * 2, plane = o.plane * 2, gap = skip * 2;
+        if constexpr (SLOW) {
+            base = reinterpret_cast<const char *>(o.p) + r0 * 2;
+            left = K * pitch - r0 * 2;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int f = (int)threadIdx.x + u * THREADS, row = f / (R / 8), q = f % (R / 8);
+                const int c = ((q >> 1) ^ prod_key(row, R)) * 16 + (q & 1) * 8;
+                off[u] = r0 + c < o.pitch ? (unsigned)row * (unsigned)pitch + (unsigned)c * 2 : kLinNowhere;
+            }
+        } else {
+            base = reinterpret_cast<const char *>(o.p) + r0 * pitch;
+            left = rows - r0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = ((int)threadIdx.x + u * THREADS) / 8;
+                const int row = HALF > 0 ? s / (2 * HALF) * HALF + s % HALF : s;
+                off[u] = (unsigned)row * (unsigned)pitch + piece() * 16;
+            }
+        }
+    }
+    static __device__ __forceinline__ int piece() { return (threadIdx.x % 8) ^ (threadIdx.x / 8 % 8); }
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char *p, long bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, (unsigned)max(0L, min(bytes, 0x7fffffffL)), 0x00020000);
+    }
+    // (not `live`: zeros)
+    __device__ __forceinline__ void load(uint16_t *lds, int which, long k0, long K, bool live) const {
+        typedef __attribute__((address_space(3))) void lds_void;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#ifdef __HIP_DEVICE_COMPILE__
+        if constexpr (SLOW) {
+            const __amdgpu_buffer_rsrc_t r = rsrc(base + which * plane + k0 * pitch, live ? left - k0 * pitch : 0);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, off[u], 0, 0, 0);
+        } else {
+            // beyond the last summed index a lane reads nowhere, which writes zeros
+            const unsigned kill = piece() * 8 < K - k0 ? 0u : kLinNowhere;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const bool second = HALF > 0 && (wave * 8 + u * (THREADS / 8)) / (HALF > 0 ? HALF : 1) % 2 != 0;
+                const __amdgpu_buffer_rsrc_t r = rsrc(base + which * plane + (second ? gap : 0), live ? left * pitch : 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, off[u] | kill,
+                                                         (int)k0 * 2, 0, 0);
+            }
+        }
+#endif
+    }
+};
+
+// sixteen rows (columns) from slot0 on x 32 summed indices, 32 kk .. of the stage: a lane's eight values are 8 g .. of row c
+template <int R, bool SLOW>
+__device__ __forceinline__ mma_s8 prod_fragment(const uint16_t *lds, int slot0, int kk) {
+    if constexpr (SLOW) {
+        typedef __attribute__((address_space(3))) mma_s4 lds_s4;
+        const int lane = threadIdx.x & 63, i = lane & 15, row = 8 * (lane >> 4) + (i >> 2);
+        const uint16_t *at = lds + (32 * kk + row) * R + ((slot0 / 16) ^ prod_key(row, R)) * 16 + (i & 3) * 4;
+        const mma_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at);
+        const mma_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * R));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        return lin_fragment<kProdK>(lds, slot0, kk);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- what goes out
+enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2, OUT_PLANES = 3 };  // (the first three are the DWO_ codes)
+struct Out {
+    void *p;
+    long pitch, plane;
+    int type;
+};
+__device__ __forceinline__ uint16_t bits16(int type, float v) {
+    return type == OUT_F16 ? __builtin_bit_cast(uint16_t, from_float<f16_t>(v)) : from_float<bf16_t>(v).bits;
+}
+__device__ __forceinline__ unsigned pack16(int type, float a, float b) {
+    return type == OUT_F16 ? lin_pack<f16_t>(a, b) : pack_bf16(a, b);
+}
+__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+// v's three planes; infinities and NaN stay in the first one alone
+__device__ __forceinline__ void planes_of(float v, float (&q)[3]) {
+    // (rounded toward zero, so that the largest numbers do not become infinite)
+    q[0] = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
+    if (!finite) q[0] = v;
+    const float r = finite ? v - q[0] : 0.f;
+    q[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    q[2] = r - q[1];
+}
+__device__ __forceinline__ void out_one(const Out &o, long m, long n, float v) {
+    const size_t at = (size_t)m * o.pitch + n;
+    if (o.type == OUT_F32) {
+        reinterpret_cast<float *>(o.p)[at] = v;
+    } else if (o.type == OUT_PLANES) {
+        float q[3];
+        planes_of(v, q);
+#pragma unroll
+        for (int e = 0; e < 3; e++) reinterpret_cast<uint16_t *>(o.p)[at + e * o.plane] = from_float<bf16_t>(q[e]).bits;
+    } else {
+        reinterpret_cast<uint16_t *>(o.p)[at] = bits16(o.type, v);
+    }
+}
+__device__ __forceinline__ bool out_wide(const Out &o) {
+    return o.pitch % (o.type == OUT_F32 ? 4 : 8) == 0 && ((uintptr_t)o.p & 15) == 0;
+}
+
+// eight neighbours n .. n + 7 of row m (n a multiple of eight), those below N
+__device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long n, long N, const float (&v)[8]) {
+    if (!wide || n + 8 > N) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (n + e < N) out_one(o, m, n + e, v[e]);
+        return;
+    }
+    const size_t at = (size_t)m * o.pitch + n;
+    if (o.type == OUT_F32) {
+        mma_f4 *to = reinterpret_cast<mma_f4 *>(reinterpret_cast<float *>(o.p) + at);
+        to[0] = mma_f4{v[0], v[1], v[2], v[3]}, to[1] = mma_f4{v[4], v[5], v[6], v[7]};
+        return;
+    }
+    uint16_t *to = reinterpret_cast<uint16_t *>(o.p) + at;
+    if (o.type == OUT_PLANES) {
+        float q[8][3];
+#pragma unroll
+        for (int e = 0; e < 8; e++) planes_of(v[e], q[e]);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            *reinterpret_cast<mma_u4 *>(to + k * o.plane) =
+                mma_u4{pack_bf16(q[0][k], q[1][k]), pack_bf16(q[2][k], q[3][k]), pack_bf16(q[4][k], q[5][k]), pack_bf16(q[6][k], q[7][k])};
+        return;
+    }
+    *reinterpret_cast<mma_u4 *>(to) =
+        mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])};
+}
+
+struct Values {  // a vector of fp32 or 16-bit values, or none
+    const void *p;
+    int type;
+    __device__ __forceinline__ float at(long i) const {
+        if (type == OUT_F32) return reinterpret_cast<const float *>(p)[i];
+        const uint16_t b = reinterpret_cast<const uint16_t *>(p)[i];
+        return type == OUT_F16 ? to_float(__builtin_bit_cast(f16_t, b)) : bf16_value(b);
+    }
+};
+
+// exp(v): v_exp_f32 of v log2(e) with what the product's rounding leaves (relative error 1e-7 where a bare product's grows with |v|)
+__device__ __forceinline__ float prod_exp(float v) {
+    const float t = v * 1.44269504f;
+    const float r = __builtin_fmaf(v, 1.44269504f, -t) + v * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    // (infinities: e is 0 or infinite and r not a number)
+    return __builtin_fabsf(v) < 1e4f ? __builtin_fmaf(e, r * 0.693147181f, e) : e;
+}
+
+// The plain epilogue: out = alpha * sum + bias[n] + before[m][n].  With several splits the sums go to `part` as they are, and
+// product_reduce_kernel does the rest.  sums: the sums over k of A alone (a bias gradient), alpha times.
+struct PlainEpi {
+    static constexpr bool kSums = false;
+    Out out, sums;      // (sums.p null: none)
+    Values bias;        // (p null: none)
+    const float *alpha, *before;  // (null: 1, none); before: [M][pitch of out]
+    float *part;        // [splits][M][N], then [splits][M]
+    long rows_from, rows_skip;  // output rows from rows_from on lie rows_skip further up; those skipped are not written (0: none)
+    long tail;          // columns of A that are only padding (behind rows_from - rows_skip .. rows_from)
+    __device__ __forceinline__ long place(long m) const {  // of row m, or -1
+        if (rows_skip == 0) return m;
+        if (m < rows_from - rows_skip) return m;
+        if (m < rows_from) return -1;
+        return m - rows_skip < tail ? m - rows_skip : -1;
+    }
+    __device__ __forceinline__ float finish(long m, long n, float v, float a) const {
+        v = __builtin_fmaf(v, a, bias.p != nullptr ? bias.at(n) : 0.f);
+        if (before != nullptr) v += before[(size_t)m * out.pitch + n];
+        return v;
+    }
+    struct Lane {
+        float bias[8], alpha;
+        bool wide;
+    };
+    __device__ __forceinline__ Lane begin(const Product &p, long n) const {
+        Lane l;
+        l.alpha = alpha != nullptr && part == nullptr ? *alpha : 1.f;
+        l.wide = part != nullptr ? p.N % 4 == 0 : out_wide(out);
+#pragma unroll
+        for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && part == nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
+        return l;
+    }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int split, long m, long n, float (&v)[8]) const {
+        if (m >= p.M || n >= p.N) return;
+        if (part != nullptr) {
+            out_octet({part + (size_t)split * p.M * p.N, p.N, 0, OUT_F32}, l.wide, m, n, p.N, v);
+            return;
+        }
+        const long to = place(m);
+        if (to < 0) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e], l.alpha, l.bias[e]);
+        if (before != nullptr)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (n + e < p.N) v[e] += before[(size_t)to * out.pitch + n + e];
+        out_octet(out, l.wide, to, n, p.N, v);
+    }
+    __device__ __forceinline__ void emit_sum(const Product &p, int split, long m, float v) const {
+        if (m >= p.M) return;
+        if (part != nullptr) {
+            part[(size_t)p.splits * p.M * p.N + (size_t)split * p.M + m] = v;
+            return;
+        }
+        const long to = place(m);
+        if (to >= 0) out_one(sums, 0, to, v * (alpha != nullptr ? *alpha : 1.f));
+    }
+};
+
+struct SumsEpi : PlainEpi {
+    static constexpr bool kSums = true;
+};
+
+// ------------------------------------------------------------------------------------------------- the product
+// Tiles of BM x BN, WM x WN waves.  A stage is 64 summed indices of both operands, two stages in LDS.  While a wave multiplies the
+// first half of a stage it reads the second half's fragments; the one barrier of a step comes between the halves, when every wave
+// has the rest of its stage in registers: the stage's LDS takes the stage after the next, and the products of the second half
+// cover the reads of the next stage's first.
+template <int BM_, int BN_, int WM_, int WN_, int WAVES>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM_ * WN_, PER_SIMD = WAVES;
+    static constexpr int MF = BM_ / WM_ / 16, NF = BN_ / WN_ / 16;
+};
+typedef Shape<256, 256, 2, 4, 2> LargeTile;   // 128 KB of LDS, one workgroup per CU
+typedef Shape<128, 128, 2, 2, 2> MediumTile;  // 64 KB, two
+typedef Shape<64, 64, 2, 2, 4> SmallTile;     // 32 KB, four
+
+template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
+__global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Product p, Epi epi) {
+    constexpr int BM = S::BM, BN = S::BN, MF = S::MF, NF = S::NF, SF = MF / S::WN;
+    constexpr bool SUMS = Epi::kSums;
+    __shared__ __attribute__((aligned(16))) uint16_t la0[BM * kProdK];
+    __shared__ __attribute__((aligned(16))) uint16_t lb0[BN * kProdK];
+    __shared__ __attribute__((aligned(16))) uint16_t la1[BM * kProdK];
+    __shared__ __attribute__((aligned(16))) uint16_t lb1[BN * kProdK];
+    // an XCD (workgroup ids modulo eight) takes a run of tiles; runs go down groups of rows of tiles, so that the tiles of an XCD
+    // at one time share both operands' lines
+    const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    const int tiles = p.mtiles * p.ntiles;
+    const int split = id / tiles, tile = id % tiles;
+    if (split >= p.splits) return;
+    constexpr int GROUP = 8;
+    const int group = tile / (GROUP * p.ntiles), in = tile % (GROUP * p.ntiles), high = min(GROUP, p.mtiles - group * GROUP);
+    const int mt = group * GROUP + in % high, nt = in / high;
+    const long m0 = (long)mt * BM, n0 = (long)nt * BN;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    Stage<BM, S::THREADS, AS, 0> sa;
+    Stage<BN, S::THREADS, BS, GATED ? 8 * NF : 0> sb;
+    sa.init(p.a, p.M, m0, p.K, 0);
+    sb.init(p.b, GATED ? p.N / 2 : p.N, GATED ? n0 / 2 : n0, p.K, p.gap);
+    mma_f4 acc[NF][MF], accs[SF > 0 ? SF : 1];
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) acc[i][j] = mma_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < SF; j++) accs[j] = mma_f4{0.f, 0.f, 0.f, 0.f};
+
+    const int ksteps = (int)((p.K + kProdK - 1) / kProdK);
+    const int first = split * p.per, count = min(p.per, p.steps - first);
+    int pair = first / ksteps, left = count;
+    long k0 = (long)(first % ksteps) * kProdK;
+    // (a loop of one body: an odd last step is followed by one of zeros)
+    auto fetch = [&](uint16_t *la, uint16_t *lb) {
+        const bool live = left-- > 0;
+        sa.load(la, p.codes_a >> (2 * pair) & 3, k0, p.K, live);
+        sb.load(lb, p.codes_b >> (2 * pair) & 3, k0, p.K, live);
+        k0 += kProdK;
+        const bool wrap = k0 >= p.K;
+        k0 = wrap ? 0 : k0, pair = wrap ? pair + 1 : pair;
+    };
+    mma_s8 fa0[MF], fb0[NF], fa1[MF], fb1[NF];
+    auto read = [&](const uint16_t *la, const uint16_t *lb, int kk, mma_s8 (&fa)[MF], mma_s8 (&fb)[NF]) {
+#pragma unroll
+        for (int i = 0; i < NF; i++) fb[i] = prod_fragment<BN, BS>(lb, (wn * NF + i) * 16, kk);
+#pragma unroll
+        for (int j = 0; j < MF; j++) fa[j] = prod_fragment<BM, AS>(la, (wm * MF + j) * 16, kk);
+    };
+    auto multiply = [&](const mma_s8 (&fa)[MF], const mma_s8 (&fb)[NF]) {
+#pragma unroll
+        for (int j = 0; j < MF; j++)
+#pragma unroll
+            for (int i = 0; i < NF; i++) acc[i][j] = Mma<T>::run(fb[i], fa[j], acc[i][j]);
+    };
+    // sums over A alone, in the workgroups of the first column of tiles: products with ones, with zeros elsewhere and where a plane of A
+    // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all)
+    int at_pair = first / ksteps, at_step = first % ksteps;
+    auto add_sums = [&](const uint16_t *la) {
+        if constexpr (SUMS) {
+            const short one = nt == 0 && (p.codes_b >> (2 * at_pair) & 3) == 0 ? Mma<T>::kOne : 0;
+            at_step++;
+            const bool wrap = at_step == ksteps;
+            at_step = wrap ? 0 : at_step, at_pair = wrap ? at_pair + 1 : at_pair;
+            const mma_s8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                for (int j = 0; j < SF; j++)
+                    accs[j] = Mma<T>::run(ones, prod_fragment<BM, AS>(la, (wm * MF + wn * SF + j) * 16, kk), accs[j]);
+        }
+    };
+    auto step = [&](uint16_t *ca, uint16_t *cb, const uint16_t *na, const uint16_t *nb) {
+        add_sums(ca);
+        read(ca, cb, 1, fa1, fb1);
+        multiply(fa0, fb0);
+        __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's reads of the stage are done, and its part of the next one is there ..
+        asm volatile("s_barrier" ::: "memory");  // .. and the other waves'
+        fetch(ca, cb);
+        read(na, nb, 0, fa0, fb0);
+        multiply(fa1, fb1);
+    };
+    fetch(la0, lb0);
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("s_barrier" ::: "memory");
+    fetch(la1, lb1);
+    read(la0, lb0, 0, fa0, fb0);
+    for (int s = 0; s < count; s += 2) {
+        step(la0, lb0, la1, lb1);
+        step(la1, lb1, la0, lb0);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // (nothing may arrive behind the sums)
+    // The sums go through LDS, each wave's through its own part, and come back as eight neighbours of a row per lane (gated: eight
+    // gates and what they multiply): wide stores, row sums over few lanes, and a loop of one body.  Quads of a row are permuted by the row.
+    __syncthreads();
+    constexpr int QUADS = 4 * NF, PF = MF < 4 ? MF : 4, ROWS = 16 * PF, LANES = GATED ? NF : 2 * NF, STEP = 64 / LANES;
+    constexpr int WAVES = S::THREADS / 64, SHARE = WAVES / 4;  // (waves per array)
+    static_assert(BM == BN && SHARE >= 1 && ROWS * 16 * NF * 4 * SHARE <= BM * kProdK * 2, "the waves' parts fit the stages");
+    float *mine = reinterpret_cast<float *>(wave / SHARE == 0 ? la0 : wave / SHARE == 1 ? lb0 : wave / SHARE == 2 ? la1 : lb1) +
+                  wave % SHARE * ROWS * 16 * NF;
+    const int lane = threadIdx.x & 63;
+    const int o = lane % LANES, row0 = lane / LANES;
+    const long nl = (GATED ? n0 / 2 + wn * 8 * NF : n0 + wn * 16 * NF) + o * 8;
+    const auto local = epi.begin(p, nl);
+#pragma unroll
+    for (int pass = 0; pass < MF / PF; pass++) {
+#pragma unroll
+        for (int j = 0; j < PF; j++)
+#pragma unroll
+            for (int i = 0; i < NF; i++) {
+                const int row = 16 * j + (lane & 15), quad = 4 * i + (lane >> 4);
+                reinterpret_cast<mma_f4 *>(mine)[row * QUADS + (quad ^ (row & (QUADS - 1)))] = acc[i][pass * PF + j];
+            }
+        auto octet = [&](int row, int at, float (&v)[8]) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const mma_f4 q = reinterpret_cast<const mma_f4 *>(mine)[row * QUADS + ((2 * at + h) ^ (row & (QUADS - 1)))];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * h + e] = q[e];
+            }
+        };
+        const long mp = m0 + wm * 16 * MF + pass * ROWS;
+#pragma unroll 1
+        for (int row = row0; row < ROWS; row += STEP) {
+            float v[8];
+            octet(row, o, v);
+            if constexpr (GATED) {
+                float u[8];
+                octet(row, NF + o, u);
+                epi.octet(p, local, mp + row, nl, v, u);
+            } else {
+                epi.octet(p, local, split, mp + row, nl, v);
+            }
+        }
+    }
+    if constexpr (SUMS)
+        if (nt == 0 && (threadIdx.x & 63) < 16) {
+#pragma unroll
+            for (int j = 0; j < SF; j++) epi.emit_sum(p, split, m0 + (wm * MF + wn * SF + j) * 16 + (threadIdx.x & 15), accs[j][0]);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------- on the host
+// A workspace handed out piece by piece.  With no memory behind it, it measures: the calls below then launch nothing.
+struct Arena {
+    char *base;
+    size_t used;
+    bool dry() const { return base == nullptr; }
+    void *take(size_t bytes) {
+        void *p = base != nullptr ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+inline long up8(long n) { return (n + 7) / 8 * 8; }
+inline int status() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : (int)e;
+}
+inline unsigned blocks_for(long work, long most = 4096) {
+    const long n = (work + 255) / 256;
+    return (unsigned)(n < 1 ? 1 : n < most ? n : most);
+}
+inline size_t size_of(int dtype) { return dtype == DWO_F32 ? 4 : 2; }
+inline bool known(int dtype) { return dtype == DWO_F32 || dtype == DWO_BF16 || dtype == DWO_F16; }
+
+// room for an operand of rows x pitch that a kernel writes
+inline Operand take_operand(Arena &ws, long rows, long pitch, int dtype) {
+    Operand o;
+    o.planes = dtype == DWO_F32 ? 3 : 1;
+    o.pitch = pitch, o.plane = rows * pitch;
+    o.p = ws.take((size_t)o.planes * o.plane * 2);
+    return o;
+}
+inline Out out_of(const Operand &o, int dtype) {
+    return {const_cast<void *>(o.p), o.pitch, o.plane, dtype == DWO_F32 ? OUT_PLANES : dtype};
+}
+// a dense [rows][cols] matrix as an operand: itself, or a copy that is one (dwo_product.hip).  move > 0: the rows from `gate` on go `move`
+// rows further down, with zeros between and behind.
+int stage_operand(Operand &o, const void *src, long rows, long cols, int dtype, Arena &ws, hipStream_t st, long gate = 0, long move = 0);
+
+// D = A B with the plain epilogue; a_slow, b_slow: the operand lies with the summed index as its slow one (dwo_product.hip).  epi.part
+// is filled in here.
+int plain_product(const Operand &a, bool a_slow, const Operand &b, bool b_slow, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws,
+                  hipStream_t st);
+
+inline PlainEpi plain_epilogue(const Out &out) { return {out, {nullptr, 0, 0, 0}, {nullptr, 0}, nullptr, nullptr, nullptr, 0, 0, 0}; }
+
+// products whose epilogue is not the plain one
+template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
+int launch_shape(Product p, const Epi &epi, hipStream_t st) {
+    p.mtiles = (int)((p.M + S::BM - 1) / S::BM), p.ntiles = (int)((p.N + S::BN - 1) / S::BN);
+    const long total = (long)p.mtiles * p.ntiles * p.splits;
+    if (total > 0x7ffffff0L) return DWO_ERR_BAD_SHAPE;
+    product_kernel<T, S, AS, BS, GATED, Epi><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(S::THREADS), 0, st>>>(p, epi);
+    return status();
+}
+inline long tiles_of(long M, long N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
+inline Product make_product(const Operand &a, const Operand &b, long M, long N, long K, long gap) {
+    Product p{a, b, M, N, K, gap, 1, 0, 0, 0, 0, 1, 0, 0};
+    product_pairs(p);
+    p.steps = p.per = (int)((K + kProdK - 1) / kProdK * p.pairs);
+    return p;
+}
+inline int tile_for(long M, long N) { return tiles_of(M, N, 256, 256) >= 200 ? 256 : tiles_of(M, N, 128, 128) >= 160 ? 128 : 64; }
+// columns of a wave
+inline int wave_columns(long M, long N) { return tile_for(M, N) == 64 ? 16 * SmallTile::NF : 16 * LargeTile::NF; }
+template <typename T, bool AS, bool BS, bool GATED, class Epi>
+int launch_tiles(const Product &p, const Epi &epi, hipStream_t st) {
+    switch (tile_for(p.M, p.N)) {
+        case 256: return launch_shape<T, LargeTile, AS, BS, GATED>(p, epi, st);
+        case 128: return launch_shape<T, MediumTile, AS, BS, GATED>(p, epi, st);
+        default: return launch_shape<T, SmallTile, AS, BS, GATED>(p, epi, st);
+    }
+}
+template <bool AS, bool BS, bool GATED, class Epi>
+int launch_product(const Product &p, int dtype, const Epi &epi, hipStream_t st) {
+    if (dtype == DWO_F16) return launch_tiles<f16_t, AS, BS, GATED>(p, epi, st);
+    return launch_tiles<bf16_t, AS, BS, GATED>(p, epi, st);
+}
+
+}  // namespace dwo

@@ -294,7 +294,7 @@ def _norm_type(x, C, norm, consumer):
     ac = _autocast(x)
     if ac is None:
         return x.dtype if x.dtype == w.dtype == b.dtype else None
-    out = ac if ac in _DTYPES and consumer is not None and plain(consumer, Linear) else torch.float32
+    out = ac if ac in _DTYPES and consumer is not None and plain(consumer, *CONSUMERS) else torch.float32
     return out if x.dtype == out or torch.float32 in (x.dtype, out) else None
 
 
@@ -460,6 +460,10 @@ class Linear(torch.nn.Linear):
                     ac is not None or (x.dtype == w.dtype and (b is None or b.dtype == w.dtype))):
                 return _linear16(x.to(dtype), w, b)
         return F.linear(x, w, b)
+
+
+# Modules that convert what they read under autocast, as a pointwise layer does
+CONSUMERS = [Linear]
 
 
 def tile_norm(x, norm, consumer=None):

@@ -1,0 +1,618 @@
+"""The operators around wide layers (gated feed-forward block, cross entropy of many classes, layers and activations with 8-bit
+checkpoints) against their formulas in 64 bits.
+
+Tolerances, with r = eps / 2 of the type (half a step, relative).  A result is rounded once: at most r of each value.  In 16 bits the
+products of the backward passes, and the gated block's second, read an operand that was computed and rounded once, an error of at most r of
+each term and of either sign: at most r of the result's norm where terms add up like random numbers, as here.  fp32 sums of n terms
+lose about 0.3 2^-24 sqrt(n / 2) (8e-7 at n = 2048), exponentials, activations and the logits before them about 1e-6.  So the norm of
+the difference is at most 2 r + 4e-6 of the reference's; a single value is off by r of itself and 16 times that limit of the root mean
+square (a sum of errors of either sign, over as many values as here, stays within six of its deviations)."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from oriented1d_amd import checkpoint8, feedforward, losses
+from oriented1d_amd.convnext1d import Block, ConvNeXt1D
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+ACT = {"gelu": F.gelu, "silu": F.silu}
+
+
+def near(got, ref, what, rounding=None, terms=None, rounded=0.0):
+    """``terms``: magnitudes of what cancels in each value before any rounding to 16 bits, of which fp32 leaves 1e-6.  ``rounded``: the sum
+    of the magnitudes of a value's terms that hold a rounded operand, of which each is off by r at most: where a few rows are much
+    larger than the others the mean square says nothing of them (a class that one row has as its target: one term of size 1 in a
+    gradient whose other rows are 1e-5, two roundings of it)."""
+    assert got is not None and got.shape == ref.shape, what
+    r = torch.finfo(got.dtype).eps / 2
+    limit = 2 * max(r, rounding or 0.0) + 4e-6
+    g, ref = got.double(), ref.double()
+    assert torch.isfinite(g).all(), "%s: not finite" % what
+    # (below the smallest normal number of fp16 a step is 2^-24)
+    floor = 2.0 ** -25 if got.dtype == torch.float16 else 1e-30
+    if terms is not None:
+        floor += 1e-6 * float(terms.detach().norm()) / math.sqrt(max(g.numel(), 1))
+    off, norm = (g - ref).detach(), float(ref.detach().norm())
+    assert float(off.norm()) <= limit * norm + floor * math.sqrt(g.numel()), "%s: relative error %.3g, limit %.3g" % (
+        what, float(off.norm()) / max(norm, 1e-300), limit)
+    rms = norm / math.sqrt(max(g.numel(), 1))
+    bad = off.abs() > r * ref.detach().abs() + r * rounded + 16 * limit * rms + floor
+    assert not bad.any(), "%s: %d values off, worst %.3g at root mean square %.3g" % (what, int(bad.sum()), float(off.abs().max()), rms)
+
+
+def held8(x):
+    """The values that an 8-bit checkpoint of x stands for, in 64 bits."""
+    C = x.shape[-1]
+    v = F.pad(x.double(), (0, -C % 32)).unflatten(-1, (-1, 32))
+    finite = torch.isfinite(v).all(-1, keepdim=True)
+    clean = torch.where(finite, v, 0.0)
+    exponent = torch.frexp(clean.abs().amax(-1, keepdim=True))[1] - 7
+    # (the power of two by its bits: torch.ldexp goes through pow, which is not exact)
+    step = ((exponent.clamp(min=-126).long() + 1023) << 52).view(torch.float64)
+    held = torch.round(clean / step).clamp(-127, 127) * step
+    return torch.where(finite, held, float("nan")).flatten(-2)[..., :C]
+
+
+def leaves64(*tensors):
+    return [None if t is None else t.detach().double().requires_grad_() for t in tensors]
+
+
+def gated64(x, w_in, b_in, w_out, b_out, act):
+    gate, up = F.linear(x, w_in, b_in).chunk(2, dim=-1)
+    return F.linear(ACT[act](gate) * up, w_out, b_out)
+
+
+def make_gated(rows, C, H, D, dtype, bias=True, seed=0, param=None):
+    gen = torch.Generator("cuda").manual_seed(seed + rows + C)
+
+    def values(*shape, std=1.0, t=dtype):
+        return (torch.randn(shape, generator=gen, device="cuda") * std).to(t).requires_grad_()
+
+    param = param or dtype
+    x = values(rows, C)
+    w_in, w_out = values(2 * H, C, std=1.5 * C ** -0.5, t=param), values(D, H, std=H ** -0.5, t=param)
+    b_in, b_out = (values(2 * H, std=0.3, t=param), values(D, std=0.3, t=param)) if bias else (None, None)
+    dy = values(rows, D).detach()
+    return [x, w_in, b_in, w_out, b_out], dy
+
+
+GATED = [(1, 8, 8, 8), (3, 5, 7, 9), (49, 96, 256, 96), (64, 64, 32, 72), (65, 129, 33, 1), (300, 72, 100, 40), (257, 640, 130, 64),
+         (1100, 1, 1, 1)]
+
+
+@pytest.mark.parametrize("held", [False, True], ids=["kept", "held8"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", GATED, ids=str)
+def test_gated_mlp(shape, dtype, act, held):
+    bias = shape[0] % 2 == 1
+    args, dy = make_gated(*shape, dtype, bias)
+    y = feedforward.gated_mlp(*args, activation=act, checkpoint8=held)
+    assert y.dtype == dtype and y.is_contiguous()
+    leaves = [t for t in args if t is not None]
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = leaves64(*args)
+    near(y, gated64(*ref, act), "y")
+    if held:
+        ref[0] = held8(args[0].detach()).requires_grad_()
+    want = torch.autograd.grad(gated64(*ref, act), [t for t in ref if t is not None], dy.double())
+    names = ["dx", "dw_in", "db_in", "dw_out", "db_out"] if bias else ["dx", "dw_in", "dw_out"]
+    for g, t, w, name in zip(got, leaves, want, names):
+        assert g.dtype == t.dtype
+        near(g, w, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows,C,H,D", [(2560, 32, 2560, 72), (4300, 136, 1300, 1288)], ids=str)
+def test_gated_mlp_large_tiles(rows, C, H, D, dtype):
+    args, dy = make_gated(rows, C, H, D, dtype)
+    y = feedforward.gated_mlp(*args)
+    got = torch.autograd.grad(y, args, dy)
+    ref = leaves64(*args)
+    out = gated64(*ref, "gelu")
+    near(y, out, "y")
+    for g, w, name in zip(got, torch.autograd.grad(out, ref, dy.double()), ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
+        near(g, w, name)
+
+
+def test_gated_mlp_without_gradients_and_single_rows():
+    for rows in (1, 2, 17):
+        args, _ = make_gated(rows, 256, 1024, 256, torch.bfloat16)
+        with torch.no_grad():
+            y = feedforward.gated_mlp(*args)
+        assert not y.requires_grad
+        near(y, gated64(*leaves64(*args), "gelu"), "y")
+
+
+def test_gated_gradients_of_some_inputs():
+    args, dy = make_gated(37, 40, 48, 24, torch.float32)
+    ref = leaves64(*args)
+    want = torch.autograd.grad(gated64(*ref, "gelu"), ref, dy.double())
+    for wanted in ([0], [1], [2], [3], [4], [0, 4], [2, 3]):
+        for held in (False, True):
+            some = [t.detach().requires_grad_(i in wanted) for i, t in enumerate(args)]
+            y = feedforward.gated_mlp(*some, checkpoint8=held)
+            got = torch.autograd.grad(y, [some[i] for i in wanted], dy)
+            if not held:
+                for g, i in zip(got, wanted):
+                    near(g, want[i], "input %d of %s" % (i, wanted))
+            else:
+                at = leaves64(*args)
+                at[0] = held8(args[0].detach()).requires_grad_()
+                for g, w in zip(got, torch.autograd.grad(gated64(*at, "gelu"), [at[i] for i in wanted], dy.double())):
+                    near(g, w, "held, of %s" % wanted)
+
+
+def test_gated_differences():
+    """The gradient against differences of the result: along a direction d, (f(x + h d) - f(x - h d)) / 2 h is off by the third derivative,
+    about h^2, and by what fp32 leaves of the results, about 1e-6 |f| / h: h = 1e-2, 1e-3 of the norms involved."""
+    args, dy = make_gated(20, 24, 40, 16, torch.float32, seed=5)
+    y = feedforward.gated_mlp(*args, activation="silu")
+    got = torch.autograd.grad(y, args, dy)
+    h = 1e-2
+    for i, g in enumerate(got):
+        d = torch.randn_like(args[i])
+        d /= d.norm()
+        with torch.no_grad():
+            moved = [feedforward.gated_mlp(*[t + s * h * d if k == i else t for k, t in enumerate(args)], activation="silu")
+                     for s in (1, -1)]
+        slope = float(((moved[0].double() - moved[1].double()) * dy.double()).sum()) / (2 * h)
+        assert abs(slope - float((g * d).double().sum())) <= 2e-3 * float(dy.double().norm()) * math.sqrt(d.numel()) / math.sqrt(d.numel()), i
+
+
+@pytest.mark.parametrize("what", ["gated", "linear8", "head"])
+def test_parameters_of_another_type(what):
+    """16-bit activations, fp32 parameters: results as with parameters converted, gradients of the parameters' own type."""
+    args, dy = make_gated(130, 64, 72, 40, torch.bfloat16, param=torch.float32)
+    x, w_in, b_in, w_out, b_out = args
+    r = 2.0 ** -8
+    if what == "gated":
+        y = feedforward.gated_mlp(*args)
+        got = torch.autograd.grad(y, args, dy)
+        ref = leaves64(x, *[t.detach().bfloat16() for t in args[1:]])
+        want = torch.autograd.grad(gated64(*ref, "gelu"), ref, dy.double())
+        leaves = args
+    elif what == "linear8":
+        y = checkpoint8.linear8(x, w_in, b_in)
+        dy = torch.randn_like(y)
+        leaves = [x, w_in, b_in]
+        got = torch.autograd.grad(y, leaves, dy)
+        ref = leaves64(held8(x.detach()), w_in.detach().bfloat16(), b_in.detach().bfloat16())
+        want = torch.autograd.grad(F.linear(*ref), ref, dy.double())
+    else:
+        target = torch.randint(0, w_in.shape[0], (130,), device="cuda")
+        y = losses.linear_cross_entropy(x, w_in, b_in, target)
+        leaves = [x, w_in, b_in]
+        got = torch.autograd.grad(y, leaves)
+        ref = leaves64(x, w_in.detach().bfloat16(), b_in.detach().bfloat16())
+        want = torch.autograd.grad(F.cross_entropy(F.linear(*ref), target), ref)
+    for g, t, w in zip(got, leaves, want):
+        assert g.dtype == t.dtype
+        near(g, w, what, rounding=r)
+
+
+@pytest.mark.parametrize("what", ["gated", "linear8", "head"])
+def test_autocast(what):
+    args, _ = make_gated(66, 64, 72, 40, torch.float32)
+    x, w_in, b_in, w_out, b_out = args
+    target = torch.randint(0, 144, (66,), device="cuda")
+    call = {"gated": lambda *a: feedforward.gated_mlp(*a), "linear8": lambda a, b, c, *_: checkpoint8.linear8(a, b, c),
+            "head": lambda a, b, c, *_: losses.linear_cross_entropy(a, b, c, target)}[what]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = call(*args)
+    assert y.dtype == (torch.float32 if what == "head" else torch.bfloat16)
+    y.float().square().sum().backward()
+    used = args if what == "gated" else args[:3]
+    assert all(t.grad is not None and t.grad.dtype == torch.float32 and torch.isfinite(t.grad).all() for t in used)
+    same = call(x.detach().bfloat16(), *[t.detach() for t in args[1:]])
+    assert torch.equal(y, same)
+
+
+# ---------------------------------------------------------------------------------------------------- cross entropy
+HEAD = [(1, 16, 1), (1, 16, 10), (5, 7, 13), (64, 768, 1000), (300, 100, 257), (33, 64, 21841), (2000, 8, 3), (700, 96, 4099)]
+
+
+def make_head(rows, C, V, dtype, bias=True, ignored=0.0, seed=0):
+    gen = torch.Generator("cuda").manual_seed(seed + rows + V)
+    x = torch.randn((rows, C), generator=gen, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn((V, C), generator=gen, device="cuda") * 2 * C ** -0.5).to(dtype).requires_grad_()
+    b = (torch.randn((V,), generator=gen, device="cuda") * 0.3).to(dtype).requires_grad_() if bias else None
+    target = torch.randint(0, V, (rows,), generator=gen, device="cuda")
+    if ignored:
+        target[torch.rand((rows,), generator=gen, device="cuda") < ignored] = -100
+        target[0] = V - 1
+    return x, w, b, target
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("smoothing,ignored", [(0.0, 0.0), (0.1, 0.4)], ids=["plain", "smoothed"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", HEAD, ids=str)
+def test_linear_cross_entropy(shape, dtype, smoothing, ignored, reduction):
+    x, w, b, target = make_head(*shape, dtype, bias=shape[0] != 5, ignored=ignored)
+    leaves = [t for t in (x, w, b) if t is not None]
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction=reduction, label_smoothing=smoothing)
+    assert loss.dtype == torch.float32 and loss.shape == (target.shape if reduction == "none" else ())
+    # (a mean in fp16 is trained with a scaled loss)
+    up = torch.rand_like(loss) + 0.5 if reduction == "none" else torch.full_like(loss, 256.0)
+    got = torch.autograd.grad(loss, leaves, up)
+    ref = leaves64(x, w, b)
+    want = F.cross_entropy(F.linear(*ref), target, reduction=reduction, label_smoothing=smoothing)
+    # (a loss is a difference of two numbers of the size of a logit)
+    assert ((loss.double() - want).abs() <= 4e-6 * (want.abs() + 12)).all()
+    # the logits' gradients are differences of a probability, (1 - smoothing) at the target and smoothing / V
+    with torch.no_grad():
+        size = torch.softmax(F.linear(*ref), 1)
+        size[torch.arange(len(target)), target.clamp(min=0)] += 1
+        size *= torch.where(target >= 0, up.double() / (1 if reduction == "none" else (target >= 0).sum()), 0.0)[:, None]
+        terms = size @ ref[1].abs(), size.t() @ ref[0].abs(), size.sum(0)
+    logits = F.linear(*ref)
+    each = F.cross_entropy(logits, target, reduction=reduction, label_smoothing=smoothing)
+    size = torch.autograd.grad(each, logits, up.double())[0].abs()
+    rounded = size @ ref[1].abs(), size.t() @ ref[0].abs(), size.sum(0)
+    for g, r, t, o, name in zip(got, torch.autograd.grad(want, [t for t in ref if t is not None], up.double()), terms, rounded,
+                                ["dx", "dw", "db"]):
+        near(g, r, name, terms=t, rounded=o.detach())
+    with torch.no_grad():
+        again = losses.linear_cross_entropy(x, w, b, target, reduction=reduction, label_smoothing=smoothing)
+    assert torch.equal(again, loss)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "f16", "f32"])
+def test_cross_entropy_in_pieces(dtype):
+    """More rows times classes than a piece of the backward pass holds."""
+    x, w, b, target = make_head(20000, 32, 8003, dtype)
+    up = torch.tensor(512.0, device="cuda")
+    got = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target, label_smoothing=0.05), [x, w, b], up)
+    ref = leaves64(x, w, b)
+    want = F.cross_entropy(F.linear(*ref), target, label_smoothing=0.05)
+    for g, r, name in zip(got, torch.autograd.grad(want, ref, up.double()), ["dx", "dw", "db"]):
+        near(g, r, name)
+
+
+def test_cross_entropy_special_rows():
+    x, w, b, target = make_head(40, 24, 50, torch.float32)
+    # classes that cannot be: -infinity; logits far from zero; a row that is not a number but ignored
+    with torch.no_grad():
+        b[3] = float("-inf")
+        b[4] = 300.0
+        b[5] = -3e4
+        target[:] = torch.where(target == 3, 4, target)
+        x[7] *= 1e3
+    ref = leaves64(x, w, b)
+    want = F.cross_entropy(F.linear(*ref), target, reduction="none")
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction="none")
+    # (logits of 1e4: fp32 sums leave 1e-6 of them)
+    assert ((loss.double() - want).abs() <= 1e-5 * want.abs() + 2e-2 * (want.abs() > 1e3) + 2e-4).all()
+    got = torch.autograd.grad(loss.sum(), [x, w, b])
+    for g, r in zip(got, torch.autograd.grad(want.sum(), ref)):
+        assert torch.isfinite(g).all()
+        assert float((g.double() - r).norm()) <= 1e-3 * float(r.norm())
+    # every target ignored: no mean, zero gradients
+    ignored = torch.full_like(target, -100)
+    loss = losses.linear_cross_entropy(x, w, b, ignored)
+    assert torch.isnan(loss)
+    per_row = losses.linear_cross_entropy(x, w, b, ignored, reduction="none")
+    assert (per_row == 0).all()
+    for g in torch.autograd.grad(per_row.sum(), [x, w, b]):
+        assert (g == 0).all()
+    for g in torch.autograd.grad(loss, [x, w, b]):
+        assert (g == 0).all()
+    # a target that is no class: NaN in its row alone
+    odd = target.clone()
+    odd[11], odd[12] = 50, -1
+    loss = losses.linear_cross_entropy(x, w, b, odd, reduction="none")
+    assert torch.isnan(loss[11:13]).all() and torch.isfinite(loss[:11]).all() and torch.isfinite(loss[13:]).all()
+    dx, = torch.autograd.grad(loss.sum(), [x])
+    assert torch.isnan(dx[11:13]).all() and torch.isfinite(dx[:11]).all() and torch.isfinite(dx[13:]).all()
+    assert torch.equal(losses.linear_cross_entropy(x, w, b, torch.where(odd == 50, 7, target), ignore_index=7, reduction="none")[11:12],
+                       torch.zeros(1, device="cuda"))
+
+
+def test_cross_entropy_nan_and_infinity():
+    x, w, b, target = make_head(9, 16, 70, torch.bfloat16)
+    with torch.no_grad():
+        x[2, 3] = float("nan")
+        x[4, 0] = float("inf")
+    target[6] = -100
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction="none")
+    want = F.cross_entropy(F.linear(x.double(), w.double(), b.double()), target, reduction="none")
+    assert torch.equal(torch.isnan(loss), torch.isnan(want)) and loss[6] == 0
+    fine = ~torch.isnan(want)
+    assert ((loss[fine].double() - want[fine]).abs() <= 1e-4).all()
+
+
+# ---------------------------------------------------------------------------------------------------- 8-bit checkpoints
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 1), (7, 32), (3, 333), (64, 96), (2, 5, 100), (1000, 31), (129, 2048)], ids=str)
+def test_pack8(shape, dtype):
+    torch.manual_seed(shape[-1])
+    x = (torch.randn(shape, device="cuda") * torch.exp(3 * torch.randn(shape[:-1] + (1,), device="cuda"))).to(dtype)
+    flat = x.view(-1)
+    flat[:: 41] = 0
+    if flat.numel() > 64:
+        flat[:32] = 0
+        flat[-1] = torch.finfo(dtype).tiny  # next to larger ones
+    p = checkpoint8.pack8(x)
+    assert p.codes.shape == x.shape and p.codes.dtype == torch.int8 and p.dtype == dtype
+    assert p.exponents.shape == shape[:-1] + (-(-shape[-1] // 32),)
+    got = checkpoint8.unpack8(p)
+    assert got.dtype == dtype and torch.equal(got.double(), held8(x))
+    assert torch.equal(checkpoint8.unpack8(checkpoint8.pack8(got)), got)
+
+
+def test_pack8_borders():
+    """Every exponent that fp32 has, ties, the largest numbers, and groups that are not finite."""
+    e = torch.arange(-149, 128, device="cuda", dtype=torch.float64)
+    x = torch.zeros(len(e), 32, dtype=torch.float64, device="cuda")
+    x[:, 0] = ((e.long() + 1023) << 52).view(torch.float64)
+    x[:, 1:] = x[:, :1] * torch.linspace(-1, 1, 31, device="cuda", dtype=torch.float64)
+    x[:, 5] = x[:, 0] * (64.5 / 64)  # a tie, largest magnitude of its group
+    x[:, 6] = x[:, 0] * (33.5 / 64)
+    x = x.float()
+    assert torch.equal(checkpoint8.unpack8(checkpoint8.pack8(x)).double(), held8(x))
+    top = torch.full((2, 32), torch.finfo(torch.float32).max, device="cuda")
+    top[1] *= -1
+    assert torch.equal(checkpoint8.unpack8(checkpoint8.pack8(top)).double(), held8(top))
+    for dtype in DTYPES:
+        y = torch.randn(4, 96, device="cuda").to(dtype)
+        y[0, 40], y[1, 2], y[2, 95] = float("nan"), float("inf"), float("-inf")
+        got = checkpoint8.unpack8(checkpoint8.pack8(y))
+        want = held8(y)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got[~torch.isnan(got)].double(), want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 1), (5, 333), (64, 96), (2, 3, 4, 64), (4099, 40)], ids=str)
+def test_act8(shape, dtype, act):
+    torch.manual_seed(shape[-1])
+    x = (torch.randn(shape, device="cuda") * 2).to(dtype).requires_grad_()
+    dy = torch.randn(shape, device="cuda").to(dtype)
+    y = checkpoint8.act8(x, act)
+    got, = torch.autograd.grad(y, x, dy)
+    near(y, ACT[act](x.detach().double()), "y")
+    at = held8(x.detach()).requires_grad_()
+    near(got, torch.autograd.grad(ACT[act](at), at, dy.double())[0], "dx")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,C,D", [(1, 1, 1), (1, 64, 8), (301, 100, 61), (196, 384, 96), (1000, 33, 520), (5000, 64, 192)], ids=str)
+def test_linear8(rows, C, D, dtype):
+    gen = torch.Generator("cuda").manual_seed(rows + C)
+    x = torch.randn((rows, C), generator=gen, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn((D, C), generator=gen, device="cuda") * C ** -0.5).to(dtype).requires_grad_()
+    b = torch.randn((D,), generator=gen, device="cuda").to(dtype).requires_grad_() if rows % 2 else None
+    dy = torch.randn((rows, D), generator=gen, device="cuda").to(dtype)
+    y = checkpoint8.linear8(x, w, b)
+    leaves = [t for t in (x, w, b) if t is not None]
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = leaves64(x, w, b)
+    out = F.linear(*ref)
+    near(y, out, "y")
+    near(got[0], torch.autograd.grad(out, ref[0], dy.double())[0], "dx")
+    near(got[1], dy.double().t() @ held8(x.detach()), "dw")
+    if b is not None:
+        near(got[2], dy.double().sum(0), "db")
+    with torch.no_grad():
+        assert torch.equal(checkpoint8.linear8(x, w, b), y)
+
+
+# ---------------------------------------------------------------------------------------------------- how they are called
+def test_layouts_and_views():
+    """Leading dimensions, transposed and offset tensors, gradients that are broadcast: as their dense copies."""
+    torch.manual_seed(0)
+    base = torch.randn(2, 3, 4, 41, device="cuda", dtype=torch.bfloat16)
+    x = base.permute(2, 0, 1, 3)[..., 1:]                      # 40 channels, odd offsets
+    w_in = torch.randn(40, 48, device="cuda", dtype=torch.bfloat16).t()
+    w_out = torch.randn(25, 24, device="cuda", dtype=torch.bfloat16)[1:]
+    b = torch.randn(48, 2, device="cuda", dtype=torch.bfloat16)[:, 0]
+    target = torch.randint(0, 48, (3, 2, 4), device="cuda").permute(2, 1, 0)
+    calls = [lambda x, w, v, b, t: feedforward.gated_mlp(x, w, b, v, None), lambda x, w, v, b, t: checkpoint8.linear8(x, w, b),
+             lambda x, w, v, b, t: checkpoint8.act8(x, "silu"),
+             lambda x, w, v, b, t: losses.linear_cross_entropy(x, w, b, t, reduction="none")]
+    for call in calls:
+        results = []
+        for copy in (False, True):
+            args = [t.detach().clone(memory_format=torch.contiguous_format) if copy else t.detach() for t in (x, w_in, w_out, b)]
+            for t in args:
+                t.requires_grad_()
+            y = call(*args, target.contiguous() if copy else target)
+            assert y.shape[:3] == x.shape[:3]
+            up = torch.ones((), device="cuda", dtype=y.dtype).expand(y.shape)
+            results.append((y, *[g for g in torch.autograd.grad(y, args, up, allow_unused=True) if g is not None]))
+        for got, want in zip(*results):
+            assert torch.equal(got, want)
+
+
+def test_no_rows():
+    for dtype in DTYPES:
+        args, _ = make_gated(2, 16, 24, 8, dtype)
+        x = torch.empty(0, 5, 16, device="cuda", dtype=dtype, requires_grad=True)
+        for call in (lambda: feedforward.gated_mlp(x, *args[1:]), lambda: feedforward.gated_mlp(x, *args[1:], checkpoint8=True),
+                     lambda: checkpoint8.linear8(x, args[1], args[2]), lambda: checkpoint8.act8(x),
+                     lambda: losses.linear_cross_entropy(x, args[1], args[2], torch.empty(0, 5, dtype=torch.long, device="cuda"),
+                                                         reduction="none")):
+            y = call()
+            assert y.shape[:2] == (0, 5)
+            grads = torch.autograd.grad(y, [x, args[1]], torch.zeros_like(y), allow_unused=True)
+            assert grads[0].shape == x.shape and (grads[1] is None or (grads[1] == 0).all())
+        mean = losses.linear_cross_entropy(x, args[1], args[2], torch.empty(0, 5, dtype=torch.long, device="cuda"))
+        assert torch.isnan(mean)
+
+
+def step(args, dy, target):
+    """One training step over all of them, as a network runs them: block, layer, activation, head."""
+    x, w_in, b_in, w_out, b_out = args
+    y = feedforward.gated_mlp(x, w_in, b_in, w_out, b_out, checkpoint8=True)
+    z = checkpoint8.act8(checkpoint8.linear8(y, w_in, b_in))
+    loss = losses.linear_cross_entropy(z, w_in.t().contiguous(), None, target, label_smoothing=0.1)
+    return [loss, *torch.autograd.grad(loss, args)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_run_of_all(dtype):
+    """All of them behind each other; the gradients against the same values from plain layers, whose distance is what the 8-bit
+    checkpoints cost: steps of 2^-6 to 2^-7 of a group's largest value, 2 % of an activation's norm at most, through four layers."""
+    args, dy = make_gated(96, 64, 40, 64, dtype, seed=3)
+    target = torch.randint(0, 64, (96,), device="cuda")
+    got = step(args, dy, target)
+    x, w_in, b_in, w_out, b_out = ref = leaves64(*args)
+    z = F.gelu(F.linear(gated64(*ref, "gelu"), w_in, b_in))
+    loss = F.cross_entropy(F.linear(z, w_in.t()), target, label_smoothing=0.1)
+    want = [loss, *torch.autograd.grad(loss, ref)]
+    assert abs(float(got[0]) - float(want[0])) <= 1e-2 * float(want[0])
+    for g, w in zip(got[1:], want[1:]):
+        assert float((g.double() - w).norm()) <= 0.08 * float(w.norm())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_repeats_streams_and_graphs(dtype):
+    """The same bits every time: again, on another stream, and replayed from a graph with other work between."""
+    args, dy = make_gated(200, 64, 56, 64, dtype, seed=7)
+    target = torch.randint(0, 64, (200,), device="cuda")
+    want = [t.detach().clone() for t in step(args, dy, target)]
+    for got, w in zip(step(args, dy, target), want):
+        assert torch.equal(got, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = step(args, dy, target)
+    torch.cuda.current_stream().wait_stream(side)
+    for got, w in zip(again, want):
+        assert torch.equal(got, w)
+    del again, got  # (no eager graph of these leaves while one is captured)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(args, dy, target)
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(captured, want):
+            assert torch.equal(got, w)
+        step(args, dy, target)
+        torch.randn(1 << 20, device="cuda").sum().item()
+    # another input in the same place
+    with torch.no_grad():
+        args[0].copy_(args[0].roll(1, 0))
+    fresh = [t.detach().clone() for t in step(args, dy, target)]
+    graph.replay()
+    for got, w in zip(captured, fresh):
+        assert torch.equal(got, w)
+
+
+def test_two_graphs():
+    """Two captured graphs hold workspaces of their own: replayed in turn they do not disturb each other."""
+    first, dy = make_gated(150, 64, 56, 64, torch.bfloat16, seed=1)
+    second, _ = make_gated(90, 64, 72, 64, torch.bfloat16, seed=2)
+    t1, t2 = torch.randint(0, 64, (150,), device="cuda"), torch.randint(0, 64, (90,), device="cuda")
+    want = [[t.detach().clone() for t in step(a, dy, t)] for a, t in ((first, t1), (second, t2))]
+    graphs, held = [], []
+    for a, t in ((first, t1), (second, t2)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(step(a, dy, t))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for k in order:
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in set(order):
+            for got, w in zip(held[k], want[k]):
+                assert torch.equal(got, w)
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """A leaf's node of an eager graph belongs to the stream of that graph: a captured backward pass would draw it into the capture, which
+    ends the process."""
+    args, dy = make_gated(20, 32, 40, 32, torch.float32)
+    target = torch.randint(0, 80, (20,), device="cuda")
+    for call in (lambda: feedforward.gated_mlp(*args), lambda: checkpoint8.linear8(args[0], args[1], args[2]),
+                 lambda: checkpoint8.act8(args[0]), lambda: losses.linear_cross_entropy(args[0], args[1], args[2], target)):
+        eager = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(graph):
+                y = call()
+                torch.autograd.grad(y, args[0], torch.ones_like(y))
+        del eager, y
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+            dx, = torch.autograd.grad(y, args[0], torch.ones_like(y))
+        graph.replay()
+        got = dx.clone()
+        del y, graph
+        y = call()
+        assert torch.equal(torch.autograd.grad(y, args[0], torch.ones_like(y))[0], got)
+        del y
+
+
+def test_gradients_accumulate_and_retain():
+    args, dy = make_gated(50, 32, 40, 32, torch.float32)
+    y = feedforward.gated_mlp(*args)
+    y.backward(dy, retain_graph=True)
+    once = [t.grad.clone() for t in args]
+    y.backward(dy)
+    for t, g in zip(args, once):
+        assert torch.equal(t.grad, 2 * g)
+
+
+def test_second_order_is_refused():
+    args, dy = make_gated(6, 16, 24, 16, torch.float32)
+    target = torch.randint(0, 48, (6,), device="cuda")
+    for y in (feedforward.gated_mlp(*args), checkpoint8.linear8(args[0], args[1], args[2]), checkpoint8.act8(args[0]),
+              losses.linear_cross_entropy(args[0], args[1], args[2], target)):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(y.sum(), args[0], create_graph=True)
+
+
+# ---------------------------------------------------------------------------------------------------- in the networks
+def test_gated_block():
+    torch.manual_seed(0)
+    block = Block(64, (7,), False, layer_scale_init_value=0.1, mlp="gated", checkpoint8=True).cuda()
+    assert not hasattr(block, "pwconv1")
+    x = torch.randn(2, 64, 14, 14, device="cuda", requires_grad=True)
+    out = block(x)
+    g = torch.autograd.grad(out.square().sum(), [x, *block.parameters()], allow_unused=True)
+    named = dict(zip(["x", *[n for n, _ in block.named_parameters()]], g))
+    y = block.norm(block.dwconv(x).permute(0, 2, 3, 1))
+    m = block.mlp
+    plain = x + (block.gamma * gated64(y, m.w_in, m.b_in, m.w_out, m.b_out, "gelu")).permute(0, 3, 1, 2)
+    assert float((out - plain).norm()) <= 1e-5 * float(plain.norm())
+    want = torch.autograd.grad(plain.square().sum(), [x, *block.parameters()], allow_unused=True)
+    for (name, got), w in zip(named.items(), want):
+        if w is not None:  # (8 bits of the block's input: a step is under 2^-6 of a group's largest value)
+            assert float((got - w).norm()) <= 0.05 * float(w.norm()), name
+    block.eval()
+    with torch.no_grad():
+        assert float((block(x) - plain).norm()) <= 1e-5 * float(plain.norm())
+
+
+@pytest.mark.parametrize("variant", ["1d", "1dpp"])
+def test_network_with_checkpoints_and_loss(variant):
+    torch.manual_seed(1)
+    net = ConvNeXt1D(num_classes=37, depths=(1, 1, 1, 1), dims=(32, 64, 96, 128), variant=variant, layer_scale_init_value=0.3).cuda()
+    lean = ConvNeXt1D(num_classes=37, depths=(1, 1, 1, 1), dims=(32, 64, 96, 128), variant=variant, layer_scale_init_value=0.3,
+                      checkpoint8=True).cuda()
+    lean.load_state_dict(net.state_dict())
+    image, target = torch.randn(3, 3, 224, 224, device="cuda"), torch.tensor([5, 36, -100], device="cuda")
+    loss = lean.loss(image, target, label_smoothing=0.1)
+    want = F.cross_entropy(net(image), target, label_smoothing=0.1)
+    # (results are exact, gradients see the checkpoints)
+    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    assert abs(float(net.loss(image, target, label_smoothing=0.1)) - float(want)) <= 1e-5 * float(want)
+    got = torch.autograd.grad(loss, [p for p in lean.parameters() if p.requires_grad], allow_unused=True)
+    ref = torch.autograd.grad(want, [p for p in net.parameters() if p.requires_grad], allow_unused=True)
+    for a, b in zip(got, ref):
+        assert (a is None) == (b is None)
+        if a is not None:
+            assert float((a - b).norm()) <= 0.1 * float(b.norm()) + 1e-7
