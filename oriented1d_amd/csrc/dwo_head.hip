@@ -21,6 +21,18 @@ struct Targets {
     }
 };
 
+// bias of the eight classes that a lane has, -infinity where there is no class: its logit is then no largest one and its exponential zero
+// (products with columns that are not there are zeros)
+struct Classes {
+    float bias[8];
+    __device__ __forceinline__ void init(const Values &b, long n, long N) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) bias[e] = n + e >= N ? -INFINITY : b.p != nullptr ? b.at(n + e) : 0.f;
+    }
+};
+// place of class t among eight from n on, or one beyond them
+__device__ __forceinline__ int place_of(long t, long n) { return t >= n && t < n + 8 ? (int)(t - n) : 8; }
+
 struct StatsEpi {
     static constexpr bool kSums = false;
     Values bias;
@@ -29,39 +41,41 @@ struct StatsEpi {
     float *sum;    // the same of sums of logits, or null
     float *at;     // [M]: the target's logit
     int width;     // classes of a wave, eight to a lane
-    struct Lane {
-        float bias[8];
-    };
+    typedef Classes Lane;
     __device__ __forceinline__ Lane begin(const Product &p, long n) const {
         Lane l;
-#pragma unroll
-        for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
+        l.init(bias, n, p.N);
         return l;
     }
     __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
-        const long t = m < p.M ? targets.of(m) : -1;
-        float most = -INFINITY, s = 0.f, all = 0.f;
+        float most = -INFINITY, s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const bool real = n + e < p.N;
-            v[e] = real ? v[e] + l.bias[e] : -INFINITY;
-            most = fmaxf(most, v[e]);
-            if (real) all += v[e];
-            if (n + e == t) at[m] = v[e];
+        for (int e = 0; e < 8; e++) v[e] += l.bias[e], most = fmaxf(most, v[e]);
+        if (m < p.M) {
+            const int k = place_of(targets.of(m), n);
+            if (k < 8) {
+                float hit = v[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) hit = k == e ? v[e] : hit;
+                at[m] = hit;
+            }
         }
         for (int off = 1; off < width / 8; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
         // (all -infinity: no exponential; NaN is in no maximum and in the sum)
         const float base = most == -INFINITY ? 0.f : most;
+        // (exponents are differences here: what rounding their multiples leaves, 2^-24 of each, is small where the term is not)
 #pragma unroll
-        for (int e = 0; e < 8; e++) s += prod_exp(v[e] - base);
-        for (int off = 1; off < width / 8; off <<= 1) {
-            s += __shfl_xor(s, off, 64);
-            if (sum != nullptr) all += __shfl_xor(all, off, 64);
-        }
-        if (n % width == 0 && n < p.N && m < p.M) {
-            const size_t to = (size_t)(n / width) * p.M + m;
-            part[to] = make_float2(most, s);
-            if (sum != nullptr) sum[to] = all;
+        for (int e = 0; e < 8; e++) s += __builtin_amdgcn_exp2f((v[e] - base) * 1.44269504f);
+        for (int off = 1; off < width / 8; off <<= 1) s += __shfl_xor(s, off, 64);
+        const bool writes = n % width == 0 && n < p.N && m < p.M;
+        const size_t to = (size_t)(n / width) * p.M + m;
+        if (writes) part[to] = make_float2(most, s);
+        if (sum != nullptr) {
+            float all = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) all += n + e < p.N ? v[e] : 0.f;
+            for (int off = 1; off < width / 8; off <<= 1) all += __shfl_xor(all, off, 64);
+            if (writes) sum[to] = all;
         }
     }
 };
@@ -128,18 +142,28 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restric
     if (threadIdx.x == 0) loss[0] = (float)(value[0] / number[0]), count[0] = (float)number[0];
 }
 
-// What G is multiplied with so that fp16 holds it, a power of two that brings the largest |up| to 2^13 .. 2^14 (G is at most |up|), and
-// its inverse: probabilities below 6e-8 would be lost otherwise.
+// What the products that read G give it back: G is held without what all its rows share.
+//   a mean: up / count (1 - eps), so that a row's largest value, about -1 at its target, is next to a number that 16 bits hold; rounded
+//   where it is, the same rounding in all rows would go into the gradients (twice their own rounding with labels smoothed)
+//   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's rows are at most 2, times 2^13, others are brought to
+//   2^13 .. 2^14 by the largest |up|
+// scale[0]: what G is multiplied with, scale[1]: what its products are.
 __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, const float *__restrict__ count, long M,
-                                                          float *__restrict__ scale) {
+                                                          float eps, int half, float *__restrict__ scale) {
+    if (count != nullptr) {
+        if (threadIdx.x == 0)
+            scale[0] = half ? 8192.f : 1.f,
+            scale[1] = count[0] > 0.f ? up[0] / count[0] * (eps < 1.f ? 1.f - eps : 1.f) * (half ? 1.f / 8192.f : 1.f) : 0.f;
+        return;
+    }
     __shared__ unsigned most[1024];
     unsigned v = 0;
-    const long n = count != nullptr ? 1 : M;
-    for (long i = threadIdx.x; i < n; i += 1024) v = max(v, __float_as_uint(count != nullptr ? up[i] / count[0] : up[i]) & 0x7fffffffu);
+    if (half)
+        for (long i = threadIdx.x; i < M; i += 1024) v = max(v, __float_as_uint(up[i]) & 0x7fffffffu);
     most[threadIdx.x] = v;
     __syncthreads();
-    for (int half = 512; half > 0; half >>= 1) {
-        if ((int)threadIdx.x < half) most[threadIdx.x] = max(most[threadIdx.x], most[threadIdx.x + half]);
+    for (int h = 512; h > 0; h >>= 1) {
+        if ((int)threadIdx.x < h) most[threadIdx.x] = max(most[threadIdx.x], most[threadIdx.x + h]);
         __syncthreads();
     }
     if (threadIdx.x == 0) {
@@ -154,27 +178,46 @@ struct GradEpi {
     Values bias;      // of the piece
     Targets targets;  // V: all classes
     long from;        // the piece's first class
-    const float *lse, *up, *count, *scale;  // count: a mean's (up has one value), or null; scale may be null
+    const float *lse, *up, *scale;  // up null: a mean
     float eps;
     Out g;            // [M][pitch]
-    struct Lane {
-        float bias[8], extra, flat;
+    struct Lane : Classes {
+        float scale, hit, flat;
     };
     __device__ __forceinline__ Lane begin(const Product &p, long n) const {
         Lane l;
-        l.extra = (scale != nullptr ? scale[0] : 1.f) * (count != nullptr ? up[0] / count[0] : 1.f), l.flat = eps / (float)targets.V;
-#pragma unroll
-        for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
+        l.init(bias, n, p.N);
+        // (a mean is held without 1 - eps)
+        const float s = scale[0], part = up == nullptr && eps < 1.f ? s / (1.f - eps) : s;
+        l.scale = part, l.hit = up == nullptr && eps < 1.f ? s : s * (1.f - eps), l.flat = part * (eps / (float)targets.V);
         return l;
     }
     __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
         if (m >= p.M || n >= g.pitch) return;
         const long t = targets.of(m);
-        const float total = lse[m], f = t == -2 ? NAN : count != nullptr ? l.extra : up[m] * l.extra;
+        const float total = lse[m], f = up != nullptr ? up[m] : 1.f;
+        if (g.type == OUT_PLANES) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float hit = from + n + e == t ? 1.f - eps : 0.f;
-            v[e] = t == -1 || n + e >= p.N ? 0.f : (prod_exp(v[e] + l.bias[e] - total) - hit - l.flat) * f;
+            for (int e = 0; e < 8; e++) v[e] = prod_exp(v[e] + l.bias[e] - total);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f((v[e] + l.bias[e] - total) * 1.44269504f);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e], l.scale, -l.flat);
+        const int k = place_of(t - from, n);
+        if (t >= from && k < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] -= k == e ? l.hit : 0.f;
+        }
+        if (up != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] *= f;
+        }
+        // rows that are ignored, or whose target is no class, and columns behind the last class
+        if (t < 0 || n + 8 > p.N) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = t == -1 || n + e >= p.N ? 0.f : t == -2 ? NAN : v[e];
         }
         out_octet(g, true, m, n, g.pitch, v);
     }
@@ -223,13 +266,13 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
     // dx is summed over the pieces in fp32
     const bool many = piece < s.V;
     float *sum = many && dx != nullptr && s.dtype != DWO_F32 ? (float *)ws.take((size_t)s.rows * s.C * sizeof(float)) : (float *)dx;
-    float *scale = s.dtype == DWO_F16 ? (float *)ws.take(2 * sizeof(float)) : nullptr;
-    if (scale != nullptr && !ws.dry()) {
-        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, count, s.rows, scale);
+    float *scale = (float *)ws.take(2 * sizeof(float));
+    if (!ws.dry()) {
+        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, count, s.rows, eps, s.dtype == DWO_F16, scale);
         if ((e = status())) return e;
     }
     const size_t size = size_of(s.dtype), grad_size = size_of(grad);
-    const float *alpha = scale != nullptr ? scale + 1 : nullptr;
+    const float *alpha = scale + 1;
     const size_t held = ws.used;
     size_t peak = held;
     for (long from = 0; from < s.V; from += piece) {
@@ -240,7 +283,7 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
         Operand gp = g;
         gp.pitch = up8(n), gp.plane = s.rows * gp.pitch;
         if (!ws.dry()) {
-            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, up, count, scale, eps,
+            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, count != nullptr ? nullptr : up, scale, eps,
                               out_of(gp, s.dtype)};
             if ((e = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st))) return e;
         }

@@ -50,74 +50,84 @@ template <int R, int THREADS, bool SLOW, int HALF>
 struct Stage {
     static constexpr int U = R * 8 / THREADS;
     static_assert(R * 8 % THREADS == 0 && THREADS % 64 == 0, "whole loads");
-    const char *base;
-    long left, pitch, plane, gap;  // bytes; left: rows (k fast) or bytes (k slow) from base to the operand's end
-    unsigned off[U];
-    __device__ __forceinline__ void init(const Operand &o, long rows, long r0, long K, long skip) {
-        pitch = o.pitch * 2, plane = o.plane * 2, gap = skip * 2;
+    const char *base, *at;  // of plane 0, and where the next stage comes from (k slow) or its plane (k fast)
+    long plane, gap, step;  // bytes
+    unsigned off[SLOW ? 1 : U], pitch;
+    // (a row or column that the operand has not is nowhere: every other access lies inside it)
+    __device__ __forceinline__ void init(const Operand &o, long rows, long r0, long skip) {
+        plane = o.plane * 2, gap = skip * 2, step = kProdK * o.pitch * 2, pitch = (unsigned)o.pitch * 2;
         if constexpr (SLOW) {
+            // (a lane's rows are a multiple of sixteen apart: their permutation is the same)
+            static_assert(THREADS / (R / 8) % 16 == 0, "one place in all rows");
             base = reinterpret_cast<const char *>(o.p) + r0 * 2;
-            left = K * pitch - r0 * 2;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int f = (int)threadIdx.x + u * THREADS, row = f / (R / 8), q = f % (R / 8);
-                const int c = ((q >> 1) ^ prod_key(row, R)) * 16 + (q & 1) * 8;
-                off[u] = r0 + c < o.pitch ? (unsigned)row * (unsigned)pitch + (unsigned)c * 2 : kLinNowhere;
-            }
+            const int q = threadIdx.x % (R / 8), c = ((q >> 1) ^ prod_key(row(0), R)) * 16 + (q & 1) * 8;
+            off[0] = r0 + c < o.pitch ? (unsigned)row(0) * pitch + (unsigned)c * 2 : kLinNowhere;
         } else {
-            base = reinterpret_cast<const char *>(o.p) + r0 * pitch;
-            left = rows - r0;
+            base = reinterpret_cast<const char *>(o.p) + r0 * o.pitch * 2;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = ((int)threadIdx.x + u * THREADS) / 8;
-                const int row = HALF > 0 ? s / (2 * HALF) * HALF + s % HALF : s;
-                off[u] = (unsigned)row * (unsigned)pitch + piece() * 16;
-            }
+            for (int u = 0; u < U; u++) off[u] = r0 + row(u) < rows ? (unsigned)row(u) * pitch + piece() * 16 : kLinNowhere;
         }
+        at = base;
+    }
+    static __device__ __forceinline__ int row(int u) {
+        const int f = (int)threadIdx.x + u * THREADS, s = SLOW ? f / (R / 8) : f / 8;
+        return HALF > 0 ? s / (2 * HALF) * HALF + s % HALF : s;
     }
     static __device__ __forceinline__ int piece() { return (threadIdx.x % 8) ^ (threadIdx.x / 8 % 8); }
-    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char *p, long bytes) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, (unsigned)max(0L, min(bytes, 0x7fffffffL)), 0x00020000);
-    }
-    // (not `live`: zeros)
-    __device__ __forceinline__ void load(uint16_t *lds, int which, long k0, long K, bool live) const {
+    __device__ __forceinline__ void seek(int which, long k0) { at = base + which * plane + (SLOW ? k0 / kProdK * step : 0); }
+    // left: summed indices from k0 to the operand's end; beyond it a lane reads nowhere, which writes zeros
+    __device__ __forceinline__ void load(uint16_t *lds, int k0, int left) const {
         typedef __attribute__((address_space(3))) void lds_void;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #ifdef __HIP_DEVICE_COMPILE__
-        if constexpr (SLOW) {
-            const __amdgpu_buffer_rsrc_t r = rsrc(base + which * plane + k0 * pitch, live ? left - k0 * pitch : 0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, 0x7fffffff, 0x00020000);
+        __amdgpu_buffer_rsrc_t r2 = r;
+        if constexpr (HALF > 0) r2 = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at + gap), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, off[u], 0, 0, 0);
-        } else {
-            // beyond the last summed index a lane reads nowhere, which writes zeros
-            const unsigned kill = piece() * 8 < K - k0 ? 0u : kLinNowhere;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const bool second = HALF > 0 && (wave * 8 + u * (THREADS / 8)) / (HALF > 0 ? HALF : 1) % 2 != 0;
-                const __amdgpu_buffer_rsrc_t r = rsrc(base + which * plane + (second ? gap : 0), live ? left * pitch : 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, off[u] | kill,
-                                                         (int)k0 * 2, 0, 0);
-            }
+        for (int u = 0; u < U; u++) {
+            const bool second = HALF > 0 && (wave * 8 + u * (THREADS / 8)) / (HALF > 0 ? HALF : 1) % 2 != 0;
+            constexpr int ROWS = THREADS / (R / 8);
+            const unsigned from = SLOW ? ((int)threadIdx.x / (R / 8) < left - u * ROWS ? off[0] : kLinNowhere)
+                                       : off[u] | (piece() * 8 < left ? 0u : kLinNowhere);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(second ? r2 : r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, from,
+                                                     SLOW ? (int)(u * ROWS * pitch) : k0 * 2, 0, 0);
         }
 #endif
     }
+    __device__ __forceinline__ void advance() {
+        if constexpr (SLOW) at += step;
+    }
 };
 
-// sixteen rows (columns) from slot0 on x 32 summed indices, 32 kk .. of the stage: a lane's eight values are 8 g .. of row c
+// A wave's fragments of a stage: sixteen rows (columns) each, from slot0 (a multiple of sixteen times their number, a power of two) on, x
+// 32 summed indices, 32 kk .. of the stage; a lane's eight values are 8 g .. of row c.
 template <int R, bool SLOW>
-__device__ __forceinline__ mma_s8 prod_fragment(const uint16_t *lds, int slot0, int kk) {
-    if constexpr (SLOW) {
-        typedef __attribute__((address_space(3))) mma_s4 lds_s4;
-        const int lane = threadIdx.x & 63, i = lane & 15, row = 8 * (lane >> 4) + (i >> 2);
-        const uint16_t *at = lds + (32 * kk + row) * R + ((slot0 / 16) ^ prod_key(row, R)) * 16 + (i & 3) * 4;
-        const mma_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at);
-        const mma_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * R));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    } else {
-        return lin_fragment<kProdK>(lds, slot0, kk);
+struct Fragments {
+    unsigned at;  // where the lane reads of fragment 0 (k slow), bytes; the others' places differ in single bits
+    int slot;
+    __device__ __forceinline__ void init(int slot0) {
+        slot = slot0;
+        if constexpr (SLOW) {
+            const int lane = threadIdx.x & 63, i = lane & 15, row = 8 * (lane >> 4) + (i >> 2);
+            at = 2 * ((unsigned)(row * R + prod_key(row, R) * 16 + (i & 3) * 4) ^ (unsigned)slot0);
+        }
     }
-}
+    // (the places are made anew each time, one instruction each: kept, they cost the registers that the fragments need)
+    __device__ __forceinline__ void start() {
+        if constexpr (SLOW) asm volatile("" : "+v"(at));
+    }
+    __device__ __forceinline__ mma_s8 read(const uint16_t *lds, int f, int kk) const {
+        if constexpr (SLOW) {
+            typedef __attribute__((address_space(3))) mma_s4 lds_s4;
+            const char *from = reinterpret_cast<const char *>(lds) + (at ^ (unsigned)(32 * f)) + 64 * kk * R;
+            const mma_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)from);
+            const mma_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(from + 8 * R));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return lin_fragment<kProdK>(lds, slot + 16 * f, kk);
+        }
+    }
+};
 
 // ------------------------------------------------------------------------------------------------- what goes out
 enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2, OUT_PLANES = 3 };  // (the first three are the DWO_ codes)
@@ -273,10 +283,10 @@ struct SumsEpi : PlainEpi {
 };
 
 // ------------------------------------------------------------------------------------------------- the product
-// Tiles of BM x BN, WM x WN waves.  A stage is 64 summed indices of both operands, two stages in LDS.  While a wave multiplies the
-// first half of a stage it reads the second half's fragments; the one barrier of a step comes between the halves, when every wave
-// has the rest of its stage in registers: the stage's LDS takes the stage after the next, and the products of the second half
-// cover the reads of the next stage's first.
+// Tiles of BM x BN, WM x WN waves.  A stage is 64 summed indices of both operands, two stages in LDS.  While a wave multiplies one
+// part of a stage it reads the fragments of the next: a stage is four parts (or eight), half of the wave's rows x half of the stage each.  The one
+// barrier of a step comes before the last part, when every wave has the rest of its stage in registers: the stage's LDS takes the
+// stage after the next, and the products of that part cover the reads of the next stage's first.
 template <int BM_, int BN_, int WM_, int WN_, int WAVES>
 struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM_ * WN_, PER_SIMD = WAVES;
@@ -307,8 +317,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
     Stage<BM, S::THREADS, AS, 0> sa;
     Stage<BN, S::THREADS, BS, GATED ? 8 * NF : 0> sb;
-    sa.init(p.a, p.M, m0, p.K, 0);
-    sb.init(p.b, GATED ? p.N / 2 : p.N, GATED ? n0 / 2 : n0, p.K, p.gap);
+    sa.init(p.a, p.M, m0, 0);
+    sb.init(p.b, GATED ? p.N / 2 : p.N, GATED ? n0 / 2 : n0, p.gap);
     mma_f4 acc[NF][MF], accs[SF > 0 ? SF : 1];
 #pragma unroll
     for (int i = 0; i < NF; i++)
@@ -319,33 +329,53 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
 
     const int ksteps = (int)((p.K + kProdK - 1) / kProdK);
     const int first = split * p.per, count = min(p.per, p.steps - first);
-    int pair = first / ksteps, left = count;
-    long k0 = (long)(first % ksteps) * kProdK;
+    int pair = first / ksteps, k0 = first % ksteps * kProdK, more = count;
+    sa.seek(p.codes_a >> (2 * pair) & 3, k0), sb.seek(p.codes_b >> (2 * pair) & 3, k0);
     // (a loop of one body: an odd last step is followed by one of zeros)
     auto fetch = [&](uint16_t *la, uint16_t *lb) {
-        const bool live = left-- > 0;
-        sa.load(la, p.codes_a >> (2 * pair) & 3, k0, p.K, live);
-        sb.load(lb, p.codes_b >> (2 * pair) & 3, k0, p.K, live);
-        k0 += kProdK;
-        const bool wrap = k0 >= p.K;
-        k0 = wrap ? 0 : k0, pair = wrap ? pair + 1 : pair;
+        const int left = more > 0 ? (int)p.K - k0 : 0;
+        sa.load(la, k0, left), sb.load(lb, k0, left);
+        sa.advance(), sb.advance();
+        k0 += kProdK, more--;
+        if (k0 >= p.K) {
+            k0 = 0, pair++;
+            sa.seek(p.codes_a >> (2 * pair) & 3, 0), sb.seek(p.codes_b >> (2 * pair) & 3, 0);
+        }
     };
-    mma_s8 fa0[MF], fb0[NF], fa1[MF], fb1[NF];
-    auto read = [&](const uint16_t *la, const uint16_t *lb, int kk, mma_s8 (&fa)[MF], mma_s8 (&fb)[NF]) {
+    // (quarters of eight fragments and not halves: sixteen registers less, which two transposing operands have not)
+    constexpr int Q = MF == 8 ? 4 : 2, MH = MF / Q;
+    mma_s8 fa[2][MH], fb[2][NF];
+    Fragments<BM, AS> part_a;
+    Fragments<BN, BS> part_b;
+    part_a.init(wm * MF * 16), part_b.init(wn * NF * 16);
+    // part t of a stage, q of Q of the rows and half kk: its A goes to fa[t % 2], its B to fb[kk] (with the first rows)
+    auto read = [&](const uint16_t *la, const uint16_t *lb, int t) {
+        const int kk = t / Q, q = t % Q;
+        part_a.start();
 #pragma unroll
-        for (int i = 0; i < NF; i++) fb[i] = prod_fragment<BN, BS>(lb, (wn * NF + i) * 16, kk);
+        for (int j = 0; j < MH; j++) fa[t % 2][j] = part_a.read(la, q * MH + j, kk);
+        if (q != 0) return;
+        part_b.start();
 #pragma unroll
-        for (int j = 0; j < MF; j++) fa[j] = prod_fragment<BM, AS>(la, (wm * MF + j) * 16, kk);
+        for (int i = 0; i < NF; i++) fb[kk][i] = part_b.read(lb, i, kk);
     };
-    auto multiply = [&](const mma_s8 (&fa)[MF], const mma_s8 (&fb)[NF]) {
+    // (what was asked for above goes out before the products, and the products before what is asked for below)
+    auto multiply = [&](int t) {
+        const int kk = t / Q, q = t % Q;
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int j = 0; j < MF; j++)
+        for (int j = 0; j < MH; j++)
 #pragma unroll
-            for (int i = 0; i < NF; i++) acc[i][j] = Mma<T>::run(fb[i], fa[j], acc[i][j]);
+            for (int i = 0; i < NF; i++) acc[i][q * MH + j] = Mma<T>::run(fb[kk][i], fa[t % 2][j], acc[i][q * MH + j]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
     };
     // sums over A alone, in the workgroups of the first column of tiles: products with ones, with zeros elsewhere and where a plane of A
     // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all)
     int at_pair = first / ksteps, at_step = first % ksteps;
+    Fragments<BM, AS> sums_of;
+    sums_of.init((wm * MF + wn * SF) * 16);
     auto add_sums = [&](const uint16_t *la) {
         if constexpr (SUMS) {
             const short one = nt == 0 && (p.codes_b >> (2 * at_pair) & 3) == 0 ? Mma<T>::kOne : 0;
@@ -353,28 +383,29 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
             const bool wrap = at_step == ksteps;
             at_step = wrap ? 0 : at_step, at_pair = wrap ? at_pair + 1 : at_pair;
             const mma_s8 ones = {one, one, one, one, one, one, one, one};
+            sums_of.start();
 #pragma unroll
             for (int kk = 0; kk < 2; kk++)
 #pragma unroll
                 for (int j = 0; j < SF; j++)
-                    accs[j] = Mma<T>::run(ones, prod_fragment<BM, AS>(la, (wm * MF + wn * SF + j) * 16, kk), accs[j]);
+                    accs[j] = Mma<T>::run(ones, sums_of.read(la, j, kk), accs[j]);
         }
     };
     auto step = [&](uint16_t *ca, uint16_t *cb, const uint16_t *na, const uint16_t *nb) {
         add_sums(ca);
-        read(ca, cb, 1, fa1, fb1);
-        multiply(fa0, fb0);
+#pragma unroll
+        for (int t = 0; t + 1 < 2 * Q; t++) read(ca, cb, t + 1), multiply(t);
         __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's reads of the stage are done, and its part of the next one is there ..
         asm volatile("s_barrier" ::: "memory");  // .. and the other waves'
         fetch(ca, cb);
-        read(na, nb, 0, fa0, fb0);
-        multiply(fa1, fb1);
+        read(na, nb, 0);
+        multiply(2 * Q - 1);
     };
     fetch(la0, lb0);
     __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("s_barrier" ::: "memory");
     fetch(la1, lb1);
-    read(la0, lb0, 0, fa0, fb0);
+    read(la0, lb0, 0);
     for (int s = 0; s < count; s += 2) {
         step(la0, lb0, la1, lb1);
         step(la1, lb1, la0, lb0);
@@ -410,7 +441,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
             }
         };
         const long mp = m0 + wm * 16 * MF + pass * ROWS;
-#pragma unroll 1
+#pragma unroll 2
         for (int row = row0; row < ROWS; row += STEP) {
             float v[8];
             octet(row, o, v);
