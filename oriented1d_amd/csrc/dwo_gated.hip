@@ -31,6 +31,8 @@ struct GluEpi {
         }
         return l;
     }
+    static constexpr int kRow = 0;
+    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
     __device__ __forceinline__ void octet(const Product &p, const Lane &l, long m, long n, float (&g)[8], float (&u)[8]) const {
         if (m >= p.M || n >= Hp) return;
 #pragma unroll
@@ -55,14 +57,23 @@ struct DgluEpi {
     int act;
     const float *keep;
     Out dg, du, h;  // dg and du: two halves of one [M][2 Hp]
-    struct Lane {};
-    __device__ __forceinline__ Lane begin(const Product &, long) const { return {}; }
-    __device__ __forceinline__ void octet(const Product &p, const Lane &, int, long m, long n, float (&d)[8]) const {
-        if (m >= p.M || n >= Hp) return;
-        float a[8], b[8], o[8];
+    static constexpr int kRow = 0;
+    __device__ __forceinline__ Nothing begin(const Product &, long) const { return {}; }
+    struct Data {
+        mma_f4 gate[2], up[2];
+    };
+    __device__ __forceinline__ Data load(const Product &p, long m, long n) const {
+        Data d;
         const mma_f4 *g = reinterpret_cast<const mma_f4 *>(keep + m * Hp + n);
         const mma_f4 *u = reinterpret_cast<const mma_f4 *>(keep + (p.M + m) * Hp + n);
-        const mma_f4 gate[2] = {g[0], g[1]}, up[2] = {u[0], u[1]};
+        if (m < p.M && n < Hp) d = {{g[0], g[1]}, {u[0], u[1]}};
+        return d;
+    }
+    __device__ __forceinline__ void octet(const Product &p, const Nothing &, const unsigned *, const Data &kept, int, long m, long n,
+                                          float (&d)[8]) const {
+        if (m >= p.M || n >= Hp) return;
+        float a[8], b[8], o[8];
+        const auto &[gate, up] = kept;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             float value, slope;

@@ -14,10 +14,10 @@ struct Targets {
     const long long *t;
     long long ignore;
     long V;
-    // the class of row m, -1 where the row is ignored, -2 where it has no class there is
-    __device__ __forceinline__ long of(long m) const {
+    // the class of row m, -1 where the row is ignored, -2 where its target is no class
+    __device__ __forceinline__ int of(long m) const {
         const long long v = t[m];
-        return v == ignore ? -1L : v >= 0 && v < V ? (long)v : -2L;
+        return v == ignore ? -1 : v >= 0 && v < V ? (int)v : -2;
     }
 };
 
@@ -30,8 +30,20 @@ struct Classes {
         for (int e = 0; e < 8; e++) bias[e] = n + e >= N ? -INFINITY : b.p != nullptr ? b.at(n + e) : 0.f;
     }
 };
+// joined over groups of four or eight lanes
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <class F>
+__device__ __forceinline__ float over_lanes(float v, bool eight, F &&join) {
+    v = join(v, from_lane<0xB1>(v));            // quad_perm [1,0,3,2]
+    v = join(v, from_lane<0x4E>(v));            // quad_perm [2,3,0,1]
+    const float w = join(v, from_lane<0x141>(v));  // row_half_mirror
+    return eight ? w : v;
+}
 // place of class t among eight from n on, or one beyond them
-__device__ __forceinline__ int place_of(long t, long n) { return t >= n && t < n + 8 ? (int)(t - n) : 8; }
+__device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
 
 struct StatsEpi {
     static constexpr bool kSums = false;
@@ -47,12 +59,17 @@ struct StatsEpi {
         l.init(bias, n, p.N);
         return l;
     }
-    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
+    static constexpr int kRow = 1;  // the target
+    __device__ __forceinline__ unsigned row(const Product &, long m, int) const { return (unsigned)targets.of(m); }
+    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
+                                          float (&v)[8]) const {
         float most = -INFINITY, s = 0.f;
+        const bool eight = width == 64;
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += l.bias[e], most = fmaxf(most, v[e]);
         if (m < p.M) {
-            const int k = place_of(targets.of(m), n);
+            const int k = place_of((int)rows[0], n);
             if (k < 8) {
                 float hit = v[0];
 #pragma unroll
@@ -60,13 +77,13 @@ struct StatsEpi {
                 at[m] = hit;
             }
         }
-        for (int off = 1; off < width / 8; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        most = over_lanes(most, eight, [](float a, float b) { return fmaxf(a, b); });
         // (all -infinity: no exponential; NaN is in no maximum and in the sum)
         const float base = most == -INFINITY ? 0.f : most;
         // (exponents are differences here: what rounding their multiples leaves, 2^-24 of each, is small where the term is not)
 #pragma unroll
         for (int e = 0; e < 8; e++) s += __builtin_amdgcn_exp2f((v[e] - base) * 1.44269504f);
-        for (int off = 1; off < width / 8; off <<= 1) s += __shfl_xor(s, off, 64);
+        s = over_lanes(s, eight, [](float a, float b) { return a + b; });
         const bool writes = n % width == 0 && n < p.N && m < p.M;
         const size_t to = (size_t)(n / width) * p.M + m;
         if (writes) part[to] = make_float2(most, s);
@@ -74,7 +91,7 @@ struct StatsEpi {
             float all = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) all += n + e < p.N ? v[e] : 0.f;
-            for (int off = 1; off < width / 8; off <<= 1) all += __shfl_xor(all, off, 64);
+            all = over_lanes(all, eight, [](float a, float b) { return a + b; });
             if (writes) sum[to] = all;
         }
     }
@@ -109,7 +126,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict
         if (m < M) {
             const float l = base + logf(s);
             lse[m] = l;
-            const long t = targets.of(m);
+            const int t = targets.of(m);
             if (t == -2) value = NAN;
             else if (t >= 0) value = (l - at[m]) * (1.f - eps);
             if (t >= 0 && sum != nullptr) value += eps * (l - all / (float)targets.V);
@@ -192,10 +209,16 @@ struct GradEpi {
         l.scale = part, l.hit = up == nullptr && eps < 1.f ? s : s * (1.f - eps), l.flat = part * (eps / (float)targets.V);
         return l;
     }
-    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int, long m, long n, float (&v)[8]) const {
+    static constexpr int kRow = 3;  // the target, the log of the sum, what arrives at the loss
+    __device__ __forceinline__ unsigned row(const Product &, long m, int k) const {
+        return k == 0 ? (unsigned)targets.of(m) : k == 1 ? __float_as_uint(lse[m]) : up != nullptr ? __float_as_uint(up[m]) : 0u;
+    }
+    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
+                                          float (&v)[8]) const {
         if (m >= p.M || n >= g.pitch) return;
-        const long t = targets.of(m);
-        const float total = lse[m], f = up != nullptr ? up[m] : 1.f;
+        const int t = (int)rows[0];
+        const float total = __uint_as_float(rows[1]), f = __uint_as_float(rows[2]);
         if (g.type == OUT_PLANES) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = prod_exp(v[e] + l.bias[e] - total);
@@ -205,8 +228,8 @@ struct GradEpi {
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e], l.scale, -l.flat);
-        const int k = place_of(t - from, n);
-        if (t >= from && k < 8) {
+        const int k = place_of(t, from + n);
+        if (k < 8) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] -= k == e ? l.hit : 0.f;
         }

@@ -199,6 +199,14 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
         mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])};
 }
 
+// An epilogue E has
+//   begin(p, n): what a lane keeps for its eight columns (n: the first) while it goes down the rows
+//   kRow, row(p, m, k): numbers of a row that wait in LDS from the start of the kernel
+//   load(p, m, n): what the epilogue reads for an octet, asked for one octet ahead
+//   octet(p, lane, rows, data, split, m, n, v): eight neighbours of a row; all lanes call it for some row, beyond the ends as well
+//   kSums, emit_sum: see SumsEpi
+struct Nothing {};
+
 struct Values {  // a vector of fp32 or 16-bit values, or none
     const void *p;
     int type;
@@ -251,7 +259,10 @@ struct PlainEpi {
         for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && part == nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
         return l;
     }
-    __device__ __forceinline__ void octet(const Product &p, const Lane &l, int split, long m, long n, float (&v)[8]) const {
+    static constexpr int kRow = 0;
+    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *, const Nothing &, int split, long m, long n,
+                                          float (&v)[8]) const {
         if (m >= p.M || n >= p.N) return;
         if (part != nullptr) {
             out_octet({part + (size_t)split * p.M * p.N, p.N, 0, OUT_F32}, l.wide, m, n, p.N, v);
@@ -304,6 +315,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     __shared__ __attribute__((aligned(16))) uint16_t lb0[BN * kProdK];
     __shared__ __attribute__((aligned(16))) uint16_t la1[BM * kProdK];
     __shared__ __attribute__((aligned(16))) uint16_t lb1[BN * kProdK];
+    __shared__ unsigned lrow[Epi::kRow > 0 ? BM * Epi::kRow : 1];
     // an XCD (workgroup ids modulo eight) takes a run of tiles; runs go down groups of rows of tiles, so that the tiles of an XCD
     // at one time share both operands' lines
     const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
@@ -327,6 +339,10 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
 #pragma unroll
     for (int j = 0; j < SF; j++) accs[j] = mma_f4{0.f, 0.f, 0.f, 0.f};
 
+    if constexpr (Epi::kRow > 0)
+        if ((int)threadIdx.x < BM && m0 + (int)threadIdx.x < p.M)
+#pragma unroll
+            for (int k = 0; k < Epi::kRow; k++) lrow[threadIdx.x * Epi::kRow + k] = epi.row(p, m0 + (int)threadIdx.x, k);
     const int ksteps = (int)((p.K + kProdK - 1) / kProdK);
     const int first = split * p.per, count = min(p.per, p.steps - first);
     int pair = first / ksteps, k0 = first % ksteps * kProdK, more = count;
@@ -441,8 +457,12 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
             }
         };
         const long mp = m0 + wm * 16 * MF + pass * ROWS;
+        auto data = epi.load(p, mp + row0, nl);
 #pragma unroll 2
         for (int row = row0; row < ROWS; row += STEP) {
+            const auto now = data;
+            data = epi.load(p, mp + row + STEP, nl);
+            const unsigned *rows = lrow + (wm * 16 * MF + pass * ROWS + row) * Epi::kRow;
             float v[8];
             octet(row, o, v);
             if constexpr (GATED) {
@@ -450,7 +470,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
                 octet(row, NF + o, u);
                 epi.octet(p, local, mp + row, nl, v, u);
             } else {
-                epi.octet(p, local, split, mp + row, nl, v);
+                epi.octet(p, local, rows, now, split, mp + row, nl, v);
             }
         }
     }
