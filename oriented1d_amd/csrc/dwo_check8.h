@@ -25,7 +25,4 @@ __device__ __forceinline__ int quantum(float v, float inverse) {
 // (a maximum of magnitudes as integers orders NaN above everything)
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// a checkpoint's values as an operand, [rows][up8(C)] with zeros behind C: one plane whatever the type, they are exact in 16 bits
-int unpack8_operand(Operand &o, const int8_t *codes, const uint8_t *exps, long rows, long C, int dtype, Arena &ws, hipStream_t st);
-
 }  // namespace dwo

@@ -92,13 +92,13 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, T *
     }
 }
 
-// The values held, or where dy is not null dx = dy act'(value); `out` has rows of `pitch` (with zeros from C on where it is wider).
+// The values held, or where dy is not null dx = dy act'(value).
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
-                                                      const T *__restrict__ dy, T *__restrict__ out, long rows, int C, int pitch,
+                                                      const T *__restrict__ dy, T *__restrict__ out, long rows, int C,
                                                       int act) {
     const int groups = (C + kGroup8 - 1) / kGroup8;
-    const long total = WIDE ? rows * C / 8 : rows * pitch;
+    const long total = WIDE ? rows * C / 8 : rows * C;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         if constexpr (WIDE) {
             float v[8];
@@ -118,16 +118,13 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__
             }
             store8(out + i * 8, v);
         } else {
-            const long row = i / pitch;
-            const int c = (int)(i % pitch);
-            float v = 0.f;
-            if (c < C) {
-                v = (float)codes[row * C + c] * group_scale(exps[row * groups + c / kGroup8]);
-                if (dy != nullptr) {
-                    float value, slope;
-                    act_wide<T>(act, v, value, slope);
-                    v = to_float(dy[row * C + c]) * slope;
-                }
+            const long row = i / C;
+            const int c = (int)(i % C);
+            float v = (float)codes[i] * group_scale(exps[row * groups + c / kGroup8]);
+            if (dy != nullptr) {
+                float value, slope;
+                act_wide<T>(act, v, value, slope);
+                v = to_float(dy[i]) * slope;
             }
             out[i] = from_float<T>(v);
         }
@@ -144,25 +141,16 @@ int launch_pack8(const void *x, void *y, void *codes, void *exps, long rows, int
     return status();
 }
 template <typename T>
-int launch_unpack8(const void *codes, const void *exps, const void *dy, void *out, long rows, int C, long pitch, int act,
-                   hipStream_t st) {
-    const bool wide = C % kGroup8 == 0 && pitch == C;
-    const dim3 grid(blocks_for(wide ? rows * C / 8 : rows * pitch, 1 << 20)), block(256);
+int launch_unpack8(const void *codes, const void *exps, const void *dy, void *out, long rows, int C, int act, hipStream_t st) {
+    const bool wide = C % kGroup8 == 0;
+    const dim3 grid(blocks_for(wide ? rows * C / 8 : rows * C, 1 << 20)), block(256);
     if (wide)
         unpack8_kernel<T, true><<<grid, block, 0, st>>>((const int8_t *)codes, (const uint8_t *)exps, (const T *)dy, (T *)out, rows, C,
-                                                        (int)pitch, act);
+                                                        act);
     else
         unpack8_kernel<T, false><<<grid, block, 0, st>>>((const int8_t *)codes, (const uint8_t *)exps, (const T *)dy, (T *)out, rows,
-                                                         C, (int)pitch, act);
+                                                         C, act);
     return status();
-}
-
-int unpack8_operand(Operand &o, const int8_t *codes, const uint8_t *exps, long rows, long C, int dtype, Arena &ws, hipStream_t st) {
-    o = take_operand(ws, rows, up8(C), DWO_BF16);
-    if (ws.dry()) return 0;
-    void *to = const_cast<void *>(o.p);
-    if (dtype == DWO_F16) return launch_unpack8<f16_t>(codes, exps, nullptr, to, rows, (int)C, o.pitch, 0, st);
-    return launch_unpack8<bf16_t>(codes, exps, nullptr, to, rows, (int)C, o.pitch, 0, st);
 }
 
 static bool sizes_ok(long rows, int C, const void *a, const void *b, const void *c, const void *d) {
@@ -171,25 +159,24 @@ static bool sizes_ok(long rows, int C, const void *a, const void *b, const void 
 
 static int layer_forward(const void *x, const void *w, const void *b, void *y, long rows, int C, int D, int dtype, Arena &ws,
                          hipStream_t st) {
-    Operand ox, ow;
-    int e;
-    if ((e = stage_operand(ox, x, rows, C, dtype, ws, st)) || (e = stage_operand(ow, w, D, C, dtype, ws, st))) return e;
+    Staging stage;
+    const Operand ox = stage.matrix(x, rows, C, dtype, ws), ow = stage.matrix(w, D, C, dtype, ws);
+    const int e = stage.launch(ws.dry(), st);
+    if (e) return e;
     PlainEpi epi = plain_epilogue({y, D, 0, dtype});
     epi.bias = {b, dtype};
     return plain_product(ox, false, ow, false, rows, D, C, dtype, epi, ws, st);
 }
 static int layer_backward(const void *dy, const int8_t *codes, const uint8_t *exps, const void *w, void *dx, void *dw, void *db,
                           long rows, int C, int D, int dtype, int grad, Arena &ws, hipStream_t st) {
-    Operand oy, ox, ow;
-    int e;
-    if ((e = stage_operand(oy, dy, rows, D, dtype, ws, st))) return e;
-    if (dx != nullptr) {
-        if ((e = stage_operand(ow, w, D, C, dtype, ws, st)) ||
-            (e = plain_product(oy, false, ow, true, rows, C, D, dtype, plain_epilogue({dx, C, 0, dtype}), ws, st)))
-            return e;
-    }
+    Staging stage;
+    const Operand oy = stage.matrix(dy, rows, D, dtype, ws);
+    const Operand ow = dx != nullptr ? stage.matrix(w, D, C, dtype, ws) : Operand{};
+    const Operand ox = dw != nullptr ? stage.held8(codes, exps, rows, C, dtype, ws) : Operand{};
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
+    if (dx != nullptr && (e = plain_product(oy, false, ow, true, rows, C, D, dtype, plain_epilogue({dx, C, 0, dtype}), ws, st))) return e;
     if (dw == nullptr) return 0;
-    if ((e = unpack8_operand(ox, codes, exps, rows, C, dtype, ws, st))) return e;
     PlainEpi epi = plain_epilogue({dw, C, 0, grad});
     epi.sums = {db, 0, 0, grad};
     return plain_product(oy, true, ox, true, D, C, rows, dtype, epi, ws, st);
@@ -220,9 +207,9 @@ int dwo_unpack8(const void *codes, const void *exps, const void *dy, void *out, 
     (void)hipGetLastError();
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-        case DWO_F32: return launch_unpack8<float>(codes, exps, dy, out, (long)rows, C, C, act, st);
-        case DWO_BF16: return launch_unpack8<bf16_t>(codes, exps, dy, out, (long)rows, C, C, act, st);
-        case DWO_F16: return launch_unpack8<f16_t>(codes, exps, dy, out, (long)rows, C, C, act, st);
+        case DWO_F32: return launch_unpack8<float>(codes, exps, dy, out, (long)rows, C, act, st);
+        case DWO_BF16: return launch_unpack8<bf16_t>(codes, exps, dy, out, (long)rows, C, act, st);
+        case DWO_F16: return launch_unpack8<f16_t>(codes, exps, dy, out, (long)rows, C, act, st);
         default: return DWO_ERR_BAD_DTYPE;
     }
 }

@@ -106,11 +106,11 @@ static int gated_hidden(const GatedSizes &s, const Operand &x, const Operand &w,
 
 static int gated_forward(const GatedSizes &s, const void *x, const void *w_in, const void *b_in, const void *w_out, const void *b_out,
                          void *y, float *keep, int act, Arena &ws, hipStream_t st) {
-    Operand ox, oi, oo;
-    int e;
-    if ((e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st)) || (e = stage_operand(oi, w_in, 2 * s.H, s.C, s.dtype, ws, st)) ||
-        (e = stage_operand(oo, w_out, s.D, s.H, s.dtype, ws, st)))
-        return e;
+    Staging stage;
+    const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), oi = stage.matrix(w_in, 2 * s.H, s.C, s.dtype, ws),
+                  oo = stage.matrix(w_out, s.D, s.H, s.dtype, ws);
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
     const Operand h = take_operand(ws, s.rows, s.Hp, s.dtype);
     if (!ws.dry() && (e = gated_hidden(s, ox, oi, b_in, act, keep, out_of(h, s.dtype), st))) return e;
     PlainEpi epi = plain_epilogue({y, s.D, 0, s.dtype});
@@ -126,21 +126,21 @@ struct GatedGrads {
 static int gated_backward(const GatedSizes &s, const void *dy, const void *x, const int8_t *codes, const uint8_t *exps, const float *keep,
                           const void *w_in, const void *b_in, const void *w_out, const GatedGrads &g, int act, Arena &ws,
                           hipStream_t st) {
-    Operand ody, ox{nullptr, 0, 0, 1}, oi, oo;
     const long move = s.Hp - s.H;
-    int e;
-    if ((e = stage_operand(ody, dy, s.rows, s.D, s.dtype, ws, st)) || (e = stage_operand(oo, w_out, s.D, s.H, s.dtype, ws, st)) ||
-        (e = stage_operand(oi, w_in, 2 * s.H, s.C, s.dtype, ws, st, s.H, move)))
-        return e;
-    if (codes != nullptr) e = unpack8_operand(ox, codes, exps, s.rows, s.C, s.dtype, ws, st);
-    else if (g.dw_in != nullptr) e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st);
+    Staging stage;
+    const Operand ody = stage.matrix(dy, s.rows, s.D, s.dtype, ws), oo = stage.matrix(w_out, s.D, s.H, s.dtype, ws),
+                  oi = stage.matrix(w_in, 2 * s.H, s.C, s.dtype, ws, s.H, move);
+    const Operand ox = codes != nullptr     ? stage.held8(codes, exps, s.rows, s.C, s.dtype, ws)
+                       : g.dw_in != nullptr ? stage.matrix(x, s.rows, s.C, s.dtype, ws)
+                                            : Operand{nullptr, 0, 0, 1};
+    int e = stage.launch(ws.dry(), st);
     if (e) return e;
     if (keep == nullptr) {
         float *again = (float *)ws.take((size_t)2 * s.rows * s.Hp * sizeof(float));
-        Operand packed = oi;  // the rows of the second half lie Hp rows behind the first's
+        // (the rows of w_in's second half lie Hp rows behind the first's)
         const GluEpi epi{{b_in, s.dtype}, s.H, s.Hp, act, again, {nullptr, 0, 0, 0}};
-        if (!ws.dry() && (e = launch_product<false, false, true>(make_product(ox, packed, s.rows, 2 * s.H, s.C, s.Hp * oi.pitch), s.dtype,
-                                                                 epi, st)))
+        if (!ws.dry() &&
+            (e = launch_product<false, false, true>(make_product(ox, oi, s.rows, 2 * s.H, s.C, s.Hp * oi.pitch), s.dtype, epi, st)))
             return e;
         keep = again;
     }

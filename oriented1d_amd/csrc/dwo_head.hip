@@ -30,17 +30,17 @@ struct Classes {
         for (int e = 0; e < 8; e++) bias[e] = n + e >= N ? -INFINITY : b.p != nullptr ? b.at(n + e) : 0.f;
     }
 };
-// joined over groups of four or eight lanes
+// joined over groups of two, four or eight lanes
 template <int CTRL>
 __device__ __forceinline__ float from_lane(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 template <class F>
-__device__ __forceinline__ float over_lanes(float v, bool eight, F &&join) {
-    v = join(v, from_lane<0xB1>(v));            // quad_perm [1,0,3,2]
-    v = join(v, from_lane<0x4E>(v));            // quad_perm [2,3,0,1]
-    const float w = join(v, from_lane<0x141>(v));  // row_half_mirror
-    return eight ? w : v;
+__device__ __forceinline__ float over_lanes(float v, int lanes, F &&join) {
+    v = join(v, from_lane<0xB1>(v));                   // quad_perm [1,0,3,2]
+    if (lanes > 2) v = join(v, from_lane<0x4E>(v));    // quad_perm [2,3,0,1]
+    if (lanes > 4) v = join(v, from_lane<0x141>(v));   // row_half_mirror
+    return v;
 }
 // place of class t among eight from n on, or one beyond them
 __device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
@@ -65,7 +65,7 @@ struct StatsEpi {
     __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
                                           float (&v)[8]) const {
         float most = -INFINITY, s = 0.f;
-        const bool eight = width == 64;
+        const int lanes = width / 8;
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += l.bias[e], most = fmaxf(most, v[e]);
         if (m < p.M) {
@@ -77,13 +77,13 @@ struct StatsEpi {
                 at[m] = hit;
             }
         }
-        most = over_lanes(most, eight, [](float a, float b) { return fmaxf(a, b); });
+        most = over_lanes(most, lanes, [](float a, float b) { return fmaxf(a, b); });
         // (all -infinity: no exponential; NaN is in no maximum and in the sum)
         const float base = most == -INFINITY ? 0.f : most;
         // (exponents are differences here: what rounding their multiples leaves, 2^-24 of each, is small where the term is not)
 #pragma unroll
         for (int e = 0; e < 8; e++) s += __builtin_amdgcn_exp2f((v[e] - base) * 1.44269504f);
-        s = over_lanes(s, eight, [](float a, float b) { return a + b; });
+        s = over_lanes(s, lanes, [](float a, float b) { return a + b; });
         const bool writes = n % width == 0 && n < p.N && m < p.M;
         const size_t to = (size_t)(n / width) * p.M + m;
         if (writes) part[to] = make_float2(most, s);
@@ -91,7 +91,7 @@ struct StatsEpi {
             float all = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) all += n + e < p.N ? v[e] : 0.f;
-            all = over_lanes(all, eight, [](float a, float b) { return a + b; });
+            all = over_lanes(all, lanes, [](float a, float b) { return a + b; });
             if (writes) sum[to] = all;
         }
     }
@@ -260,11 +260,12 @@ struct HeadSizes {
 
 static int head_forward(const HeadSizes &s, const void *x, const void *w, const void *b, Targets targets, float eps, float *lse,
                         float *loss, float *count, bool mean, Arena &ws, hipStream_t st) {
-    Operand ox, ow;
-    int e;
-    if ((e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st)) || (e = stage_operand(ow, w, s.V, s.C, s.dtype, ws, st))) return e;
+    Staging stage;
+    const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), ow = stage.matrix(w, s.V, s.C, s.dtype, ws);
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
     const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
-    const int width = wave_columns(s.rows, s.V);
+    const int width = wave_columns(tile_for(p.M, p.N, p.steps));
     const int parts = (int)((s.V + width - 1) / width), blocks = (int)((s.rows + 15) / 16);
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
     float *sum = eps > 0.f ? (float *)ws.take((size_t)parts * s.rows * sizeof(float)) : nullptr;
@@ -281,9 +282,10 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
 
 static int head_backward(const HeadSizes &s, const float *up, const void *x, const void *w, const void *b, Targets targets, float eps,
                          const float *lse, const float *count, void *dx, void *dw, void *db, int grad, Arena &ws, hipStream_t st) {
-    Operand ox, ow;
-    int e;
-    if ((e = stage_operand(ox, x, s.rows, s.C, s.dtype, ws, st)) || (e = stage_operand(ow, w, s.V, s.C, s.dtype, ws, st))) return e;
+    Staging stage;
+    const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), ow = stage.matrix(w, s.V, s.C, s.dtype, ws);
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
     const long piece = s.piece();
     const Operand g = take_operand(ws, s.rows, up8(piece), s.dtype);
     // dx is summed over the pieces in fp32

@@ -9,6 +9,8 @@
 // 2^-24 of the whole.  417 TFLOP/s at best, where the fp32 matrix instructions give 157, at the accuracy of sums in fp32.
 #pragma once
 
+#include <utility>
+
 #include "dwo_linear.h"
 
 namespace dwo {
@@ -44,7 +46,7 @@ constexpr int kProdK = 64;  // summed indices of a stage
 // values whose 32-byte units are permuted by the row, so that the eight rows of a transposing read lie on different banks.
 // HALF > 0: rows come in runs of HALF gates and the HALF rows that these multiply.
 __device__ __forceinline__ int prod_key(int row, int R) {
-    return R >= 128 ? (row & 3) | (row >> 1 & 4) : (row >> 1 & 1) | (row >> 2 & 2);
+    return R >= 128 ? (row & 3) | (row >> 1 & 4) : R == 64 ? (row >> 1 & 1) | (row >> 2 & 2) : row >> 3 & 1;
 }
 template <int R, int THREADS, bool SLOW, int HALF>
 struct Stage {
@@ -298,23 +300,48 @@ struct SumsEpi : PlainEpi {
 // part of a stage it reads the fragments of the next: a stage is four parts (or eight), half of the wave's rows x half of the stage each.  The one
 // barrier of a step comes before the last part, when every wave has the rest of its stage in registers: the stage's LDS takes the
 // stage after the next, and the products of that part cover the reads of the next stage's first.
-template <int BM_, int BN_, int WM_, int WN_, int WAVES>
+template <int BM_, int BN_, int WM_, int WN_, int WAVES, int STAGES_>
 struct Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM_ * WN_, PER_SIMD = WAVES;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM_ * WN_, PER_SIMD = WAVES, STAGES = STAGES_;
     static constexpr int MF = BM_ / WM_ / 16, NF = BN_ / WN_ / 16;
 };
-typedef Shape<256, 256, 2, 4, 2> LargeTile;   // 128 KB of LDS, one workgroup per CU
-typedef Shape<128, 128, 2, 2, 2> MediumTile;  // 64 KB, two
-typedef Shape<64, 64, 2, 2, 4> SmallTile;     // 32 KB, four
+typedef Shape<256, 256, 2, 4, 2, 2> LargeTile;   // 128 KB of LDS, one workgroup per CU
+typedef Shape<128, 128, 2, 2, 2, 2> MediumTile;  // 64 KB, two
+// Few tiles leave most of a CU's LDS free and their waves waiting for memory: more stages on their way
+typedef Shape<64, 64, 2, 2, 2, 4> SmallTile;     // 64 KB
+typedef Shape<32, 32, 2, 2, 2, 8> ThinTile;      // 64 KB
+
+// f(0), f(1), .. until one is false
+template <class F, int... I>
+__device__ __forceinline__ bool stages_of(std::integer_sequence<int, I...>, F &&f) {
+    return (f(std::integral_constant<int, I>{}) && ...);
+}
 
 template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
 __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Product p, Epi epi) {
-    constexpr int BM = S::BM, BN = S::BN, MF = S::MF, NF = S::NF, SF = MF / S::WN;
+    constexpr int BM = S::BM, BN = S::BN, MF = S::MF, NF = S::NF, SF = MF / S::WN > 0 ? MF / S::WN : 1;
     constexpr bool SUMS = Epi::kSums;
-    __shared__ __attribute__((aligned(16))) uint16_t la0[BM * kProdK];
-    __shared__ __attribute__((aligned(16))) uint16_t lb0[BN * kProdK];
-    __shared__ __attribute__((aligned(16))) uint16_t la1[BM * kProdK];
-    __shared__ __attribute__((aligned(16))) uint16_t lb1[BN * kProdK];
+    constexpr int STAGES = S::STAGES, SIZE = (BM + BN) * kProdK;
+    // (arrays of their own: a read of one then waits for no load into another)
+    __shared__ __attribute__((aligned(16))) uint16_t s0[SIZE];
+    __shared__ __attribute__((aligned(16))) uint16_t s1[SIZE];
+    __shared__ __attribute__((aligned(16))) uint16_t s2[STAGES > 2 ? SIZE : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t s3[STAGES > 2 ? SIZE : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t s4[STAGES > 4 ? SIZE : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t s5[STAGES > 4 ? SIZE : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t s6[STAGES > 4 ? SIZE : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t s7[STAGES > 4 ? SIZE : 8];
+    auto stage = [&](auto i) -> uint16_t * {
+        constexpr int k = decltype(i)::value % STAGES;
+        if constexpr (k == 0) return s0;
+        else if constexpr (k == 1) return s1;
+        else if constexpr (k == 2) return s2;
+        else if constexpr (k == 3) return s3;
+        else if constexpr (k == 4) return s4;
+        else if constexpr (k == 5) return s5;
+        else if constexpr (k == 6) return s6;
+        else return s7;
+    };
     __shared__ unsigned lrow[Epi::kRow > 0 ? BM * Epi::kRow : 1];
     // an XCD (workgroup ids modulo eight) takes a run of tiles; runs go down groups of rows of tiles, so that the tiles of an XCD
     // at one time share both operands' lines
@@ -331,7 +358,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     Stage<BN, S::THREADS, BS, GATED ? 8 * NF : 0> sb;
     sa.init(p.a, p.M, m0, 0);
     sb.init(p.b, GATED ? p.N / 2 : p.N, GATED ? n0 / 2 : n0, p.gap);
-    mma_f4 acc[NF][MF], accs[SF > 0 ? SF : 1];
+    mma_f4 acc[NF][MF], accs[SF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
@@ -348,7 +375,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     int pair = first / ksteps, k0 = first % ksteps * kProdK, more = count;
     sa.seek(p.codes_a >> (2 * pair) & 3, k0), sb.seek(p.codes_b >> (2 * pair) & 3, k0);
     // (a loop of one body: an odd last step is followed by one of zeros)
-    auto fetch = [&](uint16_t *la, uint16_t *lb) {
+    auto fetch = [&](uint16_t *la) {
+        uint16_t *lb = la + BM * kProdK;
         const int left = more > 0 ? (int)p.K - k0 : 0;
         sa.load(la, k0, left), sb.load(lb, k0, left);
         sa.advance(), sb.advance();
@@ -359,13 +387,14 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
         }
     };
     // (quarters of eight fragments and not halves: sixteen registers less, which two transposing operands have not)
-    constexpr int Q = MF == 8 ? 4 : 2, MH = MF / Q;
+    constexpr int Q = MF == 8 ? 4 : MF > 1 ? 2 : 1, MH = MF / Q;
     mma_s8 fa[2][MH], fb[2][NF];
     Fragments<BM, AS> part_a;
     Fragments<BN, BS> part_b;
     part_a.init(wm * MF * 16), part_b.init(wn * NF * 16);
     // part t of a stage, q of Q of the rows and half kk: its A goes to fa[t % 2], its B to fb[kk] (with the first rows)
-    auto read = [&](const uint16_t *la, const uint16_t *lb, int t) {
+    auto read = [&](const uint16_t *la, int t) {
+        const uint16_t *lb = la + BM * kProdK;
         const int kk = t / Q, q = t % Q;
         part_a.start();
 #pragma unroll
@@ -391,7 +420,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all)
     int at_pair = first / ksteps, at_step = first % ksteps;
     Fragments<BM, AS> sums_of;
-    sums_of.init((wm * MF + wn * SF) * 16);
+    sums_of.init((wm * MF + wn * SF % MF) * 16);
     auto add_sums = [&](const uint16_t *la) {
         if constexpr (SUMS) {
             const short one = nt == 0 && (p.codes_b >> (2 * at_pair) & 3) == 0 ? Mma<T>::kOne : 0;
@@ -407,34 +436,45 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
                     accs[j] = Mma<T>::run(ones, sums_of.read(la, j, kk), accs[j]);
         }
     };
-    auto step = [&](uint16_t *ca, uint16_t *cb, const uint16_t *na, const uint16_t *nb) {
-        add_sums(ca);
+    // all but the last `stages` stages' loads of this wave have arrived, and what it read of LDS
+    auto wait = [](auto stages) {
+        constexpr int n = decltype(stages)::value * (decltype(sa)::U + decltype(sb)::U);
+        static_assert(n < 64, "what the counter holds");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | n >> 4 << 14);
+        asm volatile("s_barrier" ::: "memory");
+    };
+    auto step = [&](auto i) {
+        uint16_t *current = stage(i);
+        add_sums(current);
 #pragma unroll
-        for (int t = 0; t + 1 < 2 * Q; t++) read(ca, cb, t + 1), multiply(t);
-        __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's reads of the stage are done, and its part of the next one is there ..
-        asm volatile("s_barrier" ::: "memory");  // .. and the other waves'
-        fetch(ca, cb);
-        read(na, nb, 0);
+        for (int t = 0; t + 1 < 2 * Q; t++) read(current, t + 1), multiply(t);
+        // this wave's reads of the stage are done, and its part of the next one is there; so are the other waves' behind the barrier
+        wait(std::integral_constant<int, STAGES - 2>{});
+        fetch(current);
+        read(stage(std::integral_constant<int, decltype(i)::value + 1>{}), 0);
         multiply(2 * Q - 1);
     };
-    fetch(la0, lb0);
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    asm volatile("s_barrier" ::: "memory");
-    fetch(la1, lb1);
-    read(la0, lb0, 0);
-    for (int s = 0; s < count; s += 2) {
-        step(la0, lb0, la1, lb1);
-        step(la1, lb1, la0, lb0);
+    if constexpr (STAGES == 2) {
+        fetch(s0);
+        wait(std::integral_constant<int, 0>{});
+        fetch(s1);
+        read(s0, 0);
+        for (int s = 0; s < count; s += 2) step(std::integral_constant<int, 0>{}), step(std::integral_constant<int, 1>{});
+    } else {
+        stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return fetch(stage(i)), true; });
+        wait(std::integral_constant<int, STAGES - 1>{});
+        read(s0, 0);
+        int s = 0;
+        while (stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return step(i), ++s < count; })) {}
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (nothing may arrive behind the sums)
     // The sums go through LDS, each wave's through its own part, and come back as eight neighbours of a row per lane (gated: eight
     // gates and what they multiply): wide stores, row sums over few lanes, and a loop of one body.  Quads of a row are permuted by the row.
     __syncthreads();
     constexpr int QUADS = 4 * NF, PF = MF < 4 ? MF : 4, ROWS = 16 * PF, LANES = GATED ? NF : 2 * NF, STEP = 64 / LANES;
-    constexpr int WAVES = S::THREADS / 64, SHARE = WAVES / 4;  // (waves per array)
-    static_assert(BM == BN && SHARE >= 1 && ROWS * 16 * NF * 4 * SHARE <= BM * kProdK * 2, "the waves' parts fit the stages");
-    float *mine = reinterpret_cast<float *>(wave / SHARE == 0 ? la0 : wave / SHARE == 1 ? lb0 : wave / SHARE == 2 ? la1 : lb1) +
-                  wave % SHARE * ROWS * 16 * NF;
+    constexpr int WAVES = S::THREADS / 64, PART = ROWS * 16 * NF, FIT = SIZE / 2 / PART < WAVES ? SIZE / 2 / PART : WAVES;
+    static_assert(2 * FIT >= WAVES, "the waves' parts fit two stages");
+    float *mine = reinterpret_cast<float *>(wave < FIT ? s0 : s1) + wave % FIT * PART;
     const int lane = threadIdx.x & 63;
     const int o = lane % LANES, row0 = lane / LANES;
     const long nl = (GATED ? n0 / 2 + wn * 8 * NF : n0 + wn * 16 * NF) + o * 8;
@@ -475,7 +515,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
         }
     }
     if constexpr (SUMS)
-        if (nt == 0 && (threadIdx.x & 63) < 16) {
+        if (nt == 0 && wn * SF < MF && (threadIdx.x & 63) < 16) {
 #pragma unroll
             for (int j = 0; j < SF; j++) epi.emit_sum(p, split, m0 + (wm * MF + wn * SF + j) * 16 + (threadIdx.x & 15), accs[j][0]);
         }
@@ -516,9 +556,38 @@ inline Operand take_operand(Arena &ws, long rows, long pitch, int dtype) {
 inline Out out_of(const Operand &o, int dtype) {
     return {const_cast<void *>(o.p), o.pitch, o.plane, dtype == DWO_F32 ? OUT_PLANES : dtype};
 }
-// a dense [rows][cols] matrix as an operand: itself, or a copy that is one (dwo_product.hip).  move > 0: the rows from `gate` on go `move`
-// rows further down, with zeros between and behind.
-int stage_operand(Operand &o, const void *src, long rows, long cols, int dtype, Arena &ws, hipStream_t st, long gate = 0, long move = 0);
+// Operands that are made before the products of a call, by one launch (dwo_product.hip).
+struct StageJob {
+    const void *src;
+    const uint8_t *exps;  // of a checkpoint (dwo_check8.h), or null
+    uint16_t *dst;
+    long rows, gate, move, all, pitch, plane;
+    int cols, type;
+};
+struct Staging {
+    StageJob jobs[4];
+    int count = 0;
+    // a dense [rows][cols] matrix as an operand: itself, or a copy that is one.  move > 0: the rows from `gate` on go `move` rows further
+    // down (the second half of gated weights whose hidden size is no multiple of eight), with zeros between and behind.
+    Operand matrix(const void *src, long rows, long cols, int dtype, Arena &ws, long gate = 0, long move = 0) {
+        if (dtype != DWO_F32 && cols % 8 == 0 && move == 0) return {src, cols, 0, 1};
+        const Operand o = take_operand(ws, rows + 2 * move, up8(cols), dtype);
+        add(o, src, nullptr, rows, cols, move == 0 ? rows : gate, move, dtype);
+        return o;
+    }
+    // the values that a checkpoint holds: one plane whatever the type, they are exact in 16 bits
+    Operand held8(const int8_t *codes, const uint8_t *exps, long rows, long cols, int dtype, Arena &ws) {
+        const Operand o = take_operand(ws, rows, up8(cols), DWO_BF16);
+        add(o, codes, exps, rows, cols, rows, 0, dtype);
+        return o;
+    }
+    int launch(bool dry, hipStream_t st);
+
+private:
+    void add(const Operand &o, const void *src, const uint8_t *exps, long rows, long cols, long gate, long move, int type) {
+        jobs[count++] = {src, exps, (uint16_t *)const_cast<void *>(o.p), rows, gate, move, rows + 2 * move, o.pitch, o.plane, (int)cols, type};
+    }
+};
 
 // D = A B with the plain epilogue; a_slow, b_slow: the operand lies with the summed index as its slow one (dwo_product.hip).  epi.part
 // is filled in here.
@@ -543,15 +612,37 @@ inline Product make_product(const Operand &a, const Operand &b, long M, long N, 
     p.steps = p.per = (int)((K + kProdK - 1) / kProdK * p.pairs);
     return p;
 }
-inline int tile_for(long M, long N) { return tiles_of(M, N, 256, 256) >= 200 ? 256 : tiles_of(M, N, 128, 128) >= 160 ? 128 : 64; }
+// Time of a product with square tiles of this size, us: workgroups that have a CU to themselves wait for memory step by step, others
+// share its units.  The numbers are fits to products of 1 to 16384 rows x 96 to 21841 columns, steps of 64 summed indices 1 to 342,
+// of which they are 10 to 15 % off.  First round: a launch with its first loads and last stores, and a step; then each round.
+struct TileCost {
+    int size;
+    float first, first_step, more, more_step;
+};
+constexpr TileCost kTileCosts[4] = {
+    {256, 13.f, 1.7f, 9.5f, 1.6f}, {128, 7.f, 0.62f, 3.f, 0.45f}, {64, 4.2f, 0.25f, 1.2f, 0.22f}, {32, 4.f, 0.14f, 1.2f, 0.09f}};
+inline float tile_time(const TileCost &c, long workgroups, long steps) {
+    if (workgroups <= kLinCus) return c.first + (float)steps * c.first_step;
+    return 3.5f + (float)((workgroups + kLinCus - 1) / kLinCus) * (c.more + (float)steps * c.more_step);
+}
+// the tile of a product that is not split
+inline int tile_for(long M, long N, long steps) {
+    int best = 0;
+    for (int i = 1; i < 4; i++)
+        if (tile_time(kTileCosts[i], tiles_of(M, N, kTileCosts[i].size, kTileCosts[i].size), steps) <
+            tile_time(kTileCosts[best], tiles_of(M, N, kTileCosts[best].size, kTileCosts[best].size), steps))
+            best = i;
+    return kTileCosts[best].size;
+}
 // columns of a wave
-inline int wave_columns(long M, long N) { return tile_for(M, N) == 64 ? 16 * SmallTile::NF : 16 * LargeTile::NF; }
+inline int wave_columns(int tile) { return tile == 32 ? 16 * ThinTile::NF : tile == 64 ? 16 * SmallTile::NF : 16 * LargeTile::NF; }
 template <typename T, bool AS, bool BS, bool GATED, class Epi>
 int launch_tiles(const Product &p, const Epi &epi, hipStream_t st) {
-    switch (tile_for(p.M, p.N)) {
+    switch (tile_for(p.M, p.N, p.steps)) {
         case 256: return launch_shape<T, LargeTile, AS, BS, GATED>(p, epi, st);
         case 128: return launch_shape<T, MediumTile, AS, BS, GATED>(p, epi, st);
-        default: return launch_shape<T, SmallTile, AS, BS, GATED>(p, epi, st);
+        case 64: return launch_shape<T, SmallTile, AS, BS, GATED>(p, epi, st);
+        default: return launch_shape<T, ThinTile, AS, BS, GATED>(p, epi, st);
     }
 }
 template <bool AS, bool BS, bool GATED, class Epi>

@@ -1,60 +1,78 @@
 // Operands of the products around wide layers, and the products with the plain epilogue.
+#include "dwo_check8.h"
 #include "dwo_product.h"
 
 namespace dwo {
 
-// rows x cols of a dense matrix as an operand: columns padded with zeros to `pitch`, fp32 taken apart into three planes.  Rows from
-// `gate` on go `move` rows further down (the second half of gated weights whose hidden size is no multiple of eight), the rest is zeros.
+// Eight neighbours per thread: columns padded with zeros to `pitch`, fp32 taken apart into three planes, checkpoints taken out of theirs.
 template <typename S>
-__global__ __launch_bounds__(256) void stage_kernel(const S *__restrict__ src, uint16_t *__restrict__ dst, long rows, int cols,
-                                                    long gate, long move, long all_rows, long pitch, long plane) {
-    const long pieces = pitch / 8, total = all_rows * pieces;
-    const bool wide = cols % (16 / (int)sizeof(S)) == 0;
+__device__ __forceinline__ void read_octet(const S *at, int c, int cols, bool real, S (&v)[8]) {
+    if (real && cols % (16 / (int)sizeof(S)) == 0 && c + 8 <= cols && sizeof(S) > 1) {
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(S) / 2; e++) reinterpret_cast<mma_u4 *>(v)[e] = reinterpret_cast<const mma_u4 *>(at)[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = real && c + e < cols ? at[e] : S(0);
+    }
+}
+struct StageJobs {
+    StageJob job[4];
+};
+__global__ __launch_bounds__(256) void stage_kernel(StageJobs jobs) {
+    const StageJob &j = jobs.job[blockIdx.y];
+    const long pieces = j.pitch / 8, total = j.all * pieces;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = i / pieces;
         const int c = (int)(i % pieces) * 8;
-        const long from = row < gate ? row : row < gate + move ? rows : row - move;
-        const S *at = src + from * cols + c;
-        S v[8];
-        if (from < rows && wide && c + 8 <= cols) {
+        const long from = row < j.gate ? row : row < j.gate + j.move ? j.rows : row - j.move;
+        const bool real = from < j.rows;
+        uint16_t *to = j.dst + row * j.pitch + c;
+        if (j.exps != nullptr) {
+            const int8_t *at = reinterpret_cast<const int8_t *>(j.src) + from * j.cols + c;
+            int8_t q[8];
+            if (real && j.cols % 8 == 0) {
+                *reinterpret_cast<mma_u2 *>(q) = *reinterpret_cast<const mma_u2 *>(at);
+            } else {
 #pragma unroll
-            for (int e = 0; e < (int)sizeof(S) / 2; e++)
-                reinterpret_cast<mma_u4 *>(v)[e] = reinterpret_cast<const mma_u4 *>(at)[e];
-        } else {
+                for (int e = 0; e < 8; e++) q[e] = real && c + e < j.cols ? at[e] : (int8_t)0;
+            }
+            // (a group's eight values lie in it: groups are 32 wide)
+            const float s = real && c < j.cols ? group_scale(j.exps[from * ((j.cols + kGroup8 - 1) / kGroup8) + c / kGroup8]) : 0.f;
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = from < rows && c + e < cols ? at[e] : S(0);
-        }
-        uint16_t *to = dst + row * pitch + c;
-        if constexpr (sizeof(S) == 4) {
-            float q[8][3];
+            for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? (float)q[e] * s : 0.f;
+            mma_u4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = pack16(j.type, v[2 * e], v[2 * e + 1]);
+            *reinterpret_cast<mma_u4 *>(to) = w;
+        } else if (j.type == DWO_F32) {
+            float v[8], q[8][3];
+            read_octet(reinterpret_cast<const float *>(j.src) + from * j.cols + c, c, j.cols, real, v);
 #pragma unroll
             for (int e = 0; e < 8; e++) planes_of(v[e], q[e]);
 #pragma unroll
             for (int k = 0; k < 3; k++)
-                *reinterpret_cast<mma_u4 *>(to + k * plane) =
+                *reinterpret_cast<mma_u4 *>(to + k * j.plane) =
                     mma_u4{pack_bf16(q[0][k], q[1][k]), pack_bf16(q[2][k], q[3][k]), pack_bf16(q[4][k], q[5][k]),
                            pack_bf16(q[6][k], q[7][k])};
         } else {
+            uint16_t v[8];
+            read_octet(reinterpret_cast<const uint16_t *>(j.src) + from * j.cols + c, c, j.cols, real, v);
             *reinterpret_cast<mma_u4 *>(to) = *reinterpret_cast<const mma_u4 *>(v);
         }
     }
 }
 
-int stage_operand(Operand &o, const void *src, long rows, long cols, int dtype, Arena &ws, hipStream_t st, long gate, long move) {
-    if (dtype != DWO_F32 && cols % 8 == 0 && move == 0) {
-        o = {src, cols, 0, 1};
-        return 0;
+int Staging::launch(bool dry, hipStream_t st) {
+    if (dry || count == 0) return 0;
+    StageJobs all;
+    long most = 0;
+    for (int i = 0; i < count; i++) {
+        all.job[i] = jobs[i];
+        const long work = jobs[i].all * jobs[i].pitch / 8;
+        most = work > most ? work : most;
     }
-    const long all = rows + 2 * move;
-    if (move == 0) gate = rows;
-    o = take_operand(ws, all, up8(cols), dtype);
-    if (ws.dry()) return 0;
-    const dim3 grid(blocks_for(all * o.pitch / 8, 16384)), block(256);
-    uint16_t *to = (uint16_t *)const_cast<void *>(o.p);
-    if (dtype == DWO_F32)
-        stage_kernel<float><<<grid, block, 0, st>>>((const float *)src, to, rows, (int)cols, gate, move, all, o.pitch, o.plane);
-    else
-        stage_kernel<uint16_t><<<grid, block, 0, st>>>((const uint16_t *)src, to, rows, (int)cols, gate, move, all, o.pitch, o.plane);
+    stage_kernel<<<dim3(blocks_for(most, 8192), (unsigned)count), dim3(256), 0, st>>>(all);
     return status();
 }
 
@@ -104,27 +122,45 @@ template <typename T>
 int plain_typed(const Product &p, int tile, bool as, bool bs, const PlainEpi &epi, hipStream_t st) {
     if (tile == 256) return plain_shape<T, LargeTile>(p, as, bs, epi, st);
     if (tile == 128) return plain_shape<T, MediumTile>(p, as, bs, epi, st);
-    return plain_shape<T, SmallTile>(p, as, bs, epi, st);
+    if (tile == 64) return plain_shape<T, SmallTile>(p, as, bs, epi, st);
+    return plain_shape<T, ThinTile>(p, as, bs, epi, st);
 }
 
+// tile and splits of a plain product
+struct PlainChoice {
+    int tile;
+    long splits;
+};
+// The least of tile_time, with splits of the sums their writing and reading (4 TB/s behind each other) and the launch that joins them
+PlainChoice plain_choice(long M, long N, int steps) {
+    PlainChoice best{0, 0};
+    float least = 0.f;
+    for (const TileCost &c : kTileCosts) {
+        const long tiles = tiles_of(M, N, c.size, c.size);
+        for (const long splits : {1L, 2L, 3L, 4L, 6L, 8L, 12L, 16L, 24L, 32L}) {
+            if (splits > 1 && (tiles * splits > 4 * kLinCus || steps < 4 * splits)) break;
+            float t = tile_time(c, tiles * splits, (steps + splits - 1) / splits);
+            if (splits > 1) t += 4.f + (float)(splits * M) * (float)N * 8.f / 4e6f;
+            if (best.tile == 0 || t < least) best = {c.size, splits}, least = t;
+        }
+    }
+    return best;
+}
+
+int plain_product_as(Product p, const PlainChoice &choice, bool as, bool bs, int dtype, PlainEpi epi, Arena &ws, hipStream_t st) {
+    p.per = (int)((p.steps + choice.splits - 1) / choice.splits);
+    p.splits = (p.steps + p.per - 1) / p.per;
+    if (p.splits > 1) epi.part = (float *)ws.take((size_t)p.splits * ((size_t)p.M * p.N + p.M) * sizeof(float));
+    if (ws.dry()) return 0;
+    const int e = dtype == DWO_F16 ? plain_typed<f16_t>(p, choice.tile, as, bs, epi, st) : plain_typed<bf16_t>(p, choice.tile, as, bs, epi, st);
+    if (e != 0 || p.splits == 1) return e;
+    product_reduce_kernel<<<dim3(blocks_for(p.M * ((p.N + 3) / 4) + p.M, 8192)), dim3(256), 0, st>>>(p, epi);
+    return status();
+}
 int plain_product(const Operand &a, bool as, const Operand &b, bool bs, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws,
                   hipStream_t st) {
-    Product p = make_product(a, b, M, N, K, 0);
-    const long large = tiles_of(M, N, 256, 256), medium = tiles_of(M, N, 128, 128), small = tiles_of(M, N, 64, 64);
-    const int tile = large >= 200 ? 256 : medium >= 160 || (medium >= 8 && p.steps >= 64) ? 128 : 64;
-    const long tiles = tile == 256 ? large : tile == 128 ? medium : small;
-    // as many splits as the chip holds workgroups, of eight steps at least
-    const long room = tile == 256 ? 1 : (tile == 128 ? 512 : 1024) / tiles;
-    long splits = p.steps / 8 < room ? p.steps / 8 : room;
-    if (splits < 1) splits = 1;
-    p.per = (int)((p.steps + splits - 1) / splits);
-    p.splits = (p.steps + p.per - 1) / p.per;
-    if (p.splits > 1) epi.part = (float *)ws.take((size_t)p.splits * ((size_t)M * N + M) * sizeof(float));
-    if (ws.dry()) return 0;
-    const int e = dtype == DWO_F16 ? plain_typed<f16_t>(p, tile, as, bs, epi, st) : plain_typed<bf16_t>(p, tile, as, bs, epi, st);
-    if (e != 0 || p.splits == 1) return e;
-    product_reduce_kernel<<<dim3(blocks_for(M * ((N + 3) / 4) + M, 8192)), dim3(256), 0, st>>>(p, epi);
-    return status();
+    const Product p = make_product(a, b, M, N, K, 0);
+    return plain_product_as(p, plain_choice(M, N, p.steps), as, bs, dtype, epi, ws, st);
 }
 
 }  // namespace dwo
