@@ -165,7 +165,7 @@ static int layer_forward(const void *x, const void *w, const void *b, void *y, l
     if (e) return e;
     PlainEpi epi = plain_epilogue({y, D, 0, dtype});
     epi.bias = {b, dtype};
-    return plain_product(ox, false, ow, false, rows, D, C, dtype, epi, ws, st);
+    return plain_product(ox, ow, rows, D, C, dtype, epi, ws, st);
 }
 static int layer_backward(const void *dy, const int8_t *codes, const uint8_t *exps, const void *w, void *dx, void *dw, void *db,
                           long rows, int C, int D, int dtype, int grad, Arena &ws, hipStream_t st) {
@@ -173,13 +173,16 @@ static int layer_backward(const void *dy, const int8_t *codes, const uint8_t *ex
     const Operand oy = stage.matrix(dy, rows, D, dtype, ws);
     const Operand ow = dx != nullptr ? stage.matrix(w, D, C, dtype, ws) : Operand{};
     const Operand ox = dw != nullptr ? stage.held8(codes, exps, rows, C, dtype, ws) : Operand{};
-    int e = stage.launch(ws.dry(), st);
+    const int e = stage.launch(ws.dry(), st);
     if (e) return e;
-    if (dx != nullptr && (e = plain_product(oy, false, ow, true, rows, C, D, dtype, plain_epilogue({dx, C, 0, dtype}), ws, st))) return e;
-    if (dw == nullptr) return 0;
-    PlainEpi epi = plain_epilogue({dw, C, 0, grad});
-    epi.sums = {db, 0, 0, grad};
-    return plain_product(oy, true, ox, true, D, C, rows, dtype, epi, ws, st);
+    ProductGroup group;
+    if (dx != nullptr) group.add(false, oy, ow, rows, C, D, plain_epilogue({dx, C, 0, dtype}));
+    if (dw != nullptr) {
+        PlainEpi epi = plain_epilogue({dw, C, 0, grad});
+        epi.sums = {db, 0, 0, grad};
+        group.add(true, oy, ox, D, C, rows, epi);
+    }
+    return group.launch(dtype, ws, st);
 }
 
 }  // namespace dwo
@@ -216,7 +219,7 @@ int dwo_unpack8(const void *codes, const void *exps, const void *dy, void *out, 
 
 size_t dwo_layer8_workspace_bytes(size_t rows, int C, int D, int backward, int dtype) {
     if (!sizes_ok((long)rows, C, nullptr, nullptr, nullptr, nullptr) || D < 1 || D > 65536 || !known(dtype)) return 0;
-    Arena ws{nullptr, 0};
+    Arena ws = Arena::measure();
     void *const any = (void *)256;  // (nothing is launched)
     if (backward)
         layer_backward(any, (const int8_t *)any, (const uint8_t *)any, any, any, any, any, (long)rows, C, D, dtype, DWO_F32, ws, nullptr);
@@ -236,7 +239,7 @@ int dwo_layer8(const void *x, const void *w, const void *bias, void *y, void *co
         const int e = dwo_pack8(x, nullptr, codes, exps, rows, C, 0, dtype, stream);
         if (e != 0) return e;
     }
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return layer_forward(x, w, bias, y, (long)rows, C, D, dtype, a, (hipStream_t)stream);
 }
 
@@ -247,7 +250,7 @@ int dwo_layer8_backward(const void *dy, const void *codes, const void *exps, con
     if (!sizes_ok((long)rows, C, dy, w, ws, codes) || D < 1 || D > 65536 || (db && !dw)) return DWO_ERR_BAD_SHAPE;
     if (ws_bytes < dwo_layer8_workspace_bytes(rows, C, D, 1, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
     (void)hipGetLastError();
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return layer_backward(dy, (const int8_t *)codes, (const uint8_t *)exps, w, dx, dw, db, (long)rows, C, D, dtype, grad_dtype, a,
                           (hipStream_t)stream);
 }

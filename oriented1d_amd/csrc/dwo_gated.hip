@@ -115,7 +115,7 @@ static int gated_forward(const GatedSizes &s, const void *x, const void *w_in, c
     if (!ws.dry() && (e = gated_hidden(s, ox, oi, b_in, act, keep, out_of(h, s.dtype), st))) return e;
     PlainEpi epi = plain_epilogue({y, s.D, 0, s.dtype});
     epi.bias = {b_out, s.dtype};
-    return plain_product(h, false, oo, false, s.rows, s.D, s.H, s.dtype, epi, ws, st);
+    return plain_product(h, oo, s.rows, s.D, s.H, s.dtype, epi, ws, st);
 }
 
 struct GatedGrads {
@@ -152,21 +152,20 @@ static int gated_backward(const GatedSizes &s, const void *dy, const void *x, co
         const DgluEpi epi{s.H, s.Hp, act, keep, dg, du, out_of(h, s.dtype)};
         if ((e = launch_product<false, true, false>(make_product(ody, oo, s.rows, s.H, s.D, 0), s.dtype, epi, st))) return e;
     }
-    if (g.dx != nullptr &&
-        (e = plain_product(da, false, oi, true, s.rows, s.C, 2 * s.Hp, s.dtype, plain_epilogue({g.dx, s.C, 0, s.dtype}), ws, st)))
-        return e;
-    if (g.dw_in != nullptr || g.db_in != nullptr) {
+    ProductGroup group;
+    if (g.dx != nullptr) group.add(false, da, oi, s.rows, s.C, 2 * s.Hp, plain_epilogue({g.dx, s.C, 0, s.dtype}));
+    if (g.dw_in != nullptr) {
         PlainEpi epi = plain_epilogue({g.dw_in, s.C, 0, g.grad});
         epi.sums = {g.db_in, 0, 0, g.grad};
         epi.rows_from = s.Hp, epi.rows_skip = move, epi.tail = 2 * s.H;
-        if ((e = plain_product(da, true, ox, true, 2 * s.Hp, s.C, s.rows, s.dtype, epi, ws, st))) return e;
+        group.add(true, da, ox, 2 * s.Hp, s.C, s.rows, epi);
     }
-    if (g.dw_out != nullptr || g.db_out != nullptr) {
+    if (g.dw_out != nullptr) {
         PlainEpi epi = plain_epilogue({g.dw_out, s.H, 0, g.grad});
         epi.sums = {g.db_out, 0, 0, g.grad};
-        if ((e = plain_product(ody, true, h, true, s.D, s.H, s.rows, s.dtype, epi, ws, st))) return e;
+        group.add(true, ody, h, s.D, s.H, s.rows, epi);
     }
-    return 0;
+    return group.launch(s.dtype, ws, st);
 }
 
 }  // namespace dwo
@@ -178,7 +177,7 @@ extern "C" {
 size_t dwo_gated_workspace_bytes(size_t rows, int C, int H, int D, int backward, int held8, int dtype) {
     const GatedSizes s(rows, C, H, D, dtype);
     if (!s.ok()) return 0;
-    Arena ws{nullptr, 0};
+    Arena ws = Arena::measure();
     void *const any = (void *)256;  // (nothing is launched)
     if (!backward) {
         gated_forward(s, any, any, any, any, any, any, nullptr, ACT_GELU, ws, nullptr);
@@ -200,7 +199,7 @@ int dwo_gated_forward(const void *x, const void *w_in, const void *b_in, const v
         return DWO_ERR_BAD_SHAPE;
     if (ws_bytes < dwo_gated_workspace_bytes(rows, C, H, D, 0, 0, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
     (void)hipGetLastError();
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return gated_forward(s, x, w_in, b_in, w_out, b_out, y, keep, act, a, (hipStream_t)stream);
 }
 
@@ -216,7 +215,7 @@ int dwo_gated_backward(const void *dy, const void *x, const void *codes, const v
         return DWO_ERR_BAD_SHAPE;
     if (ws_bytes < dwo_gated_workspace_bytes(rows, C, H, D, 1, held8, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
     (void)hipGetLastError();
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return gated_backward(s, dy, x, (const int8_t *)codes, (const uint8_t *)exps, keep, w_in, b_in, w_out,
                           {dx, dw_in, db_in, dw_out, db_out, grad_dtype}, act, a, (hipStream_t)stream);
 }

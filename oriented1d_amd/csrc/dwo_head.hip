@@ -163,20 +163,12 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restric
 //   a mean: up / count (1 - eps), so that a row's largest value, about -1 at its target, is next to a number that 16 bits hold; rounded
 //   where it is, the same rounding in all rows would go into the gradients (twice their own rounding with labels smoothed)
 //   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's rows are at most 2, times 2^13, others are brought to
-//   2^13 .. 2^14 by the largest |up|
-// scale[0]: what G is multiplied with, scale[1]: what its products are.
-__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, const float *__restrict__ count, long M,
-                                                          float eps, int half, float *__restrict__ scale) {
-    if (count != nullptr) {
-        if (threadIdx.x == 0)
-            scale[0] = half ? 8192.f : 1.f,
-            scale[1] = count[0] > 0.f ? up[0] / count[0] * (eps < 1.f ? 1.f - eps : 1.f) * (half ? 1.f / 8192.f : 1.f) : 0.f;
-        return;
-    }
+//   2^13 .. 2^14 by the largest |up|: scale[0], and its inverse, by this kernel
+constexpr float kHalfScale = 8192.f;
+__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, long M, float *__restrict__ scale) {
     __shared__ unsigned most[1024];
     unsigned v = 0;
-    if (half)
-        for (long i = threadIdx.x; i < M; i += 1024) v = max(v, __float_as_uint(up[i]) & 0x7fffffffu);
+    for (long i = threadIdx.x; i < M; i += 1024) v = max(v, __float_as_uint(up[i]) & 0x7fffffffu);
     most[threadIdx.x] = v;
     __syncthreads();
     for (int h = 512; h > 0; h >>= 1) {
@@ -195,8 +187,8 @@ struct GradEpi {
     Values bias;      // of the piece
     Targets targets;  // V: all classes
     long from;        // the piece's first class
-    const float *lse, *up, *scale;  // up null: a mean
-    float eps;
+    const float *lse, *up, *scale;  // up null: a mean; scale null: 1, or a mean's in fp16
+    float eps, mean_scale;
     Out g;            // [M][pitch]
     struct Lane : Classes {
         float scale, hit, flat;
@@ -205,7 +197,7 @@ struct GradEpi {
         Lane l;
         l.init(bias, n, p.N);
         // (a mean is held without 1 - eps)
-        const float s = scale[0], part = up == nullptr && eps < 1.f ? s / (1.f - eps) : s;
+        const float s = scale != nullptr ? scale[0] : up == nullptr ? mean_scale : 1.f, part = up == nullptr && eps < 1.f ? s / (1.f - eps) : s;
         l.scale = part, l.hit = up == nullptr && eps < 1.f ? s : s * (1.f - eps), l.flat = part * (eps / (float)targets.V);
         return l;
     }
@@ -291,13 +283,20 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
     // dx is summed over the pieces in fp32
     const bool many = piece < s.V;
     float *sum = many && dx != nullptr && s.dtype != DWO_F32 ? (float *)ws.take((size_t)s.rows * s.C * sizeof(float)) : (float *)dx;
-    float *scale = (float *)ws.take(2 * sizeof(float));
-    if (!ws.dry()) {
-        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, count, s.rows, eps, s.dtype == DWO_F16, scale);
+    const bool mean = count != nullptr, half = s.dtype == DWO_F16;
+    float *scale = half && !mean ? (float *)ws.take(2 * sizeof(float)) : nullptr;
+    if (scale != nullptr && !ws.dry()) {
+        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, s.rows, scale);
         if ((e = status())) return e;
     }
     const size_t size = size_of(s.dtype), grad_size = size_of(grad);
-    const float *alpha = scale + 1;
+    const float mean_scale = half ? kHalfScale : 1.f;
+    auto shared = [&](PlainEpi epi) {
+        epi.alpha = mean ? up : scale != nullptr ? scale + 1 : nullptr;
+        epi.over = count;
+        epi.factor = mean ? (eps < 1.f ? 1.f - eps : 1.f) / mean_scale : 1.f;
+        return epi;
+    };
     const size_t held = ws.used;
     size_t peak = held;
     for (long from = 0; from < s.V; from += piece) {
@@ -308,22 +307,23 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
         Operand gp = g;
         gp.pitch = up8(n), gp.plane = s.rows * gp.pitch;
         if (!ws.dry()) {
-            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, count != nullptr ? nullptr : up, scale, eps,
+            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, mean ? nullptr : up, scale, eps, mean_scale,
                               out_of(gp, s.dtype)};
             if ((e = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st))) return e;
         }
+        ProductGroup group;
         if (dx != nullptr) {
             const bool last = from + n == s.V;
-            PlainEpi epi = plain_epilogue({last ? dx : (void *)sum, s.C, 0, last ? s.dtype : (int)OUT_F32});
-            epi.alpha = alpha, epi.before = from > 0 ? sum : nullptr;
-            if ((e = plain_product(gp, false, wp, true, s.rows, s.C, n, s.dtype, epi, ws, st))) return e;
+            PlainEpi epi = shared(plain_epilogue({last ? dx : (void *)sum, s.C, 0, last ? s.dtype : (int)OUT_F32}));
+            epi.before = from > 0 ? sum : nullptr;
+            group.add(false, gp, wp, s.rows, s.C, n, epi);
         }
         if (dw != nullptr) {
-            PlainEpi epi = plain_epilogue({(char *)dw + (size_t)from * s.C * grad_size, s.C, 0, grad});
+            PlainEpi epi = shared(plain_epilogue({(char *)dw + (size_t)from * s.C * grad_size, s.C, 0, grad}));
             epi.sums = {db != nullptr ? (char *)db + from * grad_size : nullptr, 0, 0, grad};
-            epi.alpha = alpha;
-            if ((e = plain_product(gp, true, ox, true, n, s.C, s.rows, s.dtype, epi, ws, st))) return e;
+            group.add(true, gp, ox, n, s.C, s.rows, epi);
         }
+        if ((e = group.launch(s.dtype, ws, st))) return e;
         if (ws.used > peak) peak = ws.used;
     }
     ws.used = peak;
@@ -339,12 +339,11 @@ extern "C" {
 size_t dwo_head_workspace_bytes(size_t rows, int C, int V, int backward, int dtype) {
     const HeadSizes s(rows, C, V, dtype);
     if (!s.ok()) return 0;
-    Arena ws{nullptr, 0};
+    Arena ws = Arena::measure();
     void *const any = (void *)256;  // (nothing is launched)
     const Targets t{(const long long *)any, 0, V};
     if (backward)
-        head_backward(s, (const float *)any, any, any, any, t, 0.1f, (const float *)any, (const float *)any, any, any, any, DWO_F32, ws,
-                      nullptr);
+        head_backward(s, (const float *)any, any, any, any, t, 0.1f, (const float *)any, nullptr, any, any, any, DWO_F32, ws, nullptr);
     else
         head_forward(s, any, any, any, t, 0.1f, (float *)any, (float *)any, (float *)any, true, ws, nullptr);
     return ws.used + 256;
@@ -360,7 +359,7 @@ int dwo_head_forward(const void *x, const void *w, const void *bias, const void 
         return DWO_ERR_BAD_SHAPE;
     if (ws_bytes < dwo_head_workspace_bytes(rows, C, V, 0, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
     (void)hipGetLastError();
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return head_forward(s, x, w, bias, {(const long long *)targets, ignore, s.V}, smoothing, lse, loss, count, count != nullptr, a,
                         (hipStream_t)stream);
 }
@@ -376,7 +375,7 @@ int dwo_head_backward(const float *up, const void *x, const void *w, const void 
         return DWO_ERR_BAD_SHAPE;
     if (ws_bytes < dwo_head_workspace_bytes(rows, C, V, 1, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
     (void)hipGetLastError();
-    Arena a{(char *)ws, 0};
+    Arena a{(char *)ws, 0, ws_bytes};
     return head_backward(s, up, x, w, bias, {(const long long *)targets, ignore, s.V}, smoothing, lse, count, dx, dw, db, grad_dtype, a,
                          (hipStream_t)stream);
 }

@@ -234,7 +234,9 @@ struct PlainEpi {
     static constexpr bool kSums = false;
     Out out, sums;      // (sums.p null: none)
     Values bias;        // (p null: none)
-    const float *alpha, *before;  // (null: 1, none); before: [M][pitch of out]
+    const float *before;  // [M][pitch of out], or null
+    const float *alpha, *over;  // alpha = factor * alpha[0] / over[0], 0 where over[0] is 0 (null: 1)
+    float factor;
     float *part;        // [splits][M][N], then [splits][M]
     long rows_from, rows_skip;  // output rows from rows_from on lie rows_skip further up; those skipped are not written (0: none)
     long tail;          // columns of A that are only padding (behind rows_from - rows_skip .. rows_from)
@@ -243,6 +245,10 @@ struct PlainEpi {
         if (m < rows_from - rows_skip) return m;
         if (m < rows_from) return -1;
         return m - rows_skip < tail ? m - rows_skip : -1;
+    }
+    __device__ __forceinline__ float scale() const {
+        const float a = alpha != nullptr ? alpha[0] * factor : factor;
+        return over == nullptr ? a : over[0] > 0.f ? a / over[0] : 0.f;
     }
     __device__ __forceinline__ float finish(long m, long n, float v, float a) const {
         v = __builtin_fmaf(v, a, bias.p != nullptr ? bias.at(n) : 0.f);
@@ -255,7 +261,7 @@ struct PlainEpi {
     };
     __device__ __forceinline__ Lane begin(const Product &p, long n) const {
         Lane l;
-        l.alpha = alpha != nullptr && part == nullptr ? *alpha : 1.f;
+        l.alpha = part == nullptr ? scale() : 1.f;
         l.wide = part != nullptr ? p.N % 4 == 0 : out_wide(out);
 #pragma unroll
         for (int e = 0; e < 8; e++) l.bias[e] = bias.p != nullptr && part == nullptr && n + e < p.N ? bias.at(n + e) : 0.f;
@@ -287,7 +293,7 @@ struct PlainEpi {
             return;
         }
         const long to = place(m);
-        if (to >= 0) out_one(sums, 0, to, v * (alpha != nullptr ? *alpha : 1.f));
+        if (to >= 0) out_one(sums, 0, to, v * scale());
     }
 };
 
@@ -317,35 +323,42 @@ __device__ __forceinline__ bool stages_of(std::integer_sequence<int, I...>, F &&
     return (f(std::integral_constant<int, I>{}) && ...);
 }
 
+// The LDS of a workgroup: arrays of their own, so that a read of one waits for no load into another
+#define DWO_STAGES(S)                                                                                  \
+    constexpr int kStageSize = (S::BM + S::BN) * kProdK;                                               \
+    __shared__ __attribute__((aligned(16))) uint16_t s0[kStageSize];                                   \
+    __shared__ __attribute__((aligned(16))) uint16_t s1[kStageSize];                                   \
+    __shared__ __attribute__((aligned(16))) uint16_t s2[S::STAGES > 2 ? kStageSize : 8];               \
+    __shared__ __attribute__((aligned(16))) uint16_t s3[S::STAGES > 2 ? kStageSize : 8];               \
+    __shared__ __attribute__((aligned(16))) uint16_t s4[S::STAGES > 4 ? kStageSize : 8];               \
+    __shared__ __attribute__((aligned(16))) uint16_t s5[S::STAGES > 4 ? kStageSize : 8];               \
+    __shared__ __attribute__((aligned(16))) uint16_t s6[S::STAGES > 4 ? kStageSize : 8];               \
+    __shared__ __attribute__((aligned(16))) uint16_t s7[S::STAGES > 4 ? kStageSize : 8];               \
+    const Stages lds = {s0, s1, s2, s3, s4, s5, s6, s7}
+struct Stages {
+    uint16_t *s0, *s1, *s2, *s3, *s4, *s5, *s6, *s7;
+};
+
+// Workgroup `block` of `blocks` (a multiple of eight).  lrow: room for the rows' numbers.
 template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
-__global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Product p, Epi epi) {
+__device__ __forceinline__ void product_body(const Product &p, const Epi &epi, int block, int blocks, const Stages &lds, unsigned *lrow) {
     constexpr int BM = S::BM, BN = S::BN, MF = S::MF, NF = S::NF, SF = MF / S::WN > 0 ? MF / S::WN : 1;
     constexpr bool SUMS = Epi::kSums;
     constexpr int STAGES = S::STAGES, SIZE = (BM + BN) * kProdK;
-    // (arrays of their own: a read of one then waits for no load into another)
-    __shared__ __attribute__((aligned(16))) uint16_t s0[SIZE];
-    __shared__ __attribute__((aligned(16))) uint16_t s1[SIZE];
-    __shared__ __attribute__((aligned(16))) uint16_t s2[STAGES > 2 ? SIZE : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t s3[STAGES > 2 ? SIZE : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t s4[STAGES > 4 ? SIZE : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t s5[STAGES > 4 ? SIZE : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t s6[STAGES > 4 ? SIZE : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t s7[STAGES > 4 ? SIZE : 8];
     auto stage = [&](auto i) -> uint16_t * {
         constexpr int k = decltype(i)::value % STAGES;
-        if constexpr (k == 0) return s0;
-        else if constexpr (k == 1) return s1;
-        else if constexpr (k == 2) return s2;
-        else if constexpr (k == 3) return s3;
-        else if constexpr (k == 4) return s4;
-        else if constexpr (k == 5) return s5;
-        else if constexpr (k == 6) return s6;
-        else return s7;
+        if constexpr (k == 0) return lds.s0;
+        else if constexpr (k == 1) return lds.s1;
+        else if constexpr (k == 2) return lds.s2;
+        else if constexpr (k == 3) return lds.s3;
+        else if constexpr (k == 4) return lds.s4;
+        else if constexpr (k == 5) return lds.s5;
+        else if constexpr (k == 6) return lds.s6;
+        else return lds.s7;
     };
-    __shared__ unsigned lrow[Epi::kRow > 0 ? BM * Epi::kRow : 1];
     // an XCD (workgroup ids modulo eight) takes a run of tiles; runs go down groups of rows of tiles, so that the tiles of an XCD
     // at one time share both operands' lines
-    const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    const int per = blocks / 8, id = block % 8 * per + block / 8;
     const int tiles = p.mtiles * p.ntiles;
     const int split = id / tiles, tile = id % tiles;
     if (split >= p.splits) return;
@@ -455,15 +468,15 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
         multiply(2 * Q - 1);
     };
     if constexpr (STAGES == 2) {
-        fetch(s0);
+        fetch(lds.s0);
         wait(std::integral_constant<int, 0>{});
-        fetch(s1);
-        read(s0, 0);
+        fetch(lds.s1);
+        read(lds.s0, 0);
         for (int s = 0; s < count; s += 2) step(std::integral_constant<int, 0>{}), step(std::integral_constant<int, 1>{});
     } else {
         stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return fetch(stage(i)), true; });
         wait(std::integral_constant<int, STAGES - 1>{});
-        read(s0, 0);
+        read(lds.s0, 0);
         int s = 0;
         while (stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return step(i), ++s < count; })) {}
     }
@@ -474,7 +487,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
     constexpr int QUADS = 4 * NF, PF = MF < 4 ? MF : 4, ROWS = 16 * PF, LANES = GATED ? NF : 2 * NF, STEP = 64 / LANES;
     constexpr int WAVES = S::THREADS / 64, PART = ROWS * 16 * NF, FIT = SIZE / 2 / PART < WAVES ? SIZE / 2 / PART : WAVES;
     static_assert(2 * FIT >= WAVES, "the waves' parts fit two stages");
-    float *mine = reinterpret_cast<float *>(wave < FIT ? s0 : s1) + wave % FIT * PART;
+    float *mine = reinterpret_cast<float *>(wave < FIT ? lds.s0 : lds.s1) + wave % FIT * PART;
     const int lane = threadIdx.x & 63;
     const int o = lane % LANES, row0 = lane / LANES;
     const long nl = (GATED ? n0 / 2 + wn * 8 * NF : n0 + wn * 16 * NF) + o * 8;
@@ -521,15 +534,25 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Produc
         }
 }
 
+template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
+__global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void product_kernel(Product p, Epi epi) {
+    DWO_STAGES(S);
+    __shared__ unsigned lrow[Epi::kRow > 0 ? S::BM * Epi::kRow : 1];
+    product_body<T, S, AS, BS, GATED>(p, epi, (int)blockIdx.x, (int)gridDim.x, lds, lrow);
+}
+
 // ------------------------------------------------------------------------------------------------- on the host
 // A workspace handed out piece by piece.  With no memory behind it, it measures: the calls below then launch nothing.
 struct Arena {
     char *base;
-    size_t used;
+    size_t used, size;
+    static Arena measure() { return {nullptr, 0, (size_t)-1}; }
     bool dry() const { return base == nullptr; }
+    static size_t whole(size_t bytes) { return (bytes + 255) / 256 * 256; }
+    bool fits(size_t bytes) const { return whole(bytes) <= size - used; }
     void *take(size_t bytes) {
         void *p = base != nullptr ? base + used : nullptr;
-        used += (bytes + 255) / 256 * 256;
+        used += whole(bytes);
         return p;
     }
 };
@@ -589,12 +612,24 @@ private:
     }
 };
 
-// D = A B with the plain epilogue; a_slow, b_slow: the operand lies with the summed index as its slow one (dwo_product.hip).  epi.part
-// is filled in here.
-int plain_product(const Operand &a, bool a_slow, const Operand &b, bool b_slow, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws,
-                  hipStream_t st);
+// A [M][K] times B [N][K] with the plain epilogue, whose `part` is filled in here (dwo_product.hip)
+int plain_product(const Operand &a, const Operand &b, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws, hipStream_t st);
 
-inline PlainEpi plain_epilogue(const Out &out) { return {out, {nullptr, 0, 0, 0}, {nullptr, 0}, nullptr, nullptr, nullptr, 0, 0, 0}; }
+// Products of a backward pass that do not wait for each other, as one launch: of gradients with weights, A [M][K] times B [K][N], and of
+// gradients with activations, A [K][M] times B [K][N].  Their tiles fill the chip together, where each alone leaves a part of its last round.
+struct GroupPart {
+    Product p;
+    PlainEpi epi;
+    int kind, blocks;  // 0: A [M][K], 1: A [K][M], 2: that with sums over A
+};
+struct ProductGroup {
+    GroupPart part[3];
+    int count = 0;
+    void add(bool a_slow, const Operand &a, const Operand &b, long M, long N, long K, const PlainEpi &epi);
+    int launch(int dtype, Arena &ws, hipStream_t st);
+};
+
+inline PlainEpi plain_epilogue(const Out &out) { return {out, {nullptr, 0, 0, 0}, {nullptr, 0}, nullptr, nullptr, nullptr, 1.f, nullptr, 0, 0, 0}; }
 
 // products whose epilogue is not the plain one
 template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>

@@ -1,4 +1,7 @@
 // Operands of the products around wide layers, and the products with the plain epilogue.
+#include <cmath>
+#include <utility>
+
 #include "dwo_check8.h"
 #include "dwo_product.h"
 
@@ -76,11 +79,14 @@ int Staging::launch(bool dry, hipStream_t st) {
     return status();
 }
 
-// Sums over the splits in a fixed order, then the plain epilogue: four neighbours of a row per thread.
-__global__ __launch_bounds__(256) void product_reduce_kernel(Product p, PlainEpi epi) {
+// Sums over the splits in a fixed order, then the plain epilogue: four neighbours of a row per thread, a product per blockIdx.y.
+__global__ __launch_bounds__(256) void product_reduce_kernel(ProductGroup group) {
+    const Product &p = group.part[blockIdx.y].p;
+    const PlainEpi &epi = group.part[blockIdx.y].epi;
+    if (epi.part == nullptr) return;
     const long quads = (p.N + 3) / 4, body = p.M * quads, all = body + (epi.sums.p != nullptr ? p.M : 0);
     const size_t total = (size_t)p.M * p.N;
-    const float a = epi.alpha != nullptr ? *epi.alpha : 1.f;
+    const float a = epi.scale();
     const bool four = p.N % 4 == 0;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
         if (i >= body) {
@@ -112,55 +118,132 @@ __global__ __launch_bounds__(256) void product_reduce_kernel(Product p, PlainEpi
 }
 
 template <typename T, class S>
-int plain_shape(const Product &p, bool as, bool bs, const PlainEpi &epi, hipStream_t st) {
-    if (as && epi.sums.p != nullptr) return launch_shape<T, S, true, true, false>(p, SumsEpi{epi}, st);
-    if (as) return launch_shape<T, S, true, true, false>(p, epi, st);
-    if (bs) return launch_shape<T, S, false, true, false>(p, epi, st);
-    return launch_shape<T, S, false, false, false>(p, epi, st);
-}
-template <typename T>
-int plain_typed(const Product &p, int tile, bool as, bool bs, const PlainEpi &epi, hipStream_t st) {
-    if (tile == 256) return plain_shape<T, LargeTile>(p, as, bs, epi, st);
-    if (tile == 128) return plain_shape<T, MediumTile>(p, as, bs, epi, st);
-    if (tile == 64) return plain_shape<T, SmallTile>(p, as, bs, epi, st);
-    return plain_shape<T, ThinTile>(p, as, bs, epi, st);
+__global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void group_kernel(ProductGroup group) {
+    DWO_STAGES(S);
+    int block = (int)blockIdx.x, k = 0;
+    while (k + 1 < group.count && block >= group.part[k].blocks) block -= group.part[k++].blocks;
+    const GroupPart &q = group.part[k];
+    switch (q.kind) {
+        case 0: product_body<T, S, false, true, false>(q.p, q.epi, block, q.blocks, lds, nullptr); break;
+        case 1: product_body<T, S, true, true, false>(q.p, q.epi, block, q.blocks, lds, nullptr); break;
+        default: product_body<T, S, true, true, false>(q.p, SumsEpi{q.epi}, block, q.blocks, lds, nullptr);
+    }
 }
 
-// tile and splits of a plain product
 struct PlainChoice {
     int tile;
-    long splits;
+    long steps;  // of a split, at most
 };
-// The least of tile_time, with splits of the sums their writing and reading (4 TB/s behind each other) and the launch that joins them
-PlainChoice plain_choice(long M, long N, int steps) {
+static long splits_for(long steps, long most) { return (steps + most - 1) / most; }
+
+// The least time of the products behind each other on all CUs, but no less than that of the longest sum; with splits of the sums also
+// their writing and reading (4 TB/s behind each other) and the launch that joins them.
+static PlainChoice plain_choice(const GroupPart *part, int count) {
     PlainChoice best{0, 0};
     float least = 0.f;
+    long longest = 0;
+    for (int i = 0; i < count; i++) longest = part[i].p.steps > longest ? part[i].p.steps : longest;
     for (const TileCost &c : kTileCosts) {
-        const long tiles = tiles_of(M, N, c.size, c.size);
-        for (const long splits : {1L, 2L, 3L, 4L, 6L, 8L, 12L, 16L, 24L, 32L}) {
-            if (splits > 1 && (tiles * splits > 4 * kLinCus || steps < 4 * splits)) break;
-            float t = tile_time(c, tiles * splits, (steps + splits - 1) / splits);
-            if (splits > 1) t += 4.f + (float)(splits * M) * (float)N * 8.f / 4e6f;
-            if (best.tile == 0 || t < least) best = {c.size, splits}, least = t;
+        for (const long parts : {1L, 2L, 3L, 4L, 6L, 8L, 12L, 16L, 24L, 32L}) {
+            const long most = (longest + parts - 1) / parts;
+            if (parts > 1 && most < 4) break;
+            float shared = 0.f, join = 0.f;
+            long workgroups = 0, chain = 0;
+            for (int i = 0; i < count; i++) {
+                const Product &p = part[i].p;
+                const long splits = splits_for(p.steps, most), steps = (p.steps + splits - 1) / splits;
+                const long n = tiles_of(p.M, p.N, c.size, c.size) * splits;
+                workgroups += n, shared += (float)n * (c.more + (float)steps * c.more_step);
+                chain = steps > chain ? steps : chain;
+                if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 4.f : 0.f);
+            }
+            if (parts > 1 && workgroups > 4 * kLinCus) break;
+            // (a last round that is not full takes as long as one that is)
+            const float rounds = (float)((workgroups + kLinCus - 1) / kLinCus), mean = shared / (float)workgroups;
+            const float alone = c.first + (float)chain * c.first_step;
+            const float t = (workgroups <= kLinCus ? alone : fmaxf(alone, 3.5f + rounds * mean)) + join;
+            if (best.tile == 0 || t < least) best = {c.size, most}, least = t;
         }
     }
     return best;
 }
 
-int plain_product_as(Product p, const PlainChoice &choice, bool as, bool bs, int dtype, PlainEpi epi, Arena &ws, hipStream_t st) {
-    p.per = (int)((p.steps + choice.splits - 1) / choice.splits);
+static void split_part(GroupPart &q, const PlainChoice &choice, Arena &ws) {
+    Product &p = q.p;
+    const long splits = splits_for(p.steps, choice.steps);
+    p.per = (int)((p.steps + splits - 1) / splits);
     p.splits = (p.steps + p.per - 1) / p.per;
-    if (p.splits > 1) epi.part = (float *)ws.take((size_t)p.splits * ((size_t)p.M * p.N + p.M) * sizeof(float));
-    if (ws.dry()) return 0;
-    const int e = dtype == DWO_F16 ? plain_typed<f16_t>(p, choice.tile, as, bs, epi, st) : plain_typed<bf16_t>(p, choice.tile, as, bs, epi, st);
-    if (e != 0 || p.splits == 1) return e;
-    product_reduce_kernel<<<dim3(blocks_for(p.M * ((p.N + 3) / 4) + p.M, 8192)), dim3(256), 0, st>>>(p, epi);
+    const size_t room = (size_t)p.splits * ((size_t)p.M * p.N + p.M) * sizeof(float);
+    // (a workspace is measured for all outputs of a call: with some of them alone more splits may be chosen than it has room for)
+    if (!ws.fits(room)) p.splits = 1, p.per = p.steps;
+    q.epi.part = p.splits > 1 ? (float *)ws.take(room) : nullptr;
+}
+static int join_parts(const ProductGroup &group, hipStream_t st) {
+    long work = 0;
+    for (int i = 0; i < group.count; i++) {
+        const Product &p = group.part[i].p;
+        if (p.splits > 1 && p.M * ((p.N + 3) / 4) + p.M > work) work = p.M * ((p.N + 3) / 4) + p.M;
+    }
+    if (work == 0) return 0;
+    product_reduce_kernel<<<dim3(blocks_for(work, 8192), (unsigned)group.count), dim3(256), 0, st>>>(group);
     return status();
 }
-int plain_product(const Operand &a, bool as, const Operand &b, bool bs, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws,
-                  hipStream_t st) {
-    const Product p = make_product(a, b, M, N, K, 0);
-    return plain_product_as(p, plain_choice(M, N, p.steps), as, bs, dtype, epi, ws, st);
+
+template <typename T>
+static int plain_typed(const GroupPart &q, int tile, hipStream_t st) {
+    switch (tile) {
+        case 256: return launch_shape<T, LargeTile, false, false, false>(q.p, q.epi, st);
+        case 128: return launch_shape<T, MediumTile, false, false, false>(q.p, q.epi, st);
+        case 64: return launch_shape<T, SmallTile, false, false, false>(q.p, q.epi, st);
+        default: return launch_shape<T, ThinTile, false, false, false>(q.p, q.epi, st);
+    }
+}
+int plain_product(const Operand &a, const Operand &b, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws, hipStream_t st) {
+    ProductGroup group;
+    group.part[group.count++] = {make_product(a, b, M, N, K, 0), epi, 0, 0};
+    const PlainChoice choice = plain_choice(group.part, 1);
+    split_part(group.part[0], choice, ws);
+    if (ws.dry()) return 0;
+    const int e = dtype == DWO_F16 ? plain_typed<f16_t>(group.part[0], choice.tile, st) : plain_typed<bf16_t>(group.part[0], choice.tile, st);
+    return e != 0 ? e : join_parts(group, st);
+}
+
+void ProductGroup::add(bool a_slow, const Operand &a, const Operand &b, long M, long N, long K, const PlainEpi &epi) {
+    part[count++] = {make_product(a, b, M, N, K, 0), epi, !a_slow ? 0 : epi.sums.p == nullptr ? 1 : 2, 0};
+}
+template <typename T, class S>
+static int launch_group(ProductGroup group, hipStream_t st) {
+    long all = 0;
+    for (int i = 0; i < group.count; i++) {
+        Product &p = group.part[i].p;
+        p.mtiles = (int)((p.M + S::BM - 1) / S::BM), p.ntiles = (int)((p.N + S::BN - 1) / S::BN);
+        const long blocks = ((long)p.mtiles * p.ntiles * p.splits + 7) / 8 * 8;
+        all += blocks;
+        if (all > 0x7ffffff0L) return DWO_ERR_BAD_SHAPE;
+        group.part[i].blocks = (int)blocks;
+    }
+    group_kernel<T, S><<<dim3((unsigned)all), dim3(S::THREADS), 0, st>>>(group);
+    return status();
+}
+template <typename T>
+static int launch_group_tile(const ProductGroup &group, int tile, hipStream_t st) {
+    switch (tile) {
+        case 256: return launch_group<T, LargeTile>(group, st);
+        case 128: return launch_group<T, MediumTile>(group, st);
+        case 64: return launch_group<T, SmallTile>(group, st);
+        default: return launch_group<T, ThinTile>(group, st);
+    }
+}
+int ProductGroup::launch(int dtype, Arena &ws, hipStream_t st) {
+    if (count == 0) return 0;
+    const PlainChoice choice = plain_choice(part, count);
+    for (int i = 0; i < count; i++) split_part(part[i], choice, ws);
+    if (ws.dry()) return 0;
+    // the longest sums first: what is left at the end is short
+    for (int i = 1; i < count; i++)
+        for (int k = i; k > 0 && part[k].p.per > part[k - 1].p.per; k--) std::swap(part[k], part[k - 1]);
+    const int e = dtype == DWO_F16 ? launch_group_tile<f16_t>(*this, choice.tile, st) : launch_group_tile<bf16_t>(*this, choice.tile, st);
+    return e != 0 ? e : join_parts(*this, st);
 }
 
 }  // namespace dwo
