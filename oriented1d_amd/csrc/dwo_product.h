@@ -50,20 +50,23 @@ __device__ __forceinline__ int prod_key(int row, int R) {
 }
 template <int R, int THREADS, bool SLOW, int HALF>
 struct Stage {
-    static constexpr int U = R * 8 / THREADS;
-    static_assert(R * 8 % THREADS == 0 && THREADS % 64 == 0, "whole loads");
+    static constexpr int U = R * 8 / THREADS, ROWS = THREADS / (R / 8);
+    // k slow: a lane's rows are ROWS apart, and their permutation is the same every sixteen rows
+    static constexpr int OFFS = SLOW ? (ROWS % 16 == 0 ? 1 : 16 / ROWS) : U;
+    static_assert(R * 8 % THREADS == 0 && THREADS % 64 == 0 && (!SLOW || U % OFFS == 0), "whole loads");
     const char *base, *at;  // of plane 0, and where the next stage comes from (k slow) or its plane (k fast)
     long plane, gap, step;  // bytes
-    unsigned off[SLOW ? 1 : U], pitch;
+    unsigned off[OFFS], pitch;
     // (a row or column that the operand has not is nowhere: every other access lies inside it)
     __device__ __forceinline__ void init(const Operand &o, long rows, long r0, long skip) {
         plane = o.plane * 2, gap = skip * 2, step = kProdK * o.pitch * 2, pitch = (unsigned)o.pitch * 2;
         if constexpr (SLOW) {
-            // (a lane's rows are a multiple of sixteen apart: their permutation is the same)
-            static_assert(THREADS / (R / 8) % 16 == 0, "one place in all rows");
             base = reinterpret_cast<const char *>(o.p) + r0 * 2;
-            const int q = threadIdx.x % (R / 8), c = ((q >> 1) ^ prod_key(row(0), R)) * 16 + (q & 1) * 8;
-            off[0] = r0 + c < o.pitch ? (unsigned)row(0) * pitch + (unsigned)c * 2 : kLinNowhere;
+#pragma unroll
+            for (int u = 0; u < OFFS; u++) {
+                const int q = threadIdx.x % (R / 8), c = ((q >> 1) ^ prod_key(row(u), R)) * 16 + (q & 1) * 8;
+                off[u] = r0 + c < o.pitch ? (unsigned)row(u) * pitch + (unsigned)c * 2 : kLinNowhere;
+            }
         } else {
             base = reinterpret_cast<const char *>(o.p) + r0 * o.pitch * 2;
 #pragma unroll
@@ -77,23 +80,18 @@ struct Stage {
     }
     static __device__ __forceinline__ int piece() { return (threadIdx.x % 8) ^ (threadIdx.x / 8 % 8); }
     __device__ __forceinline__ void seek(int which, long k0) { at = base + which * plane + (SLOW ? k0 / kProdK * step : 0); }
-    // left: summed indices from k0 to the operand's end; beyond it a lane reads nowhere, which writes zeros
-    __device__ __forceinline__ void load(uint16_t *lds, int k0, int left) const {
+    // load u of a stage.  left: summed indices from k0 to the operand's end; beyond it a lane reads nowhere, which writes zeros
+    __device__ __forceinline__ void load(uint16_t *lds, int k0, int left, int u) const {
         typedef __attribute__((address_space(3))) void lds_void;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #ifdef __HIP_DEVICE_COMPILE__
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, 0x7fffffff, 0x00020000);
-        __amdgpu_buffer_rsrc_t r2 = r;
-        if constexpr (HALF > 0) r2 = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at + gap), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool second = HALF > 0 && (wave * 8 + u * (THREADS / 8)) / (HALF > 0 ? HALF : 1) % 2 != 0;
-            constexpr int ROWS = THREADS / (R / 8);
-            const unsigned from = SLOW ? ((int)threadIdx.x / (R / 8) < left - u * ROWS ? off[0] : kLinNowhere)
-                                       : off[u] | (piece() * 8 < left ? 0u : kLinNowhere);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(second ? r2 : r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, from,
-                                                     SLOW ? (int)(u * ROWS * pitch) : k0 * 2, 0, 0);
-        }
+        const bool second = HALF > 0 && (wave * 8 + u * (THREADS / 8)) / (HALF > 0 ? HALF : 1) % 2 != 0;
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(second ? at + gap : at), 0, 0x7fffffff, 0x00020000);
+        const unsigned from = SLOW ? ((int)threadIdx.x / (R / 8) < left - u * ROWS ? off[u % OFFS] : kLinNowhere)
+                                   : off[u] | (piece() * 8 < left ? 0u : kLinNowhere);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + (wave * 64 + u * THREADS) * 8), 16, from,
+                                                 SLOW ? (int)(u / OFFS * OFFS * ROWS * pitch) : k0 * 2, 0, 0);
 #endif
     }
     __device__ __forceinline__ void advance() {
@@ -387,11 +385,14 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
     const int first = split * p.per, count = min(p.per, p.steps - first);
     int pair = first / ksteps, k0 = first % ksteps * kProdK, more = count;
     sa.seek(p.codes_a >> (2 * pair) & 3, k0), sb.seek(p.codes_b >> (2 * pair) & 3, k0);
-    // (a loop of one body: an odd last step is followed by one of zeros)
-    auto fetch = [&](uint16_t *la) {
-        uint16_t *lb = la + BM * kProdK;
+    // the loads of the next stage, U in all; (a loop of one body: an odd last step is followed by one of zeros)
+    constexpr int UA = decltype(sa)::U, U = UA + decltype(sb)::U;
+    auto load = [&](uint16_t *to, int u) {
         const int left = more > 0 ? (int)p.K - k0 : 0;
-        sa.load(la, k0, left), sb.load(lb, k0, left);
+        if (u < UA) sa.load(to, k0, left, u);
+        else sb.load(to + BM * kProdK, k0, left, u - UA);
+    };
+    auto loaded = [&] {
         sa.advance(), sb.advance();
         k0 += kProdK, more--;
         if (k0 >= p.K) {
@@ -399,35 +400,38 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
             sa.seek(p.codes_a >> (2 * pair) & 3, 0), sb.seek(p.codes_b >> (2 * pair) & 3, 0);
         }
     };
+    auto fetch = [&](uint16_t *to) {
+#pragma unroll
+        for (int u = 0; u < U; u++) load(to, u);
+        loaded();
+    };
     // (quarters of eight fragments and not halves: sixteen registers less, which two transposing operands have not)
     constexpr int Q = MF == 8 ? 4 : MF > 1 ? 2 : 1, MH = MF / Q;
     mma_s8 fa[2][MH], fb[2][NF];
     Fragments<BM, AS> part_a;
     Fragments<BN, BS> part_b;
     part_a.init(wm * MF * 16), part_b.init(wn * NF * 16);
-    // part t of a stage, q of Q of the rows and half kk: its A goes to fa[t % 2], its B to fb[kk] (with the first rows)
-    auto read = [&](const uint16_t *la, int t) {
-        const uint16_t *lb = la + BM * kProdK;
-        const int kk = t / Q, q = t % Q;
-        part_a.start();
-#pragma unroll
-        for (int j = 0; j < MH; j++) fa[t % 2][j] = part_a.read(la, q * MH + j, kk);
-        if (q != 0) return;
-        part_b.start();
-#pragma unroll
-        for (int i = 0; i < NF; i++) fb[kk][i] = part_b.read(lb, i, kk);
+    // part t of a stage: q of Q of the rows and half kk; its A goes to fa[t % 2], its B to fb[kk] (with the first rows)
+    constexpr int G = MH * NF;  // products of a part
+    auto multiply = [&](int t, int k) {
+        const int kk = t / Q, q = t % Q, j = k / NF, i = k % NF;
+        acc[i][q * MH + j] = Mma<T>::run(fb[kk][i], fa[t % 2][j], acc[i][q * MH + j]);
     };
-    // (what was asked for above goes out before the products, and the products before what is asked for below)
-    auto multiply = [&](int t) {
+    auto reads = [&](int t) { return t % Q == 0 ? MH + NF : MH; };
+    auto read = [&](const uint16_t *from, int t, int r) {
         const int kk = t / Q, q = t % Q;
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
+        if (r < MH) {
+            if (r == 0) part_a.start();
+            fa[t % 2][r] = part_a.read(from, q * MH + r, kk);
+        } else {
+            if (r == MH) part_b.start();
+            fb[kk][r - MH] = part_b.read(from + BM * kProdK, r - MH, kk);
+        }
+    };
+    auto read_all = [&](const uint16_t *from, int t) {
 #pragma unroll
-        for (int j = 0; j < MH; j++)
-#pragma unroll
-            for (int i = 0; i < NF; i++) acc[i][q * MH + j] = Mma<T>::run(fb[kk][i], fa[t % 2][j], acc[i][q * MH + j]);
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int r = 0; r < MH + NF; r++)
+            if (r < reads(t)) read(from, t, r);
     };
     // sums over A alone, in the workgroups of the first column of tiles: products with ones, with zeros elsewhere and where a plane of A
     // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all)
@@ -456,27 +460,44 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
         __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | n >> 4 << 14);
         asm volatile("s_barrier" ::: "memory");
     };
+    // What goes out between the products of a part, evenly: the reads of the next part, in the last one the loads too (behind each other
+    // they hold the products up: 8192 x 8192 x 8192 in bf16 877 us, so 860)
     auto step = [&](auto i) {
         uint16_t *current = stage(i);
+        const uint16_t *next = stage(std::integral_constant<int, decltype(i)::value + 1>{});
         add_sums(current);
 #pragma unroll
-        for (int t = 0; t + 1 < 2 * Q; t++) read(current, t + 1), multiply(t);
-        // this wave's reads of the stage are done, and its part of the next one is there; so are the other waves' behind the barrier
-        wait(std::integral_constant<int, STAGES - 2>{});
-        fetch(current);
-        read(stage(std::integral_constant<int, decltype(i)::value + 1>{}), 0);
-        multiply(2 * Q - 1);
+        for (int t = 0; t < 2 * Q; t++) {
+            const bool last = t + 1 == 2 * Q;
+            // this wave's reads of the stage are done, and its part of the next one is there; so are the other waves' behind the barrier
+            if (last) wait(std::integral_constant<int, STAGES - 2>{});
+            const int after = last ? 0 : t + 1, n = reads(after);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                multiply(t, k);
+#pragma unroll
+                for (int r = 0; r < MH + NF; r++)
+                    if (r >= k * n / G && r < (k + 1) * n / G) read(last ? next : current, after, r);
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (last && u >= k * U / G && u < (k + 1) * U / G) load(current, u);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        }
+        loaded();
     };
     if constexpr (STAGES == 2) {
         fetch(lds.s0);
         wait(std::integral_constant<int, 0>{});
         fetch(lds.s1);
-        read(lds.s0, 0);
+        read_all(lds.s0, 0);
         for (int s = 0; s < count; s += 2) step(std::integral_constant<int, 0>{}), step(std::integral_constant<int, 1>{});
     } else {
         stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return fetch(stage(i)), true; });
         wait(std::integral_constant<int, STAGES - 1>{});
-        read(lds.s0, 0);
+        read_all(lds.s0, 0);
         int s = 0;
         while (stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return step(i), ++s < count; })) {}
     }
