@@ -13,7 +13,7 @@
 namespace dwo {
 
 struct GluEpi {
-    static constexpr bool kSums = false;
+    static constexpr bool kSums = false, kDirect = false;
     Values bias;  // [2 H]
     long H, Hp;
     int act;
@@ -47,12 +47,12 @@ struct GluEpi {
         if (h.p == nullptr) return;
 #pragma unroll
         for (int e = 0; e < 8; e++) g[e] = act_value(act, g[e]) * u[e];
-        out_octet(h, true, m, n, Hp, g);
+        out_octet<false>(h, true, m, n, Hp, g);
     }
 };
 
 struct DgluEpi {
-    static constexpr bool kSums = false;
+    static constexpr bool kSums = false, kDirect = false;
     long H, Hp;
     int act;
     const float *keep;
@@ -66,7 +66,9 @@ struct DgluEpi {
         Data d;
         const mma_f4 *g = reinterpret_cast<const mma_f4 *>(keep + m * Hp + n);
         const mma_f4 *u = reinterpret_cast<const mma_f4 *>(keep + (p.M + m) * Hp + n);
-        if (m < p.M && n < Hp) d = {{g[0], g[1]}, {u[0], u[1]}};
+        if (m < p.M && n < Hp)
+            d = {{__builtin_nontemporal_load(g), __builtin_nontemporal_load(g + 1)},
+                 {__builtin_nontemporal_load(u), __builtin_nontemporal_load(u + 1)}};
         return d;
     }
     __device__ __forceinline__ void octet(const Product &p, const Nothing &, const unsigned *, const Data &kept, int, long m, long n,

@@ -21,6 +21,90 @@ struct Targets {
     }
 };
 
+// bias of the classes n0 + 16 i + 4 g + r that a lane has, -infinity where there is no class: its logit is then no largest one and its
+// exponential zero (products with columns that are not there are zeros)
+__device__ __forceinline__ long class_of(long n0, int i, int r) { return n0 + 16 * i + 4 * ((threadIdx.x & 63) >> 4) + r; }
+template <int NF>
+struct RowClasses {
+    float bias[NF][4];
+    __device__ __forceinline__ void init(const Values &b, long n0, long N) {
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const long n = class_of(n0, i, r);
+                bias[i][r] = n >= N ? -INFINITY : b.p != nullptr ? b.at(n) : 0.f;
+            }
+    }
+};
+// joined over the four lanes that have a row
+template <class F>
+__device__ __forceinline__ float over_lanes(float v, F &&join) {
+    const unsigned u = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned w = __float_as_uint(join(__uint_as_float(s[0]), __uint_as_float(s[1])));
+    const auto t = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return join(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+struct StatsEpi {
+    static constexpr bool kSums = false, kDirect = true;
+    Values bias;
+    Targets targets;
+    float2 *part;  // [classes / (16 NF)][M]: largest, sum of exponentials
+    float *sum;    // the same of sums of logits, or null
+    float *at;     // [M]: the target's logit
+    static constexpr int kRow = 1;  // the target
+    __device__ __forceinline__ unsigned row(const Product &, long m, int) const { return (unsigned)targets.of(m); }
+    template <int NF>
+    __device__ __forceinline__ RowClasses<NF> begin(const Product &p, long n0) const {
+        RowClasses<NF> l;
+        l.init(bias, n0, p.N);
+        return l;
+    }
+    template <int NF>
+    __device__ __forceinline__ void emit(const Product &p, const RowClasses<NF> &l, const unsigned *rows, long m, long n0,
+                                         mma_f4 (&v)[NF]) const {
+        float most = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[i][r] += l.bias[i][r], most = fmaxf(most, v[i][r]);
+        if (m < p.M) {
+            const int t = (int)rows[0] - (int)class_of(n0, 0, 0);
+            if (t >= 0 && t < 16 * NF && (t & 15) < 4) {
+                float hit = 0.f;
+#pragma unroll
+                for (int i = 0; i < NF; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) hit = t == 16 * i + r ? v[i][r] : hit;
+                at[m] = hit;
+            }
+        }
+        most = over_lanes(most, [](float a, float b) { return fmaxf(a, b); });
+        // (all -infinity: no exponential; NaN is in no maximum and in the sum)
+        const float base = most == -INFINITY ? 0.f : most;
+        // (exponents are differences here: what rounding their multiples leaves, 2^-24 of each, is small where the term is not)
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s += __builtin_amdgcn_exp2f((v[i][r] - base) * 1.44269504f);
+        s = over_lanes(s, [](float a, float b) { return a + b; });
+        const bool writes = (threadIdx.x & 63) < 16 && n0 < p.N && m < p.M;
+        const size_t to = (size_t)(n0 / (16 * NF)) * p.M + m;
+        if (writes) part[to] = make_float2(most, s);
+        if (sum != nullptr) {
+            float all = 0.f;
+#pragma unroll
+            for (int i = 0; i < NF; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) all += class_of(n0, i, r) < p.N ? v[i][r] : 0.f;
+            all = over_lanes(all, [](float a, float b) { return a + b; });
+            if (writes) sum[to] = all;
+        }
+    }
+};
+
 // bias of the eight classes that a lane has, -infinity where there is no class: its logit is then no largest one and its exponential zero
 // (products with columns that are not there are zeros)
 struct Classes {
@@ -30,72 +114,8 @@ struct Classes {
         for (int e = 0; e < 8; e++) bias[e] = n + e >= N ? -INFINITY : b.p != nullptr ? b.at(n + e) : 0.f;
     }
 };
-// joined over groups of two, four or eight lanes
-template <int CTRL>
-__device__ __forceinline__ float from_lane(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
-template <class F>
-__device__ __forceinline__ float over_lanes(float v, int lanes, F &&join) {
-    v = join(v, from_lane<0xB1>(v));                   // quad_perm [1,0,3,2]
-    if (lanes > 2) v = join(v, from_lane<0x4E>(v));    // quad_perm [2,3,0,1]
-    if (lanes > 4) v = join(v, from_lane<0x141>(v));   // row_half_mirror
-    return v;
-}
 // place of class t among eight from n on, or one beyond them
 __device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
-
-struct StatsEpi {
-    static constexpr bool kSums = false;
-    Values bias;
-    Targets targets;
-    float2 *part;  // [classes / width][M]: largest, sum of exponentials
-    float *sum;    // the same of sums of logits, or null
-    float *at;     // [M]: the target's logit
-    int width;     // classes of a wave, eight to a lane
-    typedef Classes Lane;
-    __device__ __forceinline__ Lane begin(const Product &p, long n) const {
-        Lane l;
-        l.init(bias, n, p.N);
-        return l;
-    }
-    static constexpr int kRow = 1;  // the target
-    __device__ __forceinline__ unsigned row(const Product &, long m, int) const { return (unsigned)targets.of(m); }
-    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
-    __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
-                                          float (&v)[8]) const {
-        float most = -INFINITY, s = 0.f;
-        const int lanes = width / 8;
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += l.bias[e], most = fmaxf(most, v[e]);
-        if (m < p.M) {
-            const int k = place_of((int)rows[0], n);
-            if (k < 8) {
-                float hit = v[0];
-#pragma unroll
-                for (int e = 1; e < 8; e++) hit = k == e ? v[e] : hit;
-                at[m] = hit;
-            }
-        }
-        most = over_lanes(most, lanes, [](float a, float b) { return fmaxf(a, b); });
-        // (all -infinity: no exponential; NaN is in no maximum and in the sum)
-        const float base = most == -INFINITY ? 0.f : most;
-        // (exponents are differences here: what rounding their multiples leaves, 2^-24 of each, is small where the term is not)
-#pragma unroll
-        for (int e = 0; e < 8; e++) s += __builtin_amdgcn_exp2f((v[e] - base) * 1.44269504f);
-        s = over_lanes(s, lanes, [](float a, float b) { return a + b; });
-        const bool writes = n % width == 0 && n < p.N && m < p.M;
-        const size_t to = (size_t)(n / width) * p.M + m;
-        if (writes) part[to] = make_float2(most, s);
-        if (sum != nullptr) {
-            float all = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) all += n + e < p.N ? v[e] : 0.f;
-            all = over_lanes(all, lanes, [](float a, float b) { return a + b; });
-            if (writes) sum[to] = all;
-        }
-    }
-};
 
 // Sixteen rows per workgroup, sixteen threads a row.
 __global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict__ part, const float *__restrict__ sum,
@@ -183,7 +203,7 @@ __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restric
 }
 
 struct GradEpi {
-    static constexpr bool kSums = false;
+    static constexpr bool kSums = false, kDirect = false;
     Values bias;      // of the piece
     Targets targets;  // V: all classes
     long from;        // the piece's first class
@@ -264,7 +284,7 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
     float *at = (float *)ws.take((size_t)s.rows * sizeof(float));
     float2 *block = mean ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
     if (ws.dry()) return 0;
-    const StatsEpi epi{{b, s.dtype}, targets, part, sum, at, width};
+    const StatsEpi epi{{b, s.dtype}, targets, part, sum, at};
     if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
     head_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss, block, s.rows, parts,
                                                                   eps);

@@ -170,7 +170,16 @@ __device__ __forceinline__ bool out_wide(const Out &o) {
     return o.pitch % (o.type == OUT_F32 ? 4 : 8) == 0 && ((uintptr_t)o.p & 15) == 0;
 }
 
+// Stores of whole lines (STREAM: eight lanes have 128 bytes of a row of 16-bit values) go past the L2: what they write does not fit it, and
+// another launch reads it (4096 x 4096 x 64, all of it writing, 17.5 / 15.9 us; 25088 x 1536 x 384 59.4 / 57.3).  Pieces of lines go
+// through it (fp32 in two stores per lane: the gated block's first product, 16384 x 1024 x 8192, 466 us past it, 400 so).
+template <bool STREAM>
+__device__ __forceinline__ void store_out(void *to, const mma_u4 &v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<mma_u4 *>(to));
+    else *reinterpret_cast<mma_u4 *>(to) = v;
+}
 // eight neighbours n .. n + 7 of row m (n a multiple of eight), those below N
+template <bool STREAM = true>
 __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long n, long N, const float (&v)[8]) {
     if (!wide || n + 8 > N) {
 #pragma unroll
@@ -191,12 +200,10 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
         for (int e = 0; e < 8; e++) planes_of(v[e], q[e]);
 #pragma unroll
         for (int k = 0; k < 3; k++)
-            *reinterpret_cast<mma_u4 *>(to + k * o.plane) =
-                mma_u4{pack_bf16(q[0][k], q[1][k]), pack_bf16(q[2][k], q[3][k]), pack_bf16(q[4][k], q[5][k]), pack_bf16(q[6][k], q[7][k])};
+            store_out<STREAM>(to + k * o.plane, mma_u4{pack_bf16(q[0][k], q[1][k]), pack_bf16(q[2][k], q[3][k]), pack_bf16(q[4][k], q[5][k]), pack_bf16(q[6][k], q[7][k])});
         return;
     }
-    *reinterpret_cast<mma_u4 *>(to) =
-        mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])};
+    store_out<STREAM>(to, mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])});
 }
 
 // An epilogue E has
@@ -205,6 +212,8 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
 //   load(p, m, n): what the epilogue reads for an octet, asked for one octet ahead
 //   octet(p, lane, rows, data, split, m, n, v): eight neighbours of a row; all lanes call it for some row, beyond the ends as well
 //   kSums, emit_sum: see SumsEpi
+// or, where it writes next to nothing, kDirect and emit(p, lane, rows, m, n0, v): a row's fragments as they are in registers, columns
+// n0 + 16 i + 4 g + r, with begin(p, n0) of the wave's first column.
 struct Nothing {};
 
 struct Values {  // a vector of fp32 or 16-bit values, or none
@@ -229,7 +238,7 @@ __device__ __forceinline__ float prod_exp(float v) {
 // The plain epilogue: out = alpha * sum + bias[n] + before[m][n].  With several splits the sums go to `part` as they are, and
 // product_reduce_kernel does the rest.  sums: the sums over k of A alone (a bias gradient), alpha times.
 struct PlainEpi {
-    static constexpr bool kSums = false;
+    static constexpr bool kSums = false, kDirect = false;
     Out out, sums;      // (sums.p null: none)
     Values bias;        // (p null: none)
     const float *before;  // [M][pitch of out], or null
@@ -315,6 +324,15 @@ typedef Shape<128, 128, 2, 2, 2, 2> MediumTile;  // 64 KB, two
 typedef Shape<64, 64, 2, 2, 2, 4> SmallTile;     // 64 KB
 typedef Shape<32, 32, 2, 2, 2, 8> ThinTile;      // 64 KB
 
+// f(0), f(1), .. with constant indices, one after the other
+template <class F, int... I>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F &&f) {
+    ((f(std::integral_constant<int, I>{}), __builtin_amdgcn_sched_barrier(0)), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F &&f) {
+    each_of(std::make_integer_sequence<int, N>{}, f);
+}
 // f(0), f(1), .. until one is false
 template <class F, int... I>
 __device__ __forceinline__ bool stages_of(std::integer_sequence<int, I...>, F &&f) {
@@ -502,49 +520,61 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
         while (stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return step(i), ++s < count; })) {}
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (nothing may arrive behind the sums)
-    // The sums go through LDS, each wave's through its own part, and come back as eight neighbours of a row per lane (gated: eight
-    // gates and what they multiply): wide stores, row sums over few lanes, and a loop of one body.  Quads of a row are permuted by the row.
-    __syncthreads();
-    constexpr int QUADS = 4 * NF, PF = MF < 4 ? MF : 4, ROWS = 16 * PF, LANES = GATED ? NF : 2 * NF, STEP = 64 / LANES;
-    constexpr int WAVES = S::THREADS / 64, PART = ROWS * 16 * NF, FIT = SIZE / 2 / PART < WAVES ? SIZE / 2 / PART : WAVES;
-    static_assert(2 * FIT >= WAVES, "the waves' parts fit two stages");
-    float *mine = reinterpret_cast<float *>(wave < FIT ? lds.s0 : lds.s1) + wave % FIT * PART;
-    const int lane = threadIdx.x & 63;
-    const int o = lane % LANES, row0 = lane / LANES;
-    const long nl = (GATED ? n0 / 2 + wn * 8 * NF : n0 + wn * 16 * NF) + o * 8;
-    const auto local = epi.begin(p, nl);
+    if constexpr (Epi::kDirect) {
+        // (1141 us through LDS, 1001 so: statistics of 8192 x 1024 x 65536.  Where rows are written their pieces are too short, 64 bytes)
+        const long nw = n0 + wn * 16 * NF, mw = m0 + wm * 16 * MF + (threadIdx.x & 15);
+        const auto local = epi.template begin<NF>(p, nw);
+        each<MF>([&](auto j) {
+            mma_f4 v[NF];
 #pragma unroll
-    for (int pass = 0; pass < MF / PF; pass++) {
+            for (int i = 0; i < NF; i++) v[i] = acc[i][j];
+            epi.emit(p, local, lrow + (wm * 16 * MF + 16 * j + (threadIdx.x & 15)) * Epi::kRow, mw + 16 * j, nw, v);
+        });
+    } else {
+        // The sums go through LDS, each wave's through its own part, and come back as eight neighbours of a row per lane (gated: eight
+        // gates and what they multiply): wide stores, row sums over few lanes, and a loop of one body.  Quads of a row are permuted by the row.
+        __syncthreads();
+        constexpr int QUADS = 4 * NF, PF = MF < 4 ? MF : 4, ROWS = 16 * PF, LANES = GATED ? NF : 2 * NF, STEP = 64 / LANES;
+        constexpr int WAVES = S::THREADS / 64, PART = ROWS * 16 * NF, FIT = SIZE / 2 / PART < WAVES ? SIZE / 2 / PART : WAVES;
+        static_assert(2 * FIT >= WAVES, "the waves' parts fit two stages");
+        float *mine = reinterpret_cast<float *>(wave < FIT ? lds.s0 : lds.s1) + wave % FIT * PART;
+        const int lane = threadIdx.x & 63;
+        const int o = lane % LANES, row0 = lane / LANES;
+        const long nl = (GATED ? n0 / 2 + wn * 8 * NF : n0 + wn * 16 * NF) + o * 8;
+        const auto local = epi.begin(p, nl);
 #pragma unroll
-        for (int j = 0; j < PF; j++)
+        for (int pass = 0; pass < MF / PF; pass++) {
 #pragma unroll
-            for (int i = 0; i < NF; i++) {
-                const int row = 16 * j + (lane & 15), quad = 4 * i + (lane >> 4);
-                reinterpret_cast<mma_f4 *>(mine)[row * QUADS + (quad ^ (row & (QUADS - 1)))] = acc[i][pass * PF + j];
-            }
-        auto octet = [&](int row, int at, float (&v)[8]) {
+            for (int j = 0; j < PF; j++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const mma_f4 q = reinterpret_cast<const mma_f4 *>(mine)[row * QUADS + ((2 * at + h) ^ (row & (QUADS - 1)))];
+                for (int i = 0; i < NF; i++) {
+                    const int row = 16 * j + (lane & 15), quad = 4 * i + (lane >> 4);
+                    reinterpret_cast<mma_f4 *>(mine)[row * QUADS + (quad ^ (row & (QUADS - 1)))] = acc[i][pass * PF + j];
+                }
+            auto octet = [&](int row, int at, float (&v)[8]) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * h + e] = q[e];
-            }
-        };
-        const long mp = m0 + wm * 16 * MF + pass * ROWS;
-        auto data = epi.load(p, mp + row0, nl);
+                for (int h = 0; h < 2; h++) {
+                    const mma_f4 q = reinterpret_cast<const mma_f4 *>(mine)[row * QUADS + ((2 * at + h) ^ (row & (QUADS - 1)))];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[4 * h + e] = q[e];
+                }
+            };
+            const long mp = m0 + wm * 16 * MF + pass * ROWS;
+            auto data = epi.load(p, mp + row0, nl);
 #pragma unroll 2
-        for (int row = row0; row < ROWS; row += STEP) {
-            const auto now = data;
-            data = epi.load(p, mp + row + STEP, nl);
-            const unsigned *rows = lrow + (wm * 16 * MF + pass * ROWS + row) * Epi::kRow;
-            float v[8];
-            octet(row, o, v);
-            if constexpr (GATED) {
-                float u[8];
-                octet(row, NF + o, u);
-                epi.octet(p, local, mp + row, nl, v, u);
-            } else {
-                epi.octet(p, local, rows, now, split, mp + row, nl, v);
+            for (int row = row0; row < ROWS; row += STEP) {
+                const auto now = data;
+                data = epi.load(p, mp + row + STEP, nl);
+                const unsigned *rows = lrow + (wm * 16 * MF + pass * ROWS + row) * Epi::kRow;
+                float v[8];
+                octet(row, o, v);
+                if constexpr (GATED) {
+                    float u[8];
+                    octet(row, NF + o, u);
+                    epi.octet(p, local, mp + row, nl, v, u);
+                } else {
+                    epi.octet(p, local, rows, now, split, mp + row, nl, v);
+                }
             }
         }
     }
