@@ -314,7 +314,7 @@ int dwo_linear_norm_planes(const void *x, const float *gamma_in, const float *be
 
 /*
  * Operators around wide layers, for training and evaluation; no counterpart in the reference's extension.  Tensors are dense, of one type
- * `dtype` (DWO_F32, DWO_BF16, DWO_F16), parameters' gradients are written as grad_dtype.  rows is below 2^31, channels are at most 65536;
+ * `dtype` (DWO_F32, DWO_BF16, DWO_F16), parameters' gradients are written as grad_dtype.  rows is at most 2^30, channels are at most 65536;
  * inputs, outputs that a kernel reads again, and workspaces are 16-byte aligned.  Sums, exponentials and statistics are fp32.  ws holds at least
  * the bytes that the matching function gives (0: sizes that are not accepted); nothing in it has to survive a call, and calls that
  * overlap in time take one each.

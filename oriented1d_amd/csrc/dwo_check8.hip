@@ -154,7 +154,7 @@ int launch_unpack8(const void *codes, const void *exps, const void *dy, void *ou
 }
 
 static bool sizes_ok(long rows, int C, const void *a, const void *b, const void *c, const void *d) {
-    return rows >= 1 && rows < 1L << 31 && C >= 1 && C <= 65536 && ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 == 0;
+    return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 == 0;
 }
 
 static int layer_forward(const void *x, const void *w, const void *b, void *y, long rows, int C, int D, int dtype, Arena &ws,

@@ -95,7 +95,7 @@ struct GatedSizes {
     int dtype;
     GatedSizes(size_t r, int c, int h, int d, int t) : rows((long)r), C(c), H(h), D(d), Hp(up8(h)), dtype(t) {}
     bool ok() const {
-        return rows >= 1 && rows < 1L << 31 && C >= 1 && H >= 1 && D >= 1 && C <= 65536 && H <= 65536 && D <= 65536 && known(dtype);
+        return rows >= 1 && rows <= 1L << 30 && C >= 1 && H >= 1 && D >= 1 && C <= 65536 && H <= 65536 && D <= 65536 && known(dtype);
     }
 };
 

@@ -117,53 +117,57 @@ struct Classes {
 // place of class t among eight from n on, or one beyond them
 __device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
 
-// Sixteen rows per workgroup, sixteen threads a row.
+// The parts of a row joined, sixteen threads a row and sixteen rows at a time; `block` receives a workgroup's sum of losses and number of
+// rows that count.  One workgroup with all rows (few of them) writes the mean itself.
 __global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict__ part, const float *__restrict__ sum,
                                                         const float *__restrict__ at, Targets targets, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float2 *__restrict__ block, long M, int parts,
-                                                        float eps) {
+                                                        float *__restrict__ loss, float *__restrict__ mean, float *__restrict__ count,
+                                                        float2 *__restrict__ block, long M, int parts, float eps) {
     __shared__ float most_of[16][17], sum_of[16][17], all_of[16][17];
     __shared__ float2 rows[16];
     const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const long m = (long)blockIdx.x * 16 + r;
-    float most = -INFINITY, s = 0.f, all = 0.f;
-    if (m < M)
-        for (int p = k; p < parts; p += 16) {
-            const float2 v = part[(size_t)p * M + m];
-            const float next = fmaxf(most, v.x), base = next == -INFINITY ? 0.f : next;
-            s = s * prod_exp(most - base) + v.y * prod_exp(v.x - base);
-            most = next;
-            if (sum != nullptr) all += sum[(size_t)p * M + m];
+    double total = 0.0, number = 0.0;
+    for (long first = (long)blockIdx.x * 16; first < M; first += (long)gridDim.x * 16) {
+        const long m = first + r;
+        float most = -INFINITY, s = 0.f, all = 0.f;
+        if (m < M)
+            for (int p = k; p < parts; p += 16) {
+                const float2 v = part[(size_t)p * M + m];
+                const float next = fmaxf(most, v.x), base = next == -INFINITY ? 0.f : next;
+                s = s * prod_exp(most - base) + v.y * prod_exp(v.x - base);
+                most = next;
+                if (sum != nullptr) all += sum[(size_t)p * M + m];
+            }
+        most_of[k][r] = most, sum_of[k][r] = s, all_of[k][r] = all;
+        __syncthreads();
+        if (k == 0) {
+            for (int i = 1; i < 16; i++) most = fmaxf(most, most_of[i][r]);
+            const float base = most == -INFINITY ? 0.f : most;
+            s = 0.f, all = 0.f;
+            for (int i = 0; i < 16; i++) s += sum_of[i][r] * prod_exp(most_of[i][r] - base), all += all_of[i][r];
+            float value = 0.f, counts = 0.f;
+            if (m < M) {
+                const float l = base + logf(s);
+                lse[m] = l;
+                const int t = targets.of(m);
+                if (t == -2) value = NAN;
+                else if (t >= 0) value = (l - at[m]) * (1.f - eps);
+                if (t >= 0 && sum != nullptr) value += eps * (l - all / (float)targets.V);
+                counts = t != -1 ? 1.f : 0.f;
+                if (loss != nullptr) loss[m] = value;
+            }
+            rows[r] = make_float2(value, counts);
         }
-    most_of[k][r] = most, sum_of[k][r] = s, all_of[k][r] = all;
-    __syncthreads();
-    if (k == 0) {
-        for (int i = 1; i < 16; i++) most = fmaxf(most, most_of[i][r]);
-        const float base = most == -INFINITY ? 0.f : most;
-        s = 0.f, all = 0.f;
-        for (int i = 0; i < 16; i++) s += sum_of[i][r] * prod_exp(most_of[i][r] - base), all += all_of[i][r];
-        float value = 0.f, count = 0.f;
-        if (m < M) {
-            const float l = base + logf(s);
-            lse[m] = l;
-            const int t = targets.of(m);
-            if (t == -2) value = NAN;
-            else if (t >= 0) value = (l - at[m]) * (1.f - eps);
-            if (t >= 0 && sum != nullptr) value += eps * (l - all / (float)targets.V);
-            count = t != -1 ? 1.f : 0.f;
-            if (loss != nullptr) loss[m] = value;
-        }
-        rows[r] = make_float2(value, count);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 0; i < 16; i++) total += rows[i].x, number += rows[i].y;
     }
-    __syncthreads();
-    if (block != nullptr && threadIdx.x == 0) {
-        float2 t = make_float2(0.f, 0.f);
-        for (int i = 0; i < 16; i++) t.x += rows[i].x, t.y += rows[i].y;
-        block[blockIdx.x] = t;
-    }
+    if (threadIdx.x != 0) return;
+    if (block != nullptr) block[blockIdx.x] = make_float2((float)total, (float)number);
+    else if (mean != nullptr) mean[0] = (float)(total / number), count[0] = (float)number;
 }
 
-// loss[0] = the mean over the rows that count, count[0] how many do; one workgroup, fixed order, in 64 bits (many rows)
+// The same of many workgroups' sums, in a fixed order and in 64 bits
 __global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restrict__ block, int blocks, float *__restrict__ loss,
                                                          float *__restrict__ count) {
     __shared__ double value[1024], number[1024];
@@ -262,7 +266,7 @@ struct HeadSizes {
     long rows, C, V;
     int dtype;
     HeadSizes(size_t r, int c, int v, int t) : rows((long)r), C(c), V(v), dtype(t) {}
-    bool ok() const { return rows >= 1 && rows < 1L << 31 && C >= 1 && C <= 65536 && V >= 1 && V <= 1 << 24 && known(dtype); }
+    bool ok() const { return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && V >= 1 && V <= 1 << 24 && known(dtype); }
     // classes of a piece: G of a piece has about 2^27 values, 256 MB in 16 bits, what the last cache before memory holds
     long piece() const {
         const long most = (1L << 27) / rows / 256 * 256;
@@ -278,17 +282,18 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
     if (e) return e;
     const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
     const int width = wave_columns(tile_for(p.M, p.N, p.steps));
-    const int parts = (int)((s.V + width - 1) / width), blocks = (int)((s.rows + 15) / 16);
+    // Up to 128 rows one workgroup joins them all (64 x 1000 classes: 4.7 and 2.4 us as two launches)
+    const int parts = (int)((s.V + width - 1) / width), blocks = s.rows <= 128 ? 1 : (int)((s.rows + 15) / 16);
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
     float *sum = eps > 0.f ? (float *)ws.take((size_t)parts * s.rows * sizeof(float)) : nullptr;
     float *at = (float *)ws.take((size_t)s.rows * sizeof(float));
-    float2 *block = mean ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
+    float2 *block = mean && blocks > 1 ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
     if (ws.dry()) return 0;
     const StatsEpi epi{{b, s.dtype}, targets, part, sum, at};
     if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
-    head_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss, block, s.rows, parts,
-                                                                  eps);
-    if (mean) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
+    head_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss,
+                                                                  mean ? loss : nullptr, count, block, s.rows, parts, eps);
+    if (block != nullptr) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
     return status();
 }
 

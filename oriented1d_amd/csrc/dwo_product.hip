@@ -155,7 +155,7 @@ static PlainChoice plain_choice(const GroupPart *part, int count) {
                 const long n = tiles_of(p.M, p.N, c.size, c.size) * splits;
                 workgroups += n, shared += (float)n * (c.more + (float)steps * c.more_step);
                 chain = steps > chain ? steps : chain;
-                if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 4.f : 0.f);
+                if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 5.f : 0.f);
             }
             if (parts > 1 && workgroups > 4 * kLinCus) break;
             // (a last round that is not full takes as long as one that is)
