@@ -11,8 +11,8 @@ import math
 
 import pytest
 import torch
-import torch.nn as nn
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from oriented1d_amd import checkpoint8, feedforward, losses
 from oriented1d_amd.convnext1d import Block, ConvNeXt1D
@@ -150,7 +150,7 @@ def test_gated_gradients_of_some_inputs():
 
 def test_gated_differences():
     """The gradient against differences of the result: along a direction d, (f(x + h d) - f(x - h d)) / 2 h is off by the third derivative,
-    about h^2, and by what fp32 leaves of the results, about 1e-6 |f| / h: h = 1e-2, 1e-3 of the norms involved."""
+    about h^2, and by what fp32 leaves of the results, about 1e-6 |f| / h: with h = 1e-2 both under 1e-3 of the norm of dy."""
     args, dy = make_gated(20, 24, 40, 16, torch.float32, seed=5)
     y = feedforward.gated_mlp(*args, activation="silu")
     got = torch.autograd.grad(y, args, dy)
@@ -162,7 +162,7 @@ def test_gated_differences():
             moved = [feedforward.gated_mlp(*[t + s * h * d if k == i else t for k, t in enumerate(args)], activation="silu")
                      for s in (1, -1)]
         slope = float(((moved[0].double() - moved[1].double()) * dy.double()).sum()) / (2 * h)
-        assert abs(slope - float((g * d).double().sum())) <= 2e-3 * float(dy.double().norm()) * math.sqrt(d.numel()) / math.sqrt(d.numel()), i
+        assert abs(slope - float((g * d).double().sum())) <= 2e-3 * float(dy.double().norm()), i
 
 
 @pytest.mark.parametrize("what", ["gated", "linear8", "head"])
@@ -573,6 +573,153 @@ def test_second_order_is_refused():
               losses.linear_cross_entropy(args[0], args[1], args[2], target)):
         with pytest.raises(RuntimeError, match="create_graph"):
             torch.autograd.grad(y.sum(), args[0], create_graph=True)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap in time have workspaces of their own."""
+    sets = [make_gated(500, 64, 56, 64, torch.bfloat16, seed=s) for s in (11, 12)]
+    targets = [torch.randint(0, 64, (500,), device="cuda") for _ in sets]
+    want = [[t.detach().clone() for t in step(a, dy, t)] for (a, dy), t in zip(sets, targets)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(20):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = step(*sets[k], targets[k])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for g, w in zip(a, b):
+            assert torch.equal(g, w)
+
+
+def test_frozen_parameters():
+    gen = torch.Generator("cuda").manual_seed(2)
+    x = torch.randn((70, 48), generator=gen, device="cuda").requires_grad_()
+    w, b = torch.randn((24, 48), generator=gen, device="cuda"), torch.randn((24,), generator=gen, device="cuda")
+    target = torch.randint(0, 24, (70,), device="cuda")
+    dy = torch.randn((70, 24), generator=gen, device="cuda")
+    dx, = torch.autograd.grad(checkpoint8.linear8(x, w, b), x, dy)
+    near(dx, dy.double() @ w.double(), "dx alone")
+    dx, = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target), x)
+    ref = x.detach().double().requires_grad_()
+    near(dx, torch.autograd.grad(F.cross_entropy(F.linear(ref, w.double(), b.double()), target), ref)[0], "dx of the loss")
+    bias = b.clone().requires_grad_()
+    db, = torch.autograd.grad(checkpoint8.linear8(x.detach(), w, bias), bias, dy)
+    near(db, dy.double().sum(0), "db alone")
+    db, = torch.autograd.grad(losses.linear_cross_entropy(x.detach(), w, bias, target), bias)
+    ref = b.double().requires_grad_()
+    near(db, torch.autograd.grad(F.cross_entropy(F.linear(x.detach().double(), w.double(), ref), target), ref)[0], "db of the loss")
+
+
+def test_recomputed_and_hooked():
+    """Under torch.utils.checkpoint, with hooks on what is saved, and in inference mode."""
+    args, dy = make_gated(60, 40, 48, 40, torch.float32)
+    target = torch.randint(0, 40, (60,), device="cuda")
+
+    w = torch.randn(40, 40, device="cuda", requires_grad=True)
+
+    def f(*a):
+        return losses.linear_cross_entropy(checkpoint8.act8(feedforward.gated_mlp(*a, checkpoint8=True)), w, None, target)
+
+    want = torch.autograd.grad(f(*args), args)
+    got = torch.autograd.grad(torch.utils.checkpoint.checkpoint(f, *args, use_reentrant=False), args)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.save_on_cpu():
+        y = f(*args)
+    for a, b in zip(torch.autograd.grad(y, args), want):
+        assert torch.equal(a, b)
+    with torch.inference_mode():
+        assert torch.equal(f(*[t.detach() for t in args]), y.detach())
+
+
+def test_fp32_keeps_small_rows():
+    """fp32 products are exact to fp32 for every row by itself: rows and columns of very different magnitudes."""
+    gen = torch.Generator("cuda").manual_seed(4)
+    scale = torch.logspace(-18, 12, 200, device="cuda")
+    x = (torch.randn((200, 96), generator=gen, device="cuda") * scale[:, None]).requires_grad_()
+    w = (torch.randn((64, 96), generator=gen, device="cuda") * torch.logspace(-6, 6, 64, device="cuda")[:, None]).requires_grad_()
+    y = checkpoint8.linear8(x, w)
+    ref = x.double() @ w.double().t()
+    size = x.double().abs() @ w.double().abs().t()
+    # (sums of 96 terms: n 2^-24 of their magnitudes, and 4 2^-24 that the products of planes leave out)
+    assert ((y.double() - ref).abs() <= 100 * 2.0 ** -24 * size).all()
+    dy = torch.randn((200, 64), generator=gen, device="cuda") * torch.logspace(10, -10, 200, device="cuda")[:, None]
+    dx, = torch.autograd.grad(y, x, dy)
+    assert ((dx.double() - dy.double() @ w.double()).abs() <= 70 * 2.0 ** -24 * (dy.double().abs() @ w.double().abs())).all()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values, and more than 2^32 bytes: the last rows, against themselves in a small call."""
+    C, rows = 1024, (1 << 21) + 5
+    x = torch.empty(rows, C, device="cuda", dtype=torch.bfloat16)
+    x.view(-1, 1 << 10)[:] = torch.randn(1 << 10, device="cuda").bfloat16()
+    tail = torch.randn(37, C, device="cuda").bfloat16()
+    x[-37:] = tail
+    p, q = checkpoint8.pack8(x), checkpoint8.pack8(tail)
+    assert torch.equal(p.codes[-37:], q.codes) and torch.equal(p.exponents[-37:], q.exponents)
+    assert torch.equal(checkpoint8.unpack8(p)[-37:], checkpoint8.unpack8(q))
+    del p
+    w = (torch.randn(16, C, device="cuda") / 32).bfloat16()
+    with torch.no_grad():
+        near(checkpoint8.linear8(x, w)[-37:], tail.double() @ w.double().t(), "y")
+        target = torch.randint(0, 16, (rows,), device="cuda")
+        loss = losses.linear_cross_entropy(x, w, None, target, reduction="none")
+        want = F.cross_entropy(tail.double() @ w.double().t(), target[-37:], reduction="none")
+        assert ((loss[-37:].double() - want).abs() <= 4e-6 * (want.abs() + 12)).all()
+    # the sum over all rows: only the last ones have a gradient
+    wg = w.clone().requires_grad_()
+    xg = x.requires_grad_()
+    y = checkpoint8.linear8(xg, wg)
+    dy = torch.zeros_like(y)
+    dy[-37:] = torch.randn(37, 16, device="cuda").bfloat16()
+    dx, dw = torch.autograd.grad(y, [xg, wg], dy)
+    near(dw, dy[-37:].double().t() @ held8(tail), "dw")
+    near(dx[-37:], dy[-37:].double() @ w.double(), "dx")
+    assert not dx[:64].any() and not dx[rows // 2:rows // 2 + 64].any()
+    del x, xg, y, dx, dy
+    # many classes: the last piece of the backward pass
+    V = (1 << 21) + 7
+    x = torch.randn(3, C, device="cuda").bfloat16().requires_grad_()
+    w = torch.zeros(V, C, device="cuda", dtype=torch.bfloat16)
+    w[-5:] = torch.randn(5, C, device="cuda").bfloat16() / 4
+    w.requires_grad_()
+    target = torch.tensor([V - 1, 0, V - 4], device="cuda")
+    loss = losses.linear_cross_entropy(x, w, None, target, reduction="none")
+    logits = x.double() @ w[-5:].double().t()
+    lse = torch.logsumexp(torch.cat([logits, torch.full((3, 1), math.log(V - 5), dtype=torch.float64, device="cuda")], 1), 1)
+    want = lse - torch.stack([logits[0, 4], torch.zeros_like(lse[0]), logits[2, 1]])
+    assert ((loss.double() - want).abs() <= 4e-6 * (want.abs() + 12)).all()
+    dx, dw = torch.autograd.grad(loss.sum(), [x, w])
+    g = torch.exp(logits - lse[:, None])
+    g[0, 4] -= 1
+    g[2, 1] -= 1
+    near(dw[-5:], g.t() @ x.double(), "dw")
+    near(dx, g @ w[-5:].double(), "dx")
+
+
+SIZES = [(r, c, n) for r in (1, 31, 33, 63, 65, 127, 129, 255, 257, 511) for c, n in ((8, 248), (56, 257), (264, 63), (520, 130))]
+
+
+@pytest.mark.parametrize("rows,C,N", SIZES, ids=str)
+def test_sizes_around_tiles(rows, C, N):
+    """Sizes next to those of tiles and stages, in all types."""
+    for dtype in DTYPES:
+        gen = torch.Generator("cuda").manual_seed(rows + C + N)
+        x = torch.randn((rows, C), generator=gen, device="cuda").to(dtype).requires_grad_()
+        w = (torch.randn((2 * N, C), generator=gen, device="cuda") * C ** -0.5).to(dtype).requires_grad_()
+        v = (torch.randn((C, N), generator=gen, device="cuda") * N ** -0.5).to(dtype).requires_grad_()
+        dy = torch.randn((rows, C), generator=gen, device="cuda").to(dtype)
+        y = feedforward.gated_mlp(x, w, None, v, None, activation="silu")
+        got = torch.autograd.grad(y, [x, w, v], dy)
+        ref = leaves64(x, w, v)
+        out = gated64(ref[0], ref[1], None, ref[2], None, "silu")
+        near(y, out, "y %s" % dtype)
+        # (a row by itself has no sum that its operand's rounding disappears in: 2 r of each value; the norm's limit is 2 r as well)
+        for g, t, name in zip(got, torch.autograd.grad(out, ref, dy.double()), ["dx", "dw_in", "dw_out"]):
+            near(g, t, "%s %s" % (name, dtype), rounded=t.detach().abs())
 
 
 # ---------------------------------------------------------------------------------------------------- in the networks

@@ -1,0 +1,133 @@
+"""The operators around wide layers without a GPU: status codes of the C entry points before any GPU work, workspace sizes, and what the
+Python entry points refuse."""
+import ctypes
+
+import pytest
+import torch
+
+from oriented1d_amd import _lib, checkpoint8, feedforward, losses
+from oriented1d_amd.convnext1d import Block, ConvNeXt1D, gated_hidden
+
+ONE = ctypes.c_void_p(256)  # never dereferenced: validation fails first
+ODD = ctypes.c_void_p(264)
+F32, BF16, F16 = 0, 1, 2
+
+
+def lib():
+    return _lib.load()
+
+
+def test_workspace_sizes():
+    L = lib()
+    for dtype in (F32, BF16, F16):
+        for rows, C, H, D in [(1, 1, 1, 1), (49, 96, 256, 96), (16384, 1024, 4096, 1024), (1 << 30, 8, 8, 8)]:
+            for backward in (0, 1):
+                for held in (0, 1):
+                    assert L.dwo_gated_workspace_bytes(rows, C, H, D, backward, held, dtype) > 0
+                assert L.dwo_layer8_workspace_bytes(rows, C, D, backward, dtype) > 0
+        for rows, C, V in [(1, 1, 1), (64, 768, 1000), (8192, 1024, 65536), (1 << 30, 8, 8), (1, 8, 1 << 24)]:
+            assert all(L.dwo_head_workspace_bytes(rows, C, V, b, dtype) > 0 for b in (0, 1))
+    # a backward pass holds the logits' gradients in pieces of the classes, about 2^27 values each
+    piece = L.dwo_head_workspace_bytes(8192, 1024, 1 << 18, 1, BF16)
+    assert piece < 3 * (1 << 28) + 8192 * 1024 * 4 + (1 << 28)
+    for bad in [(0, 8, 8, 8), (1, 0, 8, 8), (1, 8, 0, 8), (1, 8, 8, 0), ((1 << 30) + 1, 8, 8, 8), (1, 65537, 8, 8), (1, 8, 65537, 8)]:
+        assert L.dwo_gated_workspace_bytes(*bad, 0, 0, BF16) == 0
+    assert L.dwo_gated_workspace_bytes(1, 8, 8, 8, 0, 0, 3) == 0
+    assert L.dwo_head_workspace_bytes(1, 8, (1 << 24) + 1, 0, BF16) == 0 and L.dwo_head_workspace_bytes(1, 8, 0, 0, BF16) == 0
+    assert L.dwo_layer8_workspace_bytes(1, 8, 65537, 0, BF16) == 0
+
+
+def test_status_codes():
+    L = lib()
+
+    def gated(x=ONE, w=ONE, y=ONE, keep=None, ws=ONE, need=1 << 40, rows=4, C=8, H=8, D=8, act=0, dtype=BF16):
+        return L.dwo_gated_forward(x, w, None, ONE, None, y, keep, ws, need, rows, C, H, D, act, dtype, None)
+
+    assert gated(x=None) == -1 and gated(y=None) == -1 and gated(ws=None) == -1
+    assert gated(rows=0) == -2 and gated(C=0) == -2 and gated(act=2) == -2 and gated(act=-1) == -2 and gated(x=ODD) == -2
+    assert gated(dtype=3) == -5 and gated(need=1) == -7
+
+    def gated_back(x=ONE, codes=None, exps=None, keep=ONE, dx=ONE, dwi=ONE, dbi=ONE, need=1 << 40, grad=F32):
+        return L.dwo_gated_backward(ONE, x, codes, exps, keep, ONE, None, ONE, dx, dwi, dbi, None, None, ONE, need, 4, 8, 8, 8, 0, BF16,
+                                    grad, None)
+
+    assert gated_back(x=None) == -1 and gated_back(keep=None) == -1
+    assert gated_back(codes=ONE, exps=ONE) == -1  # a checkpoint goes without keep
+    assert gated_back(codes=ONE, keep=None) == -1
+    assert gated_back(dwi=None) == -2  # a bias gradient without its weight's
+    assert gated_back(grad=4) == -5 and gated_back(need=1) == -7
+
+    def head(x=ONE, targets=ONE, smoothing=0.0, need=1 << 40, V=10, dtype=BF16):
+        return L.dwo_head_forward(x, ONE, None, targets, -100, smoothing, ONE, ONE, ONE, ONE, need, 4, 8, V, dtype, None)
+
+    assert head(x=None) == -1 and head(targets=None) == -1
+    assert head(V=0) == -2 and head(smoothing=1.5) == -2 and head(smoothing=float("nan")) == -2 and head(targets=ctypes.c_void_p(260)) == -2
+    assert head(dtype=7) == -5 and head(need=1) == -7
+    assert L.dwo_head_backward(ONE, ONE, ONE, None, ONE, -100, 0.0, ONE, None, ONE, None, ONE, ONE, 1 << 40, 4, 8, 10, BF16, F32, None) == -2
+    assert L.dwo_head_backward(None, ONE, ONE, None, ONE, -100, 0.0, ONE, None, ONE, ONE, ONE, ONE, 1 << 40, 4, 8, 10, BF16, F32, None) == -1
+
+    assert L.dwo_pack8(None, None, ONE, ONE, 4, 8, 0, BF16, None) == -1
+    assert L.dwo_pack8(ONE, None, ONE, ONE, 0, 8, 0, BF16, None) == -2 and L.dwo_pack8(ONE, None, ONE, ONE, 4, 8, 2, BF16, None) == -2
+    assert L.dwo_pack8(ONE, None, ONE, ONE, 4, 8, 0, 9, None) == -5
+    assert L.dwo_unpack8(ONE, None, None, ONE, 4, 8, 0, BF16, None) == -1 and L.dwo_unpack8(ODD, ONE, None, ONE, 4, 8, 0, BF16, None) == -2
+    assert L.dwo_layer8(ONE, ONE, None, ONE, ONE, None, ONE, 1 << 40, 4, 8, 8, BF16, None) == -1  # codes without exponents
+    assert L.dwo_layer8(ONE, ONE, None, ONE, None, None, ONE, 1, 4, 8, 8, BF16, None) == -7
+    assert L.dwo_layer8_backward(ONE, ONE, ONE, ONE, ONE, None, ONE, ONE, 1 << 40, 4, 8, 8, BF16, F32, None) == -2
+
+
+def test_python_refusals():
+    x, w, b, w_out = torch.randn(4, 8), torch.randn(16, 8), torch.randn(16), torch.randn(8, 8)
+    target = torch.zeros(4, dtype=torch.long)
+    for call in (lambda: feedforward.gated_mlp(x, w, b, torch.randn(8, 8), None), lambda: checkpoint8.linear8(x, w, b),
+                 lambda: checkpoint8.act8(x), lambda: checkpoint8.pack8(x), lambda: losses.linear_cross_entropy(x, w, b, target)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
+    with pytest.raises(ValueError, match="activation"):
+        feedforward.gated_mlp(x, w, b, torch.randn(8, 8), None, activation="relu")
+    with pytest.raises(ValueError, match="activation"):
+        checkpoint8.act8(x, "tanh")
+    with pytest.raises(ValueError, match="activation"):
+        feedforward.GatedMLP(8, 16, activation="relu")
+    with pytest.raises(ValueError, match="at least 1"):
+        feedforward.GatedMLP(8, 0)
+    with pytest.raises(ValueError, match="reduction"):
+        losses.linear_cross_entropy(x, w, b, target, reduction="sum")
+    for value in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="label_smoothing"):
+            losses.linear_cross_entropy(x, w, b, target, label_smoothing=value)
+    for call in (lambda: torch.func.vmap(lambda v: checkpoint8.linear8(v, w, b))(x[None]),
+                 lambda: torch.func.vmap(lambda v: feedforward.gated_mlp(v, w, b, w_out, None, checkpoint8=True))(x[None])):
+        with pytest.raises(RuntimeError, match="ordinary tensors"):
+            call()
+
+
+def test_transforms_compose_the_same_values():
+    x, w, b, v = torch.randn(3, 4, 8), torch.randn(16, 8), torch.randn(16), torch.randn(5, 8)
+    gate, up = torch.nn.functional.linear(x, w, b).chunk(2, -1)
+    want = torch.nn.functional.linear(torch.nn.functional.silu(gate) * up, v)
+    got = torch.func.vmap(lambda a: feedforward.gated_mlp(a, w, b, v, None, activation="silu"))(x)
+    assert torch.allclose(got, want, atol=1e-5)
+    target = torch.tensor([[0, 3, -100, 15]] * 3)
+    want = torch.nn.functional.cross_entropy(torch.nn.functional.linear(x, w, b).flatten(0, 1), target.flatten(), reduction="none")
+    got = torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, b, t, reduction="none"))(x, target)
+    assert torch.allclose(got.flatten(), want, atol=1e-5)
+
+
+def test_networks_with_gated_blocks():
+    assert [gated_hidden(d) for d in (96, 128, 192, 768, 1)] == [256, 344, 512, 2048, 8]
+    block = Block(96, (31,), False, mlp="gated")
+    assert block.mlp.w_in.shape == (512, 96) and block.mlp.w_out.shape == (96, 256)
+    names = dict(block.named_parameters())
+    assert "mlp.w_in" in names and not any(n.startswith("pwconv") for n in names)
+    plain = dict(Block(96, (31,), False).named_parameters())
+    assert not any(n.startswith("mlp") for n in plain) and "pwconv1.weight" in plain
+    # as many weights as the two pointwise layers
+    assert abs(sum(names[n].numel() for n in names if n.startswith("mlp.w")) / (8 * 96 * 96) - 1) < 0.01
+    with pytest.raises(ValueError, match="gated"):
+        Block(96, (15, 31), True, mlp="gated")
+    with pytest.raises(ValueError, match="mlp"):
+        Block(96, (31,), False, mlp="glu")
+    net = ConvNeXt1D(depths=(1, 1, 1, 1), dims=(16, 24, 32, 40), mlp="gated", checkpoint8=True)
+    assert all(stage[0].mlp.checkpoint8 for stage in net.stages)
+    with pytest.raises(ValueError, match="classes"):
+        ConvNeXt1D(depths=(1, 1, 1, 1), dims=(16, 24, 32, 40), out_stages=True).loss(torch.zeros(1, 3, 32, 32), torch.zeros(1))
