@@ -136,9 +136,55 @@ struct PlainChoice {
 };
 static long splits_for(long steps, long most) { return (steps + most - 1) / most; }
 
-// The least time of the products behind each other on all CUs, but no less than that of the longest sum; with splits of the sums also
-// their writing and reading (4 TB/s behind each other) and the launch that joins them.
-static PlainChoice plain_choice(const GroupPart *part, int count) {
+// When the last of the workgroups ends that go to 256 CUs one after the other, each to the CU that is free first, longest first:
+// `count` kinds of them, numbers[i] of times[i]
+static float makespan(const long *numbers, const float *times, int count) {
+    struct Span {
+        float end;
+        long cus;
+    } spans[16] = {{0.f, kLinCus}};
+    int used = 1, order[3] = {0, 1, 2};
+    for (int i = 1; i < count; i++)
+        for (int k = i; k > 0 && times[order[k]] > times[order[k - 1]]; k--) std::swap(order[k], order[k - 1]);
+    for (int i = 0; i < count; i++) {
+        long n = numbers[order[i]];
+        const float time = times[order[i]];
+        // (of many only the last rounds are dealt out)
+        if (n > 8 * kLinCus) {
+            const long whole = n / kLinCus - 6;
+            for (int k = 0; k < used; k++) spans[k].end += (float)whole * time;
+            n -= whole * kLinCus;
+        }
+        while (n > 0) {
+            int at = 0;
+            for (int k = 1; k < used; k++)
+                if (spans[k].end < spans[at].end) at = k;
+            const long take = n < spans[at].cus ? n : spans[at].cus;
+            const float end = spans[at].end + time;
+            int same = 0;
+            while (same < used && (same == at || spans[same].end != end)) same++;
+            if (same == used && take == spans[at].cus) {
+                spans[at].end = end;
+            } else {
+                if (same == used) {
+                    if (used == 16) return end;
+                    spans[used++] = {end, 0};
+                }
+                spans[same].cus += take, spans[at].cus -= take;
+                if (spans[at].cus == 0) spans[at] = spans[--used];
+            }
+            n -= take;
+        }
+    }
+    float last = 0.f;
+    for (int k = 0; k < used; k++) last = spans[k].end > last ? spans[k].end : last;
+    return last;
+}
+
+// The least of the products' time by tile_time's numbers, with splits of the sums also their writing and reading (4 TB/s behind each
+// other) and the launch that joins them.  8192 x 1024 from 16384 and 16384 x 1024 from 8192, bf16: both in tiles of 256 without splits 430 us,
+// the first one split in two, as it would be by itself, 470 and 33 for the join.
+static PlainChoice find_choice(const GroupPart *part, int count) {
     PlainChoice best{0, 0};
     float least = 0.f;
     long longest = 0;
@@ -147,25 +193,46 @@ static PlainChoice plain_choice(const GroupPart *part, int count) {
         for (const long parts : {1L, 2L, 3L, 4L, 6L, 8L, 12L, 16L, 24L, 32L}) {
             const long most = (longest + parts - 1) / parts;
             if (parts > 1 && most < 4) break;
-            float shared = 0.f, join = 0.f;
-            long workgroups = 0, chain = 0;
+            float join = 0.f, times[3];
+            long workgroups = 0, chain = 0, numbers[3];
             for (int i = 0; i < count; i++) {
                 const Product &p = part[i].p;
                 const long splits = splits_for(p.steps, most), steps = (p.steps + splits - 1) / splits;
-                const long n = tiles_of(p.M, p.N, c.size, c.size) * splits;
-                workgroups += n, shared += (float)n * (c.more + (float)steps * c.more_step);
+                numbers[i] = tiles_of(p.M, p.N, c.size, c.size) * splits, times[i] = c.more + (float)steps * c.more_step;
+                workgroups += numbers[i];
                 chain = steps > chain ? steps : chain;
                 if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 5.f : 0.f);
             }
             if (parts > 1 && workgroups > 4 * kLinCus) break;
-            // (a last round that is not full takes as long as one that is)
-            const float rounds = (float)((workgroups + kLinCus - 1) / kLinCus), mean = shared / (float)workgroups;
             const float alone = c.first + (float)chain * c.first_step;
-            const float t = (workgroups <= kLinCus ? alone : fmaxf(alone, 3.5f + rounds * mean)) + join;
+            const float t = join + (workgroups <= kLinCus ? alone : fmaxf(alone, 3.5f + makespan(numbers, times, count)));
             if (best.tile == 0 || t < least) best = {c.size, most}, least = t;
         }
     }
     return best;
+}
+// (a call asks three times for the same sizes, measuring its workspace and launching, and the next one often does: 64 answers are kept per
+// thread, by all that they follow from)
+static PlainChoice plain_choice(const GroupPart *part, int count) {
+    struct Known {
+        long key[9];
+        PlainChoice choice;
+    };
+    static thread_local Known known[64] = {};
+    long key[9] = {};
+    size_t hash = 0;
+    for (int i = 0; i < count; i++) {
+        key[3 * i] = part[i].p.M, key[3 * i + 1] = part[i].p.N, key[3 * i + 2] = part[i].p.steps;
+        for (int k = 0; k < 3; k++) hash = (hash ^ (size_t)key[3 * i + k]) * 0x9e3779b97f4a7c15ull, hash ^= hash >> 29;
+    }
+    Known &slot = known[hash % 64];
+    bool same = slot.choice.tile != 0;
+    for (int k = 0; k < 9; k++) same = same && slot.key[k] == key[k];
+    if (!same) {
+        for (int k = 0; k < 9; k++) slot.key[k] = key[k];
+        slot.choice = find_choice(part, count);
+    }
+    return slot.choice;
 }
 
 static void split_part(GroupPart &q, const PlainChoice &choice, Arena &ws) {
