@@ -425,22 +425,23 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
     };
     // (quarters of eight fragments and not halves: sixteen registers less, which two transposing operands have not)
     constexpr int Q = MF == 8 ? 4 : MF > 1 ? 2 : 1, MH = MF / Q;
-    mma_s8 fa[2][MH], fb[2][NF];
+    mma_s8 fa[4][MH], fb[2][NF];  // (at most three of the four hold anything at one time)
     Fragments<BM, AS> part_a;
     Fragments<BN, BS> part_b;
     part_a.init(wm * MF * 16), part_b.init(wn * NF * 16);
-    // part t of a stage: q of Q of the rows and half kk; its A goes to fa[t % 2], its B to fb[kk] (with the first rows)
+    // part t of a stage: q of Q of the rows and half kk; its A goes to fa[t % 4], its B to fb[kk] (with the first rows)
     constexpr int G = MH * NF;  // products of a part
+    static_assert(Q > 1 || G == 1);  // (a part alone in its half reads over itself: behind its only product)
     auto multiply = [&](int t, int k) {
         const int kk = t / Q, q = t % Q, j = k / NF, i = k % NF;
-        acc[i][q * MH + j] = Mma<T>::run(fb[kk][i], fa[t % 2][j], acc[i][q * MH + j]);
+        acc[i][q * MH + j] = Mma<T>::run(fb[kk][i], fa[t % 4][j], acc[i][q * MH + j]);
     };
     auto reads = [&](int t) { return t % Q == 0 ? MH + NF : MH; };
     auto read = [&](const uint16_t *from, int t, int r) {
         const int kk = t / Q, q = t % Q;
         if (r < MH) {
             if (r == 0) part_a.start();
-            fa[t % 2][r] = part_a.read(from, q * MH + r, kk);
+            fa[t % 4][r] = part_a.read(from, q * MH + r, kk);
         } else {
             if (r == MH) part_b.start();
             fb[kk][r - MH] = part_b.read(from + BM * kProdK, r - MH, kk);
@@ -478,28 +479,28 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
         __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | n >> 4 << 14);
         asm volatile("s_barrier" ::: "memory");
     };
-    // What goes out between the products of a part, evenly: the reads of the next part, in the last one the loads too (behind each other
-    // they hold the products up: 8192 x 8192 x 8192 in bf16 877 us, so 860)
+    // What goes out between the products of a part, evenly: the reads of the part after the next, in the last two the loads too (8192 x 8192 x
+    // 8192 in bf16: 859 us, with the reads of the next part only 872; transposing operands 964, and 987)
     auto step = [&](auto i) {
         uint16_t *current = stage(i);
         const uint16_t *next = stage(std::integral_constant<int, decltype(i)::value + 1>{});
         add_sums(current);
 #pragma unroll
         for (int t = 0; t < 2 * Q; t++) {
-            const bool last = t + 1 == 2 * Q;
             // this wave's reads of the stage are done, and its part of the next one is there; so are the other waves' behind the barrier
-            if (last) wait(std::integral_constant<int, STAGES - 2>{});
-            const int after = last ? 0 : t + 1, n = reads(after);
+            if (t == 2 * Q - 2) wait(std::integral_constant<int, STAGES - 2>{});
+            const bool late = t >= 2 * Q - 2;
+            const int after = late ? t + 2 - 2 * Q : t + 2, n = reads(after), first = (t - (2 * Q - 2)) * G;
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int k = 0; k < G; k++) {
                 multiply(t, k);
 #pragma unroll
                 for (int r = 0; r < MH + NF; r++)
-                    if (r >= k * n / G && r < (k + 1) * n / G) read(last ? next : current, after, r);
+                    if (r >= k * n / G && r < (k + 1) * n / G) read(late ? next : current, after, r);
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (last && u >= k * U / G && u < (k + 1) * U / G) load(current, u);
+                    if (late && u >= (first + k) * U / (2 * G) && u < (first + k + 1) * U / (2 * G)) load(current, u);
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
@@ -510,12 +511,12 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
         fetch(lds.s0);
         wait(std::integral_constant<int, 0>{});
         fetch(lds.s1);
-        read_all(lds.s0, 0);
+        read_all(lds.s0, 0), read_all(lds.s0, 1);
         for (int s = 0; s < count; s += 2) step(std::integral_constant<int, 0>{}), step(std::integral_constant<int, 1>{});
     } else {
         stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return fetch(stage(i)), true; });
         wait(std::integral_constant<int, STAGES - 1>{});
-        read_all(lds.s0, 0);
+        read_all(lds.s0, 0), read_all(lds.s0, 1);
         int s = 0;
         while (stages_of(std::make_integer_sequence<int, STAGES>{}, [&](auto i) { return step(i), ++s < count; })) {}
     }
