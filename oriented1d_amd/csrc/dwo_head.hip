@@ -117,41 +117,62 @@ struct Classes {
 // place of class t among eight from n on, or one beyond them
 __device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
 
-// The parts of a row joined, sixteen threads a row and sixteen rows at a time; `block` receives a workgroup's sum of losses and number of
-// rows that count.  One workgroup with all rows (few of them) writes the mean itself.
-__global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict__ part, const float *__restrict__ sum,
-                                                        const float *__restrict__ at, Targets targets, float *__restrict__ lse,
-                                                        float *__restrict__ loss, float *__restrict__ mean, float *__restrict__ count,
-                                                        float2 *__restrict__ block, long M, int parts, float eps) {
-    __shared__ float most_of[16][17], sum_of[16][17], all_of[16][17];
-    __shared__ float2 rows[16];
-    const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
+// exp of what a logit is below another: the multiple's rounding is 2^-24 of the difference, which is at most the log of a part's width where
+// the part counts
+__device__ __forceinline__ float below(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
+
+// The parts of a row joined, K threads a row and R rows at a time; `block` receives a workgroup's sum of losses and number of rows that
+// count.  One workgroup with all rows (few of them) writes the mean itself.
+// A read of 8 bytes (12 with labels smoothed) a row and part, bound by its latency: four parts a thread are read before the first is joined
+// (8192 rows of 1024 parts, 67 MB: 15.3 us, one at a time 32.3).
+template <int R, int K>
+__global__ __launch_bounds__(R *K) void head_join_kernel(const float2 *__restrict__ part, const float *__restrict__ sum,
+                                                           const float *__restrict__ at, Targets targets, float *__restrict__ lse,
+                                                           float *__restrict__ loss, float *__restrict__ mean, float *__restrict__ count,
+                                                           float2 *__restrict__ block, long M, int parts, float eps) {
+    __shared__ float most_of[K][R + 1], sum_of[K][R + 1], all_of[K][R + 1];
+    __shared__ float2 rows[R];
+    const int r = threadIdx.x % R, k = threadIdx.x / R;
     double total = 0.0, number = 0.0;
-    for (long first = (long)blockIdx.x * 16; first < M; first += (long)gridDim.x * 16) {
+    for (long first = (long)blockIdx.x * R; first < M; first += (long)gridDim.x * R) {
         const long m = first + r;
         float most = -INFINITY, s = 0.f, all = 0.f;
+        const bool ends = k == 0 && m < M;  // (what the end reads, before the parts)
+        const int t = ends ? targets.of(m) : -1;
+        const float hit = ends ? at[m] : 0.f;  // (of rows that count)
         if (m < M)
-            for (int p = k; p < parts; p += 16) {
-                const float2 v = part[(size_t)p * M + m];
-                const float next = fmaxf(most, v.x), base = next == -INFINITY ? 0.f : next;
-                s = s * prod_exp(most - base) + v.y * prod_exp(v.x - base);
+            for (int p = k; p < parts; p += 4 * K) {
+                float2 v[4];
+                float next = most;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int q = p + K * u;
+                    v[u] = q < parts ? part[(size_t)q * M + m] : make_float2(-INFINITY, 0.f);
+                    if (sum != nullptr && q < parts) all += sum[(size_t)q * M + m];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) next = fmaxf(next, v[u].x);
+                const float base = next == -INFINITY ? 0.f : next;
+                s *= below(most - base);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s += v[u].y * below(v[u].x - base);
                 most = next;
-                if (sum != nullptr) all += sum[(size_t)p * M + m];
             }
         most_of[k][r] = most, sum_of[k][r] = s, all_of[k][r] = all;
         __syncthreads();
         if (k == 0) {
-            for (int i = 1; i < 16; i++) most = fmaxf(most, most_of[i][r]);
+#pragma unroll
+            for (int i = 1; i < K; i++) most = fmaxf(most, most_of[i][r]);
             const float base = most == -INFINITY ? 0.f : most;
             s = 0.f, all = 0.f;
-            for (int i = 0; i < 16; i++) s += sum_of[i][r] * prod_exp(most_of[i][r] - base), all += all_of[i][r];
+#pragma unroll
+            for (int i = 0; i < K; i++) s += sum_of[i][r] * below(most_of[i][r] - base), all += all_of[i][r];
             float value = 0.f, counts = 0.f;
             if (m < M) {
                 const float l = base + logf(s);
                 lse[m] = l;
-                const int t = targets.of(m);
                 if (t == -2) value = NAN;
-                else if (t >= 0) value = (l - at[m]) * (1.f - eps);
+                else if (t >= 0) value = (l - hit) * (1.f - eps);
                 if (t >= 0 && sum != nullptr) value += eps * (l - all / (float)targets.V);
                 counts = t != -1 ? 1.f : 0.f;
                 if (loss != nullptr) loss[m] = value;
@@ -160,7 +181,8 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2 *__restrict
         }
         __syncthreads();
         if (threadIdx.x == 0)
-            for (int i = 0; i < 16; i++) total += rows[i].x, number += rows[i].y;
+#pragma unroll 16
+            for (int i = 0; i < R; i++) total += rows[i].x, number += rows[i].y;
     }
     if (threadIdx.x != 0) return;
     if (block != nullptr) block[blockIdx.x] = make_float2((float)total, (float)number);
@@ -282,8 +304,11 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
     if (e) return e;
     const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
     const int width = wave_columns(tile_for(p.M, p.N, p.steps));
-    // Up to 128 rows one workgroup joins them all (64 x 1000 classes: 4.7 and 2.4 us as two launches)
-    const int parts = (int)((s.V + width - 1) / width), blocks = s.rows <= 128 ? 1 : (int)((s.rows + 15) / 16);
+    // Up to 128 rows one workgroup joins them all (64 x 1000 classes: 6.3 us, as two launches 4.7 and 2.4); with no more than sixteen parts four
+    // threads have a row (32768 x 150 classes: 8.3 us for both launches, sixteen 9.6; 64 rows of 63 parts need the sixteen)
+    const int parts = (int)((s.V + width - 1) / width);
+    const bool few = s.rows <= 128, narrow = !few && parts <= 16;
+    const int group = few || narrow ? 64 : 16, blocks = few ? 1 : (int)((s.rows + group - 1) / group);
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
     float *sum = eps > 0.f ? (float *)ws.take((size_t)parts * s.rows * sizeof(float)) : nullptr;
     float *at = (float *)ws.take((size_t)s.rows * sizeof(float));
@@ -291,8 +316,9 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
     if (ws.dry()) return 0;
     const StatsEpi epi{{b, s.dtype}, targets, part, sum, at};
     if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
-    head_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss,
-                                                                  mean ? loss : nullptr, count, block, s.rows, parts, eps);
+    auto *const join = few ? head_join_kernel<64, 16> : narrow ? head_join_kernel<64, 4> : head_join_kernel<16, 16>;
+    join<<<dim3((unsigned)blocks), dim3(few ? 1024 : 256), 0, st>>>(part, sum, at, targets, lse, mean ? nullptr : loss, mean ? loss : nullptr,
+                                                                    count, block, s.rows, parts, eps);
     if (block != nullptr) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
     return status();
 }
