@@ -700,14 +700,16 @@ inline Product make_product(const Operand &a, const Operand &b, long M, long N, 
     return p;
 }
 // Time of a product with square tiles of this size, us: workgroups that have a CU to themselves wait for memory step by step, others
-// share its units.  The numbers are fits to products of 1 to 16384 rows x 96 to 21841 columns, steps of 64 summed indices 1 to 342,
-// of which they are 10 to 15 % off.  First round: a launch with its first loads and last stores, and a step; then each round.
+// share its units.  The numbers are fits to 450 bf16 products of 64 to 25088 rows x 384 to 8192 columns x 64 to 16384 summed indices, operands
+// of every order, which they meet within 10 % (root of the mean square; 13 % the smallest tile); the tile that they choose is 0.2 % slower
+// than the fastest of the four in the geometric mean, 9 % at the most.  First round: a launch with its first loads and last stores, and a
+// step; then each round.
 struct TileCost {
     int size;
     float first, first_step, more, more_step;
 };
 constexpr TileCost kTileCosts[4] = {
-    {256, 13.f, 1.7f, 9.5f, 1.6f}, {128, 7.f, 0.62f, 3.f, 0.45f}, {64, 4.2f, 0.25f, 1.2f, 0.22f}, {32, 4.f, 0.14f, 1.2f, 0.09f}};
+    {256, 11.6f, 1.19f, 10.f, 1.41f}, {128, 6.7f, 0.54f, 2.65f, 0.44f}, {64, 4.2f, 0.275f, 1.25f, 0.195f}, {32, 4.f, 0.15f, 1.2f, 0.105f}};
 inline float tile_time(const TileCost &c, long workgroups, long steps) {
     if (workgroups <= kLinCus) return c.first + (float)steps * c.first_step;
     return 3.5f + (float)((workgroups + kLinCus - 1) / kLinCus) * (c.more + (float)steps * c.more_step);
