@@ -7,6 +7,11 @@
 // g and u are kept for the backward pass in fp32, eight bytes a hidden unit and row: what a composition of layers in 16 bits keeps as
 // four tensors, without their roundings (dx would be 1.8 times a rounding off instead of 1.4).  Or nothing but x in 8 bits is kept, and the
 // backward pass makes g and u again, into its workspace.  h, dg and du are rounded to the activations' type, as operands of the matrix cores.
+//
+// 16384 x 1024 -> 4096 -> 1024 in bf16: the gated product 380 us and the one behind dy 335, bound by what goes out and comes in behind their
+// sums (678 MB written; 537 MB read, 405 written: with the products' own reads 2.9 and 3.6 TB/s, matrix cores busy 29 and 15 %); the second
+// product 135 (1018 TFLOP/s) and the group of the three gradients 680 (1010).  Tiles of 128, two workgroups a CU of which one writes while the
+// other multiplies, take 474 and 341.  One row: 9.0 and 4.7 us, and 4.1 for the join, 25 MB of weights at 1.4 TB/s.
 #include "dwo_act.h"
 #include "dwo_check8.h"
 
