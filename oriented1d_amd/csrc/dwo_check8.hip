@@ -3,7 +3,7 @@
 // passes run at a large copy's rate and at the issue slots' at once: there 36 us (194 MB, 5.3 TB/s; 92 % of the slots), back 33 us (5.9 TB/s;
 // 82 %).  A layer of 25088 x 384 -> 1536 packs its input in 7 us and stages it again in 9, of 150 both ways.
 #include "dwo_check8.h"
-#include "dwo_act.h"
+#include "dwo_few.h"
 
 namespace dwo {
 
@@ -161,6 +161,8 @@ static bool sizes_ok(long rows, int C, const void *a, const void *b, const void 
 
 static int layer_forward(const void *x, const void *w, const void *b, void *y, long rows, int C, int D, int dtype, Arena &ws,
                          hipStream_t st) {
+    if (few(rows, C, dtype))
+        return ws.dry() ? 0 : launch_few(x, w, C, D, 0, rows, dtype, FewPlain{{b, dtype}, {y, D, 0, dtype}}, st);
     Staging stage;
     const Operand ox = stage.matrix(x, rows, C, dtype, ws), ow = stage.matrix(w, D, C, dtype, ws);
     const int e = stage.launch(ws.dry(), st);

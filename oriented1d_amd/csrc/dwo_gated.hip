@@ -11,9 +11,9 @@
 // 16384 x 1024 -> 4096 -> 1024 in bf16: the gated product 380 us and the one behind dy 335, bound by what goes out and comes in behind their
 // sums (678 MB written; 537 MB read, 405 written: with the products' own reads 2.9 and 3.6 TB/s, matrix cores busy 29 and 15 %); the second
 // product 135 (1018 TFLOP/s) and the group of the three gradients 680 (1010).  Tiles of 128, two workgroups a CU of which one writes while the
-// other multiplies, take 474 and 341.  One row: 9.0 and 4.7 us, and 4.1 for the join, 25 MB of weights at 1.4 TB/s.
-#include "dwo_act.h"
+// other multiplies, take 474 and 341.  One row (dwo_few.h): 7.0 us, 25 MB of weights at 3.6 TB/s.
 #include "dwo_check8.h"
+#include "dwo_few.h"
 
 namespace dwo {
 
@@ -113,6 +113,13 @@ static int gated_hidden(const GatedSizes &s, const Operand &x, const Operand &w,
 
 static int gated_forward(const GatedSizes &s, const void *x, const void *w_in, const void *b_in, const void *w_out, const void *b_out,
                          void *y, float *keep, int act, Arena &ws, hipStream_t st) {
+    if (few(s.rows, s.C, s.dtype) && few(s.rows, s.H, s.dtype)) {
+        void *const h = ws.take((size_t)s.rows * s.H * size_of(s.dtype));
+        if (ws.dry()) return 0;
+        const FewGlu glu{{b_in, s.dtype}, s.rows, s.H, s.Hp, act, keep, {h, s.H, 0, s.dtype}};
+        const int e = launch_few(x, w_in, s.C, s.H, s.H, s.rows, s.dtype, glu, st);
+        return e != 0 ? e : launch_few(h, w_out, s.H, s.D, 0, s.rows, s.dtype, FewPlain{{b_out, s.dtype}, {y, s.D, 0, s.dtype}}, st);
+    }
     Staging stage;
     const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), oi = stage.matrix(w_in, 2 * s.H, s.C, s.dtype, ws),
                   oo = stage.matrix(w_out, s.D, s.H, s.dtype, ws);

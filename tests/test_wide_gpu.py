@@ -129,6 +129,42 @@ def test_gated_mlp_without_gradients_and_single_rows():
         near(y, gated64(*leaves64(*args), "gelu"), "y")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9])
+@pytest.mark.parametrize("C,H,D", [(8, 8, 1), (24, 12, 7), (520, 264, 61), (1032, 2056, 96), (4104, 16, 4099)], ids=str)
+def test_few_rows(C, H, D, rows, dtype):
+    """Columns that waves share, or not, whole and partial pieces of a sum, kept halves with padding, and the layer alone."""
+    args, dy = make_gated(rows, C, H, D, dtype, bias=rows % 2 == 1)
+    y = feedforward.gated_mlp(*args, activation="silu")
+    leaves = [t for t in args if t is not None]
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = leaves64(*args)
+    out = gated64(*ref, "silu")
+    near(y, out, "y")
+    for g, w in zip(got, torch.autograd.grad(out, [t for t in ref if t is not None], dy.double())):
+        near(g, w, "gradient")
+    with torch.no_grad():
+        assert torch.equal(feedforward.gated_mlp(*args, activation="silu"), y)
+        near(checkpoint8.linear8(args[0], args[1], args[2]), F.linear(*ref[:3]), "layer")
+
+
+def test_few_rows_of_all_kinds_of_numbers():
+    # a row that is not finite leaves the others as they are
+    w = torch.randn(70, 520, device="cuda")
+    for dtype in DTYPES:
+        x = torch.randn(4, 520, device="cuda").to(dtype)
+        clean = checkpoint8.linear8(x, w.to(dtype))
+        x[1, 3], x[2, 519] = float("nan"), float("inf")
+        y = checkpoint8.linear8(x, w.to(dtype))
+        assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+        assert y[1].isnan().all() and not y[2].isfinite().any()
+    # fp16 below its smallest normal number: multiples of 2^-24 times 512, every product and sum of which is a multiple of 2^-15 below 2^9
+    q = torch.randint(-1023, 1024, (40, 64), device="cuda")
+    x = torch.full((3, 64), 512.0, device="cuda", dtype=torch.float16)
+    y = checkpoint8.linear8(x, (q.double() * 2.0 ** -24).half())
+    assert torch.equal(y, (q.double().sum(1) * 2.0 ** -15).half().expand(3, 40))
+
+
 def test_gated_gradients_of_some_inputs():
     args, dy = make_gated(37, 40, 48, 24, torch.float32)
     ref = leaves64(*args)
