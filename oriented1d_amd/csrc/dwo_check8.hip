@@ -162,7 +162,7 @@ static bool sizes_ok(long rows, int C, const void *a, const void *b, const void 
 static int layer_forward(const void *x, const void *w, const void *b, void *y, long rows, int C, int D, int dtype, Arena &ws,
                          hipStream_t st) {
     if (few(rows, C, dtype))
-        return ws.dry() ? 0 : launch_few(x, w, C, D, 0, rows, dtype, FewPlain{{b, dtype}, {y, D, 0, dtype}}, st);
+        return ws.dry() ? 0 : launch_few<false>(x, w, C, D, 0, rows, dtype, FewPlain{{b, dtype}, {y, D, 0, dtype}}, st);
     Staging stage;
     const Operand ox = stage.matrix(x, rows, C, dtype, ws), ow = stage.matrix(w, D, C, dtype, ws);
     const int e = stage.launch(ws.dry(), st);

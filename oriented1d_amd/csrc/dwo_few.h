@@ -11,22 +11,28 @@ namespace dwo {
 
 constexpr int kFewWaves = 4096;  // sixteen a CU: their loads in flight keep its memory busy
 
-// sixteen bytes of a row times those of another: pairs of 16-bit values by the instruction that adds two products to a sum in fp32
-__device__ __forceinline__ float few_dot(const mma_u4 &a, const mma_u4 &b, float sum, float) {
+// sixteen bytes of a row of w times as many values of x: pairs of 16-bit values by the instruction that adds two products to a sum in fp32
+template <int N>
+struct FewPiece {
+    mma_u4 v[N];
+};
+template <typename T>
+__device__ __forceinline__ float few_dot(const mma_u4 &a, const FewPiece<sizeof(float) / sizeof(T)> &x, float sum, T, float) {
+    const T *w = reinterpret_cast<const T *>(&a);
 #pragma unroll
-    for (int e = 0; e < 4; e++) sum = __builtin_fmaf(__uint_as_float(a[e]), __uint_as_float(b[e]), sum);
+    for (int e = 0; e < 16 / (int)sizeof(T); e++) sum = __builtin_fmaf(to_float(w[e]), __uint_as_float(x.v[e / 4][e % 4]), sum);
     return sum;
 }
-__device__ __forceinline__ float few_dot(const mma_u4 &a, const mma_u4 &b, float sum, bf16_t) {
+__device__ __forceinline__ float few_dot(const mma_u4 &a, const FewPiece<1> &x, float sum, bf16_t, bf16_t) {
     typedef __bf16 two __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, (unsigned)a[e]), __builtin_bit_cast(two, (unsigned)b[e]), sum, false);
+    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, (unsigned)a[e]), __builtin_bit_cast(two, (unsigned)x.v[0][e]), sum, false);
     return sum;
 }
-__device__ __forceinline__ float few_dot(const mma_u4 &a, const mma_u4 &b, float sum, f16_t) {
+__device__ __forceinline__ float few_dot(const mma_u4 &a, const FewPiece<1> &x, float sum, f16_t, f16_t) {
     typedef _Float16 two __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(two, (unsigned)a[e]), __builtin_bit_cast(two, (unsigned)b[e]), sum, false);
+    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(two, (unsigned)a[e]), __builtin_bit_cast(two, (unsigned)x.v[0][e]), sum, false);
     return sum;
 }
 template <int CTRL>
@@ -60,18 +66,18 @@ struct FewGlu {
     long rows, H, Hp;
     int act;
     float *keep;  // g, then u, [rows][Hp] each; or null
-    Out h;
+    float *h;  // [rows][H]
     __device__ __forceinline__ void operator()(long m, long n, const float (&v)[2]) const {
         const float g = v[0] + (bias.p != nullptr ? bias.at(n) : 0.f), u = v[1] + (bias.p != nullptr ? bias.at(H + n) : 0.f);
         if (keep != nullptr) keep[m * Hp + n] = g, keep[(rows + m) * Hp + n] = u;
-        out_one(h, m, n, act_value(act, g) * u);
+        h[m * H + n] = act_value(act, g) * u;
     }
 };
 
 // along: waves that share a column, 1, 2 or 4.  K in whole pieces of sixteen bytes.  From three rows on a wave has two columns: a row's piece is read
 // for both.
-template <typename T, int R, class End>
-__global__ __launch_bounds__(256) void few_kernel(const T *__restrict__ x, const T *__restrict__ w, long K, long N, long gap, int rows,
+template <typename TX, typename T, int R, class End>
+__global__ __launch_bounds__(256) void few_kernel(const TX *__restrict__ x, const T *__restrict__ w, long K, long N, long gap, int rows,
                                                   int along, End end) {
     constexpr int V = 16 / (int)sizeof(T), COLS = End::kCols, U = R > 2 ? 2 : 1;
     __shared__ float part[4][COLS][U * R];
@@ -88,11 +94,11 @@ __global__ __launch_bounds__(256) void few_kernel(const T *__restrict__ x, const
                 a[u][c] = *reinterpret_cast<const mma_u4 *>(w + ((n0 + u < N ? n0 + u : N - 1) + c * gap) * K + k);
 #pragma unroll
         for (int m = 0; m < R; m++) {
-            const mma_u4 b = *reinterpret_cast<const mma_u4 *>(x + (m < rows ? m : rows - 1) * K + k);
+            const auto b = *reinterpret_cast<const FewPiece<sizeof(TX) / sizeof(T)> *>(x + (m < rows ? m : rows - 1) * K + k);
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int c = 0; c < COLS; c++) sum[u][c][m] = few_dot(a[u][c], b, sum[u][c][m], T{});
+                for (int c = 0; c < COLS; c++) sum[u][c][m] = few_dot(a[u][c], b, sum[u][c][m], T{}, TX{});
         }
     }
     float mine[COLS] = {};  // lane u R + m: of column u and row m
@@ -120,24 +126,25 @@ __global__ __launch_bounds__(256) void few_kernel(const T *__restrict__ x, const
     if (wave == first && lane < U * R && m < rows && n < N) end(m, n, mine);
 }
 
-template <typename T, class End>
+template <typename TX, typename T, class End>
 int launch_few_typed(const void *x, const void *w, long K, long N, long gap, int rows, const End &end, hipStream_t st) {
     const long piece = 64 * 16 / (long)sizeof(T), units = rows > 2 ? (N + 1) / 2 : N;
     int along = 1;
     while (along < 4 && units * along < kFewWaves && K >= 2 * along * piece) along *= 2;
     const dim3 grid((unsigned)((units * along + 3) / 4)), block(256);
-    auto *kernel = rows == 1 ? few_kernel<T, 1, End> : rows == 2 ? few_kernel<T, 2, End> : few_kernel<T, 4, End>;
+    auto *kernel = rows == 1 ? few_kernel<TX, T, 1, End> : rows == 2 ? few_kernel<TX, T, 2, End> : few_kernel<TX, T, 4, End>;
     if constexpr (sizeof(T) == 4)
-        if (rows > 4) kernel = few_kernel<T, 8, End>;
-    kernel<<<grid, block, 0, st>>>((const T *)x, (const T *)w, K, N, gap, rows, along, end);
+        if (rows > 4) kernel = few_kernel<TX, T, 8, End>;
+    kernel<<<grid, block, 0, st>>>((const TX *)x, (const T *)w, K, N, gap, rows, along, end);
     return status();
 }
-template <class End>
+// FLOAT: x in fp32 whatever w is
+template <bool FLOAT, class End>
 int launch_few(const void *x, const void *w, long K, long N, long gap, long rows, int dtype, const End &end, hipStream_t st) {
     switch (dtype) {
-        case DWO_F32: return launch_few_typed<float>(x, w, K, N, gap, (int)rows, end, st);
-        case DWO_BF16: return launch_few_typed<bf16_t>(x, w, K, N, gap, (int)rows, end, st);
-        default: return launch_few_typed<f16_t>(x, w, K, N, gap, (int)rows, end, st);
+        case DWO_F32: return launch_few_typed<float, float>(x, w, K, N, gap, (int)rows, end, st);
+        case DWO_BF16: return launch_few_typed<std::conditional_t<FLOAT, float, bf16_t>, bf16_t>(x, w, K, N, gap, (int)rows, end, st);
+        default: return launch_few_typed<std::conditional_t<FLOAT, float, f16_t>, f16_t>(x, w, K, N, gap, (int)rows, end, st);
     }
 }
 // Up to eight rows in fp32, whose tiles take three planes made by another launch (gated block 1024 -> 4096 -> 1024: 13 us for one row and 25 for

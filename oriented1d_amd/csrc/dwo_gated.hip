@@ -6,7 +6,8 @@
 //
 // g and u are kept for the backward pass in fp32, eight bytes a hidden unit and row: what a composition of layers in 16 bits keeps as
 // four tensors, without their roundings (dx would be 1.8 times a rounding off instead of 1.4).  Or nothing but x in 8 bits is kept, and the
-// backward pass makes g and u again, into its workspace.  h, dg and du are rounded to the activations' type, as operands of the matrix cores.
+// backward pass makes g and u again, into its workspace.  h, dg and du are rounded to the activations' type, as operands of the matrix cores,
+// or to two of them where the work is small (kHalvesWork).
 //
 // 16384 x 1024 -> 4096 -> 1024 in bf16: the gated product 380 us and the one behind dy 335, bound by what goes out and comes in behind their
 // sums (678 MB written; 537 MB read, 405 written: with the products' own reads 2.9 and 3.6 TB/s, matrix cores busy 29 and 15 %); the second
@@ -52,7 +53,7 @@ struct GluEpi {
         if (h.p == nullptr) return;
 #pragma unroll
         for (int e = 0; e < 8; e++) g[e] = act_value(act, g[e]) * u[e];
-        out_octet<false>(h, true, m, n, Hp, g);
+        operand_octet<false>(h, m, n, Hp, g);
     }
 };
 
@@ -89,9 +90,9 @@ struct DgluEpi {
             const float v = up[e / 4][e % 4];
             a[e] = real ? d[e] * v * slope : 0.f, b[e] = real ? d[e] * value : 0.f, o[e] = real ? value * v : 0.f;
         }
-        out_octet(dg, true, m, n, Hp, a);
-        out_octet(du, true, m, n, Hp, b);
-        out_octet(h, true, m, n, Hp, o);
+        operand_octet(dg, m, n, Hp, a);
+        operand_octet(du, m, n, Hp, b);
+        operand_octet(h, m, n, Hp, o);
     }
 };
 
@@ -99,6 +100,7 @@ struct GatedSizes {
     long rows, C, H, D, Hp;
     int dtype;
     GatedSizes(size_t r, int c, int h, int d, int t) : rows((long)r), C(c), H(h), D(d), Hp(up8(h)), dtype(t) {}
+    double work() const { return (double)rows * (double)H * (double)(2 * C + D); }
     bool ok() const {
         return rows >= 1 && rows <= 1L << 30 && C >= 1 && H >= 1 && D >= 1 && C <= 65536 && H <= 65536 && D <= 65536 && known(dtype);
     }
@@ -114,18 +116,18 @@ static int gated_hidden(const GatedSizes &s, const Operand &x, const Operand &w,
 static int gated_forward(const GatedSizes &s, const void *x, const void *w_in, const void *b_in, const void *w_out, const void *b_out,
                          void *y, float *keep, int act, Arena &ws, hipStream_t st) {
     if (few(s.rows, s.C, s.dtype) && few(s.rows, s.H, s.dtype)) {
-        void *const h = ws.take((size_t)s.rows * s.H * size_of(s.dtype));
+        float *const h = (float *)ws.take((size_t)s.rows * s.H * sizeof(float));  // (few values: not rounded)
         if (ws.dry()) return 0;
-        const FewGlu glu{{b_in, s.dtype}, s.rows, s.H, s.Hp, act, keep, {h, s.H, 0, s.dtype}};
-        const int e = launch_few(x, w_in, s.C, s.H, s.H, s.rows, s.dtype, glu, st);
-        return e != 0 ? e : launch_few(h, w_out, s.H, s.D, 0, s.rows, s.dtype, FewPlain{{b_out, s.dtype}, {y, s.D, 0, s.dtype}}, st);
+        const FewGlu glu{{b_in, s.dtype}, s.rows, s.H, s.Hp, act, keep, h};
+        const int e = launch_few<false>(x, w_in, s.C, s.H, s.H, s.rows, s.dtype, glu, st);
+        return e != 0 ? e : launch_few<true>(h, w_out, s.H, s.D, 0, s.rows, s.dtype, FewPlain{{b_out, s.dtype}, {y, s.D, 0, s.dtype}}, st);
     }
     Staging stage;
     const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), oi = stage.matrix(w_in, 2 * s.H, s.C, s.dtype, ws),
                   oo = stage.matrix(w_out, s.D, s.H, s.dtype, ws);
     int e = stage.launch(ws.dry(), st);
     if (e) return e;
-    const Operand h = take_operand(ws, s.rows, s.Hp, s.dtype);
+    const Operand h = take_operand(ws, s.rows, s.Hp, s.dtype, s.work());
     if (!ws.dry() && (e = gated_hidden(s, ox, oi, b_in, act, keep, out_of(h, s.dtype), st))) return e;
     PlainEpi epi = plain_epilogue({y, s.D, 0, s.dtype});
     epi.bias = {b_out, s.dtype};
@@ -158,7 +160,7 @@ static int gated_backward(const GatedSizes &s, const void *dy, const void *x, co
             return e;
         keep = again;
     }
-    const Operand da = take_operand(ws, s.rows, 2 * s.Hp, s.dtype), h = take_operand(ws, s.rows, s.Hp, s.dtype);
+    const Operand da = take_operand(ws, s.rows, 2 * s.Hp, s.dtype, s.work()), h = take_operand(ws, s.rows, s.Hp, s.dtype, s.work());
     if (!ws.dry()) {
         const Out dg = out_of(da, s.dtype);
         Out du = dg;

@@ -4,7 +4,7 @@
 //
 // Forward: one product over all classes whose epilogue leaves, for a row and a wave's classes, their largest logit and the sum of
 // exponentials below it; a second kernel joins them.  Backward, in pieces of the classes: the product again, its sums turned into G, which
-// alone goes through memory, rounded to the activations' type for the two products that read it.  Eight products of rows x
+// alone goes through memory, rounded to the activations' type (kHalvesWork: to two) for the two products that read it.  Eight products of rows x
 // classes x channels in place of the six of a pass that keeps its logits; what would be kept is two or more bytes a row and class.
 // Bound by the matrix cores: 8192 x 1024 x 65536 in bf16, statistics 1022 us (1075 TFLOP/s), G 4 x 310 (890; 268 MB of G each go out behind
 // the sums, which nothing covers), its two products 4 x 460 (1195).  In fp32, 1024 x 512 x 21841: 137, 176 and 323 us, products of six planes at
@@ -260,7 +260,7 @@ struct GradEpi {
         if (m >= p.M || n >= g.pitch) return;
         const int t = (int)rows[0];
         const float total = __uint_as_float(rows[1]), f = __uint_as_float(rows[2]);
-        if (g.type == OUT_PLANES) {
+        if (g.plane != 0) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = prod_exp(v[e] + l.bias[e] - total);
         } else {
@@ -283,7 +283,7 @@ struct GradEpi {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = t == -1 || n + e >= p.N ? 0.f : t == -2 ? NAN : v[e];
         }
-        out_octet(g, true, m, n, g.pitch, v);
+        operand_octet(g, m, n, g.pitch, v);
     }
 };
 
@@ -333,7 +333,7 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
     int e = stage.launch(ws.dry(), st);
     if (e) return e;
     const long piece = s.piece();
-    const Operand g = take_operand(ws, s.rows, up8(piece), s.dtype);
+    const Operand g = take_operand(ws, s.rows, up8(piece), s.dtype, (double)s.rows * (double)s.C * (double)s.V);
     // dx is summed over the pieces in fp32
     const bool many = piece < s.V;
     float *sum = many && dx != nullptr && s.dtype != DWO_F32 ? (float *)ws.take((size_t)s.rows * s.C * sizeof(float)) : (float *)dx;

@@ -18,7 +18,7 @@ namespace dwo {
 struct Operand {  // rows of `pitch` values (a multiple of eight), 16-byte aligned; `plane` values from one plane to the next
     const void *p;
     long pitch, plane;
-    int planes;  // 1 or 3
+    int planes;  // 1, 2 (halves of 16-bit operands made between products) or 3 (fp32)
 };
 struct Product {
     Operand a, b;
@@ -30,12 +30,12 @@ struct Product {
     int per, steps;  // steps of 64 per split, in all
 };
 
-// (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); where one operand has a single plane, the other's planes
+// (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); where one operand has a single plane, the other's planes (two halves meet single planes only)
 inline void product_pairs(Product &p) {
-    const bool a = p.a.planes == 3, b = p.b.planes == 3;
-    p.pairs = a && b ? 6 : a || b ? 3 : 1;
-    p.codes_a = a && b ? 0x052 : a ? 0x006 : 0;
-    p.codes_b = a && b ? 0x118 : b ? 0x006 : 0;
+    const int a = p.a.planes, b = p.b.planes;
+    p.pairs = a == 3 && b == 3 ? 6 : a > b ? a : b;
+    p.codes_a = a == 3 && b == 3 ? 0x052 : a == 3 ? 0x006 : a == 2 ? 0x001 : 0;
+    p.codes_b = a == 3 && b == 3 ? 0x118 : b == 3 ? 0x006 : b == 2 ? 0x001 : 0;
 }
 
 // ------------------------------------------------------------------------------------------------- stages in LDS
@@ -204,6 +204,19 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
         return;
     }
     store_out<STREAM>(to, mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])});
+}
+// eight neighbours of an operand's row; in two halves (o.plane of 16-bit values) the second is what the first one's rounding leaves
+template <bool STREAM = true>
+__device__ __forceinline__ void operand_octet(const Out &o, long m, long n, long N, const float (&v)[8]) {
+    out_octet<STREAM>(o, true, m, n, N, v);
+    if (o.type == OUT_PLANES || o.plane == 0) return;
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float h = o.type == OUT_F16 ? to_float(from_float<f16_t>(v[e])) : bf16_value(bits16(OUT_BF16, v[e]));
+        r[e] = (__float_as_uint(h) & 0x7f800000u) != 0x7f800000u ? v[e] - h : 0.f;
+    }
+    out_octet<STREAM>({reinterpret_cast<uint16_t *>(o.p) + o.plane, o.pitch, 0, o.type}, true, m, n, N, r);
 }
 
 // An epilogue E has
@@ -622,16 +635,22 @@ inline unsigned blocks_for(long work, long most = 4096) {
 inline size_t size_of(int dtype) { return dtype == DWO_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == DWO_F32 || dtype == DWO_BF16 || dtype == DWO_F16; }
 
+// Where an operator's forward pass has no more multiply-adds than this, the 16-bit operands that one of its products makes for another are held
+// in two halves, 16 bits more, and their rounding is in no result.  Where results are large it takes them from one rounding off to 1.41; of a few
+// values by up to twice, and there the second half costs little: forward and backward, bf16, in a graph, gated block 49 x 768 -> 2048 42 us, so 48,
+// 784 x 192 -> 512 32, 44, loss of 256 x 768 x 1000 29, 35 (from Python's calls, 75 to 100 us either way); at twice the limit 1000 x 256 -> 680 41, 57,
+// 32768 x 96 x 150 56, 74.
+constexpr double kHalvesWork = 1 << 28;
 // room for an operand of rows x pitch that a kernel writes
-inline Operand take_operand(Arena &ws, long rows, long pitch, int dtype) {
+inline Operand take_operand(Arena &ws, long rows, long pitch, int dtype, double work = 2 * kHalvesWork) {
     Operand o;
-    o.planes = dtype == DWO_F32 ? 3 : 1;
+    o.planes = dtype == DWO_F32 ? 3 : work <= kHalvesWork ? 2 : 1;
     o.pitch = pitch, o.plane = rows * pitch;
     o.p = ws.take((size_t)o.planes * o.plane * 2);
     return o;
 }
 inline Out out_of(const Operand &o, int dtype) {
-    return {const_cast<void *>(o.p), o.pitch, o.plane, dtype == DWO_F32 ? OUT_PLANES : dtype};
+    return {const_cast<void *>(o.p), o.pitch, o.planes > 1 ? o.plane : 0, dtype == DWO_F32 ? OUT_PLANES : dtype};
 }
 // Operands that are made before the products of a call, by one launch (dwo_product.hip).
 struct StageJob {

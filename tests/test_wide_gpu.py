@@ -148,6 +148,34 @@ def test_few_rows(C, H, D, rows, dtype):
         near(checkpoint8.linear8(args[0], args[1], args[2]), F.linear(*ref[:3]), "layer")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows", [2, 37, 200])
+def test_small_work_rounds_once(rows, dtype):
+    """Operands that one product makes for another are held in two halves there: a result is off by its own rounding, and by what remains of
+    its terms, 2^-18 of each: of sums of any number of them, as random as they are, sixteen times 2^-18 of their root mean square."""
+    def once(got, ref, what):
+        r = torch.finfo(dtype).eps / 2
+        ref = ref.detach()
+        rms = float(ref.norm()) / math.sqrt(ref.numel())
+        off = (got.double() - ref).abs() - r * ref.abs() - 2.0 ** -14 * rms - (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        assert float(off.max()) <= 0.0, "%s: %.3g beyond one rounding at root mean square %.3g" % (what, float(off.max()), rms)
+
+    args, dy = make_gated(rows, 40, 96, 72, dtype)
+    y = feedforward.gated_mlp(*args)
+    ref = leaves64(*args)
+    out = gated64(*ref, "gelu")
+    once(y, out, "y")
+    for g, w, name in zip(torch.autograd.grad(y, args, dy), torch.autograd.grad(out, ref, dy.double()),
+                          ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
+        once(g, w, name)
+    x, w, b, target = make_head(rows, 72, 130, dtype)
+    loss = losses.linear_cross_entropy(x, w, b, target)
+    ref = leaves64(x, w, b)
+    want = torch.autograd.grad(F.cross_entropy(F.linear(*ref), target), ref)
+    for g, t, name in zip(torch.autograd.grad(loss, [x, w, b]), want, ["dx", "dw", "db"]):
+        once(g, t, name)
+
+
 def test_few_rows_of_all_kinds_of_numbers():
     # a row that is not finite leaves the others as they are
     w = torch.randn(70, 520, device="cuda")
