@@ -4,8 +4,8 @@
 //
 // Forward: one product over all classes whose epilogue leaves, for a row and a wave's classes, their largest logit and the sum of
 // exponentials below it; a second kernel joins them.  Backward, in pieces of the classes: the product again, its sums turned into G, which
-// alone goes through memory, rounded to the activations' type (kHalvesWork: to two) for the two products that read it.  Eight products of rows x
-// classes x channels in place of the six of a pass that keeps its logits; what would be kept is two or more bytes a row and class.
+// alone goes through memory, rounded to the activations' type (kHalvesWork: to two) for the two products that read it.  Eight operations per
+// row, class and channel in place of the six of a pass that keeps its logits; what would be kept is two or more bytes a row and class.
 // Bound by the matrix cores: 8192 x 1024 x 65536 in bf16, statistics 1022 us (1075 TFLOP/s), G 4 x 310 (890; 268 MB of G each go out behind
 // the sums, which nothing covers), its two products 4 x 460 (1195).  In fp32, 1024 x 512 x 21841: 137, 176 and 323 us, products of six planes at
 // 167, 130 and 142 TFLOP/s of the function's own.
