@@ -333,6 +333,8 @@ struct Shape {
 };
 typedef Shape<256, 256, 2, 4, 2, 2> LargeTile;   // 128 KB of LDS, one workgroup per CU
 typedef Shape<128, 128, 2, 2, 2, 2> MediumTile;  // 64 KB, two
+// The same where no CU has two: twice the waves, and four stages (2048 x 2048 x 2048: 21 us, as the former 27; both transposed 23, 30)
+typedef Shape<128, 128, 4, 2, 2, 4> AloneTile;   // 128 KB
 // Few tiles leave most of a CU's LDS free and their waves waiting for memory: more stages on their way
 typedef Shape<64, 64, 2, 2, 2, 4> SmallTile;     // 64 KB
 typedef Shape<32, 32, 2, 2, 2, 8> ThinTile;      // 64 KB
@@ -723,14 +725,14 @@ inline Product make_product(const Operand &a, const Operand &b, long M, long N, 
 // Time of a product with square tiles of this size, us: workgroups that have a CU to themselves wait for memory step by step, others
 // share its units.  The numbers are fits to 450 bf16 products of 64 to 25088 rows x 384 to 8192 columns x 64 to 16384 summed indices, operands
 // of every order, which they meet within 10 % (root of the mean square; 13 % the smallest tile); the tile that they choose is 0.2 % slower
-// than the fastest of the four in the geometric mean, 9 % at the most.  First round: a launch with its first loads and last stores, and a
+// than the fastest of the four in the geometric mean, 9 % at the most (with MediumTile in AloneTile's place).  First round: a launch with its first loads and last stores, and a
 // step; then each round.
 struct TileCost {
     int size;
     float first, first_step, more, more_step;
 };
 constexpr TileCost kTileCosts[4] = {
-    {256, 11.6f, 1.19f, 10.f, 1.41f}, {128, 6.7f, 0.54f, 2.65f, 0.44f}, {64, 4.2f, 0.275f, 1.25f, 0.195f}, {32, 4.f, 0.15f, 1.2f, 0.105f}};
+    {256, 11.6f, 1.19f, 10.f, 1.41f}, {128, 5.8f, 0.49f, 2.65f, 0.44f}, {64, 4.2f, 0.275f, 1.25f, 0.195f}, {32, 4.f, 0.15f, 1.2f, 0.105f}};
 inline float tile_time(const TileCost &c, long workgroups, long steps) {
     if (workgroups <= kLinCus) return c.first + (float)steps * c.first_step;
     return 3.5f + (float)((workgroups + kLinCus - 1) / kLinCus) * (c.more + (float)steps * c.more_step);
@@ -744,16 +746,23 @@ inline int tile_for(long M, long N, long steps) {
             best = i;
     return kTileCosts[best].size;
 }
+// f(shape) for tiles of this size in so many workgroups
+template <class F>
+inline int with_tile(int tile, long workgroups, F &&f) {
+    switch (tile) {
+        case 256: return f(LargeTile{});
+        case 128: return workgroups <= kLinCus ? f(AloneTile{}) : f(MediumTile{});
+        case 64: return f(SmallTile{});
+        default: return f(ThinTile{});
+    }
+}
 // columns of a wave
 inline int wave_columns(int tile) { return tile == 32 ? 16 * ThinTile::NF : tile == 64 ? 16 * SmallTile::NF : 16 * LargeTile::NF; }
 template <typename T, bool AS, bool BS, bool GATED, class Epi>
 int launch_tiles(const Product &p, const Epi &epi, hipStream_t st) {
-    switch (tile_for(p.M, p.N, p.steps)) {
-        case 256: return launch_shape<T, LargeTile, AS, BS, GATED>(p, epi, st);
-        case 128: return launch_shape<T, MediumTile, AS, BS, GATED>(p, epi, st);
-        case 64: return launch_shape<T, SmallTile, AS, BS, GATED>(p, epi, st);
-        default: return launch_shape<T, ThinTile, AS, BS, GATED>(p, epi, st);
-    }
+    const int tile = tile_for(p.M, p.N, p.steps);
+    return with_tile(tile, tiles_of(p.M, p.N, tile, tile),
+                     [&](auto shape) { return launch_shape<T, decltype(shape), AS, BS, GATED>(p, epi, st); });
 }
 template <bool AS, bool BS, bool GATED, class Epi>
 int launch_product(const Product &p, int dtype, const Epi &epi, hipStream_t st) {

@@ -258,12 +258,8 @@ static int join_parts(const ProductGroup &group, hipStream_t st) {
 
 template <typename T>
 static int plain_typed(const GroupPart &q, int tile, hipStream_t st) {
-    switch (tile) {
-        case 256: return launch_shape<T, LargeTile, false, false, false>(q.p, q.epi, st);
-        case 128: return launch_shape<T, MediumTile, false, false, false>(q.p, q.epi, st);
-        case 64: return launch_shape<T, SmallTile, false, false, false>(q.p, q.epi, st);
-        default: return launch_shape<T, ThinTile, false, false, false>(q.p, q.epi, st);
-    }
+    return with_tile(tile, tiles_of(q.p.M, q.p.N, tile, tile) * q.p.splits,
+                     [&](auto shape) { return launch_shape<T, decltype(shape), false, false, false>(q.p, q.epi, st); });
 }
 int plain_product(const Operand &a, const Operand &b, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws, hipStream_t st) {
     ProductGroup group;
@@ -294,12 +290,9 @@ static int launch_group(ProductGroup group, hipStream_t st) {
 }
 template <typename T>
 static int launch_group_tile(const ProductGroup &group, int tile, hipStream_t st) {
-    switch (tile) {
-        case 256: return launch_group<T, LargeTile>(group, st);
-        case 128: return launch_group<T, MediumTile>(group, st);
-        case 64: return launch_group<T, SmallTile>(group, st);
-        default: return launch_group<T, ThinTile>(group, st);
-    }
+    long workgroups = 0;
+    for (int i = 0; i < group.count; i++) workgroups += tiles_of(group.part[i].p.M, group.part[i].p.N, tile, tile) * group.part[i].p.splits;
+    return with_tile(tile, workgroups, [&](auto shape) { return launch_group<T, decltype(shape)>(group, st); });
 }
 int ProductGroup::launch(int dtype, Arena &ws, hipStream_t st) {
     if (count == 0) return 0;
