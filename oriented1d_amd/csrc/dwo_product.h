@@ -336,10 +336,11 @@ typedef Shape<128, 128, 2, 2, 2, 2> MediumTile;  // 64 KB, two
 // The same where no CU has two: twice the waves, and four stages (2048 x 2048 x 2048: 21 us, as the former 27; both transposed 23, 30)
 typedef Shape<128, 128, 4, 2, 2, 4> AloneTile;   // 128 KB
 // The same for short sums, whose first loads and last stores are much of a tile's time: twice the waves (25088 x 1536 x 384: 45 us, as
-// MediumTile 48; x 64 34.5, 39.4; 4096 x 4096 x 2048 63, 61; the
-// gated block's product behind dy, 3136 x 2048 from 768, 39.5, 37.4)
+// MediumTile 48; x 64 34.5, 39.4; 4096 x 4096 x 768 29.1, 30.4; x 2048
+// 63, 61; two gradients of 32768 rows, 256 columns and 150 classes 21.4, 24.3).  Not where an epilogue reads, which half the registers delay (the gated
+// block's product behind dy, 3136 x 2048 from 768, 39.5, 37.4)
 typedef Shape<128, 128, 4, 2, 4, 2> ShortTile;
-constexpr long kShortSteps = 8;
+constexpr long kShortSteps = 16;
 // Few tiles leave most of a CU's LDS free and their waves waiting for memory: more stages on their way
 typedef Shape<64, 64, 2, 2, 2, 4> SmallTile;     // 64 KB
 typedef Shape<32, 32, 2, 2, 2, 8> ThinTile;      // 64 KB
@@ -751,12 +752,21 @@ inline int tile_for(long M, long N, long steps) {
             best = i;
     return kTileCosts[best].size;
 }
-// f(shape) for tiles of this size in so many workgroups of so many steps
-template <class F>
+template <class E>
+constexpr bool epilogue_reads() {
+    if constexpr (E::kDirect) return false;
+    else return !std::is_same<decltype(std::declval<E>().load(std::declval<Product>(), 0, 0)), Nothing>::value;
+}
+// f(shape) for tiles of this size in so many workgroups of so many steps, with epilogue E
+template <class E, class F>
 inline int with_tile(int tile, long workgroups, long steps, F &&f) {
     switch (tile) {
         case 256: return f(LargeTile{});
-        case 128: return workgroups <= kLinCus ? f(AloneTile{}) : steps <= kShortSteps ? f(ShortTile{}) : f(MediumTile{});
+        case 128:
+            if (workgroups <= kLinCus) return f(AloneTile{});
+            if constexpr (!epilogue_reads<E>())
+                if (steps <= kShortSteps) return f(ShortTile{});
+            return f(MediumTile{});
         case 64: return f(SmallTile{});
         default: return f(ThinTile{});
     }
@@ -766,7 +776,7 @@ inline int wave_columns(int tile) { return tile == 32 ? 16 * ThinTile::NF : tile
 template <typename T, bool AS, bool BS, bool GATED, class Epi>
 int launch_tiles(const Product &p, const Epi &epi, hipStream_t st) {
     const int tile = tile_for(p.M, p.N, p.steps);
-    return with_tile(tile, tiles_of(p.M, p.N, tile, tile), p.steps,
+    return with_tile<Epi>(tile, tiles_of(p.M, p.N, tile, tile), p.steps,
                      [&](auto shape) { return launch_shape<T, decltype(shape), AS, BS, GATED>(p, epi, st); });
 }
 template <bool AS, bool BS, bool GATED, class Epi>

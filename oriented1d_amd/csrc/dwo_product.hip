@@ -258,7 +258,7 @@ static int join_parts(const ProductGroup &group, hipStream_t st) {
 
 template <typename T>
 static int plain_typed(const GroupPart &q, int tile, hipStream_t st) {
-    return with_tile(tile, tiles_of(q.p.M, q.p.N, tile, tile) * q.p.splits, q.p.per,
+    return with_tile<PlainEpi>(tile, tiles_of(q.p.M, q.p.N, tile, tile) * q.p.splits, q.p.per,
                      [&](auto shape) { return launch_shape<T, decltype(shape), false, false, false>(q.p, q.epi, st); });
 }
 int plain_product(const Operand &a, const Operand &b, long M, long N, long K, int dtype, PlainEpi epi, Arena &ws, hipStream_t st) {
@@ -296,7 +296,7 @@ static int launch_group_tile(const ProductGroup &group, int tile, hipStream_t st
         workgroups += tiles_of(p.M, p.N, tile, tile) * p.splits;
         steps = p.per > steps ? p.per : steps;
     }
-    return with_tile(tile, workgroups, steps, [&](auto shape) { return launch_group<T, decltype(shape)>(group, st); });
+    return with_tile<PlainEpi>(tile, workgroups, steps, [&](auto shape) { return launch_group<T, decltype(shape)>(group, st); });
 }
 int ProductGroup::launch(int dtype, Arena &ws, hipStream_t st) {
     if (count == 0) return 0;
