@@ -148,6 +148,44 @@ def test_few_rows(C, H, D, rows, dtype):
         near(checkpoint8.linear8(args[0], args[1], args[2]), F.linear(*ref[:3]), "layer")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [3, 40])
+def test_rows_that_are_not_finite_stay_apart(rows, dtype):
+    args, dy = make_gated(rows, 40, 96, 72, dtype)
+    clean = feedforward.gated_mlp(*args)
+    clean_dx, = torch.autograd.grad(clean, args[0], dy)
+    with torch.no_grad():
+        args[0][1, 3], args[0][2, 39] = float("nan"), float("inf")
+    y = feedforward.gated_mlp(*args)
+    dx, = torch.autograd.grad(y, args[0], dy)
+    others = [m for m in range(rows) if m not in (1, 2)]
+    assert torch.equal(y[others], clean[others]) and torch.equal(dx[others], clean_dx[others])
+    assert y[1].isnan().all() and dx[1].isnan().all() and not y[2].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_few_rows_in_a_graph_and_on_another_stream(dtype):
+    args, _ = make_gated(2, 264, 512, 96, dtype)
+    args = [t.detach() for t in args]
+    want, layer = feedforward.gated_mlp(*args), checkpoint8.linear8(args[0], args[1], args[2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = feedforward.gated_mlp(*args)
+    side.synchronize()
+    assert torch.equal(got, want)
+    x = torch.zeros_like(args[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, z = feedforward.gated_mlp(x, *args[1:]), checkpoint8.linear8(x, args[1], args[2])
+    for _ in range(3):
+        x.copy_(args[0])
+        graph.replay()
+        assert torch.equal(y, want) and torch.equal(z, layer)
+        x.fill_(7)
+        torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("rows", [2, 37, 200])
 def test_small_work_rounds_once(rows, dtype):
@@ -174,6 +212,29 @@ def test_small_work_rounds_once(rows, dtype):
     want = torch.autograd.grad(F.cross_entropy(F.linear(*ref), target), ref)
     for g, t, name in zip(torch.autograd.grad(loss, [x, w, b]), want, ["dx", "dw", "db"]):
         once(g, t, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,C,N", [(1601, 1030, 2041), (25003, 100, 603), (25003, 328, 603)], ids=str)
+def test_tiles_of_128(rows, C, N, dtype):
+    """Tiles that have a CU to themselves, of short sums and of longer ones; sizes that end inside a tile."""
+    args, dy = make_gated(rows, C, N // 2, 40, dtype)
+    y = feedforward.gated_mlp(*args)
+    ref = leaves64(*args)
+    out = gated64(*ref, "gelu")
+    near(y, out, "y")
+    for g, w, name in zip(torch.autograd.grad(y, args, dy), torch.autograd.grad(out, ref, dy.double()),
+                          ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
+        near(g, w, name)
+    x, w, b, target = make_head(rows, C, N, dtype, ignored=0.1)
+    up = torch.randn(rows, device="cuda")
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction="none")
+    ref = leaves64(x, w, b)
+    want = F.cross_entropy(F.linear(*ref), target, reduction="none", ignore_index=-100)
+    near(loss, want, "loss")
+    for g, t, name in zip(torch.autograd.grad(loss, [x, w, b], up), torch.autograd.grad(want, ref, up.double()), ["dx", "dw", "db"]):
+        near(g, t, name)
+    near(checkpoint8.linear8(x, w, b), F.linear(*ref), "layer")
 
 
 def test_few_rows_of_all_kinds_of_numbers():
