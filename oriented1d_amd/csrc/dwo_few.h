@@ -1,15 +1,18 @@
 // Products of few rows, as one token or image makes them:  D[m][n] = sum_k x[m][k] w[n][k],  rows of both as they lie in memory.
 //
-// Bound by reading w once.  Tiles would fill sixteen rows or more with zeros and take w through LDS; here a wave has a column (gated: a gate and what it
-// multiplies), its lanes sixteen bytes of w at a time straight to registers, and multiplies them with every row in fp32.  Where columns
-// are few, two or four waves share one's sum.
+// Bound by reading w once.  Tiles would fill sixteen rows or more with zeros and take w through LDS; here a wave has a column (gated: a
+// gate and what it multiplies), its lanes sixteen bytes of w at a time straight to registers, and multiplies them with every row in
+// fp32.  Where columns are few, two or four waves share one's sum; where they are many and rows three or more, a wave has two.
 #pragma once
 
 #include "dwo_act.h"
 
 namespace dwo {
 
-constexpr int kFewWaves = 4096;  // sixteen a CU: their loads in flight keep its memory busy
+// Sixteen waves a CU: their loads in flight keep its memory busy.  Below it waves share columns (gated block 1024 -> 4096 -> 1024 in bf16, one row
+// 7.0 us, without 8.3; four rows 11.2, 18.2), from it on two columns go to a wave from three rows on, whose pieces are then read for both
+// (4096 -> 16384 -> 4096, four rows 101 us, 119 with one; 96 -> 256 -> 96 8.2, 6.2).
+constexpr int kFewWaves = 4096;
 
 // sixteen bytes of a row of w times as many values of x: pairs of 16-bit values by the instruction that adds two products to a sum in fp32
 template <int N>
@@ -74,12 +77,11 @@ struct FewGlu {
     }
 };
 
-// along: waves that share a column, 1, 2 or 4.  K in whole pieces of sixteen bytes.  From three rows on a wave has two columns: a row's piece is read
-// for both.
-template <typename TX, typename T, int R, class End>
+// U columns per wave.  along: waves that share them, 1, 2 or 4.  K in whole pieces of sixteen bytes.
+template <typename TX, typename T, int R, int U, class End>
 __global__ __launch_bounds__(256) void few_kernel(const TX *__restrict__ x, const T *__restrict__ w, long K, long N, long gap, int rows,
                                                   int along, End end) {
-    constexpr int V = 16 / (int)sizeof(T), COLS = End::kCols, U = R > 2 ? 2 : 1;
+    constexpr int V = 16 / (int)sizeof(T), COLS = End::kCols;
     __shared__ float part[4][COLS][U * R];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave & ~(along - 1);
     const long n0 = ((long)blockIdx.x * 4 + wave) / along * U;
@@ -128,13 +130,17 @@ __global__ __launch_bounds__(256) void few_kernel(const TX *__restrict__ x, cons
 
 template <typename TX, typename T, class End>
 int launch_few_typed(const void *x, const void *w, long K, long N, long gap, int rows, const End &end, hipStream_t st) {
-    const long piece = 64 * 16 / (long)sizeof(T), units = rows > 2 ? (N + 1) / 2 : N;
+    const bool two = rows > 2 && N >= kFewWaves;
+    const long piece = 64 * 16 / (long)sizeof(T), units = two ? (N + 1) / 2 : N;
     int along = 1;
     while (along < 4 && units * along < kFewWaves && K >= 2 * along * piece) along *= 2;
     const dim3 grid((unsigned)((units * along + 3) / 4)), block(256);
-    auto *kernel = rows == 1 ? few_kernel<TX, T, 1, End> : rows == 2 ? few_kernel<TX, T, 2, End> : few_kernel<TX, T, 4, End>;
+    auto *kernel = rows == 1   ? few_kernel<TX, T, 1, 1, End>
+                   : rows == 2 ? few_kernel<TX, T, 2, 1, End>
+                   : two       ? few_kernel<TX, T, 4, 2, End>
+                               : few_kernel<TX, T, 4, 1, End>;
     if constexpr (sizeof(T) == 4)
-        if (rows > 4) kernel = few_kernel<TX, T, 8, End>;
+        if (rows > 4) kernel = two ? few_kernel<TX, T, 8, 2, End> : few_kernel<TX, T, 8, 1, End>;
     kernel<<<grid, block, 0, st>>>((const TX *)x, (const T *)w, K, N, gap, rows, along, end);
     return status();
 }

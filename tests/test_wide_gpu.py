@@ -131,7 +131,7 @@ def test_gated_mlp_without_gradients_and_single_rows():
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9])
-@pytest.mark.parametrize("C,H,D", [(8, 8, 1), (24, 12, 7), (520, 264, 61), (1032, 2056, 96), (4104, 16, 4099)], ids=str)
+@pytest.mark.parametrize("C,H,D", [(8, 8, 1), (24, 12, 7), (520, 264, 61), (1032, 2056, 96), (4104, 16, 4099), (40, 4104, 24)], ids=str)
 def test_few_rows(C, H, D, rows, dtype):
     """Columns that waves share, or not, whole and partial pieces of a sum, kept halves with padding, and the layer alone."""
     args, dy = make_gated(rows, C, H, D, dtype, bias=rows % 2 == 1)
