@@ -244,8 +244,9 @@ __device__ __forceinline__ float prod_exp(float v) {
     const float t = v * 1.44269504f;
     const float r = __builtin_fmaf(v, 1.44269504f, -t) + v * 1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(t);
-    // (infinities: e is 0 or infinite and r not a number)
-    return __builtin_fabsf(v) < 1e4f ? __builtin_fmaf(e, r * 0.693147181f, e) : e;
+    // From 88.72 on (exp overflows at 88.7228) e is infinite and, r being of either sign, e + e r would not be a number; below -88.72 e is no
+    // normal number, and r of infinities is none
+    return __builtin_fabsf(v) < 88.72f ? __builtin_fmaf(e, r * 0.693147181f, e) : e;
 }
 
 // The plain epilogue: out = alpha * sum + bias[n] + before[m][n].  With several splits the sums go to `part` as they are, and
