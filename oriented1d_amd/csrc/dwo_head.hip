@@ -9,6 +9,8 @@
 // Bound by the matrix cores: 8192 x 1024 x 65536 in bf16, statistics 1022 us (1075 TFLOP/s), G 4 x 310 (890; 268 MB of G each go out behind
 // the sums, which nothing covers), its two products 4 x 460 (1195).  In fp32, 1024 x 512 x 21841: 137, 176 and 323 us, products of six planes at
 // 167, 130 and 142 TFLOP/s of the function's own.
+#include <cmath>
+
 #include "dwo_product.h"
 
 namespace dwo {
@@ -211,9 +213,13 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restric
 // What the products that read G give it back: G is held without what all its rows share.
 //   a mean: up / count (1 - eps), so that a row's largest value, about -1 at its target, is next to a number that 16 bits hold; rounded
 //   where it is, the same rounding in all rows would go into the gradients (twice their own rounding with labels smoothed)
-//   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's rows are at most 2, times 2^13, others are brought to
-//   2^13 .. 2^14 by the largest |up|: scale[0], and its inverse, by this kernel
+//   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's values are at most 1 / (1 - eps) and 1 at the target, times
+//   2^13 or, above a smoothing of 3/4, what brings 1 / (1 - eps) to 2^14 .. 2^15; others are brought to 2^13 .. 2^14 by the largest |up|:
+//   scale[0], and its inverse, by this kernel
 constexpr float kHalfScale = 8192.f;
+static float half_mean_scale(float eps) {
+    return eps < 1.f ? fminf(kHalfScale, ldexpf(4.f * kHalfScale, ilogbf(1.f - eps))) : kHalfScale;
+}
 __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, long M, float *__restrict__ scale) {
     __shared__ unsigned most[1024];
     unsigned v = 0;
@@ -344,7 +350,7 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
         if ((e = status())) return e;
     }
     const size_t size = size_of(s.dtype), grad_size = size_of(grad);
-    const float mean_scale = half ? kHalfScale : 1.f;
+    const float mean_scale = half ? half_mean_scale(eps) : 1.f;
     auto shared = [&](PlainEpi epi) {
         epi.alpha = mean ? up : scale != nullptr ? scale + 1 : nullptr;
         epi.over = count;

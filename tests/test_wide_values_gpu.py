@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from oriented1d_amd import checkpoint8, feedforward
+from oriented1d_amd import checkpoint8, feedforward, losses
 from test_wide_gpu import DTYPES, IDS, gated64, held8, leaves64, make_gated, near
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,55 @@ def test_gated_block_with_large_gates(rows, dtype, held):
     want = torch.autograd.grad(gated64(*ref, "silu"), ref, dy.double())
     for g, w, name in zip(got, want, ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
         near(g, w, name)
+
+
+# ---------------------------------------------------------------------------------------------------- label smoothing up to 1
+def make_sure(rows, C, V, dtype, sure, seed=0):
+    """A classifier that is sure of a class in every row (probability 0.9 and more), the target in some rows and not in others; and one that is
+    not (``sure`` 0)."""
+    gen = torch.Generator("cuda").manual_seed(seed + rows + V)
+    x = torch.randn((rows, C), generator=gen, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn((V, C), generator=gen, device="cuda") * C ** -0.5).to(dtype)
+    guess = torch.randint(0, V, (rows,), generator=gen, device="cuda")
+    with torch.no_grad():
+        # (V classes and as many channels: a row's own channel says what it is sure of)
+        if sure:
+            w.zero_()
+            w[torch.arange(V), torch.arange(V)] = sure
+            x[:, :V] = 0
+            x[torch.arange(rows), guess] = 1
+    w.requires_grad_()
+    b = (torch.randn((V,), generator=gen, device="cuda") * 0.3).to(dtype).requires_grad_()
+    target = torch.where(torch.rand((rows,), generator=gen, device="cuda") < 0.5, guess, torch.randint(0, V, (rows,), generator=gen, device="cuda"))
+    return x, w, b, target
+
+
+@pytest.mark.parametrize("smoothing", [0.5, 0.75, 0.8, 0.875, 0.9, 0.99, 0.9999, 1.0])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,C,V", [(40, 72, 10), (5000, 272, 257)], ids=str)
+@pytest.mark.parametrize("sure", [0.0, 9.0])
+def test_much_smoothing(rows, C, V, dtype, reduction, smoothing, sure):
+    x, w, b, target = make_sure(rows, C, V, dtype, sure)
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction=reduction, label_smoothing=smoothing)
+    up = torch.full_like(loss, 512.0 if reduction == "mean" else 1.0)  # (a mean in fp16 is trained with a scaled loss)
+    got = torch.autograd.grad(loss, [x, w, b], up)
+    ref = leaves64(x, w, b)
+    logits = F.linear(*ref)
+    want = F.cross_entropy(logits, target, reduction=reduction, label_smoothing=smoothing)
+    assert ((loss.double() - want).abs() <= 4e-6 * (want.abs() + 12)).all()
+    # A logit's gradient is p - smoothing / V - (1 - smoothing) [target]: what fp32 leaves of these, 1e-6 of each, and its rounding as an operand, r of
+    # it.  They may have the same sign in all rows (a class that nobody has is off by the same rounding in each), so the limit is the sum of the
+    # magnitudes; then the result's rounding, and what fp32 sums lose.
+    r = torch.finfo(dtype).eps / 2
+    up64 = up.double().reshape(-1, 1) / (rows if reduction == "mean" else 1)
+    size = torch.softmax(logits, 1).detach() + smoothing / V
+    size[torch.arange(rows), target] += 1 - smoothing
+    held = torch.autograd.grad(want, logits, up.double(), retain_graph=True)[0].abs()
+    size = 1e-6 * size * up64 + (r + 4e-6) * held
+    limits = size @ ref[1].detach().abs(), size.t() @ ref[0].detach().abs(), size.sum(0)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-30
+    for g, t, m, name in zip(got, torch.autograd.grad(want, ref, up.double()), limits, ["dx", "dw", "db"]):
+        assert torch.isfinite(g).all(), "%s: %d not finite" % (name, int((~torch.isfinite(g)).sum()))
+        off = (g.double() - t).abs() - r * t.abs() - m - tiny
+        assert float(off.max()) <= 0.0, "%s: %.3g beyond the limit" % (name, float(off.max()))
