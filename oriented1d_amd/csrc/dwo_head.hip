@@ -214,16 +214,20 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restric
 //   a mean: up / count (1 - eps), so that a row's largest value, about -1 at its target, is next to a number that 16 bits hold; rounded
 //   where it is, the same rounding in all rows would go into the gradients (twice their own rounding with labels smoothed)
 //   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's values are at most 1 / (1 - eps) and 1 at the target, times
-//   2^13 or, above a smoothing of 3/4, what brings 1 / (1 - eps) to 2^14 .. 2^15; others are brought to 2^13 .. 2^14 by the largest |up|:
-//   scale[0], and its inverse, by this kernel
+//   2^13 or, above a smoothing of 3/4, what brings 1 / (1 - eps) to 2^14 .. 2^15; others are brought to 2^13 .. 2^14 by the largest finite |up| of a
+//   row with a class (whatever arrives at the others changes nothing): scale[0], and its inverse, by this kernel
 constexpr float kHalfScale = 8192.f;
 static float half_mean_scale(float eps) {
     return eps < 1.f ? fminf(kHalfScale, ldexpf(4.f * kHalfScale, ilogbf(1.f - eps))) : kHalfScale;
 }
-__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, long M, float *__restrict__ scale) {
+__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, Targets targets, long M,
+                                                          float *__restrict__ scale) {
     __shared__ unsigned most[1024];
     unsigned v = 0;
-    for (long i = threadIdx.x; i < M; i += 1024) v = max(v, __float_as_uint(up[i]) & 0x7fffffffu);
+    for (long i = threadIdx.x; i < M; i += 1024) {
+        const unsigned u = __float_as_uint(up[i]) & 0x7fffffffu;
+        v = u < 0x7f800000u && targets.of(i) >= 0 ? max(v, u) : v;
+    }
     most[threadIdx.x] = v;
     __syncthreads();
     for (int h = 512; h > 0; h >>= 1) {
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restric
     }
     if (threadIdx.x == 0) {
         const int e = (int)(most[0] >> 23);  // biased exponent; the scale's is 254 + 13 - e
-        const int k = e == 0 || e == 255 ? 127 : min(max(267 - e, 1), 253);
+        const int k = e == 0 ? 127 : min(max(267 - e, 1), 253);
         scale[0] = __uint_as_float((unsigned)k << 23), scale[1] = __uint_as_float((unsigned)(254 - k) << 23);
     }
 }
@@ -346,7 +350,7 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
     const bool mean = count != nullptr, half = s.dtype == DWO_F16;
     float *scale = half && !mean ? (float *)ws.take(2 * sizeof(float)) : nullptr;
     if (scale != nullptr && !ws.dry()) {
-        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, s.rows, scale);
+        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, targets, s.rows, scale);
         if ((e = status())) return e;
     }
     const size_t size = size_of(s.dtype), grad_size = size_of(grad);

@@ -5,7 +5,7 @@ import torch
 import torch.nn.functional as F
 
 from oriented1d_amd import checkpoint8, feedforward, losses
-from test_wide_gpu import DTYPES, IDS, gated64, held8, leaves64, make_gated, near
+from test_wide_gpu import DTYPES, IDS, gated64, held8, leaves64, make_gated, make_head, near
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,38 @@ def test_much_smoothing(rows, C, V, dtype, reduction, smoothing, sure):
         assert torch.isfinite(g).all(), "%s: %d not finite" % (name, int((~torch.isfinite(g)).sum()))
         off = (g.double() - t).abs() - r * t.abs() - m - tiny
         assert float(off.max()) <= 0.0, "%s: %.3g beyond the limit" % (name, float(off.max()))
+
+
+# ---------------------------------------------------------------------------------------------------- what arrives at rows that do not count
+@pytest.mark.parametrize("value", [1e30, float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_what_arrives_at_ignored_rows_changes_nothing(dtype, value):
+    """A weight of a masked row may be anything, 1 / 0 among it: the other rows' gradients are as with a zero there, bit for bit."""
+    x, w, b, target = make_head(300, 64, 130, dtype, ignored=0.3)
+    up = torch.rand(300, device="cuda") + 0.5
+    results = []
+    for at_ignored in (0.0, value):
+        loss = losses.linear_cross_entropy(x, w, b, target, reduction="none")
+        results.append(torch.autograd.grad(loss, [x, w, b], torch.where(target == -100, at_ignored, up)))
+    for clean, got in zip(*results):
+        assert torch.isfinite(got).all() and torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_a_row_with_an_infinite_weight_stays_apart(dtype):
+    x, w, b, target = make_head(200, 64, 130, dtype)
+    up = torch.rand(200, device="cuda") + 0.5
+    up[7] = 0
+    clean, = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target, reduction="none"), x, up)
+    for value in (float("inf"), float("nan")):
+        up[7] = value
+        dx, = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target, reduction="none"), x, up)
+        assert not torch.isfinite(dx[7]).any()
+        dx[7] = clean[7]
+        assert torch.equal(dx, clean)
+    # nor does one whose target is no class
+    target[9], up[7], up[9] = 130, 1.0, 0.0
+    first, = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target, reduction="none"), x, up)
+    up[9] = 1e30
+    dx, = torch.autograd.grad(losses.linear_cross_entropy(x, w, b, target, reduction="none"), x, up)
+    assert dx[9].isnan().all() and torch.equal(torch.cat([dx[:9], dx[10:]]), torch.cat([first[:9], first[10:]]))
