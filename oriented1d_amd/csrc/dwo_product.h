@@ -5,8 +5,9 @@
 //
 // Either operand lies in memory with k fast (A [M][K]) or with k slow (A [K][M], what the product of a gradient reads), so that no
 // tensor is transposed.  Values are 16 bits wide, sums 32.  fp32 operands come as three planes of bf16 whose sum they are (8 + 8 + 8
-// bits of mantissa, stage_kernel), and their product is six of the nine products of planes, small ones first: what is left out is below
-// 2^-24 of the whole.  417 TFLOP/s at best, where the fp32 matrix instructions give 157, at the accuracy of sums in fp32.
+// bits of mantissa, planes_of), and their product is six of the nine products of planes, small ones first: what is left out, two products of
+// 2^-8 and 2^-17 at the most of their operands, is 2^-24 of a product at the most and of either sign.  417 TFLOP/s at best, where the fp32
+// matrix instructions give 157, at the accuracy of sums in fp32.
 #pragma once
 
 #include <utility>
@@ -143,14 +144,17 @@ __device__ __forceinline__ unsigned pack16(int type, float a, float b) {
     return type == OUT_F16 ? lin_pack<f16_t>(a, b) : pack_bf16(a, b);
 }
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-// v's three planes; infinities and NaN stay in the first one alone
+__device__ __forceinline__ float bf16_nearest(float v) { return bf16_value(from_float<bf16_t>(v).bits); }
+// v's three planes, each the nearest value of eight bits to what those before it leave (what the products of planes leave out has either sign
+// then; with planes cut toward zero it is 0.6 2^-24 of a product in the mean and up to 8, always toward zero); infinities and NaN stay in
+// the first one alone
 __device__ __forceinline__ void planes_of(float v, float (&q)[3]) {
-    // (rounded toward zero, so that the largest numbers do not become infinite)
-    q[0] = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-    if (!finite) q[0] = v;
+    const bool finite = __builtin_fabsf(v) < INFINITY;
+    q[0] = bf16_nearest(v);
+    // (the largest numbers do not become infinite)
+    if (finite && __builtin_fabsf(q[0]) == INFINITY) q[0] = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
     const float r = finite ? v - q[0] : 0.f;
-    q[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    q[1] = bf16_nearest(r);
     q[2] = r - q[1];
 }
 __device__ __forceinline__ void out_one(const Out &o, long m, long n, float v) {
