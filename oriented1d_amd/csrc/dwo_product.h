@@ -146,16 +146,18 @@ __device__ __forceinline__ unsigned pack16(int type, float a, float b) {
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 __device__ __forceinline__ float bf16_nearest(float v) { return bf16_value(from_float<bf16_t>(v).bits); }
 // v's three planes, each the nearest value of eight bits to what those before it leave (what the products of planes leave out has either sign
-// then; with planes cut toward zero it is 0.6 2^-24 of a product in the mean and up to 8, always toward zero); infinities and NaN stay in
-// the first one alone
+// then; with planes cut toward zero it is 0.6 2^-24 of a product in the mean and up to 8, always toward zero).  Infinities and NaN are in
+// the last one, which meets nothing but the other operand's first, whose sign and zeros are the operand's own: the products are infinite
+// where those of fp32 are.  In front of them is 1 with their sign, so that this holds for two infinities as well.
 __device__ __forceinline__ void planes_of(float v, float (&q)[3]) {
     const bool finite = __builtin_fabsf(v) < INFINITY;
     q[0] = bf16_nearest(v);
     // (the largest numbers do not become infinite)
     if (finite && __builtin_fabsf(q[0]) == INFINITY) q[0] = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    const float r = finite ? v - q[0] : 0.f;
+    const float r = v - q[0];
     q[1] = bf16_nearest(r);
     q[2] = r - q[1];
+    if (!finite) q[0] = __builtin_copysignf(1.f, v), q[1] = 0.f, q[2] = v;
 }
 __device__ __forceinline__ void out_one(const Out &o, long m, long n, float v) {
     const size_t at = (size_t)m * o.pitch + n;

@@ -163,3 +163,63 @@ def test_fp32_errors_have_either_sign():
     for got, want in ((y, x.double() @ w.double().t()), (dx, dy.double() @ w.double())):
         error = float(((got.double() - want) / want).mean()) * 2.0 ** 24
         assert abs(error) <= 0.5, error
+
+
+# ---------------------------------------------------------------------------------------------------- infinities
+def same_kind(got, ref, what):
+    """Infinite, with its sign, and not a number where the reference is."""
+    got, ref = got.double(), ref.double()
+    assert torch.equal(got.isnan(), ref.isnan()), "%s: %d, not %d that are no numbers" % (what, int(got.isnan().sum()), int(ref.isnan().sum()))
+    assert torch.equal(torch.where(got.isinf(), got, 0), torch.where(ref.isinf(), ref, 0)), "%s: infinities" % what
+
+
+def products64(a, b):
+    """a b^T in 64 bits, term by term."""
+    return (a.double()[:, None] * b.double()[None]).sum(-1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [8, 9, 40, 300])
+def test_infinities_of_a_layer(rows, dtype):
+    """As the formula has them at any number of rows: infinite of the products' sign, no number where they meet zero or each other."""
+    gen = torch.Generator("cuda").manual_seed(rows)
+    x = torch.randn((rows, 72), generator=gen, device="cuda").to(dtype)
+    w = torch.randn((40, 72), generator=gen, device="cuda").to(dtype)
+    dy = torch.randn((rows, 40), generator=gen, device="cuda").to(dtype)
+    inf = float("inf")
+    w[0], w[1] = 1, -0.5  # (values of a few bits)
+    w[2, 3], w[3, 5] = 0, -inf
+    x[1, 3], x[2, 71], x[4, 5], x[5, 0], x[5, 1] = inf, -inf, inf, inf, -inf
+    dy[1, 7], dy[3, 39], dy[6, 3] = -inf, inf, inf
+    b = torch.randn((40,), generator=gen, device="cuda").to(dtype)
+    x, w, b = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    y = checkpoint8.linear8(x, w, b)
+    same_kind(y, products64(x.detach(), w.detach()) + b.detach().double(), "y")
+    with torch.no_grad():
+        same_kind(checkpoint8.linear8(x, w, b), y, "y")
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    same_kind(dx, products64(dy, w.detach().t()), "dx")
+    same_kind(dw, products64(dy.t(), held8(x.detach()).t()), "dw")
+    same_kind(db, dy.double().sum(0), "db")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
+@pytest.mark.parametrize("rows", [3, 9, 40, 300])
+@pytest.mark.parametrize("place", ["w_out", "dy", "x"])
+def test_infinities_of_the_gated_block(place, rows, dtype):
+    args, dy = make_gated(rows, 40, 96, 72, dtype)
+    with torch.no_grad():
+        if place == "w_out":
+            args[3][5, 17], args[3][6, 18] = float("inf"), float("-inf")
+        elif place == "dy":
+            dy[1, 5], dy[2, 71] = float("inf"), float("-inf")
+        else:
+            args[0][1, 3] = float("inf")
+    y = feedforward.gated_mlp(*args)
+    ref = leaves64(*args)
+    out = gated64(*ref, "gelu")
+    same_kind(y, out, "y")
+    got = torch.autograd.grad(y, args, dy)
+    want = torch.autograd.grad(out, ref, dy.double())
+    for g, t, name in zip(got, want, ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
+        same_kind(g, t, name)
