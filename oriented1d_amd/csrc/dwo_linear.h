@@ -37,7 +37,7 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16_t> {
-    static constexpr short kOne = 0x3f80;
+    static constexpr short kOne = 0x3f80, kHalf = 0x3f00;
     static __device__ __forceinline__ mma_f4 run(mma_s8 a, mma_s8 b, mma_f4 c) {
         typedef __bf16 v8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0,
@@ -46,7 +46,7 @@ struct Mma<bf16_t> {
 };
 template <>
 struct Mma<f16_t> {
-    static constexpr short kOne = 0x3c00;
+    static constexpr short kOne = 0x3c00, kHalf = 0x3800;
     static __device__ __forceinline__ mma_f4 run(mma_s8 a, mma_s8 b, mma_f4 c) {
         typedef _Float16 v8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0,

@@ -27,6 +27,7 @@ struct Product {
     long gap;  // gated weights: values from the row of a gate to that of what it multiplies (0: rows as they come)
     int pairs;
     unsigned codes_a, codes_b;  // the planes of each pair, two bits a pair
+    unsigned summed;            // the pairs, a bit each, whose planes of A are in its sums
     int mtiles, ntiles, splits;
     int per, steps;  // steps of 64 per split, in all
 };
@@ -37,6 +38,7 @@ inline void product_pairs(Product &p) {
     p.pairs = a == 3 && b == 3 ? 6 : a > b ? a : b;
     p.codes_a = a == 3 && b == 3 ? 0x052 : a == 3 ? 0x006 : a == 2 ? 0x001 : 0;
     p.codes_b = a == 3 && b == 3 ? 0x118 : b == 3 ? 0x006 : b == 2 ? 0x001 : 0;
+    p.summed = a == 3 && b == 3 ? 0x29 : b == 3 ? 0x4 : 0x7;
 }
 
 // ------------------------------------------------------------------------------------------------- stages in LDS
@@ -211,18 +213,30 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
     }
     store_out<STREAM>(to, mma_u4{pack16(o.type, v[0], v[1]), pack16(o.type, v[2], v[3]), pack16(o.type, v[4], v[5]), pack16(o.type, v[6], v[7])});
 }
-// eight neighbours of an operand's row; in two halves (o.plane of 16-bit values) the second is what the first one's rounding leaves
+// Eight neighbours of an operand's row; in two halves (o.plane of 16-bit values) the second is what the first one's rounding leaves.  It has
+// the first one's sign and is not zero, for which the first goes a step down where it has to (the second is then at most 3/2 steps and not
+// 1/2, its own rounding twice as far): an infinite value of the other operand, whose products with both halves are added, is infinite in the sum
+// and not NaN.  The second half of infinities and NaN is 1 with their sign.
 template <bool STREAM = true>
 __device__ __forceinline__ void operand_octet(const Out &o, long m, long n, long N, const float (&v)[8]) {
     out_octet<STREAM>(o, true, m, n, N, v);
     if (o.type == OUT_PLANES || o.plane == 0) return;
-    float r[8];
+    // (the first half is written again: with these values in front of the first store the gated block's product behind dy, 16384 x 4096 from 1024,
+    // which has no halves, takes 340 us, so 334)
+    auto value = [&](uint16_t b) { return o.type == OUT_F16 ? to_float(__builtin_bit_cast(f16_t, b)) : bf16_value(b); };
+    float first[8], second[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float h = o.type == OUT_F16 ? to_float(from_float<f16_t>(v[e])) : bf16_value(bits16(OUT_BF16, v[e]));
-        r[e] = (__float_as_uint(h) & 0x7f800000u) != 0x7f800000u ? v[e] - h : 0.f;
+        const uint16_t b = bits16(o.type, v[e]);
+        float h = value(b), rest = v[e] - h;
+        const float r = value(bits16(o.type, rest));
+        const bool apart = r == 0.f || ((__float_as_uint(r) ^ __float_as_uint(h)) >> 31) != 0;
+        const bool finite = __builtin_fabsf(h) < INFINITY;
+        if (apart && (b & 0x7fff) > 1) h = value(b - 1), rest = v[e] - h;
+        first[e] = finite ? h : v[e], second[e] = finite ? rest : __builtin_copysignf(1.f, v[e]);
     }
-    out_octet<STREAM>({reinterpret_cast<uint16_t *>(o.p) + o.plane, o.pitch, 0, o.type}, true, m, n, N, r);
+    out_octet<STREAM>(o, true, m, n, N, first);
+    out_octet<STREAM>({reinterpret_cast<uint16_t *>(o.p) + o.plane, o.pitch, 0, o.type}, true, m, n, N, second);
 }
 
 // An epilogue E has
@@ -481,13 +495,15 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
             if (r < reads(t)) read(from, t, r);
     };
     // sums over A alone, in the workgroups of the first column of tiles: products with ones, with zeros elsewhere and where a plane of A
-    // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all)
+    // meets another than B's first, once more (a branch would cost more than these products, one in sixteen of all).  Where A's only plane
+    // meets both halves of B, with 1/2 both times: its infinities are not to meet zeros (of three planes the one that holds them does not)
     int at_pair = first / ksteps, at_step = first % ksteps;
     Fragments<BM, AS> sums_of;
     sums_of.init((wm * MF + wn * SF % MF) * 16);
+    const short unit = nt != 0 ? 0 : p.b.planes == 2 ? Mma<T>::kHalf : Mma<T>::kOne;
     auto add_sums = [&](const uint16_t *la) {
         if constexpr (SUMS) {
-            const short one = nt == 0 && (p.codes_b >> (2 * at_pair) & 3) == 0 ? Mma<T>::kOne : 0;
+            const short one = p.summed >> at_pair & 1 ? unit : 0;
             at_step++;
             const bool wrap = at_step == ksteps;
             at_step = wrap ? 0 : at_step, at_pair = wrap ? at_pair + 1 : at_pair;
@@ -730,7 +746,7 @@ int launch_shape(Product p, const Epi &epi, hipStream_t st) {
 }
 inline long tiles_of(long M, long N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 inline Product make_product(const Operand &a, const Operand &b, long M, long N, long K, long gap) {
-    Product p{a, b, M, N, K, gap, 1, 0, 0, 0, 0, 1, 0, 0};
+    Product p{a, b, M, N, K, gap, 1, 0, 0, 0, 0, 0, 1, 0, 0};
     product_pairs(p);
     p.steps = p.per = (int)((K + kProdK - 1) / kProdK * p.pairs);
     return p;

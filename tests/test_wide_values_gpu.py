@@ -203,7 +203,7 @@ def test_infinities_of_a_layer(rows, dtype):
     same_kind(db, dy.double().sum(0), "db")
 
 
-@pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows", [3, 9, 40, 300])
 @pytest.mark.parametrize("place", ["w_out", "dy", "x"])
 def test_infinities_of_the_gated_block(place, rows, dtype):
