@@ -3,10 +3,31 @@
 The forward pass leaves a row's log-sum-exp and nothing of its logits; the backward pass computes them again, in pieces of the classes, and
 turns them into the gradients of input, weight and bias.
 """
+import torch
 import torch.nn.functional as F
 
 from . import _lib, fused
 from .dwoconv1d import ordinary
+
+
+def _composed(x, weight, bias, target, reduction, ignore_index, label_smoothing):
+    """The same values from PyTorch ops, for any leading dimensions and none."""
+    if target.shape != x.shape[:-1] or target.dtype != torch.int64:
+        raise RuntimeError("target must be int64, one class for every row of x")
+    logits = F.linear(x, weight, bias).float()
+    counts = target != ignore_index
+    is_class = counts & (target >= 0) & (target < logits.shape[-1])
+    # rows that are ignored may hold anything, and those whose target is no class are NaN, as are their gradients
+    logits = torch.where(counts.unsqueeze(-1), logits, 0.0) + torch.where(counts & ~is_class, float("nan"), 0.0).unsqueeze(-1)
+    logs = F.log_softmax(logits, -1)
+    loss = -logs.gather(-1, torch.where(is_class, target, 0).unsqueeze(-1)).squeeze(-1)
+    if label_smoothing > 0:
+        loss = (1 - label_smoothing) * loss - label_smoothing * logs.mean(-1)
+    loss = torch.where(counts, loss, 0.0)
+    if reduction == "none":
+        return loss
+    number = counts.sum()
+    return torch.where(number > 0, loss.sum() / number.clamp(min=1), float("nan"))
 
 
 def linear_cross_entropy(x, weight, bias, target, *, reduction="mean", ignore_index=-100, label_smoothing=0.0):
@@ -22,10 +43,7 @@ def linear_cross_entropy(x, weight, bias, target, *, reduction="mean", ignore_in
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError("label_smoothing must be between 0 and 1")
     if not ordinary(x, weight, bias, target):
-        logits = F.linear(x, weight, bias).float()
-        loss = F.cross_entropy(logits.flatten(0, -2), target.flatten(), ignore_index=ignore_index, reduction=reduction,
-                               label_smoothing=label_smoothing)
-        return loss if reduction == "mean" else loss.unflatten(0, target.shape)
+        return _composed(x, weight, bias, target, reduction, ignore_index, label_smoothing)
     dtype = fused._autocast(x)
     return _lib.host(x.get_device()).head(x if dtype is None else x.to(dtype), weight, bias, target, reduction == "mean",
                                           int(ignore_index), float(label_smoothing))

@@ -131,3 +131,46 @@ def test_networks_with_gated_blocks():
     assert all(stage[0].mlp.checkpoint8 for stage in net.stages)
     with pytest.raises(ValueError, match="classes"):
         ConvNeXt1D(depths=(1, 1, 1, 1), dims=(16, 24, 32, 40), out_stages=True).loss(torch.zeros(1, 3, 32, 32), torch.zeros(1))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_transforms_over_rows(reduction):
+    """Per-sample gradients: x [C] and a target of no dimensions inside."""
+    F = torch.nn.functional
+    x, w, b = torch.randn(4, 8), torch.randn(16, 8), torch.randn(16)
+    target = torch.tensor([0, 3, -100, 15])
+    each = F.cross_entropy(F.linear(x, w, b), target, reduction="none", label_smoothing=0.1)
+    want = torch.where(target == -100, float("nan"), each) if reduction == "mean" else each  # (a mean over no rows)
+
+    def call(row, t, weight):
+        return losses.linear_cross_entropy(row, weight, b, t, reduction=reduction, label_smoothing=0.1)
+
+    got = torch.func.vmap(call, (0, 0, None))(x, target, w)
+    assert torch.allclose(got, want, atol=1e-5, equal_nan=True)
+    grads = torch.func.vmap(torch.func.grad(call, argnums=2), (0, 0, None))(x, target, w)
+    leaf = w.clone().requires_grad_()
+    for k in range(4):
+        loss = F.cross_entropy(F.linear(x[k], leaf, b)[None], target[k:k + 1], reduction="sum", label_smoothing=0.1)
+        assert torch.allclose(grads[k], torch.autograd.grad(loss, leaf)[0], atol=1e-5)
+
+
+def test_transforms_of_targets_that_are_no_class():
+    """NaN in the row and its gradient alone, as outside of a transform; and targets to ignore that are a class."""
+    F = torch.nn.functional
+    x, w, b = torch.randn(3, 5, 8), torch.randn(6, 8), torch.randn(6)
+    target = torch.tensor([[0, 6, -1, 5, -100]] * 3)
+    got = torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, b, t, reduction="none"))(x, target)
+    assert got[:, 1:3].isnan().all() and torch.isfinite(got[:, [0, 3]]).all() and (got[:, 4] == 0).all()
+    dx = torch.func.vmap(torch.func.grad(lambda a, t: losses.linear_cross_entropy(a, w, b, t, reduction="none").sum()))(x, target)
+    assert dx[:, 1:3].isnan().all() and torch.isfinite(dx[:, [0, 3]]).all() and (dx[:, 4] == 0).all()
+    assert torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, b, t))(x, target).isnan().all()
+    target = torch.tensor([[0, 5, 2, 5, 1]] * 3)
+    want = torch.stack([F.cross_entropy(F.linear(a, w, b), t, ignore_index=5) for a, t in zip(x, target)])
+    got = torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, b, t, ignore_index=5))(x, target)
+    assert torch.allclose(got, want, atol=1e-5)
+    # a row that is ignored may hold anything
+    x[:, 1] = float("nan")
+    got = torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, b, t, ignore_index=5))(x, target)
+    assert torch.isfinite(got).all()
+    dx = torch.func.vmap(torch.func.grad(lambda a, t: losses.linear_cross_entropy(a, w, b, t, ignore_index=5)))(x, target)
+    assert torch.isfinite(dx).all() and (dx[:, 1] == 0).all()
