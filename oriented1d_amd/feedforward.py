@@ -28,8 +28,8 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, activation="gelu", checkpoint8=False)
     if not ordinary(x, w_in, b_in, w_out, b_out):
         if checkpoint8:
             require_ordinary("gated_mlp(checkpoint8=True)", x, w_in, b_in, w_out, b_out)
-        gate, up = F.linear(x, w_in, b_in).chunk(2, dim=-1)
-        return F.linear(_FUNCTIONS[activation](gate) * up, w_out, b_out)
+        gate, up = fused.linear_as(x, w_in, b_in).chunk(2, dim=-1)
+        return fused.linear_as(_FUNCTIONS[activation](gate) * up, w_out, b_out)
     dtype = fused._autocast(x)
     return _lib.host(x.get_device()).gated(x if dtype is None else x.to(dtype), w_in, b_in, w_out, b_out, code, bool(checkpoint8))
 

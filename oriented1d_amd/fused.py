@@ -462,6 +462,11 @@ class Linear(torch.nn.Linear):
         return F.linear(x, w, b)
 
 
+def linear_as(x, weight, bias):
+    """``F.linear`` with the parameters converted to the type of x."""
+    return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
+
+
 # Modules that convert what they read under autocast, as a pointwise layer does
 CONSUMERS = [Linear]
 

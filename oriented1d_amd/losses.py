@@ -14,7 +14,7 @@ def _composed(x, weight, bias, target, reduction, ignore_index, label_smoothing)
     """The same values from PyTorch ops, for any leading dimensions and none."""
     if target.shape != x.shape[:-1] or target.dtype != torch.int64:
         raise RuntimeError("target must be int64, one class for every row of x")
-    logits = F.linear(x, weight, bias).float()
+    logits = fused.linear_as(x, weight, bias).float()
     counts = target != ignore_index
     is_class = counts & (target >= 0) & (target < logits.shape[-1])
     # rows that are ignored may hold anything, and those whose target is no class are NaN, as are their gradients

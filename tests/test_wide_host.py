@@ -174,3 +174,27 @@ def test_transforms_of_targets_that_are_no_class():
     assert torch.isfinite(got).all()
     dx = torch.func.vmap(torch.func.grad(lambda a, t: losses.linear_cross_entropy(a, w, b, t, ignore_index=5)))(x, target)
     assert torch.isfinite(dx).all() and (dx[:, 1] == 0).all()
+
+
+def test_transforms_with_parameters_of_another_type():
+    """16-bit activations and fp32 parameters: converted as outside of a transform, gradients of the parameters' own type."""
+    x, w, b, v, c = torch.randn(3, 4, 8).bfloat16(), torch.randn(16, 8), torch.randn(16), torch.randn(5, 8), torch.randn(5)
+    target = torch.tensor([[0, 3, -100, 15]] * 3)
+
+    def loss(a, t, w, b):
+        return losses.linear_cross_entropy(a, w, b, t)
+
+    def block(a, w, b, v, c):
+        return feedforward.gated_mlp(a, w, b, v, c)
+
+    got = torch.func.vmap(loss, (0, 0, None, None))(x, target, w, b)
+    assert torch.equal(got, torch.func.vmap(loss, (0, 0, None, None))(x, target, w.bfloat16(), b.bfloat16()))
+    dw, db = torch.func.grad(loss, argnums=(2, 3))(x[0], target[0], w, b)
+    assert dw.dtype == torch.float32 and db.dtype == torch.float32 and torch.isfinite(dw).all()
+    got = torch.func.vmap(block, (0, None, None, None, None))(x, w, b, v, c)
+    same = torch.func.vmap(block, (0, None, None, None, None))(x, *[t.bfloat16() for t in (w, b, v, c)])
+    assert got.dtype == torch.bfloat16 and torch.equal(got, same)
+    grads = torch.func.grad(lambda *p: block(x, *p).float().sum(), argnums=(0, 1, 2, 3))(w, b, v, c)
+    assert all(g.dtype == torch.float32 and torch.isfinite(g).all() for g in grads)
+    assert torch.equal(torch.func.vmap(block, (0, None, None, None, None))(x, w, None, v, None),
+                       torch.func.vmap(block, (0, None, None, None, None))(x, w.bfloat16(), None, v.bfloat16(), None))
