@@ -9,6 +9,7 @@
 // Bound by the matrix cores: 8192 x 1024 x 65536 in bf16, statistics 1022 us (1075 TFLOP/s), G 4 x 310 (890; 268 MB of G each go out behind
 // the sums, which nothing covers), its two products 4 x 460 (1195).  In fp32, 1024 x 512 x 21841: 137, 176 and 323 us, products of six planes at
 // 167, 130 and 142 TFLOP/s of the function's own.
+#include <algorithm>
 #include <cmath>
 
 #include "dwo_product.h"
@@ -310,10 +311,10 @@ struct HeadSizes {
     int dtype;
     HeadSizes(size_t r, int c, int v, int t) : rows((long)r), C(c), V(v), dtype(t) {}
     bool ok() const { return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && V >= 1 && V <= 1 << 24 && known(dtype); }
-    // classes of a piece: G of a piece has about 2^27 values, 256 MB in 16 bits, what the last cache before memory holds
+    // classes of a piece: G of a piece has about 2^27 values, 256 MB in 16 bits, what the last cache before memory holds, or 1024 classes
     long piece() const {
-        const long most = (1L << 27) / rows / 256 * 256;
-        return V <= most ? V : most < 1024 ? 1024 : most;
+        const long most = std::max((1L << 27) / rows / 256 * 256, 1024L);
+        return std::min(V, most);
     }
 };
 

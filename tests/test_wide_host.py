@@ -198,3 +198,12 @@ def test_transforms_with_parameters_of_another_type():
     assert all(g.dtype == torch.float32 and torch.isfinite(g).all() for g in grads)
     assert torch.equal(torch.func.vmap(block, (0, None, None, None, None))(x, w, None, v, None),
                        torch.func.vmap(block, (0, None, None, None, None))(x, w.bfloat16(), None, v.bfloat16(), None))
+
+
+def test_workspace_of_many_rows_and_few_classes():
+    """The logits' gradients have room for the classes that there are, padded to eight: beside them the inputs' gradient and the partial
+    sums of the weights', which are small."""
+    for rows, C, V in [(1 << 20, 32, 150), (1 << 24, 32, 10), (1 << 30, 8, 8), (200000, 64, 1000)]:
+        for dtype, size in ((F32, 6), (BF16, 2), (F16, 2)):
+            staged = rows * C * size if dtype == F32 else 0
+            assert lib().dwo_head_workspace_bytes(rows, C, V, 1, dtype) <= rows * -(-V // 8) * 8 * size + staged + (1 << 26)
