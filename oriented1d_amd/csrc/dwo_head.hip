@@ -330,7 +330,8 @@ static int head_forward(const HeadSizes &s, const void *x, const void *w, const 
     // threads have a row (32768 x 150 classes: 8.3 us for both launches, sixteen 9.6; 64 rows of 63 parts need the sixteen)
     const int parts = (int)((s.V + width - 1) / width);
     const bool few = s.rows <= 128, narrow = !few && parts <= 16;
-    const int group = few || narrow ? 64 : 16, blocks = few ? 1 : (int)((s.rows + group - 1) / group);
+    const int group = few || narrow ? 64 : 16;
+    const int blocks = few ? 1 : (int)std::min((s.rows + group - 1) / group, 1L << 20);  // (a launch has fewer than 2^32 threads)
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
     float *sum = eps > 0.f ? (float *)ws.take((size_t)parts * s.rows * sizeof(float)) : nullptr;
     float *at = (float *)ws.take((size_t)s.rows * sizeof(float));

@@ -735,12 +735,16 @@ struct ProductGroup {
 
 inline PlainEpi plain_epilogue(const Out &out) { return {out, {nullptr, 0, 0, 0}, {nullptr, 0}, nullptr, nullptr, nullptr, 1.f, nullptr, 0, 0, 0}; }
 
+// Workgroups of a launch: it has fewer than 2^32 threads, and these have 512 at most.  Products of more tiles than that take larger ones; of 256 x 256
+// it is as many as 2^39 results need.
+constexpr long kMostGroups = (1L << 23) - 8;
+
 // products whose epilogue is not the plain one
 template <typename T, class S, bool AS, bool BS, bool GATED, class Epi>
 int launch_shape(Product p, const Epi &epi, hipStream_t st) {
     p.mtiles = (int)((p.M + S::BM - 1) / S::BM), p.ntiles = (int)((p.N + S::BN - 1) / S::BN);
     const long total = (long)p.mtiles * p.ntiles * p.splits;
-    if (total > 0x7ffffff0L) return DWO_ERR_BAD_SHAPE;
+    if (total > kMostGroups) return DWO_ERR_BAD_SHAPE;
     product_kernel<T, S, AS, BS, GATED, Epi><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(S::THREADS), 0, st>>>(p, epi);
     return status();
 }
@@ -769,10 +773,12 @@ inline float tile_time(const TileCost &c, long workgroups, long steps) {
 // the tile of a product that is not split
 inline int tile_for(long M, long N, long steps) {
     int best = 0;
-    for (int i = 1; i < 4; i++)
-        if (tile_time(kTileCosts[i], tiles_of(M, N, kTileCosts[i].size, kTileCosts[i].size), steps) <
-            tile_time(kTileCosts[best], tiles_of(M, N, kTileCosts[best].size, kTileCosts[best].size), steps))
+    for (int i = 1; i < 4; i++) {
+        const long tiles = tiles_of(M, N, kTileCosts[i].size, kTileCosts[i].size);
+        if (tiles <= kMostGroups && tile_time(kTileCosts[i], tiles, steps) <
+                                        tile_time(kTileCosts[best], tiles_of(M, N, kTileCosts[best].size, kTileCosts[best].size), steps))
             best = i;
+    }
     return kTileCosts[best].size;
 }
 template <class E>

@@ -204,6 +204,7 @@ static PlainChoice find_choice(const GroupPart *part, int count) {
                 if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 5.f : 0.f);
             }
             if (parts > 1 && workgroups > 4 * kLinCus) break;
+            if (c.size < kTileCosts[0].size && workgroups > kMostGroups - 8 * count) break;  // (each part's are rounded up to eight)
             const float alone = c.first + (float)chain * c.first_step;
             const float t = join + (workgroups <= kLinCus ? alone : fmaxf(alone, 3.5f + makespan(numbers, times, count)));
             if (best.tile == 0 || t < least) best = {c.size, most}, least = t;
@@ -282,7 +283,7 @@ static int launch_group(ProductGroup group, hipStream_t st) {
         p.mtiles = (int)((p.M + S::BM - 1) / S::BM), p.ntiles = (int)((p.N + S::BN - 1) / S::BN);
         const long blocks = ((long)p.mtiles * p.ntiles * p.splits + 7) / 8 * 8;
         all += blocks;
-        if (all > 0x7ffffff0L) return DWO_ERR_BAD_SHAPE;
+        if (all > kMostGroups) return DWO_ERR_BAD_SHAPE;
         group.part[i].blocks = (int)blocks;
     }
     group_kernel<T, S><<<dim3((unsigned)all), dim3(S::THREADS), 0, st>>>(group);

@@ -223,3 +223,33 @@ def test_infinities_of_the_gated_block(place, rows, dtype):
     want = torch.autograd.grad(out, ref, dy.double())
     for g, t, name in zip(got, want, ["dx", "dw_in", "db_in", "dw_out", "db_out"]):
         same_kind(g, t, name)
+
+
+# ---------------------------------------------------------------------------------------------------- as many rows as there may be
+def test_as_many_rows_as_there_may_be():
+    """2^30 rows of few channels: more tiles of the smaller sizes than a launch has room for, and more rows than a pass over them has
+    threads.  The first and last rows, the others being zeros and ignored."""
+    rows, C = 1 << 30, 8
+    x = torch.zeros(rows, C, device="cuda", dtype=torch.bfloat16)
+    ends = torch.randn(74, C, device="cuda").bfloat16()
+    x[:37], x[-37:] = ends[:37], ends[37:]
+    w, b = torch.randn(8, C, device="cuda").bfloat16(), torch.randn(8, device="cuda").bfloat16()
+    with torch.no_grad():
+        y = checkpoint8.linear8(x, w, b)
+    near(torch.cat([y[:37], y[-37:]]), ends.double() @ w.double().t() + b.double(), "y")
+    for m in (37, rows // 3, rows // 2 + 5, rows - 38):
+        assert torch.equal(y[m], b)
+    del y
+    target = torch.full((rows,), -100, device="cuda")
+    some = torch.randint(0, 8, (74,), device="cuda")
+    target[:37], target[-37:] = some[:37], some[37:]
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = losses.linear_cross_entropy(x, w, b, target)
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    ref = leaves64(ends, w)
+    want = F.cross_entropy(F.linear(*ref, b.double()), some)
+    assert abs(float(loss) - float(want)) <= 4e-6 * (abs(float(want)) + 12)
+    for g, t, name in zip((torch.cat([dx[:37], dx[-37:]]), dw), torch.autograd.grad(want, ref), ["dx", "dw"]):
+        near(g, t, name)
+    assert not dx[37:1000].any() and not dx[rows // 2:rows // 2 + 1000].any() and not dx[-1000:-37].any()
