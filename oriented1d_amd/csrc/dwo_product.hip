@@ -189,7 +189,9 @@ static PlainChoice find_choice(const GroupPart *part, int count) {
     float least = 0.f;
     long longest = 0;
     for (int i = 0; i < count; i++) longest = part[i].p.steps > longest ? part[i].p.steps : longest;
+    bool many = false;  // more than four workgroups a CU in the largest tiles
     for (const TileCost &c : kTileCosts) {
+        bool chained = false;  // with fewer splits the longest sum takes more time than a CU's share of all
         for (const long parts : {1L, 2L, 3L, 4L, 6L, 8L, 12L, 16L, 24L, 32L}) {
             const long most = (longest + parts - 1) / parts;
             if (parts > 1 && most < 4) break;
@@ -203,10 +205,16 @@ static PlainChoice find_choice(const GroupPart *part, int count) {
                 chain = steps > chain ? steps : chain;
                 if (splits > 1) join += (float)(splits * p.M) * (float)p.N * 8.f / 4e6f + (join == 0.f ? 5.f : 0.f);
             }
-            if (parts > 1 && workgroups > 4 * kLinCus) break;
+            if (parts == 1 && c.size == kTileCosts[0].size) many = workgroups > 4 * kLinCus;
+            // (one product may have that many without splits, and another's long sums be what is left to split: loss and gradients of 4 * 10^6 rows, 64
+            // channels and 150 classes in bf16 3.2 ms, with that product in one piece 21; 10^6 x 32 x 16 0.45 and 2.55)
+            if (parts > 1 && workgroups > 4 * kLinCus && !(many && chained)) break;
             if (c.size < kTileCosts[0].size && workgroups > kMostGroups - 8 * count) break;  // (each part's are rounded up to eight)
             const float alone = c.first + (float)chain * c.first_step;
             const float t = join + (workgroups <= kLinCus ? alone : fmaxf(alone, 3.5f + makespan(numbers, times, count)));
+            float share = 0.f, most_time = 0.f;
+            for (int i = 0; i < count; i++) share += (float)numbers[i] * times[i] / kLinCus, most_time = fmaxf(most_time, times[i]);
+            chained = most_time > share;
             if (best.tile == 0 || t < least) best = {c.size, most}, least = t;
         }
     }

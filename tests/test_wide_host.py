@@ -207,3 +207,15 @@ def test_workspace_of_many_rows_and_few_classes():
         for dtype, size in ((F32, 6), (BF16, 2), (F16, 2)):
             staged = rows * C * size if dtype == F32 else 0
             assert lib().dwo_head_workspace_bytes(rows, C, V, 1, dtype) <= rows * -(-V // 8) * 8 * size + staged + (1 << 26)
+
+
+def test_long_sums_are_split_beside_many_tiles():
+    """Weight gradients over many rows have room for their partial sums (eight splits or more) also where the inputs' gradient alone has more tiles than
+    fill the chip: in one piece they would be one workgroup's."""
+    L = lib()
+    for rows, C, V in [(1000000, 32, 16), (1 << 22, 64, 150), (1 << 24, 32, 10)]:
+        for dtype in (BF16, F16):
+            held = rows * -(-V // 8) * 8 * 2
+            assert L.dwo_head_workspace_bytes(rows, C, V, 1, dtype) >= held + 8 * V * C * 4
+            odd = 0 if V % 8 == 0 else held  # (a copy of dy with whole pieces of eight)
+            assert L.dwo_layer8_workspace_bytes(rows, C, V, 1, dtype) >= rows * C * 2 + odd + 8 * V * C * 4

@@ -253,3 +253,23 @@ def test_as_many_rows_as_there_may_be():
     for g, t, name in zip((torch.cat([dx[:37], dx[-37:]]), dw), torch.autograd.grad(want, ref), ["dx", "dw"]):
         near(g, t, name)
     assert not dx[37:1000].any() and not dx[rows // 2:rows // 2 + 1000].any() and not dx[-1000:-37].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_rows_and_few_classes(dtype):
+    """A product of many tiles next to one of long sums, which are split."""
+    rows, C, V = 400003, 24, 20
+    x, w, b, target = make_head(rows, C, V, dtype, ignored=0.1)
+    up = torch.randn(rows, device="cuda")
+    loss = losses.linear_cross_entropy(x, w, b, target, reduction="none")
+    ref = leaves64(x, w, b)
+    want = F.cross_entropy(F.linear(*ref), target, reduction="none", ignore_index=-100)
+    near(loss, want, "loss")
+    for g, t, name in zip(torch.autograd.grad(loss, [x, w, b], up), torch.autograd.grad(want, ref, up.double()), ["dx", "dw", "db"]):
+        near(g, t, name)
+    y = checkpoint8.linear8(x, w, b)
+    dy = torch.randn_like(y)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    near(dx, dy.double() @ w.double(), "dx")
+    near(dw, dy.double().t() @ held8(x.detach()), "dw")
+    near(db, dy.double().sum(0), "db")
