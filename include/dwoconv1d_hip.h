@@ -321,7 +321,8 @@ int dwo_linear_norm_planes(const void *x, const float *gamma_in, const float *be
  *
  * dwo_pack8:   8-bit checkpoints: x [rows,C] -> codes [rows,C] (signed bytes q) and exps [rows,ceil(C/32)] (bytes), standing for q * 2^(exp -
  *              127): groups of 32 neighbours along a row, scale 2^(floor(log2(largest magnitude)) - 6), at least 2^-126, q rounded to even
- *              and at most 127; exp 0: zeros, 255: a group with an infinity or NaN, all NaN.  Where y is not null also y = act(x).
+ *              and at most 127; exp 0: zeros, 255: a group with an infinity or NaN, all NaN.  Where y is not null also y = act(x), and with
+ *              codes null y alone.
  * dwo_unpack8: out [rows,C] = the values held, or where dy is not null dy * act'(value held).
  * dwo_layer8:  y [rows,D] = x [rows,C] w^T + bias for w [D,C] (bias may be null), and where codes is not null x's checkpoint.
  *              _backward: dx = dy w, dw = dy^T (values held), db = sum over rows of dy; each may be null, db only goes with dw.

@@ -41,8 +41,8 @@ __device__ __forceinline__ void codes8(mma_u2 w, float (&q)[8]) {
     for (int e = 0; e < 8; e++) q[e] = (float)((int)(w[e / 4] << (24 - 8 * (e % 4))) >> 24);
 }
 
-// codes of x and, where y is not null, y = act(x).  WIDE: rows of whole groups, eight values per lane; otherwise half a wave takes a group,
-// a value per lane.
+// Codes of x, where codes is not null, and where y is not null y = act(x).  WIDE: rows of whole groups, eight values per lane; otherwise half a
+// wave takes a group, a value per lane.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, T *__restrict__ y, int8_t *__restrict__ codes,
                                                     uint8_t *__restrict__ exps, long rows, int C, int act) {
@@ -54,19 +54,21 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, T *
         if constexpr (WIDE) {
             float v[8];
             load8(x + i * 8, v);
-            unsigned most = 0;
+            if (codes != nullptr) {
+                unsigned most = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) most = max(most, magnitude(v[e]));
-            most = max(most, (unsigned)__shfl_xor((int)most, 1, 64));
-            most = max(most, (unsigned)__shfl_xor((int)most, 2, 64));
-            const unsigned e = group_exponent(__uint_as_float(most));
-            const float inverse = group_inverse(e);
-            mma_u2 w = mma_u2{0u, 0u};
+                for (int e = 0; e < 8; e++) most = max(most, magnitude(v[e]));
+                most = max(most, (unsigned)__shfl_xor((int)most, 1, 64));
+                most = max(most, (unsigned)__shfl_xor((int)most, 2, 64));
+                const unsigned e = group_exponent(__uint_as_float(most));
+                const float inverse = group_inverse(e);
+                mma_u2 w = mma_u2{0u, 0u};
 #pragma unroll
-            for (int k = 0; k < 8; k++) w[k / 4] |= (unsigned)(quantum(v[k], inverse) & 0xff) << (8 * (k % 4));
-            if (e == 255u) w = mma_u2{0u, 0u};
-            reinterpret_cast<mma_u2 *>(codes)[i] = w;
-            if (i % LANES == 0) exps[group] = (uint8_t)e;
+                for (int k = 0; k < 8; k++) w[k / 4] |= (unsigned)(quantum(v[k], inverse) & 0xff) << (8 * (k % 4));
+                if (e == 255u) w = mma_u2{0u, 0u};
+                reinterpret_cast<mma_u2 *>(codes)[i] = w;
+                if (i % LANES == 0) exps[group] = (uint8_t)e;
+            }
             if (y != nullptr) {
                 float o[8], slope;
 #pragma unroll
@@ -79,12 +81,14 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, T *
             const bool real = c < C;
             const long at = row * C + c;
             const float v = real ? to_float(x[at]) : 0.f;
-            unsigned most = magnitude(v);
+            if (codes != nullptr) {
+                unsigned most = magnitude(v);
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, off, 64));
-            const unsigned e = group_exponent(__uint_as_float(most));
-            if (real) codes[at] = e == 255u ? 0 : (int8_t)quantum(v, group_inverse(e));
-            if (i % LANES == 0) exps[group] = (uint8_t)e;
+                for (int off = 16; off > 0; off >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, off, 64));
+                const unsigned e = group_exponent(__uint_as_float(most));
+                if (real) codes[at] = e == 255u ? 0 : (int8_t)quantum(v, group_inverse(e));
+                if (i % LANES == 0) exps[group] = (uint8_t)e;
+            }
             if (y != nullptr && real) {
                 float o, slope;
                 act_wide<T>(act, v, o, slope);
@@ -196,7 +200,7 @@ using namespace dwo;
 extern "C" {
 
 int dwo_pack8(const void *x, void *y, void *codes, void *exps, size_t rows, int C, int act, int dtype, void *stream) {
-    if (!x || !codes || !exps) return DWO_ERR_NULL_POINTER;
+    if (!x || (codes != nullptr ? !exps : !y)) return DWO_ERR_NULL_POINTER;
     if (!sizes_ok((long)rows, C, x, y, codes, nullptr) || act < 0 || act > ACT_SILU) return DWO_ERR_BAD_SHAPE;
     (void)hipGetLastError();
     hipStream_t st = (hipStream_t)stream;

@@ -65,16 +65,19 @@ void backward_allowed(const Place &at) {
 Tensor as_type(const Tensor &t, at::ScalarType type) { return !t.defined() || t.scalar_type() == type ? t : t.to(type); }
 
 // ------------------------------------------------------------------------------------------------- 8-bit checkpoints
-// (codes, exponents, act(x) or nothing)
-std::tuple<Tensor, Tensor, Tensor> pack8(const Tensor &x_, int64_t act, bool with_value) {
+// (codes and exponents or nothing, act(x) or nothing)
+std::tuple<Tensor, Tensor, Tensor> pack8(const Tensor &x_, int64_t act, bool with_codes, bool with_value) {
     const Rows r(x_, "x");
     const Place at(x_);
     const Tensor x = dense(x_);
-    Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    Tensor exps = at::empty(with_last(x, up(r.C, 32)), x.options().dtype(at::kByte));
+    Tensor codes, exps;
+    if (with_codes) {
+        codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+        exps = at::empty(with_last(x, up(r.C, 32)), x.options().dtype(at::kByte));
+    }
     Tensor y = with_value ? at::empty(x.sizes(), x.options()) : Tensor();
     if (r.rows > 0)
-        check(lib.pack8(ptr(x), mptr(y), codes.data_ptr(), exps.data_ptr(), (size_t)r.rows, as_int(r.C), (int)act, dtype_code(x), at.stream),
+        check(lib.pack8(ptr(x), mptr(y), mptr(codes), mptr(exps), (size_t)r.rows, as_int(r.C), (int)act, dtype_code(x), at.stream),
               "dwo_pack8");
     return {codes, exps, y};
 }
@@ -102,7 +105,7 @@ Tensor unpack8(const Tensor &codes_, const Tensor &exps_, const OptTensor &dy_, 
 struct Act8 : torch::autograd::Function<Act8> {
     static Tensor forward(Context *ctx, const Tensor &x, int64_t act) {
         ctx->set_materialize_grads(false);
-        auto [codes, exps, y] = pack8(x, act, true);
+        auto [codes, exps, y] = pack8(x, act, true, true);
         ctx->save_for_backward({codes, exps});
         ctx->saved_data["act"] = act, ctx->saved_data["type"] = (int64_t)x.scalar_type();
         return y;
@@ -117,11 +120,12 @@ struct Act8 : torch::autograd::Function<Act8> {
 };
 Tensor act8(const Tensor &x, int64_t act) {
     py::gil_scoped_release nogil;
-    return Act8::apply(x, act);
+    if (at::GradMode::is_enabled() && trains(x)) return Act8::apply(x, act);
+    return std::get<2>(pack8(x, act, false, true));
 }
 std::tuple<Tensor, Tensor> pack8_entry(const Tensor &x) {
     py::gil_scoped_release nogil;
-    auto [codes, exps, none] = pack8(x.detach(), 0, false);
+    auto [codes, exps, none] = pack8(x.detach(), 0, true, false);
     return {codes, exps};
 }
 Tensor unpack8_entry(const Tensor &codes, const Tensor &exps, at::ScalarType type) {
@@ -229,7 +233,7 @@ struct Gated : torch::autograd::Function<Gated> {
         const int64_t rows = x.numel() / x.size(-1), H = w_out.size(1);
         Tensor held = x, exps, keep;
         if (held8) {
-            auto [codes, e, none] = pack8(x, 0, false);
+            auto [codes, e, none] = pack8(x, 0, true, false);
             held = codes, exps = e;
         } else {
             keep = at::empty({2, rows, up8(H)}, x.options().dtype(at::kFloat));

@@ -219,3 +219,10 @@ def test_long_sums_are_split_beside_many_tiles():
             assert L.dwo_head_workspace_bytes(rows, C, V, 1, dtype) >= held + 8 * V * C * 4
             odd = 0 if V % 8 == 0 else held  # (a copy of dy with whole pieces of eight)
             assert L.dwo_layer8_workspace_bytes(rows, C, V, 1, dtype) >= rows * C * 2 + odd + 8 * V * C * 4
+
+
+def test_values_without_codes():
+    L = lib()
+    assert L.dwo_pack8(ONE, None, None, None, 4, 8, 0, BF16, None) == -1  # neither
+    assert L.dwo_pack8(ONE, ONE, ONE, None, 4, 8, 0, BF16, None) == -1  # codes without exponents
+    assert L.dwo_pack8(ONE, ONE, None, None, 0, 8, 0, BF16, None) == -2  # (accepted, but for its rows)

@@ -273,3 +273,21 @@ def test_many_rows_and_few_classes(dtype):
     near(dx, dy.double() @ w.double(), "dx")
     near(dw, dy.double().t() @ held8(x.detach()), "dw")
     near(db, dy.double().sum(0), "db")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_activation_without_gradients_keeps_nothing(dtype, act):
+    """The same bits as with them; no codes are made where nothing will read them."""
+    for shape in ((4096, 1024), (1000, 333), (7,), (0, 64)):
+        x = (3 * torch.randn(shape, device="cuda")).to(dtype)
+        want = checkpoint8.act8(x.clone().requires_grad_(), act).detach()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = checkpoint8.act8(x, act)
+        taken = torch.cuda.max_memory_allocated() - before
+        # (codes are a byte a value; what the allocator hands out beyond what is asked for is at most 1 MB)
+        assert taken <= y.numel() * y.element_size() + max(y.numel() // 2, 1 << 20)
+        assert torch.equal(y, want)
+        with torch.no_grad():
+            assert torch.equal(checkpoint8.act8(x.clone().requires_grad_(), act), want)
