@@ -328,20 +328,23 @@ class ConvNeXt1D(nn.Module):
             return outs
         return self.norm(x.mean((-2, -1)))
 
-    def forward(self, x):
+    def forward(self, x, target=None, label_smoothing=0.0, ignore_index=-100):
+        """The logits (or stage outputs) of the images x; with ``target`` their ``loss``, so that what wraps or hooks the network's call
+        sees a training step that takes it (a data-parallel wrapper: ``wrapper(x, target)``)."""
+        if target is not None and self.out_stages:
+            raise ValueError("a network of stage outputs has no classes")
         x = self.forward_features(x)
-        return x if self.out_stages else self.head(x)
+        if target is None:
+            return x if self.out_stages else self.head(x)
+        if not fused.plain(self.head, nn.Linear):
+            return F.cross_entropy(self.head(x).float(), target, ignore_index=ignore_index, label_smoothing=label_smoothing)
+        return losses.linear_cross_entropy(x, self.head.weight, self.head.bias, target, ignore_index=ignore_index,
+                                           label_smoothing=label_smoothing)
 
     def loss(self, x, target, label_smoothing=0.0, ignore_index=-100):
         """Mean softmax cross entropy of the images x against int64 classes, as fp32: ``F.cross_entropy(self(x), target, ...)`` without
-        its logits in memory."""
-        if self.out_stages:
-            raise ValueError("a network of stage outputs has no classes")
-        features = self.forward_features(x)
-        if not fused.plain(self.head, nn.Linear):
-            return F.cross_entropy(self.head(features).float(), target, ignore_index=ignore_index, label_smoothing=label_smoothing)
-        return losses.linear_cross_entropy(features, self.head.weight, self.head.bias, target, ignore_index=ignore_index,
-                                           label_smoothing=label_smoothing)
+        its logits in memory.  It is the network's call with a target: hooks see it, with the loss as the result."""
+        return self(x, target, label_smoothing, ignore_index)
 
 
 def convnext_tiny_1d(variant="1d", **kw):

@@ -5,6 +5,7 @@ import torch
 import torch.nn.functional as F
 
 from oriented1d_amd import checkpoint8, feedforward, losses
+from oriented1d_amd.convnext1d import ConvNeXt1D
 from test_wide_gpu import DTYPES, IDS, gated64, held8, leaves64, make_gated, make_head, near
 
 pytestmark = pytest.mark.gpu
@@ -291,3 +292,29 @@ def test_activation_without_gradients_keeps_nothing(dtype, act):
         assert torch.equal(y, want)
         with torch.no_grad():
             assert torch.equal(checkpoint8.act8(x.clone().requires_grad_(), act), want)
+
+
+# ---------------------------------------------------------------------------------------------------- the networks' loss
+def test_loss_goes_through_the_networks_call():
+    """Hooks on the network see it, and a wrapper of its call can take it."""
+    torch.manual_seed(0)
+    net = ConvNeXt1D(num_classes=11, depths=(1, 1, 1, 1), dims=(32, 32, 64, 64)).cuda()
+    image, target = torch.randn(2, 3, 64, 64, device="cuda"), torch.tensor([3, -1], device="cuda")
+    want = F.cross_entropy(net(image), target, ignore_index=-1, label_smoothing=0.2)
+
+    class Wrapper(torch.nn.Module):
+        def __init__(self, module):
+            super().__init__()
+            self.module = module
+
+        def forward(self, *args, **kwargs):
+            return self.module(*args, **kwargs)
+
+    seen = []
+    handle = net.register_forward_hook(lambda module, args, out: seen.append(out))
+    for loss in (net.loss(image, target, ignore_index=-1, label_smoothing=0.2),
+                 Wrapper(net)(image, target, ignore_index=-1, label_smoothing=0.2)):
+        assert loss.shape == () and abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    handle.remove()
+    assert len(seen) == 2 and seen[0].shape == ()
+    assert net(image).shape == (2, 11)
