@@ -238,6 +238,13 @@ class Block(nn.Module):
             return fused.linear_tail(y, self.pwconv2, self.gamma, x)
         return self._join(x, held.linear8(y, self.pwconv2.weight, self.pwconv2.bias) if lean else self.pwconv2(y))
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        # (blocks pickled before there were gated ones and checkpoints)
+        self.__dict__.setdefault("checkpoint8", False)
+        if "mlp" not in self._modules:
+            self.__dict__.setdefault("mlp", None)
+
     def _join(self, x, y):
         """The residual branch's end: layer scale, planes and the sum with the block's input."""
         if self.gamma is not None:

@@ -226,3 +226,18 @@ def test_values_without_codes():
     assert L.dwo_pack8(ONE, None, None, None, 4, 8, 0, BF16, None) == -1  # neither
     assert L.dwo_pack8(ONE, ONE, ONE, None, 4, 8, 0, BF16, None) == -1  # codes without exponents
     assert L.dwo_pack8(ONE, ONE, None, None, 0, 8, 0, BF16, None) == -2  # (accepted, but for its rows)
+
+
+def test_blocks_pickled_before_they_had_an_mlp_of_their_own():
+    import copy
+    import pickle
+
+    block = Block(16, (7,), False)
+    state = block.__getstate__() if hasattr(block, "__getstate__") else block.__dict__
+    state = {k: v for k, v in copy.copy(state if state is not None else block.__dict__).items() if k not in ("mlp", "checkpoint8")}
+    old = Block.__new__(Block)
+    old.__setstate__(state)
+    assert old.mlp is None and old.checkpoint8 is False
+    for mlp in ("plain", "gated"):
+        kept = pickle.loads(pickle.dumps(Block(16, (7,), False, mlp=mlp, checkpoint8=True)))
+        assert kept.checkpoint8 and (kept.mlp is None) == (mlp == "plain")
