@@ -317,7 +317,8 @@ int dwo_linear_norm_planes(const void *x, const float *gamma_in, const float *be
  * `dtype` (DWO_F32, DWO_BF16, DWO_F16), parameters' gradients are written as grad_dtype.  rows is at most 2^30, channels are at most 65536;
  * inputs, outputs that a kernel reads again, and workspaces are 16-byte aligned.  Sums, exponentials and statistics are fp32.  ws holds at least
  * the bytes that the matching function gives (0: sizes that are not accepted); nothing in it has to survive a call, and calls that
- * overlap in time take one each.
+ * overlap in time take one each.  16-bit operands that one product of a call makes for another are rounded to `dtype` once, or where the
+ * forward pass has no more than 2^28 multiply-adds held in two such values.
  *
  * dwo_pack8:   8-bit checkpoints: x [rows,C] -> codes [rows,C] (signed bytes q) and exps [rows,ceil(C/32)] (bytes), standing for q * 2^(exp -
  *              127): groups of 32 neighbours along a row, scale 2^(floor(log2(largest magnitude)) - 6), at least 2^-126, q rounded to even

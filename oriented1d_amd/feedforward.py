@@ -23,7 +23,11 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, activation="gelu", checkpoint8=False)
 
     CUDA tensors of type float32, bfloat16 and float16; parameters may have another of these types and get gradients of their own.  Under
     autocast x and parameters are converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose
-    the same values from PyTorch ops, which ``checkpoint8`` cannot; gradients of gradients are refused."""
+    the same values from PyTorch ops, which ``checkpoint8`` cannot; gradients of gradients are refused.
+
+    In 16 bits what one product makes for another (hidden units and their gradients) is rounded to the type of x; where rows * H * (2 C + D)
+    is at most 2^28 it is held in two such values, and in a forward pass of up to four rows the hidden units are fp32.  So the same row may come
+    out with other last bits in a small batch than in a large one, nearer to the formula."""
     code = activation_code(activation)
     if not ordinary(x, w_in, b_in, w_out, b_out):
         if checkpoint8:

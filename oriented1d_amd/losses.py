@@ -37,7 +37,11 @@ def linear_cross_entropy(x, weight, bias, target, *, reduction="mean", ignore_in
 
     CUDA tensors of type float32, bfloat16 and float16; parameters may have another of these types and get gradients of their own.  Under
     autocast x and parameters are converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose the
-    same values from PyTorch ops; gradients of gradients are refused."""
+    same values from PyTorch ops; gradients of gradients are refused.
+
+    Losses are computed in fp32.  In 16 bits the logits' gradients are rounded to the type of x for the products that read them; where rows *
+    V * C is at most 2^28 they are held in two such values, so that a row's gradient may have other last bits in a small batch than in a
+    large one, nearer to the formula."""
     if reduction not in ("mean", "none"):
         raise ValueError("reduction must be 'mean' or 'none'")
     if not 0.0 <= label_smoothing <= 1.0:
