@@ -18,7 +18,8 @@ def _composed(x, weight, bias, target, reduction, ignore_index, label_smoothing)
     counts = target != ignore_index
     is_class = counts & (target >= 0) & (target < logits.shape[-1])
     # rows that are ignored may hold anything, and those whose target is no class are NaN, as are their gradients
-    logits = torch.where(counts.unsqueeze(-1), logits, 0.0) + torch.where(counts & ~is_class, float("nan"), 0.0).unsqueeze(-1)
+    nothing = torch.where(counts & ~is_class, float("nan"), 0.0).to(logits.dtype)
+    logits = torch.where(counts.unsqueeze(-1), logits, 0.0) + nothing.unsqueeze(-1)
     logs = F.log_softmax(logits, -1)
     loss = -logs.gather(-1, torch.where(is_class, target, 0).unsqueeze(-1)).squeeze(-1)
     if label_smoothing > 0:

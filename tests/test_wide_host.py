@@ -241,3 +241,14 @@ def test_blocks_pickled_before_they_had_an_mlp_of_their_own():
     for mlp in ("plain", "gated"):
         kept = pickle.loads(pickle.dumps(Block(16, (7,), False, mlp=mlp, checkpoint8=True)))
         assert kept.checkpoint8 and (kept.mlp is None) == (mlp == "plain")
+
+
+def test_transforms_give_fp32_losses_whatever_the_default_type():
+    x, w, target = torch.randn(3, 4, 8), torch.randn(16, 8), torch.zeros(3, 4, dtype=torch.long)
+    torch.set_default_dtype(torch.float64)
+    try:
+        for reduction in ("mean", "none"):
+            got = torch.func.vmap(lambda a, t: losses.linear_cross_entropy(a, w, None, t, reduction=reduction))(x, target)
+            assert got.dtype == torch.float32
+    finally:
+        torch.set_default_dtype(torch.float32)

@@ -254,6 +254,8 @@ def test_as_many_rows_as_there_may_be():
     for g, t, name in zip((torch.cat([dx[:37], dx[-37:]]), dw), torch.autograd.grad(want, ref), ["dx", "dw"]):
         near(g, t, name)
     assert not dx[37:1000].any() and not dx[rows // 2:rows // 2 + 1000].any() and not dx[-1000:-37].any()
+    del x, target, loss, dx, g
+    torch.cuda.empty_cache()  # (80 GB)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -318,3 +320,33 @@ def test_loss_goes_through_the_networks_call():
     handle.remove()
     assert len(seen) == 2 and seen[0].shape == ()
     assert net(image).shape == (2, 11)
+
+
+# ---------------------------------------------------------------------------------------------------- one row without leading dimensions
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_without_leading_dimensions(dtype):
+    """x [C]: as a batch of one, in every operator, with any of the biases, and the composed forms on the GPU beside them."""
+    args, _ = make_gated(1, 40, 24, 24, dtype)
+    x, w_in, b_in, w_out, b_out = args
+    target = torch.tensor(5, device="cuda")
+    calls = [lambda a, t: checkpoint8.act8(a), lambda a, t: checkpoint8.linear8(a, w_in, b_in),
+             lambda a, t: feedforward.gated_mlp(a, w_in, None, w_out, b_out), lambda a, t: feedforward.gated_mlp(a, w_in, b_in, w_out, None),
+             lambda a, t: losses.linear_cross_entropy(a, w_in, b_in, t, reduction="none"),
+             lambda a, t: losses.linear_cross_entropy(a, w_in, None, t, label_smoothing=0.1)]
+    for k, call in enumerate(calls):
+        leaf = x.detach()[0].requires_grad_()
+        y, batch = call(leaf, target), call(x, target[None])
+        assert torch.equal(y.reshape(-1), batch.reshape(-1)) and y.dim() == (0 if k > 3 else 1)
+        some = [t for t in (w_in, b_in, w_out, b_out)]
+        got = torch.autograd.grad(y, [leaf, *some], torch.ones_like(y), allow_unused=True)
+        want = torch.autograd.grad(batch, [x, *some], torch.ones_like(batch), allow_unused=True)
+        for g, t in zip(got, want):
+            assert (g is None) == (t is None) and (g is None or torch.equal(g.reshape(-1), t.reshape(-1)))
+    packed = checkpoint8.pack8(x.detach()[0])
+    assert torch.equal(checkpoint8.unpack8(packed).double(), held8(x.detach())[0])
+    r = torch.finfo(dtype).eps / 2
+    for k in (2, 3, 4, 5):
+        got = torch.func.vmap(calls[k])(x.detach().expand(3, -1).contiguous(), target.expand(3))
+        size = float(calls[k](x, target[None]).abs().max())
+        # (composed of layers: roundings of g, u, their product and the result, each of a half's size at most, through sums of 24 and 40 terms)
+        assert (got - calls[k](x, target[None])).abs().max() <= 8 * r * (size + 1)
