@@ -360,6 +360,37 @@ int dwo_head_backward(const float *up, const void *x, const void *w, const void 
                       float smoothing, const float *lse, const float *count, void *dx, void *dw, void *db, void *ws,
                       size_t ws_bytes, size_t rows, int C, int V, int dtype, int grad_dtype, void *stream);
 
+/*
+ * Operators between a teacher and its student; no counterpart in the reference's extension.  Types, sizes, alignment and workspaces as above.
+ *
+ * dwo_int8_rows:   x [rows,C] as 8-bit integers: with a the largest magnitude of a row, codes [rows,C'] (C' the next multiple of sixteen, zeros behind
+ *                  C) = 127 x / a to the nearest, ties to even, and steps [rows] = a / 127.  A row with an infinity or NaN has codes of zero and
+ *                  a step that is NaN.
+ * dwo_int8_linear: y [rows,D] = act((sum_c q_c p_c) (a / 127) steps + bias) for x [rows,C], whose codes q are made as above, and a weight's codes
+ *                  p [D,C'] and steps [D]; whole numbers are summed.  bias (of x's type) may be null; act is DWO_GELU, DWO_SILU or -1.
+ * dwo_top:         values [rows,k] (x's type) and places [rows,k] (64 bits) of the k largest values of each row of x [rows,V], largest first, of equal
+ *                  ones the lowest place first; NaN is above everything.  V at most 2^24, k at most 1024 and V, rows * V at most 2^40.
+ * dwo_distill:     loss of logits l = x w^T + bias for w [V,C] against entries of a teacher, k (at most 1024) a row: logits [rows,k] of logits_dtype and
+ *                  classes [rows,k] (64 bits): T^2 sum_j p_j (log p_j - log softmax(l / T)[class_j]), p the softmax of a row's logits / T, T the
+ *                  temperature (1e-4 to 1e4).  Entries of class -1 or logit -infinity are absent; a row without entries is 0, one with another class
+ *                  that is none, or a logit that is NaN or infinite, NaN.  count null: loss [rows]; else loss[0] is the mean over the rows with
+ *                  entries and count[0] receives their number.  keep [rows * (3 k + 2)] and count are what the backward pass takes, up [rows], or
+ *                  up[0] for a mean, the gradient of the loss; dx, dw and db may be null, db only goes with dw.
+ */
+int dwo_int8_rows(const void *x, void *codes, float *steps, size_t rows, int C, int dtype, void *stream);
+size_t dwo_int8_workspace_bytes(size_t rows, int C, int D, int dtype);
+int dwo_int8_linear(const void *x, const void *codes, const float *steps, const void *bias, void *y, void *ws, size_t ws_bytes, size_t rows,
+                    int C, int D, int act, int dtype, void *stream);
+size_t dwo_top_workspace_bytes(size_t rows, int V, int k, int dtype);
+int dwo_top(const void *x, void *values, void *places, void *ws, size_t ws_bytes, size_t rows, int V, int k, int dtype, void *stream);
+size_t dwo_distill_workspace_bytes(size_t rows, int C, int V, int k, int backward, int dtype);
+int dwo_distill_forward(const void *x, const void *w, const void *bias, const void *logits, const void *classes, float temperature, float *keep,
+                        float *loss, float *count, void *ws, size_t ws_bytes, size_t rows, int C, int V, int k, int dtype, int logits_dtype,
+                        void *stream);
+int dwo_distill_backward(const float *up, const void *x, const void *w, const void *bias, const float *keep, float temperature, const float *count,
+                         void *dx, void *dw, void *db, void *ws, size_t ws_bytes, size_t rows, int C, int V, int k, int dtype, int grad_dtype,
+                         void *stream);
+
 #ifdef __cplusplus
 }
 #endif

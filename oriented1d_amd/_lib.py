@@ -61,6 +61,14 @@ SIGNATURES = {
     "dwo_head_workspace_bytes": (_sz, [_sz] + [_i] * 4),
     "dwo_head_forward": (_i, [_vp] * 4 + [ctypes.c_longlong, ctypes.c_float] + [_vp] * 4 + [_sz, _sz] + [_i] * 3 + [_vp]),
     "dwo_head_backward": (_i, [_vp] * 5 + [ctypes.c_longlong, ctypes.c_float] + [_vp] * 6 + [_sz, _sz] + [_i] * 4 + [_vp]),
+    "dwo_int8_rows": (_i, [_vp] * 3 + [_sz] + [_i] * 2 + [_vp]),
+    "dwo_int8_workspace_bytes": (_sz, [_sz] + [_i] * 3),
+    "dwo_int8_linear": (_i, [_vp] * 6 + [_sz, _sz] + [_i] * 4 + [_vp]),
+    "dwo_top_workspace_bytes": (_sz, [_sz] + [_i] * 3),
+    "dwo_top": (_i, [_vp] * 4 + [_sz, _sz] + [_i] * 3 + [_vp]),
+    "dwo_distill_workspace_bytes": (_sz, [_sz] + [_i] * 5),
+    "dwo_distill_forward": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_sz, _sz] + [_i] * 5 + [_vp]),
+    "dwo_distill_backward": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 5 + [_sz, _sz] + [_i] * 5 + [_vp]),
 }
 
 _lib = None

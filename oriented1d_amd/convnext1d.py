@@ -17,6 +17,7 @@ import torch.nn.functional as F
 
 from . import checkpoint8 as held, fused, losses
 from .feedforward import GatedMLP
+from .int8 import LinearInt8
 from .dwoconv1d import DepthwiseOrientedConv1d
 
 # (block kernel sizes, stem kernel size) per variant -- models/convnext.py:485-492
@@ -222,7 +223,8 @@ class Block(nn.Module):
         if self.mlp is not None:
             y = self.mlp(y)
             return fused.nhwc_scale_add_nchw(y, self.gamma, x) if fuse else self._join(x, y)
-        if fuse and not self.plus_plus:
+        held1, held2 = isinstance(self.pwconv1, LinearInt8), isinstance(self.pwconv2, LinearInt8)
+        if fuse and not self.plus_plus and not (held1 or held2):
             out = fused.block_mlp(y, self.pwconv1, self.pwconv2, self.gamma, x)
             if out is not None:
                 return out
@@ -231,10 +233,12 @@ class Block(nn.Module):
         if lean:
             y = held.act8(held.linear8(y, self.pwconv1.weight, self.pwconv1.bias))
         else:
-            y = fused.linear_gelu(y, self.pwconv1)
+            y = self.pwconv1(y, activation="gelu") if held1 else fused.linear_gelu(y, self.pwconv1)
         if self.plus_plus:
             y = self.dwconv2(y)
         if fuse:  # layer scale + permute + residual behind the layer (no stochastic depth in eval)
+            if held2:
+                return fused.nhwc_scale_add_nchw(self.pwconv2(y), self.gamma, x)
             return fused.linear_tail(y, self.pwconv2, self.gamma, x)
         return self._join(x, held.linear8(y, self.pwconv2.weight, self.pwconv2.bias) if lean else self.pwconv2(y))
 
@@ -335,12 +339,19 @@ class ConvNeXt1D(nn.Module):
             return outs
         return self.norm(x.mean((-2, -1)))
 
-    def forward(self, x, target=None, label_smoothing=0.0, ignore_index=-100):
-        """The logits (or stage outputs) of the images x; with ``target`` their ``loss``, so that what wraps or hooks the network's call
-        sees a training step that takes it (a data-parallel wrapper: ``wrapper(x, target)``)."""
-        if target is not None and self.out_stages:
+    def forward(self, x, target=None, label_smoothing=0.0, ignore_index=-100, teacher=None, temperature=1.0):
+        """The logits (or stage outputs) of the images x; with ``target`` their ``loss``, with ``teacher`` (a teacher's top logits and their
+        classes) what ``distill`` gives, so that what wraps or hooks the network's call sees a training step that takes it (a data-parallel
+        wrapper: ``wrapper(x, target)``, ``wrapper(x, teacher=top)``)."""
+        if (target is not None or teacher is not None) and self.out_stages:
             raise ValueError("a network of stage outputs has no classes")
+        if target is not None and teacher is not None:
+            raise ValueError("a target or a teacher, not both: add the losses of two calls")
         x = self.forward_features(x)
+        if teacher is not None:
+            if not fused.plain(self.head, nn.Linear):
+                return losses.distillation_of(self.head(x), *teacher, temperature)
+            return losses.linear_distillation(x, self.head.weight, self.head.bias, *teacher, temperature=temperature)
         if target is None:
             return x if self.out_stages else self.head(x)
         if not fused.plain(self.head, nn.Linear):
@@ -352,6 +363,16 @@ class ConvNeXt1D(nn.Module):
         """Mean softmax cross entropy of the images x against int64 classes, as fp32: ``F.cross_entropy(self(x), target, ...)`` without
         its logits in memory.  It is the network's call with a target: hooks see it, with the loss as the result."""
         return self(x, target, label_smoothing, ignore_index)
+
+    def distill(self, x, teacher, temperature=1.0):
+        """``losses.linear_distillation`` of the images x against ``teacher``, the ``losses.TopLogits`` of another network on them (its
+        ``top_logits``), without the network's own logits in memory.  It is the network's call with a teacher, as ``loss``."""
+        return self(x, teacher=teacher, temperature=temperature)
+
+    def top_logits(self, x, k):
+        """The ``k`` largest logits of each of the images x and their classes, without gradients: what a student learns from."""
+        with torch.no_grad():
+            return losses.top_logits(self(x), k)
 
 
 def convnext_tiny_1d(variant="1d", **kw):

@@ -1,0 +1,423 @@
+// The loss of a linear layer over many classes against a teacher's top logits, without keeping its own logits.  Row m has entries j: a class c_j and the
+// teacher's logit t_j; those of class -1, or whose logit is -infinity, are absent.
+//   p = softmax over the entries that are there of t / T,  l = x w^T + b,  q = softmax over all classes of l / T
+//   loss = T^2 sum_j p_j (log p_j - log q_{c_j}),  G_v = up T (q_v - sum over j with c_j = v of p_j),  dx = G w,  dw = G^T x,  db = sum over rows of G
+// A row without entries has no loss, no gradient, and does not count in the mean.
+//
+// A first pass makes each row's distribution, with its entries in the order of their classes, and a table that says for each run of 64 classes which
+// entries lie in it: so the product over all classes, whose epilogue leaves the statistics of l (dwo_head.hip), finds the few sums that are some
+// entry's logit among its own and leaves them too.  Backward, in pieces of the classes: the product again, its sums turned into up T q; a pass over the
+// entries then puts up T (q - p) in their places, computed from the logits left by the forward pass in fp32 and rounded once.
+#include "dwo_head.h"
+
+namespace dwo {
+
+constexpr int kDistillMost = 1024;  // entries of a row
+constexpr int kRun = 64;            // classes of a word of the table, no fewer than a wave's columns in any tile
+// A run's word: the first entry's place in the run, its place among the row's entries, and how many there are
+__device__ __forceinline__ unsigned run_word(int place, int start, int count) { return (unsigned)place | (unsigned)start << 6 | (unsigned)count << 16; }
+__device__ __forceinline__ int run_place(unsigned w) { return w & 63; }
+__device__ __forceinline__ int run_start(unsigned w) { return w >> 6 & 1023; }
+__device__ __forceinline__ int run_count(unsigned w) { return w >> 16; }
+static long run_pitch(long V) { return ((V + kRun - 1) / kRun + 3) / 4 * 4; }
+
+enum { ROW_OUT = -1, ROW_BAD = -2 };  // a row's state: without entries; a class that is none or a logit that is no number; 0 otherwise
+struct RowStates {
+    const int *state;
+    __device__ __forceinline__ int of(long m) const { return state[m]; }
+};
+// what the backward pass takes of the forward one: [M][k] each but the last two, [M]
+struct Kept {
+    int *classes;  // in order, absent ones behind the others
+    float *p, *at;  // and the layer's logit there (not written for absent ones)
+    int *state;
+    float *lse;  // T log sum exp (l / T)
+    Kept(float *keep, long rows, int k) {
+        const size_t all = (size_t)rows * k;
+        classes = (int *)keep, p = keep + all, at = keep + 2 * all, state = (int *)(keep + 3 * all), lse = keep + 3 * all + rows;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------- the teacher's entries
+// A wave a row, N entries a lane (j = lane + 64 i).  An entry's place in the order of classes is the number of those in front of it.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restrict__ logits, const long long *__restrict__ classes, Kept kept,
+                                                              unsigned *__restrict__ table, long rows, long V, int k, long pitch, float per) {
+    __shared__ int sorted[4][64 * N];
+    const int lane = threadIdx.x & 63;
+    int *const mine = sorted[threadIdx.x >> 6];
+    for (long first = (long)blockIdx.x * 4; first < rows; first += (long)gridDim.x * 4) {
+        const long row = first + (threadIdx.x >> 6);
+        const bool real = row < rows;
+        float t[N];
+        int c[N];
+        bool bad = false;
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int j = lane + 64 * i;
+            t[i] = -INFINITY, c[i] = 0x7fffffff;
+            if (real && j < k) {
+                const long long v = classes[row * k + j];
+                const float f = to_float(logits[row * k + j]);
+                const bool there = v != -1 && f != -INFINITY;
+                bad |= v != -1 && (v < 0 || v >= V || !(f < INFINITY));
+                if (there) t[i] = f, c[i] = v >= 0 && v < V ? (int)v : 0x7fffffff;
+                most = fmaxf(most, there ? f : -INFINITY);
+            }
+            mine[j] = c[i];
+        }
+        const bool any_bad = __any(bad);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        const bool some = most > -INFINITY;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            t[i] = some && !any_bad && t[i] > -INFINITY ? prod_exp((t[i] - most) * per) : 0.f;
+            sum += t[i];
+        }
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
+        const float part = some && !any_bad ? 1.f / sum : 0.f;
+        if (real && lane == 0) kept.state[row] = any_bad ? ROW_BAD : some ? 0 : ROW_OUT;
+        if (real)
+            for (long b = lane; b < pitch / 4; b += 64) reinterpret_cast<mma_u4 *>(table + row * pitch)[b] = mma_u4{0u, 0u, 0u, 0u};
+        __syncthreads();  // (the classes are in LDS, and the zeros in front of the words that replace some)
+        int rank[N] = {}, same[N] = {}, ahead[N] = {};
+        for (int j = 0; j < k; j++) {
+            const int other = mine[j];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int before = other < c[i] || (other == c[i] && j < lane + 64 * i), run = other / kRun == c[i] / kRun;
+                rank[i] += before, same[i] += run, ahead[i] += before & run;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (real && lane + 64 * i < k) {
+                kept.classes[row * k + rank[i]] = c[i];
+                kept.p[row * k + rank[i]] = t[i] * part;
+                if (c[i] != 0x7fffffff && ahead[i] == 0) table[row * pitch + c[i] / kRun] = run_word(c[i] % kRun, rank[i], same[i]);
+            }
+        __syncthreads();
+    }
+}
+template <typename T>
+static int launch_entries(const void *logits, const long long *classes, const Kept &kept, unsigned *table, long rows, long V, int k, float per,
+                          hipStream_t st) {
+    auto *kernel = k <= 64 ? distill_entries_kernel<T, 1> : k <= 256 ? distill_entries_kernel<T, 4> : distill_entries_kernel<T, 16>;
+    const long blocks = (rows + 3) / 4;
+    kernel<<<dim3((unsigned)std::min(blocks, 1L << 20)), dim3(256), 0, st>>>((const T *)logits, classes, kept, table, rows, V, k, run_pitch(V), per);
+    return status();
+}
+
+// ------------------------------------------------------------------------------------------------- statistics
+struct DistillStatsEpi {
+    static constexpr bool kSums = false, kDirect = true;
+    Values bias;
+    const unsigned *table;
+    long pitch;
+    const int *classes;
+    int k;
+    float *at;     // [M][k]
+    float2 *part;  // [classes / (16 NF)][M]: largest logit, sum of exponentials of those / T below it
+    float scale;   // log2(e) / T
+    static constexpr int kRow = 4;  // the words of the 256 classes around the tile
+    __device__ __forceinline__ unsigned row(const Product &, long m, long n0, int i) const {
+        const long b = n0 / (4 * kRun) * 4 + i;
+        return b < pitch ? table[m * pitch + b] : 0u;
+    }
+    template <int NF>
+    __device__ __forceinline__ RowClasses<NF> begin(const Product &p, long n0) const {
+        RowClasses<NF> l;
+        l.init(bias, n0, p.N);
+        return l;
+    }
+    template <int NF>
+    __device__ __forceinline__ void emit(const Product &p, const RowClasses<NF> &l, const unsigned *rows, long m, long n0,
+                                         mma_f4 (&v)[NF]) const {
+        static_assert(16 * NF <= kRun, "a wave's columns are in one run");
+        float most = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[i][r] += l.bias[i][r], most = fmaxf(most, v[i][r]);
+        const unsigned word = rows[n0 / kRun % 4];
+        if (m < p.M && word != 0) {
+            const int lane_class = (int)class_of(n0, 0, 0), start = run_start(word), count = run_count(word);
+            int t = (int)(n0 / kRun) * kRun + run_place(word) - lane_class;
+            for (int j = 0;;) {
+                if (t >= 0 && t < 16 * NF && (t & 15) < 4) {
+                    float hit = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NF; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) hit = t == 16 * i + r ? v[i][r] : hit;
+                    at[m * k + start + j] = hit;
+                }
+                if (++j >= count) break;
+                t = classes[m * k + start + j] - lane_class;
+            }
+        }
+        most = over_lanes(most, [](float a, float b) { return fmaxf(a, b); });
+        // (all -infinity: no exponential; NaN is in no maximum and in the sum)
+        const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s += __builtin_amdgcn_exp2f((v[i][r] - base) * scale);
+        s = over_lanes(s, [](float a, float b) { return a + b; });
+        if ((threadIdx.x & 63) < 16 && n0 < p.N && m < p.M) part[(size_t)(n0 / (16 * NF)) * p.M + m] = make_float2(most, s);
+    }
+};
+
+// The parts of a row joined and its loss, K threads a row and R rows at a time, as head_join_kernel has them
+template <int R, int K>
+__global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__restrict__ part, Kept kept, float *__restrict__ loss,
+                                                            float *__restrict__ mean, float *__restrict__ count, float2 *__restrict__ block, long M,
+                                                            int parts, int entries, float T) {
+    __shared__ float most_of[K][R + 1], sum_of[K][R + 1];
+    __shared__ float2 rows[R];
+    const int r = threadIdx.x % R, k = threadIdx.x / R;
+    const float per = 1.f / T, scale = 1.44269504f * per;
+    double total = 0.0, number = 0.0;
+    for (long first = (long)blockIdx.x * R; first < M; first += (long)gridDim.x * R) {
+        const long m = first + r;
+        float most = -INFINITY, s = 0.f;
+        const int state = m < M ? kept.state[m] : (int)ROW_OUT;
+        if (m < M)
+            for (int p = k; p < parts; p += 4 * K) {
+                float2 v[4];
+                float next = most;
+#pragma unroll
+                for (int u = 0; u < 4; u++) v[u] = p + K * u < parts ? part[(size_t)(p + K * u) * M + m] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int u = 0; u < 4; u++) next = fmaxf(next, v[u].x);
+                const float base = next == -INFINITY ? 0.f : next;
+                s *= __builtin_amdgcn_exp2f((most - base) * scale);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s += v[u].y * __builtin_amdgcn_exp2f((v[u].x - base) * scale);
+                most = next;
+            }
+        most_of[k][r] = most, sum_of[k][r] = s;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < K; i++) most = fmaxf(most, most_of[i][r]);
+        const float base = most == -INFINITY ? 0.f : most;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < K; i++) s += sum_of[i][r] * __builtin_amdgcn_exp2f((most_of[i][r] - base) * scale);
+        const float lse = base + T * logf(s);
+        __syncthreads();
+        // sum of p (log p - log q): both logarithms are of one size where the layer follows the teacher
+        float value = 0.f;
+        if (state == 0)
+            for (int j = k; j < entries; j += K) {
+                const float p = kept.p[m * entries + j];
+                if (p > 0.f) value = __builtin_fmaf(p, logf(p) - (kept.at[m * entries + j] - lse) * per, value);
+            }
+        sum_of[k][r] = value;
+        __syncthreads();
+        if (k == 0) {
+#pragma unroll
+            for (int i = 1; i < K; i++) value += sum_of[i][r];
+            value = state == ROW_OUT ? 0.f : state == ROW_BAD ? NAN : T * T * value;
+            if (m < M) {
+                kept.lse[m] = lse;
+                if (loss != nullptr) loss[m] = value;
+            }
+            rows[r] = make_float2(value, state != ROW_OUT ? 1.f : 0.f);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0)
+#pragma unroll 16
+            for (int i = 0; i < R; i++) total += rows[i].x, number += rows[i].y;
+    }
+    if (threadIdx.x != 0) return;
+    if (block != nullptr) block[blockIdx.x] = make_float2((float)total, (float)number);
+    else if (mean != nullptr) mean[0] = (float)(total / number), count[0] = (float)number;
+}
+
+// ------------------------------------------------------------------------------------------------- gradients of the logits
+// q times what each row's loss receives, without what all rows share (T, and a mean's up / count); in fp16 times a power of two, as dwo_head.hip has it
+struct DistillGrad {
+    const int *state;
+    const float *lse, *up, *scale;  // up null: a mean; scale null: `fixed`
+    float per, fixed;               // 1 / T
+};
+struct DistillGradEpi {
+    static constexpr bool kSums = false, kDirect = false;
+    Values bias;  // of the piece
+    DistillGrad d;
+    Out g;  // [M][pitch]
+    struct Lane : Classes {
+        float scale;
+    };
+    __device__ __forceinline__ Lane begin(const Product &p, long n) const {
+        Lane l;
+        l.init(bias, n, p.N);
+        l.scale = d.scale != nullptr ? d.scale[0] : d.fixed;
+        return l;
+    }
+    static constexpr int kRow = 3;  // the state, the log of the sum, what arrives at the loss
+    __device__ __forceinline__ unsigned row(const Product &, long m, long, int k) const {
+        return k == 0 ? (unsigned)d.state[m] : k == 1 ? __float_as_uint(d.lse[m]) : __float_as_uint(d.up != nullptr ? d.up[m] : 1.f);
+    }
+    __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
+    __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
+                                          float (&v)[8]) const {
+        if (m >= p.M || n >= g.pitch) return;
+        const int state = (int)rows[0];
+        const float lse = __uint_as_float(rows[1]), f = __uint_as_float(rows[2]) * l.scale;
+        if (g.plane != 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = prod_exp((v[e] + l.bias[e] - lse) * d.per) * f;
+        } else {
+            const float scale = 1.44269504f * d.per;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f((v[e] + l.bias[e] - lse) * scale) * f;
+        }
+        // rows without entries, or with an entry that is none, and columns behind the last class
+        if (state < 0 || n + 8 > p.N) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = state == ROW_OUT || n + e >= p.N ? 0.f : state == ROW_BAD ? NAN : v[e];
+        }
+        operand_octet(g, m, n, g.pitch, v);
+    }
+};
+// The same at the entries' places, from class `from` on, less their p.  Entries of one class are neighbours: the first writes for all.
+__global__ __launch_bounds__(256) void distill_places_kernel(Kept kept, DistillGrad d, Out g, long rows, int k, long from, long n) {
+    const long total = rows * k;
+    const float scale = d.scale != nullptr ? d.scale[0] : d.fixed;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const int c = kept.classes[i];
+        if (c < from || c >= from + n) continue;
+        const long m = i / k;
+        const int j = (int)(i % k);
+        if (kept.state[m] != 0 || (j > 0 && kept.classes[i - 1] == c)) continue;
+        float p = kept.p[i];
+        for (int o = 1; j + o < k && kept.classes[i + o] == c; o++) p += kept.p[i + o];
+        const float f = (d.up != nullptr ? d.up[m] : 1.f) * scale;
+        operand_one(g, m, c - from, (prod_exp((kept.at[i] - d.lse[m]) * d.per) - p) * f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- on the host
+struct DistillSizes : HeadSizes {
+    int k, teacher;  // the teacher's type
+    DistillSizes(size_t r, int c, int v, int entries, int t, int tt) : HeadSizes(r, c, v, t), k(entries), teacher(tt) {}
+    bool ok() const { return HeadSizes::ok() && k >= 1 && k <= kDistillMost && known(teacher); }
+};
+// (T and 1 / T, their squares, and logits times either stay numbers of fp32 by far)
+static bool temperature_ok(float T) { return T >= 1e-4f && T <= 1e4f; }
+
+static int distill_forward(const DistillSizes &s, const void *x, const void *w, const void *b, const void *logits, const long long *classes, float T,
+                           float *keep, float *loss, float *count, bool mean, Arena &ws, hipStream_t st) {
+    Staging stage;
+    const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), ow = stage.matrix(w, s.V, s.C, s.dtype, ws);
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
+    const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
+    const int width = wave_columns(tile_for(p.M, p.N, p.steps));
+    const int parts = (int)((s.V + width - 1) / width);
+    // (rows of a workgroup as in head_forward)
+    const bool few = s.rows <= 128, narrow = !few && parts <= 16;
+    const int group = few || narrow ? 64 : 16;
+    const int blocks = few ? 1 : (int)std::min((s.rows + group - 1) / group, 1L << 20);
+    float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
+    unsigned *table = (unsigned *)ws.take((size_t)s.rows * run_pitch(s.V) * sizeof(unsigned));
+    float2 *block = mean && blocks > 1 ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
+    if (ws.dry()) return 0;
+    const Kept kept(keep, s.rows, s.k);
+    const float per = 1.f / T;
+    auto *const entries = s.teacher == DWO_F32 ? launch_entries<float> : s.teacher == DWO_BF16 ? launch_entries<bf16_t> : launch_entries<f16_t>;
+    if ((e = entries(logits, classes, kept, table, s.rows, s.V, s.k, per, st))) return e;
+    const DistillStatsEpi epi{{b, s.dtype}, table, run_pitch(s.V), kept.classes, s.k, kept.at, part, 1.44269504f * per};
+    if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
+    auto *const join = few ? distill_join_kernel<64, 16> : narrow ? distill_join_kernel<64, 4> : distill_join_kernel<16, 16>;
+    join<<<dim3((unsigned)blocks), dim3(few ? 1024 : 256), 0, st>>>(part, kept, mean ? nullptr : loss, mean ? loss : nullptr, count, block, s.rows, parts,
+                                                                    s.k, T);
+    if (block != nullptr) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
+    return status();
+}
+
+static int distill_backward(const DistillSizes &s, const float *up, const void *x, const void *w, const void *b, const float *keep, float T,
+                            const float *count, void *dx, void *dw, void *db, int grad, Arena &ws, hipStream_t st) {
+    Staging stage;
+    const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), ow = stage.matrix(w, s.V, s.C, s.dtype, ws);
+    int e = stage.launch(ws.dry(), st);
+    if (e) return e;
+    const Operand g = take_operand(ws, s.rows, up8(s.piece()), s.dtype, (double)s.rows * (double)s.C * (double)s.V);
+    const bool mean = count != nullptr, half = s.dtype == DWO_F16;
+    float *scale = half && !mean ? (float *)ws.take(2 * sizeof(float)) : nullptr;
+    const Kept kept(const_cast<float *>(keep), s.rows, s.k);
+    if (scale != nullptr && !ws.dry()) {
+        head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, RowStates{kept.state}, s.rows, scale);
+        if ((e = status())) return e;
+    }
+    const DistillGrad d{kept.state, kept.lse, mean ? nullptr : up, scale, 1.f / T, half && mean ? kHalfScale : 1.f};
+    auto make = [&](long from, long n, const Operand &wp, const Operand &gp) {
+        const DistillGradEpi epi{{b != nullptr ? (const char *)b + from * size_of(s.dtype) : nullptr, s.dtype}, d, out_of(gp, s.dtype)};
+        const int status_of = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st);
+        if (status_of) return status_of;
+        distill_places_kernel<<<dim3(blocks_for(s.rows * s.k, 8192)), dim3(256), 0, st>>>(kept, d, out_of(gp, s.dtype), s.rows, s.k, from, n);
+        return status();
+    };
+    auto shared = [&](PlainEpi epi) {
+        epi.alpha = mean ? up : scale != nullptr ? scale + 1 : nullptr;
+        epi.over = count;
+        epi.factor = T / (half && mean ? kHalfScale : 1.f);
+        return epi;
+    };
+    return head_pieces(s, ox, ow, g, dx, dw, db, grad, make, shared, ws, st);
+}
+
+}  // namespace dwo
+
+using namespace dwo;
+
+extern "C" {
+
+size_t dwo_distill_workspace_bytes(size_t rows, int C, int V, int k, int backward, int dtype) {
+    const DistillSizes s(rows, C, V, k, dtype, DWO_F32);
+    if (!s.ok()) return 0;
+    Arena ws = Arena::measure();
+    void *const any = (void *)256;  // (nothing is launched)
+    if (backward)
+        distill_backward(s, (const float *)any, any, any, any, (const float *)any, 1.f, nullptr, any, any, any, DWO_F32, ws, nullptr);
+    else
+        distill_forward(s, any, any, any, any, (const long long *)any, 1.f, (float *)any, (float *)any, (float *)any, true, ws, nullptr);
+    return ws.used + 256;
+}
+
+int dwo_distill_forward(const void *x, const void *w, const void *bias, const void *logits, const void *classes, float temperature, float *keep,
+                        float *loss, float *count, void *ws, size_t ws_bytes, size_t rows, int C, int V, int k, int dtype, int logits_dtype,
+                        void *stream) {
+    if (!x || !w || !logits || !classes || !keep || !loss || !ws) return DWO_ERR_NULL_POINTER;
+    if (!known(dtype) || !known(logits_dtype)) return DWO_ERR_BAD_DTYPE;
+    const DistillSizes s(rows, C, V, k, dtype, logits_dtype);
+    if (!s.ok() || !temperature_ok(temperature) || ((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) % 16 != 0 || (uintptr_t)classes % 8 != 0 ||
+        (uintptr_t)keep % 4 != 0 || (uintptr_t)logits % size_of(logits_dtype) != 0)
+        return DWO_ERR_BAD_SHAPE;
+    if (ws_bytes < dwo_distill_workspace_bytes(rows, C, V, k, 0, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
+    (void)hipGetLastError();
+    Arena a{(char *)ws, 0, ws_bytes};
+    return distill_forward(s, x, w, bias, logits, (const long long *)classes, temperature, keep, loss, count, count != nullptr, a, (hipStream_t)stream);
+}
+
+int dwo_distill_backward(const float *up, const void *x, const void *w, const void *bias, const float *keep, float temperature, const float *count,
+                         void *dx, void *dw, void *db, void *ws, size_t ws_bytes, size_t rows, int C, int V, int k, int dtype, int grad_dtype,
+                         void *stream) {
+    if (!up || !x || !w || !keep || !ws) return DWO_ERR_NULL_POINTER;
+    if (!known(dtype) || !known(grad_dtype)) return DWO_ERR_BAD_DTYPE;
+    const DistillSizes s(rows, C, V, k, dtype, DWO_F32);
+    if (!s.ok() || !temperature_ok(temperature) || ((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) % 16 != 0 || (uintptr_t)keep % 4 != 0 || (db && !dw))
+        return DWO_ERR_BAD_SHAPE;
+    if (ws_bytes < dwo_distill_workspace_bytes(rows, C, V, k, 1, dtype)) return DWO_ERR_SCRATCH_TOO_SMALL;
+    (void)hipGetLastError();
+    Arena a{(char *)ws, 0, ws_bytes};
+    return distill_backward(s, up, x, w, bias, keep, temperature, count, dx, dw, db, grad_dtype, a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -9,10 +9,7 @@
 // Bound by the matrix cores: 8192 x 1024 x 65536 in bf16, statistics 1022 us (1075 TFLOP/s), G 4 x 310 (890; 268 MB of G each go out behind
 // the sums, which nothing covers), its two products 4 x 460 (1195).  In fp32, 1024 x 512 x 21841: 137, 176 and 323 us, products of six planes at
 // 167, 130 and 142 TFLOP/s of the function's own.
-#include <algorithm>
-#include <cmath>
-
-#include "dwo_product.h"
+#include "dwo_head.h"
 
 namespace dwo {
 
@@ -27,32 +24,6 @@ struct Targets {
     }
 };
 
-// bias of the classes n0 + 16 i + 4 g + r that a lane has, -infinity where there is no class: its logit is then no largest one and its
-// exponential zero (products with columns that are not there are zeros)
-__device__ __forceinline__ long class_of(long n0, int i, int r) { return n0 + 16 * i + 4 * ((threadIdx.x & 63) >> 4) + r; }
-template <int NF>
-struct RowClasses {
-    float bias[NF][4];
-    __device__ __forceinline__ void init(const Values &b, long n0, long N) {
-#pragma unroll
-        for (int i = 0; i < NF; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const long n = class_of(n0, i, r);
-                bias[i][r] = n >= N ? -INFINITY : b.p != nullptr ? b.at(n) : 0.f;
-            }
-    }
-};
-// joined over the four lanes that have a row
-template <class F>
-__device__ __forceinline__ float over_lanes(float v, F &&join) {
-    const unsigned u = __float_as_uint(v);
-    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const unsigned w = __float_as_uint(join(__uint_as_float(s[0]), __uint_as_float(s[1])));
-    const auto t = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return join(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-
 struct StatsEpi {
     static constexpr bool kSums = false, kDirect = true;
     Values bias;
@@ -61,7 +32,7 @@ struct StatsEpi {
     float *sum;    // the same of sums of logits, or null
     float *at;     // [M]: the target's logit
     static constexpr int kRow = 1;  // the target
-    __device__ __forceinline__ unsigned row(const Product &, long m, int) const { return (unsigned)targets.of(m); }
+    __device__ __forceinline__ unsigned row(const Product &, long m, long, int) const { return (unsigned)targets.of(m); }
     template <int NF>
     __device__ __forceinline__ RowClasses<NF> begin(const Product &p, long n0) const {
         RowClasses<NF> l;
@@ -111,21 +82,8 @@ struct StatsEpi {
     }
 };
 
-// bias of the eight classes that a lane has, -infinity where there is no class: its logit is then no largest one and its exponential zero
-// (products with columns that are not there are zeros)
-struct Classes {
-    float bias[8];
-    __device__ __forceinline__ void init(const Values &b, long n, long N) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) bias[e] = n + e >= N ? -INFINITY : b.p != nullptr ? b.at(n + e) : 0.f;
-    }
-};
 // place of class t among eight from n on, or one beyond them
 __device__ __forceinline__ int place_of(int t, long n) { return t >= (int)n && t < (int)n + 8 ? t - (int)n : 8; }
-
-// exp of what a logit is below another: the multiple's rounding is 2^-24 of the difference, which is at most the log of a part's width where
-// the part counts
-__device__ __forceinline__ float below(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
 
 // The parts of a row joined, K threads a row and R rows at a time; `block` receives a workgroup's sum of losses and number of rows that
 // count.  One workgroup with all rows (few of them) writes the mean itself.
@@ -195,59 +153,14 @@ __global__ __launch_bounds__(R *K) void head_join_kernel(const float2 *__restric
     else if (mean != nullptr) mean[0] = (float)(total / number), count[0] = (float)number;
 }
 
-// The same of many workgroups' sums, in a fixed order and in 64 bits
-__global__ __launch_bounds__(1024) void head_mean_kernel(const float2 *__restrict__ block, int blocks, float *__restrict__ loss,
-                                                         float *__restrict__ count) {
-    __shared__ double value[1024], number[1024];
-    double a = 0.0, b = 0.0;
-    for (int i = threadIdx.x; i < blocks; i += 1024) a += block[i].x, b += block[i].y;
-    value[threadIdx.x] = a, number[threadIdx.x] = b;
-    __syncthreads();
-    for (int half = 512; half > 0; half >>= 1) {
-        if ((int)threadIdx.x < half)
-            value[threadIdx.x] += value[threadIdx.x + half], number[threadIdx.x] += number[threadIdx.x + half];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) loss[0] = (float)(value[0] / number[0]), count[0] = (float)number[0];
-}
-
 // What the products that read G give it back: G is held without what all its rows share.
 //   a mean: up / count (1 - eps), so that a row's largest value, about -1 at its target, is next to a number that 16 bits hold; rounded
 //   where it is, the same rounding in all rows would go into the gradients (twice their own rounding with labels smoothed)
 //   fp16: a power of two besides, or probabilities below 6e-8 would be lost; a mean's values are at most 1 / (1 - eps) and 1 at the target, times
 //   2^13 or, above a smoothing of 3/4, what brings 1 / (1 - eps) to 2^14 .. 2^15; others are brought to 2^13 .. 2^14 by the largest finite |up| of a
-//   row with a class (whatever arrives at the others changes nothing): scale[0], and its inverse, by this kernel
-constexpr float kHalfScale = 8192.f;
+//   row with a class (whatever arrives at the others changes nothing): scale[0], and its inverse, by head_scale_kernel
 static float half_mean_scale(float eps) {
     return eps < 1.f ? fminf(kHalfScale, ldexpf(4.f * kHalfScale, ilogbf(1.f - eps))) : kHalfScale;
-}
-__global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ up, Targets targets, long M,
-                                                          float *__restrict__ scale) {
-    __shared__ unsigned most[1024];
-    unsigned v = 0;
-    // (one workgroup, bound by the reads' latency: eight rows of a thread are asked for at once; 10^6 rows 170 us, one at a time 610)
-    for (long i = threadIdx.x; i < M; i += 8 * 1024) {
-        unsigned u[8];
-        int t[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const long m = min(i + 1024 * k, M - 1);
-            u[k] = __float_as_uint(up[m]) & 0x7fffffffu, t[k] = targets.of(m);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) v = u[k] < 0x7f800000u && t[k] >= 0 ? max(v, u[k]) : v;
-    }
-    most[threadIdx.x] = v;
-    __syncthreads();
-    for (int h = 512; h > 0; h >>= 1) {
-        if ((int)threadIdx.x < h) most[threadIdx.x] = max(most[threadIdx.x], most[threadIdx.x + h]);
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        const int e = (int)(most[0] >> 23);  // biased exponent; the scale's is 254 + 13 - e
-        const int k = e == 0 ? 127 : min(max(267 - e, 1), 253);
-        scale[0] = __uint_as_float((unsigned)k << 23), scale[1] = __uint_as_float((unsigned)(254 - k) << 23);
-    }
 }
 
 struct GradEpi {
@@ -270,7 +183,7 @@ struct GradEpi {
         return l;
     }
     static constexpr int kRow = 3;  // the target, the log of the sum, what arrives at the loss
-    __device__ __forceinline__ unsigned row(const Product &, long m, int k) const {
+    __device__ __forceinline__ unsigned row(const Product &, long m, long, int k) const {
         return k == 0 ? (unsigned)targets.of(m) : k == 1 ? __float_as_uint(lse[m]) : up != nullptr ? __float_as_uint(up[m]) : 0u;
     }
     __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
@@ -303,18 +216,6 @@ struct GradEpi {
             for (int e = 0; e < 8; e++) v[e] = t == -1 || n + e >= p.N ? 0.f : t == -2 ? NAN : v[e];
         }
         operand_octet(g, m, n, g.pitch, v);
-    }
-};
-
-struct HeadSizes {
-    long rows, C, V;
-    int dtype;
-    HeadSizes(size_t r, int c, int v, int t) : rows((long)r), C(c), V(v), dtype(t) {}
-    bool ok() const { return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && V >= 1 && V <= 1 << 24 && known(dtype); }
-    // classes of a piece: G of a piece has about 2^27 values, 256 MB in 16 bits, what the last cache before memory holds, or 1024 classes
-    long piece() const {
-        const long most = std::max((1L << 27) / rows / 256 * 256, 1024L);
-        return std::min(V, most);
     }
 };
 
@@ -352,56 +253,26 @@ static int head_backward(const HeadSizes &s, const float *up, const void *x, con
     const Operand ox = stage.matrix(x, s.rows, s.C, s.dtype, ws), ow = stage.matrix(w, s.V, s.C, s.dtype, ws);
     int e = stage.launch(ws.dry(), st);
     if (e) return e;
-    const long piece = s.piece();
-    const Operand g = take_operand(ws, s.rows, up8(piece), s.dtype, (double)s.rows * (double)s.C * (double)s.V);
-    // dx is summed over the pieces in fp32
-    const bool many = piece < s.V;
-    float *sum = many && dx != nullptr && s.dtype != DWO_F32 ? (float *)ws.take((size_t)s.rows * s.C * sizeof(float)) : (float *)dx;
+    const Operand g = take_operand(ws, s.rows, up8(s.piece()), s.dtype, (double)s.rows * (double)s.C * (double)s.V);
     const bool mean = count != nullptr, half = s.dtype == DWO_F16;
     float *scale = half && !mean ? (float *)ws.take(2 * sizeof(float)) : nullptr;
     if (scale != nullptr && !ws.dry()) {
         head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, targets, s.rows, scale);
         if ((e = status())) return e;
     }
-    const size_t size = size_of(s.dtype), grad_size = size_of(grad);
     const float mean_scale = half ? half_mean_scale(eps) : 1.f;
+    auto make = [&](long from, long n, const Operand &wp, const Operand &gp) {
+        const GradEpi epi{{b != nullptr ? (const char *)b + from * size_of(s.dtype) : nullptr, s.dtype}, targets, from, lse, mean ? nullptr : up, scale,
+                          eps, mean_scale, out_of(gp, s.dtype)};
+        return launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st);
+    };
     auto shared = [&](PlainEpi epi) {
         epi.alpha = mean ? up : scale != nullptr ? scale + 1 : nullptr;
         epi.over = count;
         epi.factor = mean ? (eps < 1.f ? 1.f - eps : 1.f) / mean_scale : 1.f;
         return epi;
     };
-    const size_t held = ws.used;
-    size_t peak = held;
-    for (long from = 0; from < s.V; from += piece) {
-        const long n = s.V - from < piece ? s.V - from : piece;
-        ws.used = held;  // (the pieces' partial sums take the same place)
-        Operand wp = ow;
-        wp.p = (const char *)ow.p + (size_t)from * ow.pitch * 2;
-        Operand gp = g;
-        gp.pitch = up8(n), gp.plane = s.rows * gp.pitch;
-        if (!ws.dry()) {
-            const GradEpi epi{{b != nullptr ? (const char *)b + from * size : nullptr, s.dtype}, targets, from, lse, mean ? nullptr : up, scale, eps, mean_scale,
-                              out_of(gp, s.dtype)};
-            if ((e = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st))) return e;
-        }
-        ProductGroup group;
-        if (dx != nullptr) {
-            const bool last = from + n == s.V;
-            PlainEpi epi = shared(plain_epilogue({last ? dx : (void *)sum, s.C, 0, last ? s.dtype : (int)OUT_F32}));
-            epi.before = from > 0 ? sum : nullptr;
-            group.add(false, gp, wp, s.rows, s.C, n, epi);
-        }
-        if (dw != nullptr) {
-            PlainEpi epi = shared(plain_epilogue({(char *)dw + (size_t)from * s.C * grad_size, s.C, 0, grad}));
-            epi.sums = {db != nullptr ? (char *)db + from * grad_size : nullptr, 0, 0, grad};
-            group.add(true, gp, ox, n, s.C, s.rows, epi);
-        }
-        if ((e = group.launch(s.dtype, ws, st))) return e;
-        if (ws.used > peak) peak = ws.used;
-    }
-    ws.used = peak;
-    return 0;
+    return head_pieces(s, ox, ow, g, dx, dw, db, grad, make, shared, ws, st);
 }
 
 }  // namespace dwo

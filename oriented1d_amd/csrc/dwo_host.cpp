@@ -65,6 +65,14 @@ struct Library {
     decltype(&::dwo_head_workspace_bytes) head_workspace_bytes;
     decltype(&::dwo_head_forward) head_forward;
     decltype(&::dwo_head_backward) head_backward;
+    decltype(&::dwo_int8_rows) int8_rows;
+    decltype(&::dwo_int8_workspace_bytes) int8_workspace_bytes;
+    decltype(&::dwo_int8_linear) int8_linear;
+    decltype(&::dwo_top_workspace_bytes) top_workspace_bytes;
+    decltype(&::dwo_top) top;
+    decltype(&::dwo_distill_workspace_bytes) distill_workspace_bytes;
+    decltype(&::dwo_distill_forward) distill_forward;
+    decltype(&::dwo_distill_backward) distill_backward;
 } lib;
 
 [[noreturn]] void fail(const std::string &msg) { throw std::runtime_error(msg); }
@@ -114,6 +122,14 @@ void bind_library(const std::string &path) {
     find(lib.head_workspace_bytes, "dwo_head_workspace_bytes");
     find(lib.head_forward, "dwo_head_forward");
     find(lib.head_backward, "dwo_head_backward");
+    find(lib.int8_rows, "dwo_int8_rows");
+    find(lib.int8_workspace_bytes, "dwo_int8_workspace_bytes");
+    find(lib.int8_linear, "dwo_int8_linear");
+    find(lib.top_workspace_bytes, "dwo_top_workspace_bytes");
+    find(lib.top, "dwo_top");
+    find(lib.distill_workspace_bytes, "dwo_distill_workspace_bytes");
+    find(lib.distill_forward, "dwo_distill_forward");
+    find(lib.distill_backward, "dwo_distill_backward");
 }
 
 void check(int status, const char *what) {
@@ -738,6 +754,7 @@ Tensor conv_norm(const Tensor &x, const Tensor &w, const OptTensor &bias, const 
 }
 
 #include "dwo_host_wide.h"
+#include "dwo_host_teach.h"
 
 }  // namespace
 
@@ -764,6 +781,10 @@ PYBIND11_MODULE(_host, m) {
     m.def("linear8", &linear8);
     m.def("gated", &gated);
     m.def("head", &head);
+    m.def("int8_rows", &int8_rows);
+    m.def("int8_linear", &int8_linear);
+    m.def("top", &top);
+    m.def("distill", &distill);
     m.def("ln_rows", &ln_rows);
     m.def("ln_rows_backward", &ln_rows_backward);
     m.def("ln_tile", &ln_tile);

@@ -217,31 +217,43 @@ __device__ __forceinline__ void out_octet(const Out &o, bool wide, long m, long 
 // the first one's sign and is not zero, for which the first goes a step down where it has to (the second is then at most 3/2 steps and not
 // 1/2, its own rounding twice as far): an infinite value of the other operand, whose products with both halves are added, is infinite in the sum
 // and not NaN.  The second half of infinities and NaN is 1 with their sign.
+__device__ __forceinline__ void halves_of(int type, float v, float &first, float &second) {
+    auto value = [&](uint16_t b) { return type == OUT_F16 ? to_float(__builtin_bit_cast(f16_t, b)) : bf16_value(b); };
+    const uint16_t b = bits16(type, v);
+    float h = value(b), rest = v - h;
+    const float r = value(bits16(type, rest));
+    const bool apart = r == 0.f || ((__float_as_uint(r) ^ __float_as_uint(h)) >> 31) != 0;
+    const bool finite = __builtin_fabsf(h) < INFINITY;
+    if (apart && (b & 0x7fff) > 1) h = value(b - 1), rest = v - h;
+    first = finite ? h : v, second = finite ? rest : __builtin_copysignf(1.f, v);
+}
 template <bool STREAM = true>
 __device__ __forceinline__ void operand_octet(const Out &o, long m, long n, long N, const float (&v)[8]) {
     out_octet<STREAM>(o, true, m, n, N, v);
     if (__builtin_expect(o.type == OUT_PLANES || o.plane == 0, 1)) return;
     // (rare, and behind the first store, whose half is written again: with these values in front of it the gated block's product behind dy, 16384 x
     // 4096 from 1024, which has no second halves, takes 12 of 328 us more)
-    auto value = [&](uint16_t b) { return o.type == OUT_F16 ? to_float(__builtin_bit_cast(f16_t, b)) : bf16_value(b); };
     float first[8], second[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const uint16_t b = bits16(o.type, v[e]);
-        float h = value(b), rest = v[e] - h;
-        const float r = value(bits16(o.type, rest));
-        const bool apart = r == 0.f || ((__float_as_uint(r) ^ __float_as_uint(h)) >> 31) != 0;
-        const bool finite = __builtin_fabsf(h) < INFINITY;
-        if (apart && (b & 0x7fff) > 1) h = value(b - 1), rest = v[e] - h;
-        first[e] = finite ? h : v[e], second[e] = finite ? rest : __builtin_copysignf(1.f, v[e]);
-    }
+    for (int e = 0; e < 8; e++) halves_of(o.type, v[e], first[e], second[e]);
     out_octet<STREAM>(o, true, m, n, N, first);
     out_octet<STREAM>({reinterpret_cast<uint16_t *>(o.p) + o.plane, o.pitch, 0, o.type}, true, m, n, N, second);
+}
+// one value of an operand
+__device__ __forceinline__ void operand_one(const Out &o, long m, long n, float v) {
+    if (o.type == OUT_PLANES || o.plane == 0) {
+        out_one(o, m, n, v);
+        return;
+    }
+    float first, second;
+    halves_of(o.type, v, first, second);
+    out_one(o, m, n, first);
+    out_one({reinterpret_cast<uint16_t *>(o.p) + o.plane, o.pitch, 0, o.type}, m, n, second);
 }
 
 // An epilogue E has
 //   begin(p, n): what a lane keeps for its eight columns (n: the first) while it goes down the rows
-//   kRow, row(p, m, k): numbers of a row that wait in LDS from the start of the kernel
+//   kRow, row(p, m, n0, k): numbers of a row that wait in LDS from the start of the kernel (n0: the tile's first column)
 //   load(p, m, n): what the epilogue reads for an octet, asked for one octet ahead
 //   octet(p, lane, rows, data, split, m, n, v): eight neighbours of a row; all lanes call it for some row, beyond the ends as well
 //   kSums, emit_sum: see SumsEpi
@@ -440,7 +452,7 @@ __device__ __forceinline__ void product_body(const Product &p, const Epi &epi, i
     if constexpr (Epi::kRow > 0)
         if ((int)threadIdx.x < BM && m0 + (int)threadIdx.x < p.M)
 #pragma unroll
-            for (int k = 0; k < Epi::kRow; k++) lrow[threadIdx.x * Epi::kRow + k] = epi.row(p, m0 + (int)threadIdx.x, k);
+            for (int k = 0; k < Epi::kRow; k++) lrow[threadIdx.x * Epi::kRow + k] = epi.row(p, m0 + (int)threadIdx.x, n0, k);
     const int ksteps = (int)((p.K + kProdK - 1) / kProdK);
     const int first = split * p.per, count = min(p.per, p.steps - first);
     int pair = first / ksteps, k0 = first % ksteps * kProdK, more = count;

@@ -1,0 +1,82 @@
+"""Linear layers at inference as products of 8-bit integers, with a scale for each row and each output channel.
+
+A row x with largest magnitude a is held as whole numbers ``q = round(127 x / a)``, ties to even, times ``a / 127``.  A layer's weight is held so
+once, row by row (``quantize_rows``); ``linear_int8`` takes the rows of its input the same way, call by call, sums the products of whole numbers
+exactly and scales the sums.  Half the bytes of 16-bit weights, and twice their products' rate.
+
+CUDA tensors of type float32, bfloat16 and float16.  There are no gradients: calls that would need them are refused.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+import torch.nn as nn
+
+from . import _lib, fused
+from .checkpoint8 import activation_code, require_ordinary
+
+
+class QuantizedRows(NamedTuple):
+    """Rows in 8-bit integers: ``codes`` int8, rows filled up with zeros to a multiple of sixteen, and ``scales`` fp32, what a step of each row's
+    codes stands for."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_rows(x):
+    """``x`` [..., C] in 8-bit integers, without its history: codes [..., C'] (C' the next multiple of sixteen) and scales [...].  A row with an
+    infinity or NaN has codes of zero and a scale that is NaN."""
+    require_ordinary("quantize_rows", x)
+    return QuantizedRows(*_lib.host(x.get_device()).int8_rows(x))
+
+
+def linear_int8(x, weight, bias=None, activation=None):
+    """``act(F.linear(x, W, bias))`` for ``x`` [..., C], W the rows that ``weight``, the ``quantize_rows`` of a [D, C] matrix, holds, and x's rows held the
+    same way; ``activation``: None, "gelu" (exact) or "silu".  The result has x's type and is rounded once.  A row or output channel that holds an
+    infinity or NaN is NaN.  Under autocast x and bias are converted as for ``F.linear``."""
+    code = -1 if activation is None else activation_code(activation)
+    require_ordinary("linear_int8", x, weight.codes, weight.scales, bias)
+    dtype = fused._autocast(x)
+    return _lib.host(x.get_device()).int8_linear(x if dtype is None else x.to(dtype), weight.codes, weight.scales, bias, code)
+
+
+class LinearInt8(nn.Module):
+    """A linear layer for inference whose weight is held in 8-bit integers; ``of`` makes one of an ``nn.Linear``."""
+
+    def __init__(self, weight: QuantizedRows, in_features: int, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, weight.codes.shape[0]
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    @classmethod
+    def of(cls, linear):
+        return cls(quantize_rows(linear.weight), linear.in_features, linear.bias)
+
+    def _apply(self, fn, recurse=True):
+        # (the scales stay fp32 when a network goes to another type)
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:
+            self.scales = scales.to(self.scales.device)
+        return self
+
+    def extra_repr(self):
+        return "%d, %d, bias=%r" % (self.in_features, self.out_features, self.bias is not None)
+
+    def forward(self, x, activation=None):
+        return linear_int8(x, QuantizedRows(self.codes, self.scales), self.bias, activation)
+
+
+def quantize_network(network):
+    """Puts a ``LinearInt8`` in the place of every wide layer of a network of ``convnext1d``: the pointwise layers of its plain blocks and its
+    classifier.  (The stem, the operators, the norms and gated blocks stay as they are.)  The network is then for inference alone; returned."""
+    from .convnext1d import Block, ConvNeXt1D
+
+    for module in list(network.modules()):
+        names = ("pwconv1", "pwconv2") if isinstance(module, Block) else ("head",) if isinstance(module, ConvNeXt1D) else ()
+        for name in names:
+            layer = module._modules.get(name)
+            if isinstance(layer, nn.Linear):
+                setattr(module, name, LinearInt8.of(layer))
+    return network

@@ -1,8 +1,12 @@
-"""Softmax cross entropy of a linear classifier, without keeping its logits: what a network's head and its loss are in a training step.
+"""Losses of a linear classifier, without keeping its logits: what a network's head and its loss are in a training step.
 
-The forward pass leaves a row's log-sum-exp and nothing of its logits; the backward pass computes them again, in pieces of the classes, and
-turns them into the gradients of input, weight and bias.
+``linear_cross_entropy`` is softmax cross entropy against classes, ``linear_distillation`` that against a teacher's top logits, which
+``top_logits`` takes of a row.  The forward pass leaves a row's log-sum-exp, and the few logits that the loss reads; the backward pass computes
+them again, in pieces of the classes, and turns them into the gradients of input, weight and bias.
 """
+import operator
+from typing import NamedTuple
+
 import torch
 import torch.nn.functional as F
 
@@ -52,3 +56,76 @@ def linear_cross_entropy(x, weight, bias, target, *, reduction="mean", ignore_in
     dtype = fused._autocast(x)
     return _lib.host(x.get_device()).head(x if dtype is None else x.to(dtype), weight, bias, target, reduction == "mean",
                                           int(ignore_index), float(label_smoothing))
+
+
+class TopLogits(NamedTuple):
+    """The k largest logits of each row and their classes (int64), largest first."""
+    values: torch.Tensor
+    classes: torch.Tensor
+
+
+def top_logits(logits, k):
+    """The ``k`` largest of ``logits`` [..., V] and their classes as ``TopLogits``, [..., k] each, without their history: largest first, of equal
+    ones the lowest class first.  NaN is above everything, and the zeros are equal.
+
+    A CUDA tensor of type float32, bfloat16 or float16; V is at most 2^24, k at most 1024 and V.  Calls under compilation, tracing or torch.func
+    transforms take the same from a stable sort."""
+    k = operator.index(k)
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], 1024):
+        raise ValueError("k must be from 1 to 1024 and no more than there are classes")
+    if not ordinary(logits):
+        values, classes = torch.sort(logits.detach(), dim=-1, descending=True, stable=True)
+        return TopLogits(values[..., :k], classes[..., :k])
+    return TopLogits(*_lib.host(logits.get_device()).top(logits, k))
+
+
+def distillation_of(logits, teacher_logits, teacher_classes, temperature=1.0, reduction="mean"):
+    """``linear_distillation`` of a classifier's own ``logits`` [..., V], from PyTorch ops: for any leading dimensions and none."""
+    if teacher_logits.shape != teacher_classes.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_classes.dtype != torch.int64:
+        raise RuntimeError("teacher_classes must be int64, one class for every teacher logit, and both have entries for every row of x")
+    t = teacher_logits.detach().float()
+    classes = teacher_classes
+    bad = (classes != -1) & ((classes < 0) | (classes >= logits.shape[-1]) | ~(t < float("inf")))
+    there = (classes != -1) & (t != float("-inf")) & ~bad
+    bad, some = bad.any(-1), there.any(-1)
+    counts = bad | some
+    nothing = torch.where(bad, float("nan"), 0.0).to(torch.float32)
+    # (rows that do not count may hold anything)
+    own = torch.where(counts.unsqueeze(-1), logits.float(), 0.0) + nothing.unsqueeze(-1)
+    logs = F.log_softmax(own / temperature, -1).gather(-1, torch.where(there, classes, 0))
+    t = torch.where(there, t / temperature, float("-inf"))
+    log_p = F.log_softmax(torch.where(some.unsqueeze(-1), t, 0.0), -1)
+    p = torch.where(there, torch.exp(log_p), 0.0)
+    loss = temperature * temperature * torch.where(p > 0, p * (log_p - logs), 0.0).sum(-1) + nothing
+    loss = torch.where(counts, loss, 0.0)
+    if reduction == "none":
+        return loss
+    number = counts.sum()
+    return torch.where(number > 0, loss.sum() / number.clamp(min=1), float("nan"))
+
+
+def linear_distillation(x, weight, bias, teacher_logits, teacher_classes, *, temperature=1.0, reduction="mean"):
+    """The loss of a linear classifier, ``l = F.linear(x, weight, bias)`` for ``x`` [..., C], ``weight`` [V, C] and ``bias`` [V] or None, against the
+    largest logits of a teacher, ``teacher_logits`` [..., k] and their int64 ``teacher_classes`` [..., k] (``top_logits``):
+    ``temperature ** 2 * sum_j p_j (log p_j - log q_j)`` with ``p`` the softmax over the row's entries of ``teacher_logits / temperature`` and ``q_j``
+    that of ``l / temperature`` over all classes at ``teacher_classes[j]``.  As fp32: the mean over the rows with entries (NaN where there are none),
+    or with reduction "none" a loss for every row.
+
+    An entry of class -1, or whose logit is -infinity, is absent, whatever else it holds; a row without entries has no loss (0), no gradient and
+    does not count.  Another class that is none, or a teacher's logit that is NaN or infinite, gives NaN, in the row's loss and gradient.  Entries of the
+    same class count each for itself.
+
+    CUDA tensors of type float32, bfloat16 and float16; the teacher's logits and the parameters may have another of these types, the parameters get
+    gradients of their own, the teacher's logits none.  k is at most 1024, the temperature from 1e-4 to 1e4.  Under autocast x and parameters are
+    converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose the same values from PyTorch ops; gradients of
+    gradients are refused.  The loss and what goes into 16-bit products are computed and held as for ``linear_cross_entropy``."""
+    if reduction not in ("mean", "none"):
+        raise ValueError("reduction must be 'mean' or 'none'")
+    temperature = float(temperature)
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError("temperature must be from 1e-4 to 1e4")
+    if not ordinary(x, weight, bias, teacher_logits, teacher_classes):
+        return distillation_of(fused.linear_as(x, weight, bias), teacher_logits, teacher_classes, temperature, reduction)
+    dtype = fused._autocast(x)
+    return _lib.host(x.get_device()).distill(x if dtype is None else x.to(dtype), weight, bias, teacher_logits, teacher_classes, temperature,
+                                             reduction == "mean")
