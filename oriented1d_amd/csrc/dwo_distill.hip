@@ -12,6 +12,8 @@
 
 namespace dwo {
 
+typedef int mma_i4 __attribute__((ext_vector_type(4)));
+
 constexpr int kDistillMost = 1024;  // entries of a row
 constexpr int kRun = 64;            // classes of a word of the table, no fewer than a wave's columns in any tile
 // A run's word: the first entry's place in the run, its place among the row's entries, and how many there are
@@ -39,37 +41,46 @@ struct Kept {
 };
 
 // ------------------------------------------------------------------------------------------------- the teacher's entries
-// A wave a row, N entries a lane (j = lane + 64 i).  An entry's place in the order of classes is the number of those in front of it.
-template <typename T, int N>
+// G lanes a row, N entries a lane (j = lane + G i).  An entry's place in the order of classes is the number of those in front of it; entries of one
+// class, which are rare, stay in their order.  (8192 rows of 64 entries, 65536 classes: 14 us, 33 MB of them the table; each row's words are written as
+// zeros, and those of its runs again.)
+template <typename T, int G, int N>
 __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restrict__ logits, const long long *__restrict__ classes, Kept kept,
                                                               unsigned *__restrict__ table, long rows, long V, int k, long pitch, float per) {
-    __shared__ int sorted[4][64 * N];
-    const int lane = threadIdx.x & 63;
-    int *const mine = sorted[threadIdx.x >> 6];
-    for (long first = (long)blockIdx.x * 4; first < rows; first += (long)gridDim.x * 4) {
-        const long row = first + (threadIdx.x >> 6);
+    constexpr int ROWS = 256 / G, NOWHERE = 0x7fffffff;
+    constexpr int PITCH = G * N + 4;  // (rows of a wave on different banks)
+    __shared__ __attribute__((aligned(16))) int lds[ROWS][PITCH];
+    const int lane = threadIdx.x % G;
+    int *const mine = lds[threadIdx.x / G];
+    auto join = [](float v, auto &&f) {
+#pragma unroll
+        for (int off = 1; off < G; off <<= 1) v = f(v, __shfl_xor(v, off, 64));
+        return v;
+    };
+    for (long first = (long)blockIdx.x * ROWS; first < rows; first += (long)gridDim.x * ROWS) {
+        const long row = first + threadIdx.x / G;
         const bool real = row < rows;
         float t[N];
         int c[N];
-        bool bad = false;
-        float most = -INFINITY;
+        float bad = 0.f, most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int j = lane + 64 * i;
-            t[i] = -INFINITY, c[i] = 0x7fffffff;
+            const int j = lane + G * i;
+            t[i] = -INFINITY, c[i] = NOWHERE;
             if (real && j < k) {
                 const long long v = classes[row * k + j];
                 const float f = to_float(logits[row * k + j]);
-                const bool there = v != -1 && f != -INFINITY;
-                bad |= v != -1 && (v < 0 || v >= V || !(f < INFINITY));
-                if (there) t[i] = f, c[i] = v >= 0 && v < V ? (int)v : 0x7fffffff;
-                most = fmaxf(most, there ? f : -INFINITY);
+                const bool is = v >= 0 && v < V;
+                if (v != -1 && (!is || !(f < INFINITY))) bad = 1.f;
+                if (is && f != -INFINITY) t[i] = f, c[i] = (int)v;
             }
+            most = fmaxf(most, t[i]);
             mine[j] = c[i];
         }
-        const bool any_bad = __any(bad);
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        if (real)
+            for (long b = lane; b < pitch / 4; b += G) reinterpret_cast<mma_u4 *>(table + row * pitch)[b] = mma_u4{0u, 0u, 0u, 0u};
+        const bool any_bad = join(bad, [](float a, float b) { return fmaxf(a, b); }) != 0.f;
+        most = join(most, [](float a, float b) { return fmaxf(a, b); });
         const bool some = most > -INFINITY;
         float sum = 0.f;
 #pragma unroll
@@ -77,28 +88,43 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
             t[i] = some && !any_bad && t[i] > -INFINITY ? prod_exp((t[i] - most) * per) : 0.f;
             sum += t[i];
         }
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
+        sum = join(sum, [](float a, float b) { return a + b; });
         const float part = some && !any_bad ? 1.f / sum : 0.f;
         if (real && lane == 0) kept.state[row] = any_bad ? ROW_BAD : some ? 0 : ROW_OUT;
-        if (real)
-            for (long b = lane; b < pitch / 4; b += 64) reinterpret_cast<mma_u4 *>(table + row * pitch)[b] = mma_u4{0u, 0u, 0u, 0u};
-        __syncthreads();  // (the classes are in LDS, and the zeros in front of the words that replace some)
-        int rank[N] = {}, same[N] = {}, ahead[N] = {};
-        for (int j = 0; j < k; j++) {
-            const int other = mine[j];
+        __syncthreads();  // (the classes are in LDS)
+        int rank[N] = {}, same[N] = {};
+        for (int j = 0; j < k; j += 4) {  // (behind the last entry there is none)
+            const mma_i4 other = *reinterpret_cast<const mma_i4 *>(mine + j);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int before = other < c[i] || (other == c[i] && j < lane + 64 * i), run = other / kRun == c[i] / kRun;
-                rank[i] += before, same[i] += run, ahead[i] += before & run;
-            }
+            for (int h = 0; h < 4; h++)
+#pragma unroll
+                for (int i = 0; i < N; i++) rank[i] += other[h] < c[i] ? 1 : 0, same[i] += other[h] == c[i] ? 1 : 0;
         }
+        int most_same = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) most_same = max(most_same, lane + G * i < k ? same[i] : 0);
+        if (__any(most_same > 1))
+            for (int j = 0; j < k; j++) {
+                const int other = mine[j];
+#pragma unroll
+                for (int i = 0; i < N; i++) rank[i] += other == c[i] && j < lane + G * i ? 1 : 0;
+            }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (real && lane + 64 * i < k) {
-                kept.classes[row * k + rank[i]] = c[i];
-                kept.p[row * k + rank[i]] = t[i] * part;
-                if (c[i] != 0x7fffffff && ahead[i] == 0) table[row * pitch + c[i] / kRun] = run_word(c[i] % kRun, rank[i], same[i]);
+            if (lane + G * i < k) mine[rank[i]] = c[i];
+        __syncthreads();  // (in order; and the zeros are in memory in front of the words that replace some)
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (real && lane + G * i < k) {
+                const int at = rank[i], run = c[i] / kRun;
+                kept.classes[row * k + at] = c[i];
+                kept.p[row * k + at] = t[i] * part;
+                if (c[i] != NOWHERE && (at == 0 || mine[at - 1] / kRun != run)) {
+                    int count = 1;
+                    while (at + count < k && mine[at + count] / kRun == run) count++;
+                    table[row * pitch + run] = run_word(c[i] % kRun, at, count);
+                }
             }
         __syncthreads();
     }
@@ -106,9 +132,16 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
 template <typename T>
 static int launch_entries(const void *logits, const long long *classes, const Kept &kept, unsigned *table, long rows, long V, int k, float per,
                           hipStream_t st) {
-    auto *kernel = k <= 64 ? distill_entries_kernel<T, 1> : k <= 256 ? distill_entries_kernel<T, 4> : distill_entries_kernel<T, 16>;
-    const long blocks = (rows + 3) / 4;
-    kernel<<<dim3((unsigned)std::min(blocks, 1L << 20)), dim3(256), 0, st>>>((const T *)logits, classes, kept, table, rows, V, k, run_pitch(V), per);
+    auto go = [&](auto *kernel, int lanes) {
+        const long each = 256 / lanes, blocks = (rows + each - 1) / each;
+        kernel<<<dim3((unsigned)std::min(blocks, 1L << 20)), dim3(256), 0, st>>>((const T *)logits, classes, kept, table, rows, V, k, run_pitch(V), per);
+    };
+    if (k <= 8) go(distill_entries_kernel<T, 8, 1>, 8);
+    else if (k <= 16) go(distill_entries_kernel<T, 16, 1>, 16);
+    else if (k <= 32) go(distill_entries_kernel<T, 32, 1>, 32);
+    else if (k <= 64) go(distill_entries_kernel<T, 64, 1>, 64);
+    else if (k <= 256) go(distill_entries_kernel<T, 64, 4>, 64);
+    else go(distill_entries_kernel<T, 64, 16>, 64);
     return status();
 }
 
@@ -134,6 +167,21 @@ struct DistillStatsEpi {
         l.init(bias, n0, p.N);
         return l;
     }
+    // v[t / 16][t % 4], by the bits of t
+    template <int NF>
+    static __device__ __forceinline__ float pick(const mma_f4 (&v)[NF], int t) {
+        float w[NF];
+#pragma unroll
+        for (int i = 0; i < NF; i++) {
+            const float lo = t & 1 ? v[i][1] : v[i][0], hi = t & 1 ? v[i][3] : v[i][2];
+            w[i] = t & 2 ? hi : lo;
+        }
+#pragma unroll
+        for (int n = NF / 2, bit = 16 * n; n > 0; n /= 2, bit /= 2)
+#pragma unroll
+            for (int i = 0; i < n; i++) w[i] = t & bit ? w[i + n] : w[i];
+        return w[0];
+    }
     template <int NF>
     __device__ __forceinline__ void emit(const Product &p, const RowClasses<NF> &l, const unsigned *rows, long m, long n0,
                                          mma_f4 (&v)[NF]) const {
@@ -146,18 +194,17 @@ struct DistillStatsEpi {
         const unsigned word = rows[n0 / kRun % 4];
         if (m < p.M && word != 0) {
             const int lane_class = (int)class_of(n0, 0, 0), start = run_start(word), count = run_count(word);
-            int t = (int)(n0 / kRun) * kRun + run_place(word) - lane_class;
-            for (int j = 0;;) {
-                if (t >= 0 && t < 16 * NF && (t & 15) < 4) {
-                    float hit = 0.f;
+            auto hit = [&](int t, int j) {
+                if (t >= 0 && t < 16 * NF && (t & 15) < 4) at[m * k + start + j] = pick(v, t);
+            };
+            hit((int)(n0 / kRun) * kRun + run_place(word) - lane_class, 0);
+            for (int j = 1; j < count; j += 4) {  // (of few classes many a run has several: four are asked for at a time)
+                int c[4];
 #pragma unroll
-                    for (int i = 0; i < NF; i++)
+                for (int u = 0; u < 4; u++) c[u] = classes[m * k + start + min(j + u, count - 1)];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) hit = t == 16 * i + r ? v[i][r] : hit;
-                    at[m * k + start + j] = hit;
-                }
-                if (++j >= count) break;
-                t = classes[m * k + start + j] - lane_class;
+                for (int u = 0; u < 4; u++)
+                    if (j + u < count) hit(c[u] - lane_class, j + u);
             }
         }
         most = over_lanes(most, [](float a, float b) { return fmaxf(a, b); });

@@ -79,10 +79,18 @@ def top_logits(logits, k):
     return TopLogits(*_lib.host(logits.get_device()).top(logits, k))
 
 
+def _temperature(value):
+    value = float(value)
+    if not 1e-4 <= value <= 1e4:
+        raise ValueError("temperature must be from 1e-4 to 1e4")
+    return value
+
+
 def distillation_of(logits, teacher_logits, teacher_classes, temperature=1.0, reduction="mean"):
     """``linear_distillation`` of a classifier's own ``logits`` [..., V], from PyTorch ops: for any leading dimensions and none."""
     if teacher_logits.shape != teacher_classes.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_classes.dtype != torch.int64:
         raise RuntimeError("teacher_classes must be int64, one class for every teacher logit, and both have entries for every row of x")
+    temperature = _temperature(temperature)
     t = teacher_logits.detach().float()
     classes = teacher_classes
     bad = (classes != -1) & ((classes < 0) | (classes >= logits.shape[-1]) | ~(t < float("inf")))
@@ -121,9 +129,7 @@ def linear_distillation(x, weight, bias, teacher_logits, teacher_classes, *, tem
     gradients are refused.  The loss and what goes into 16-bit products are computed and held as for ``linear_cross_entropy``."""
     if reduction not in ("mean", "none"):
         raise ValueError("reduction must be 'mean' or 'none'")
-    temperature = float(temperature)
-    if not 1e-4 <= temperature <= 1e4:
-        raise ValueError("temperature must be from 1e-4 to 1e4")
+    temperature = _temperature(temperature)
     if not ordinary(x, weight, bias, teacher_logits, teacher_classes):
         return distillation_of(fused.linear_as(x, weight, bias), teacher_logits, teacher_classes, temperature, reduction)
     dtype = fused._autocast(x)

@@ -250,7 +250,8 @@ def check_top(x, k):
 
 TOP = [(1, 1, 1), (3, 5, 5), (7, 64, 64), (5, 65, 1), (64, 150, 8), (9, 256, 64), (10, 257, 33), (6, 1000, 64), (6, 1000, 65), (4, 1024, 16), (3, 1025, 20),
        (3, 1025, 1024), (5, 4097, 100), (2, 16376, 256), (2, 16377, 7), (3, 16384, 64), (2, 21841, 100), (2, 65528, 64), (2, 65536, 64), (1, 65537, 64),
-       (3, 131072, 1), (2, 150001, 256), (1, 600000, 1024), (2, 70000, 1000)]
+       (3, 131072, 1), (2, 150001, 256), (1, 600000, 1024), (2, 70000, 1000),
+       (4, 9000, 1024), (4, 5000, 900), (4, 3000, 256), (600, 8193, 3), (9, 512, 17), (5, 255, 16)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -567,6 +568,50 @@ def test_distillation_refusals():
                 dict(teacher_logits=logits.repeat(1, 205), teacher_classes=classes.repeat(1, 205))):
         with pytest.raises(RuntimeError):
             L(**{**dict(x=x, weight=w, bias=b, teacher_logits=logits, teacher_classes=classes), **bad})
+
+
+# ---------------------------------------------------------------------------------------------------- beyond 32 bits
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes, and 2^31 values, in front of the last rows."""
+    # top logits: rows by themselves, and short rows
+    for V, k in ((65536, 64), (150, 8)):
+        rows = (1 << 31) // V + 40
+        x = torch.zeros(rows, V, device="cuda", dtype=torch.bfloat16)
+        x[-30:] = values(30, V, dtype=torch.bfloat16)
+        got = losses.top_logits(x, k)
+        want = top64(x[-30:], k)
+        assert torch.equal(got.classes[-30:].cpu(), want[1]) and same_values(got.values[-30:], want[0])
+        assert torch.equal(got.classes[0].cpu(), torch.arange(k))
+        del x, got
+    # rows of codes, many short rows and others
+    for C in (96, 1100):
+        rows = (1 << 31) // C + 70
+        x = torch.zeros(rows, C, device="cuda", dtype=torch.bfloat16)
+        x[-50:] = values(50, C, dtype=torch.bfloat16)
+        w = values(8, C)
+        y = int8.linear_int8(x, int8.quantize_rows(w))
+        assert not y[:-50].any()
+        int8_near(y[-50:], *int8_64(x[-50:], w, None, None))
+        del x, y
+    rows = (1 << 31) // 40 + 100
+    w = values(40, 96)
+    x = torch.zeros(rows, 96, device="cuda", dtype=torch.bfloat16)
+    x[-50:] = values(50, 96, dtype=torch.bfloat16)
+    y = int8.linear_int8(x, int8.quantize_rows(w))
+    int8_near(y[-50:], *int8_64(x[-50:], w, None, None))
+    del x, y
+    # distillation: entries, and logits' gradients in pieces
+    rows, C, V, k = (1 << 31) // 128 + 60, 8, 16, 128
+    x, w, b = values(rows, C, dtype=torch.bfloat16).requires_grad_(), values(V, C, dtype=torch.bfloat16), values(V, dtype=torch.bfloat16)
+    logits, classes = torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16), torch.full((rows, k), -1, device="cuda")
+    logits[-40:], classes[-40:] = values(40, k, dtype=torch.bfloat16), torch.randint(0, V, (40, k), device="cuda")
+    loss = losses.linear_distillation(x, w, b, logits, classes, reduction="none")
+    dx, = torch.autograd.grad(loss.sum(), x)
+    ref = x[-40:].detach().double().requires_grad_()
+    want = distill64(ref, w.double(), b.double(), logits[-40:], classes[-40:], 1.0, "none")
+    assert not loss[:-40].any() and ((loss[-40:].double() - want).abs() <= 1e-4).all()
+    near(dx[-40:], torch.autograd.grad(want.sum(), ref)[0], "dx")
+    assert not dx[:-40].any()
 
 
 # ---------------------------------------------------------------------------------------------------- together
