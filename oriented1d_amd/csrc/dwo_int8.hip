@@ -6,6 +6,8 @@
 //   others: a pass over x that leaves its codes and every row's a, and a product in tiles (dwo_product.h), whose epilogue does the rest.
 // The tiles run at about the rate of the 16-bit products in operations a second times two; a product of short sums is bound by its results on their way out,
 // which the 18 us of 77 MB are not hidden behind, and by the activation's 16 instructions a value.
+#include <algorithm>
+
 #include "dwo_act.h"
 #include "dwo_int8.h"
 
@@ -274,16 +276,17 @@ __device__ __forceinline__ void rows_to_lds(const T *__restrict__ x, const Resid
 __device__ __forceinline__ int code_place(int k, int g) { return k / 2 * 128 + g * 32 + k % 2 * 16; }
 template <int NF>
 struct WeightRows {
-    const int8_t *row[NF];
+    unsigned row[NF];  // (weights of these kernels have fewer bytes)
     __device__ __forceinline__ void seek(const Resident &q, int n0) {
         const int c = threadIdx.x & 15;
 #pragma unroll
-        for (int i = 0; i < NF; i++) row[i] = q.codes + (size_t)min(n0 + c / 4 * 4 * NF + 4 * i + c % 4, q.D - 1) * q.pitch;
+        for (int i = 0; i < NF; i++) row[i] = (unsigned)min(n0 + c / 4 * 4 * NF + 4 * i + c % 4, q.D - 1) * (unsigned)q.pitch;
     }
     __device__ __forceinline__ void fetch(const Resident &q, int k, mma_s8 (&b)[NF]) const {
-        const int at = code_place(k, (threadIdx.x & 63) >> 4), to = at < q.pitch ? at : 0;
+        const int at = code_place(k, (threadIdx.x & 63) >> 4);
+        const unsigned to = at < q.pitch ? (unsigned)at : 0u;
 #pragma unroll
-        for (int i = 0; i < NF; i++) b[i] = *reinterpret_cast<const mma_s8 *>(row[i] + to);
+        for (int i = 0; i < NF; i++) b[i] = *reinterpret_cast<const mma_s8 *>(q.codes + (row[i] + to));
     }
 };
 
@@ -402,7 +405,7 @@ struct Int8Sizes {
     bool ok() const { return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && D >= 1 && D <= 65536 && known(dtype); }
 };
 // Up to sixteen rows of codes that fit LDS, and a weight whose reading does not take over (bf16, us, as rows of codes and tiles: 1 x 1024 -> 4096 6.8,
-// 9.9; 16 x 1024 -> 4096 6.8, 9.9; 1 x 4096 -> 1024 7.7, 12.8; of 32 and 64 MB 16 x 1024 -> 32768 16.7, 12.4; 1 x 4096 -> 16384 18.6, 17.4)
+// 9.9; 16 x 1024 -> 4096 6.8, 9.9; 1 x 4096 -> 1024 7.7, 12.8; up to 64 rows, whose codes every workgroup makes again, 32 x 768 -> 2048 10.7, 9.5; of 32 and 64 MB 16 x 1024 -> 32768 16.7, 12.4; 1 x 4096 -> 16384 18.6, 17.4)
 static bool few_rows(const Int8Sizes &s) {
     return s.rows <= 16 && s.C <= 4096 && s.rows * s.C <= 16384 && s.D * code_pitch(s.C) <= 1L << 24;
 }
@@ -412,16 +415,16 @@ static bool few_rows(const Int8Sizes &s) {
 static bool many_short_rows(const Int8Sizes &s) {
     return s.C <= 768 && s.rows >= 10L * s.C && s.rows <= 1L << 24 && s.D * code_pitch(s.C) <= 1L << 23;
 }
-// Tiles of 64 rows and 32 columns a wave, two steps ahead, three workgroups a CU (25088 x 384 -> 1536: 59 us; 64 columns, two workgroups: 70; steps
-// further ahead no faster, 32 rows 73: each reads the weight once more)
-constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTilePerCu = 3;
-// Parts of the columns, such that the last of the workgroups ends early: a workgroup's time goes with the columns of its waves, and as much as one group
-// of these for its rows (the case above in 1, 2, 3, 4 and 6 parts: 71, 77, 59, 67 and 72 us, by this 13, 14, 10, 12 and 12)
-static int resident_parts(long tiles, int groups) {
+// Tiles of 64 rows and 32 columns a wave, two steps ahead, four workgroups a CU (25088 x 384 -> 1536: 56 us, with three 59; 64 columns, two workgroups:
+// 70; steps further ahead no faster, 32 rows 73: each reads the weight once more)
+constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTilePerCu = 4;
+// Parts of the columns, such that the last of the workgroups, `per` a CU, ends early: a workgroup's time goes with the columns of its waves, and as much as
+// one group of these for its rows (the case above, three a CU, in 1, 2, 3, 4 and 6 parts: 71, 77, 59, 67 and 72 us, by this 13, 14, 10, 12 and 12)
+static int resident_parts(long tiles, int groups, long per) {
     int best = 1;
     long least = 0;
     for (int parts = 1; parts <= (groups + 3) / 4 && (parts == 1 || tiles * parts <= 1L << 22); parts++) {
-        const long rounds = (tiles * parts + kLinCus * kTilePerCu - 1) / (kLinCus * kTilePerCu);
+        const long rounds = (tiles * parts + kLinCus * per - 1) / (kLinCus * per);
         const long t = rounds * (1 + ((groups + parts - 1) / parts + 3) / 4);
         if (parts == 1 || t < least) best = parts, least = t;
     }
@@ -440,12 +443,13 @@ static int resident_typed(const Int8Sizes &s, const void *x, Resident q, hipStre
         return status();
     }
     const long tiles = (s.rows + 16 * kTileRows - 1) / (16 * kTileRows);
-    const int groups = (s.D + 16 * kTileColumns - 1) / (16 * kTileColumns), parts = resident_parts(tiles, groups);
+    const size_t bytes = (size_t)(16 * kTileRows) * q.stride;
+    const int groups = (s.D + 16 * kTileColumns - 1) / (16 * kTileColumns), parts = resident_parts(tiles, groups, std::min((long)kTilePerCu, (160L << 10) / (long)(bytes + 512)));
     q.groups = ((groups + parts - 1) / parts + 3) / 4 * 4, q.parts = (groups + q.groups - 1) / q.groups;
     auto *kernel = pieces <= 32   ? int8_resident_kernel<T, kTileRows, kTileColumns, 2, kTileAhead, kTilePerCu>
                    : pieces <= 64 ? int8_resident_kernel<T, kTileRows, kTileColumns, 4, kTileAhead, kTilePerCu>
                                   : int8_resident_kernel<T, kTileRows, kTileColumns, 6, kTileAhead, kTilePerCu>;
-    kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(256), (size_t)(16 * kTileRows) * q.stride, st>>>((const T *)x, q);
+    kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(256), bytes, st>>>((const T *)x, q);
     return status();
 }
 
