@@ -311,7 +311,7 @@ template <int THREADS>
 constexpr int kTopEntries = THREADS >= 512 ? 4096 : 2048;
 // `parts` parts of `length` values a row
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, THREADS >= 512 ? 8 : 4) void top_kernel(const T *__restrict__ x, T *__restrict__ values, long long *__restrict__ places,
+__global__ __launch_bounds__(THREADS, THREADS < 512 ? 4 : sizeof(T) == 4 ? 6 : 8) void top_kernel(const T *__restrict__ x, T *__restrict__ values, long long *__restrict__ places,
                                                       u64 *__restrict__ out, long rows, long V, int k, int parts, long length) {
     constexpr int WAVES = THREADS / 64, UNITS = kTopUnits, CAP = kTopEntries<THREADS>;  // (k is at most twice THREADS)
     constexpr unsigned NONE = (unsigned)(-kTopInf<T>) ^ 0x80000000u;
@@ -343,15 +343,15 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 8 : 4) void top_kernel(co
         TopRange<T> all;
         {
             TopRange<T> range[UNITS];
-            constexpr int AHEAD = sizeof(T) == 4 ? UNITS : 2 * UNITS;  // pieces on their way
-            for (int p = (int)threadIdx.x; p < q; p += AHEAD * THREADS) {
-                TopPiece<T> piece[AHEAD];
+            // (one piece of each unit on its way: with two of 16 bits the registers of two thousand threads a CU do not suffice, 222 us and 72 MB of spills)
+            for (int p = (int)threadIdx.x; p < q; p += UNITS * THREADS) {
+                TopPiece<T> piece[UNITS];
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++)
+                for (int u = 0; u < UNITS; u++)
                     if (p + u * THREADS < q) piece[u].read(inner + 8L * (p + u * THREADS));
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++)
-                    if (p + u * THREADS < q) range[u % UNITS].meet(piece[u]);
+                for (int u = 0; u < UNITS; u++)
+                    if (p + u * THREADS < q) range[u].meet(piece[u]);
             }
             int low = kTopInf<T>, high = -kTopInf<T>;
 #pragma unroll
