@@ -285,6 +285,23 @@ def test_top_logits_of_special_rows(V, k, dtype):
     base[14].view(torch.int32 if dtype == torch.float32 else torch.int16)[1] = -1  # (a NaN with the sign)
     base[15] = torch.finfo(dtype).min
     check_top(base, k)
+    # fewer values that are no number than k, more, and of both signs, at the ends of a row and inside; and ties behind them
+    more = values(8, V, dtype=dtype, seed=3)
+    bits = more.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    more[0, :k // 2 + 1] = float("nan")
+    more[1, -(k // 2) - 1:] = float("nan")
+    bits[2, 1::3] = -1
+    bits[3, 5], bits[3, V - 2] = -1, -1
+    more[3, 7] = float("nan")
+    more[4] = 0.0
+    more[4, 3::7] = float("nan")
+    more[5] = 2.0
+    bits[5, 8] = -1
+    more[6] = float("inf")
+    more[6, V // 2:] = float("nan")
+    more[7] = float("-inf")
+    more[7, 1] = float("nan")
+    check_top(more, k)
 
 
 def test_top_logits_shapes_and_strides():
