@@ -237,9 +237,9 @@ struct Resident {
 };
 // Rows of x from `first` on, `have` of them (ROWS at the most), as codes into LDS, LANES threads a row, up to U pieces a thread; their largest magnitudes
 // into `most`.  A thread asks for all its rows, or as many as 64 registers hold, before it waits for one.
-template <typename T, int ROWS, int LANES, int U>
+template <typename T, int THREADS, int ROWS, int LANES, int U>
 __device__ __forceinline__ void rows_to_lds(const T *__restrict__ x, const Resident &q, long first, int have, char *lds, float *most) {
-    constexpr int PASS = 256 / LANES, TURNS = (ROWS + PASS - 1) / PASS, FIT = 32 / (int)sizeof(T) / U, R = TURNS < FIT ? TURNS : FIT < 1 ? 1 : FIT;
+    constexpr int PASS = THREADS / LANES, TURNS = (ROWS + PASS - 1) / PASS, FIT = 32 / (int)sizeof(T) / U, R = TURNS < FIT ? TURNS : FIT < 1 ? 1 : FIT;
     const int l = threadIdx.x % LANES, pieces = q.depth / 8;
     const bool wide = q.C % 8 == 0;
     for (int r0 = (int)threadIdx.x / LANES; r0 < have; r0 += R * PASS) {
@@ -290,10 +290,15 @@ struct WeightRows {
     }
 };
 
+// Tiles of 64 rows, 32 columns a wave, two steps ahead, two workgroups of eight waves a CU (25088 x 384 -> 1536 with GELU: 54 us, in twice as many of four,
+// which make the codes of the same rows twice, 56; 25088 x 96 -> 384 16.3 and 19.9; 64 columns, eight waves a CU: 70; steps further ahead no faster, 32 rows
+// 73: each reads the weight once more)
+constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTileWaves = 8, kTilePerCu = 2;
+
 // 16 MF rows of x, taken to codes on the way into LDS, times the weight's columns, which come from the caches straight to registers, two steps ahead: a
 // wave has 16 NF columns at a time and waits for no other.  The sums' registers hold a row's neighbours: nothing goes through LDS behind them.
-template <typename T, int MF, int NF, int U, int AHEAD, int PER_SIMD>
-__global__ __launch_bounds__(256, PER_SIMD) void int8_resident_kernel(const T *__restrict__ x, Resident q) {
+template <typename T, int MF, int NF, int U, int AHEAD>
+__global__ __launch_bounds__(64 * kTileWaves, 4) void int8_resident_kernel(const T *__restrict__ x, Resident q) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float most[16 * MF];
     constexpr int ROWS = 16 * MF;
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(256, PER_SIMD) void int8_resident_kernel(const T *_
     w.seek(q, group * 16 * NF);
 #pragma unroll
     for (int u = 0; u < AHEAD; u++) w.fetch(q, u, b[u]);
-    rows_to_lds<T, ROWS, 16, U>(x, q, m0, have, lds, most);
+    rows_to_lds<T, 64 * kTileWaves, ROWS, 16, U>(x, q, m0, have, lds, most);
     __syncthreads();
     float a[MF];
     const char *from[MF];  // (rows that are not there read the last one's codes, and are not written)
@@ -320,7 +325,7 @@ __global__ __launch_bounds__(256, PER_SIMD) void int8_resident_kernel(const T *_
         const int r = min(16 * j + c, have - 1);
         a[j] = most[r], from[j] = lds + r * q.stride;
     }
-    for (; group < end; group += 4) {
+    for (; group < end; group += kTileWaves) {
         mma_f4 acc[MF][NF];
 #pragma unroll
         for (int j = 0; j < MF; j++)
@@ -340,7 +345,7 @@ __global__ __launch_bounds__(256, PER_SIMD) void int8_resident_kernel(const T *_
         for (; k + AHEAD < steps; k += AHEAD)
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) step(k + u, k + u + AHEAD, b[u]);
-        w.seek(q, (group + 4) * 16 * NF);  // (the next group's; behind the last, a column that is there)
+        w.seek(q, (group + kTileWaves) * 16 * NF);  // (the next group's; behind the last, a column that is there)
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) step(k + u, u, b[u]);
         const int n = group * 16 * NF + 4 * NF * g;
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(256, 4) void int8_few_kernel(const T *__restrict__ 
     w.seek(q, n0);
 #pragma unroll
     for (int u = 0; u < AHEAD; u++) w.fetch(q, 2 * wave + u / 2 * 8 + u % 2, b[u]);
-    rows_to_lds<T, 16, 64, U>(x, q, 0, have, lds, most);
+    rows_to_lds<T, 256, 16, 64, U>(x, q, 0, have, lds, most);
     __syncthreads();
     const int r = min(c, have - 1);
     const char *const from = lds + r * q.stride;
@@ -409,23 +414,21 @@ struct Int8Sizes {
 static bool few_rows(const Int8Sizes &s) {
     return s.rows <= 16 && s.C <= 4096 && s.rows * s.C <= 16384 && s.D * code_pitch(s.C) <= 1L << 24;
 }
-// Many short rows, and a weight not far beyond an XCD's L2 (bf16 with GELU, C -> 4 C, us, as rows of codes and tiles: 1024 x 96 9.2, 10.6; 65536 x 192 61.5,
-// 91.9; 16384 x 384 37, 46; 4096 x 384 17.2, 18.2 but 1024 x 384 11.7, 10.6; 16384 x 512 52, 69; 4096 x 512 23.2, 20.8; 16384 x 768 -> 2048 65, 77;
-// 4096 x 768 -> 2048 28, 24; weights of 4 and 6 MB, 16384 x 512 -> 8192 217, 262; 16384 x 384 -> 16384 395, 503)
+// Many short rows, and a weight not far beyond an XCD's L2 (bf16 with GELU, C -> 4 C, us, as rows of codes and tiles: 1024 x 96 8.4, 10.4; 65536 x 192 51,
+// 78; 16384 x 384 33, 47; 4096 x 384 17.8, 17.9 but 1024 x 384 12.1, 11.2; 16384 x 512 46, 62; 4096 x 512 20.8, 19.9; 16384 x 768 -> 2048 60, 68;
+// 4096 x 768 -> 2048 25, 23; weights of 4 and 6 MB, with workgroups of four waves, 16384 x 512 -> 8192 217, 262; 16384 x 384 -> 16384 395, 503)
 static bool many_short_rows(const Int8Sizes &s) {
     return s.C <= 768 && s.rows >= 10L * s.C && s.rows <= 1L << 24 && s.D * code_pitch(s.C) <= 1L << 23;
 }
-// Tiles of 64 rows and 32 columns a wave, two steps ahead, four workgroups a CU (25088 x 384 -> 1536: 56 us, with three 59; 64 columns, two workgroups:
-// 70; steps further ahead no faster, 32 rows 73: each reads the weight once more)
-constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTilePerCu = 4;
-// Parts of the columns, such that the last of the workgroups, `per` a CU, ends early: a workgroup's time goes with the columns of its waves, and as much as
-// one group of these for its rows (the case above, three a CU, in 1, 2, 3, 4 and 6 parts: 71, 77, 59, 67 and 72 us, by this 13, 14, 10, 12 and 12)
-static int resident_parts(long tiles, int groups, long per) {
+// Parts of the columns, such that the last of the workgroups ends early: a workgroup's time goes with the columns of its waves, and as much as one group of
+// these for its rows (the case above with three workgroups of four waves a CU, in 1, 2, 3, 4 and 6 parts: 71, 77, 59, 67 and 72 us, by this 13, 14, 10, 12
+// and 12)
+static int resident_parts(long tiles, int groups) {
     int best = 1;
     long least = 0;
-    for (int parts = 1; parts <= (groups + 3) / 4 && (parts == 1 || tiles * parts <= 1L << 22); parts++) {
-        const long rounds = (tiles * parts + kLinCus * per - 1) / (kLinCus * per);
-        const long t = rounds * (1 + ((groups + parts - 1) / parts + 3) / 4);
+    for (int parts = 1; parts <= (groups + kTileWaves - 1) / kTileWaves && (parts == 1 || tiles * parts <= 1L << 21); parts++) {
+        const long rounds = (tiles * parts + kLinCus * kTilePerCu - 1) / (kLinCus * kTilePerCu);
+        const long t = rounds * (1 + ((groups + parts - 1) / parts + kTileWaves - 1) / kTileWaves);
         if (parts == 1 || t < least) best = parts, least = t;
     }
     return best;
@@ -443,13 +446,12 @@ static int resident_typed(const Int8Sizes &s, const void *x, Resident q, hipStre
         return status();
     }
     const long tiles = (s.rows + 16 * kTileRows - 1) / (16 * kTileRows);
-    const size_t bytes = (size_t)(16 * kTileRows) * q.stride;
-    const int groups = (s.D + 16 * kTileColumns - 1) / (16 * kTileColumns), parts = resident_parts(tiles, groups, std::min((long)kTilePerCu, (160L << 10) / (long)(bytes + 512)));
-    q.groups = ((groups + parts - 1) / parts + 3) / 4 * 4, q.parts = (groups + q.groups - 1) / q.groups;
-    auto *kernel = pieces <= 32   ? int8_resident_kernel<T, kTileRows, kTileColumns, 2, kTileAhead, kTilePerCu>
-                   : pieces <= 64 ? int8_resident_kernel<T, kTileRows, kTileColumns, 4, kTileAhead, kTilePerCu>
-                                  : int8_resident_kernel<T, kTileRows, kTileColumns, 6, kTileAhead, kTilePerCu>;
-    kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(256), bytes, st>>>((const T *)x, q);
+    const int groups = (s.D + 16 * kTileColumns - 1) / (16 * kTileColumns), parts = resident_parts(tiles, groups);
+    q.groups = ((groups + parts - 1) / parts + kTileWaves - 1) / kTileWaves * kTileWaves, q.parts = (groups + q.groups - 1) / q.groups;
+    auto *kernel = pieces <= 32   ? int8_resident_kernel<T, kTileRows, kTileColumns, 2, kTileAhead>
+                   : pieces <= 64 ? int8_resident_kernel<T, kTileRows, kTileColumns, 4, kTileAhead>
+                                  : int8_resident_kernel<T, kTileRows, kTileColumns, 6, kTileAhead>;
+    kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(64 * kTileWaves), (size_t)(16 * kTileRows) * q.stride, st>>>((const T *)x, q);
     return status();
 }
 
