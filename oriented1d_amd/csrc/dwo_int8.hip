@@ -2,7 +2,7 @@
 //   q = round(127 x / a), a the row's largest magnitude;  y = act((sum_c q_c p_c) (a / 127) s + b) for weights held as codes p and steps s.
 //
 // Whole numbers are summed, below 2^30 for 65536 channels: sums are exact and in any order, so that a row comes out the same whichever way it goes:
-//   few rows, and many short ones: a kernel that takes its rows to codes on their way into LDS (int8_few_kernel, int8_resident_kernel);
+//   few rows, some, and many short ones: a kernel that takes its rows to codes on their way into LDS (int8_few_kernel, int8_resident_kernel);
 //   others: a pass over x that leaves its codes and every row's a, and a product in tiles (dwo_product.h), whose epilogue does the rest.
 // The tiles run at about the rate of the 16-bit products in operations a second times two; a product of short sums is bound by its results on their way out,
 // which the 18 us of 77 MB are not hidden behind, and by the activation's 16 instructions a value.
@@ -297,7 +297,7 @@ constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTileWaves = 8, k
 
 // 16 MF rows of x, taken to codes on the way into LDS, times the weight's columns, which come from the caches straight to registers, two steps ahead: a
 // wave has 16 NF columns at a time and waits for no other.  The sums' registers hold a row's neighbours: nothing goes through LDS behind them.
-template <typename T, int MF, int NF, int U, int AHEAD>
+template <typename T, int MF, int NF, int LANES, int U, int AHEAD>
 __global__ __launch_bounds__(64 * kTileWaves, 4) void int8_resident_kernel(const T *__restrict__ x, Resident q) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float most[16 * MF];
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 4) void int8_resident_kernel(const
     w.seek(q, group * 16 * NF);
 #pragma unroll
     for (int u = 0; u < AHEAD; u++) w.fetch(q, u, b[u]);
-    rows_to_lds<T, 64 * kTileWaves, ROWS, 16, U>(x, q, m0, have, lds, most);
+    rows_to_lds<T, 64 * kTileWaves, ROWS, LANES, U>(x, q, m0, have, lds, most);
     __syncthreads();
     float a[MF];
     const char *from[MF];  // (rows that are not there read the last one's codes, and are not written)
@@ -414,6 +414,10 @@ struct Int8Sizes {
 static bool few_rows(const Int8Sizes &s) {
     return s.rows <= 16 && s.C <= 4096 && s.rows * s.C <= 16384 && s.D * code_pitch(s.C) <= 1L << 24;
 }
+// Some rows, in tiles of sixteen, whose readings of the weight do not add up to much (bf16 with GELU, us, as rows of codes and larger tiles: 128 x 437 ->
+// 2720 7.1, 10.9; 300 x 384 -> 1536 9.2, 9.8; 48 x 2000 -> 500 10.0, 11.2; 800 x 96 -> 384 7.0, 9.6; beyond, 300 x 437 -> 2720 12.3, 11.0; 800 x 384 -> 1536
+// 13.3, 10.8; 30000 x 32 -> 64 11.2, in tiles of 64 rows 9.5)
+static bool some_rows(const Int8Sizes &s) { return s.rows <= 1 << 14 && s.C <= 2048 && (s.rows + 15) / 16 * s.D * code_pitch(s.C) <= 1L << 24; }
 // Many short rows, and a weight not far beyond an XCD's L2 (bf16 with GELU, C -> 4 C, us, as rows of codes and tiles: 1024 x 96 8.4, 10.4; 65536 x 192 51,
 // 78; 16384 x 384 33, 47; 4096 x 384 17.8, 17.9 but 1024 x 384 12.1, 11.2; 16384 x 512 46, 62; 4096 x 512 20.8, 19.9; 16384 x 768 -> 2048 60, 68;
 // 4096 x 768 -> 2048 25, 23; weights of 4 and 6 MB, with workgroups of four waves, 16384 x 512 -> 8192 217, 262; 16384 x 384 -> 16384 395, 503)
@@ -433,32 +437,39 @@ static int resident_parts(long tiles, int groups) {
     }
     return best;
 }
+template <typename T, int MF, int NF, int LANES, int U, int AHEAD>
+static int launch_resident(const Int8Sizes &s, const void *x, Resident q, hipStream_t st) {
+    const long tiles = (s.rows + 16 * MF - 1) / (16 * MF);
+    const int groups = (s.D + 16 * NF - 1) / (16 * NF), parts = resident_parts(tiles, groups);
+    q.groups = ((groups + parts - 1) / parts + kTileWaves - 1) / kTileWaves * kTileWaves, q.parts = (groups + q.groups - 1) / q.groups;
+    // (rows an odd number of sixteen bytes apart, so that sixteen rows' pieces lie on different banks)
+    q.depth = (q.pitch + 64 * AHEAD - 1) / (64 * AHEAD) * 64 * AHEAD, q.stride = q.depth + 16;
+    int8_resident_kernel<T, MF, NF, LANES, U, AHEAD>
+        <<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(64 * kTileWaves), (size_t)(16 * MF) * q.stride, st>>>((const T *)x, q);
+    return status();
+}
 template <typename T>
 static int resident_typed(const Int8Sizes &s, const void *x, Resident q, hipStream_t st) {
-    const bool few = few_rows(s);
-    // whole rounds of steps; and an odd number of sixteen bytes a row, so that sixteen rows' pieces lie on different banks
-    const int round = few ? 1024 : 64 * kTileAhead;
-    q.depth = (q.pitch + round - 1) / round * round, q.stride = q.depth + 16;
-    const int pieces = q.depth / 8;
-    if (few) {
-        auto *kernel = pieces <= 128 ? int8_few_kernel<T, 2> : int8_few_kernel<T, 8>;
+    if (few_rows(s)) {
+        q.depth = (q.pitch + 1023) / 1024 * 1024, q.stride = q.depth + 16;
+        auto *kernel = q.depth <= 1024 ? int8_few_kernel<T, 2> : int8_few_kernel<T, 8>;
         kernel<<<dim3((unsigned)((s.D + 15) / 16)), dim3(256), (size_t)s.rows * q.stride, st>>>((const T *)x, q);
         return status();
     }
-    const long tiles = (s.rows + 16 * kTileRows - 1) / (16 * kTileRows);
-    const int groups = (s.D + 16 * kTileColumns - 1) / (16 * kTileColumns), parts = resident_parts(tiles, groups);
-    q.groups = ((groups + parts - 1) / parts + kTileWaves - 1) / kTileWaves * kTileWaves, q.parts = (groups + q.groups - 1) / q.groups;
-    auto *kernel = pieces <= 32   ? int8_resident_kernel<T, kTileRows, kTileColumns, 2, kTileAhead>
-                   : pieces <= 64 ? int8_resident_kernel<T, kTileRows, kTileColumns, 4, kTileAhead>
-                                  : int8_resident_kernel<T, kTileRows, kTileColumns, 6, kTileAhead>;
-    kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8 * q.parts)), dim3(64 * kTileWaves), (size_t)(16 * kTileRows) * q.stride, st>>>((const T *)x, q);
-    return status();
+    if (some_rows(s)) {
+        if (q.pitch <= 512) return launch_resident<T, 1, 1, 32, 2, 4>(s, x, q, st);
+        if (q.pitch <= 1024) return launch_resident<T, 1, 1, 32, 4, 4>(s, x, q, st);
+        return launch_resident<T, 1, 1, 32, 8, 4>(s, x, q, st);
+    }
+    if (q.pitch <= 256) return launch_resident<T, kTileRows, kTileColumns, 16, 2, kTileAhead>(s, x, q, st);
+    if (q.pitch <= 512) return launch_resident<T, kTileRows, kTileColumns, 16, 4, kTileAhead>(s, x, q, st);
+    return launch_resident<T, kTileRows, kTileColumns, 16, 6, kTileAhead>(s, x, q, st);
 }
 
 static int int8_linear(const Int8Sizes &s, const void *x, const int8_t *codes, const float *steps, const void *bias, void *y, int act, Arena &ws,
                        hipStream_t st) {
     const long pitch = code_pitch(s.C);
-    const bool resident = few_rows(s) || many_short_rows(s);
+    const bool resident = few_rows(s) || some_rows(s) || many_short_rows(s);
     int8_t *q = (int8_t *)ws.take(resident ? 0 : (size_t)s.rows * pitch);
     float *most = (float *)ws.take(resident ? 0 : (size_t)s.rows * sizeof(float));
     if (ws.dry()) return 0;

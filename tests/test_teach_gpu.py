@@ -132,7 +132,8 @@ def int8_near(y, ref, size, what=""):
 
 
 INT8 = [(1, 1, 1), (1, 16, 7), (1, 1024, 4096), (2, 333, 61), (3, 4096, 40), (4, 48, 5000), (5, 100, 33), (8, 2048, 96), (9, 520, 130), (16, 64, 64),
-        (17, 1040, 72), (37, 333, 61), (64, 768, 1000), (130, 31, 257), (300, 2064, 200), (1100, 384, 1536), (2049, 136, 640), (33, 8200, 24)]
+        (17, 1040, 72), (37, 333, 61), (64, 768, 1000), (130, 31, 257), (300, 2064, 200), (1100, 384, 1536), (2049, 136, 640), (33, 8200, 24),
+        (40, 2000, 70), (100, 1500, 33), (3000, 17, 30), (4000, 384, 300), (17000, 40, 16)]
 
 
 @pytest.mark.parametrize("act", [None, "gelu", "silu"], ids=str)
@@ -194,6 +195,17 @@ def test_linear_int8_rows_stay_apart():
             z = int8.linear_int8(x[:n], w, b, "gelu")
             others = [m for m in range(n) if m not in (3, 7)]
             assert z[3].isnan().all() and z[7].isnan().all() and torch.equal(z[others], y[others])
+
+
+@pytest.mark.parametrize("act", [None, "gelu", "silu"], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_linear_int8_is_the_same_whichever_way_a_row_goes(dtype, act):
+    """Few rows, some, many short ones, and tiles: whole numbers are summed, and what follows is rounded alike."""
+    w, b = int8.quantize_rows(values(800, 200, dtype=dtype)), values(800, dtype=dtype)
+    x = values(2100, 200, dtype=dtype) * torch.exp(3 * values(2100, 1)).to(dtype).clamp(max=1000)
+    y = int8.linear_int8(x, w, b, act)
+    for n in (1, 16, 17, 200, 1900):
+        assert torch.equal(int8.linear_int8(x[:n], w, b, act), y[:n]), n
 
 
 def test_linear_int8_scales_of_all_sizes():
