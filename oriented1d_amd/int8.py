@@ -70,13 +70,19 @@ class LinearInt8(nn.Module):
 
 def quantize_network(network):
     """Puts a ``LinearInt8`` in the place of every wide layer of a network of ``convnext1d``: the pointwise layers of its plain blocks and its
-    classifier.  (The stem, the operators, the norms and gated blocks stay as they are.)  The network is then for inference alone; returned."""
+    classifier.  (The stem, the operators, the norms and gated blocks stay as they are.)  The network is then for inference alone; returned.
+    Where one of these layers is a subclass of its own, or has hooks, which would be lost, the call is refused and changes nothing."""
     from .convnext1d import Block, ConvNeXt1D
 
-    for module in list(network.modules()):
+    found = []
+    for module in network.modules():
         names = ("pwconv1", "pwconv2") if isinstance(module, Block) else ("head",) if isinstance(module, ConvNeXt1D) else ()
         for name in names:
             layer = module._modules.get(name)
             if isinstance(layer, nn.Linear):
-                setattr(module, name, LinearInt8.of(layer))
+                if not fused.plain(layer, nn.Linear, fused.Linear):
+                    raise ValueError("%s of a %s is more than a linear layer, or has hooks" % (name, type(module).__name__))
+                found.append((module, name, layer))
+    for module, name, layer in [(m, n, LinearInt8.of(l)) for m, n, l in found]:
+        setattr(module, name, layer)
     return network

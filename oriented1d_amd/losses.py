@@ -91,7 +91,9 @@ def distillation_of(logits, teacher_logits, teacher_classes, temperature=1.0, re
     if teacher_logits.shape != teacher_classes.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_classes.dtype != torch.int64:
         raise RuntimeError("teacher_classes must be int64, one class for every teacher logit, and both have entries for every row of x")
     temperature = _temperature(temperature)
-    t = teacher_logits.detach().float()
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise RuntimeError("the teacher's logits get no gradient: detach them")
+    t = teacher_logits.float()
     classes = teacher_classes
     bad = (classes != -1) & ((classes < 0) | (classes >= logits.shape[-1]) | ~(t < float("inf")))
     there = (classes != -1) & (t != float("-inf")) & ~bad
@@ -124,9 +126,9 @@ def linear_distillation(x, weight, bias, teacher_logits, teacher_classes, *, tem
     same class count each for itself.
 
     CUDA tensors of type float32, bfloat16 and float16; the teacher's logits and the parameters may have another of these types, the parameters get
-    gradients of their own, the teacher's logits none.  k is at most 1024, the temperature from 1e-4 to 1e4.  Under autocast x and parameters are
-    converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose the same values from PyTorch ops; gradients of
-    gradients are refused.  The loss and what goes into 16-bit products are computed and held as for ``linear_cross_entropy``."""
+    gradients of their own; teacher's logits that require one are refused.  k is at most 1024, the temperature from 1e-4 to 1e4.  Under autocast x
+    and parameters are converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose the same values from
+    PyTorch ops; gradients of gradients are refused.  The loss and what goes into 16-bit products are computed and held as for ``linear_cross_entropy``."""
     if reduction not in ("mean", "none"):
         raise ValueError("reduction must be 'mean' or 'none'")
     temperature = _temperature(temperature)
