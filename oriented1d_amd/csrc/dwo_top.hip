@@ -493,7 +493,10 @@ __global__ __launch_bounds__(512) void top_join_kernel(const u64 *__restrict__ i
         __syncthreads();
         const TopOut<T> to = {x + row * V, out != nullptr ? nullptr : values + row * k, out != nullptr ? nullptr : places + row * k,
                               out != nullptr ? out + job * k : nullptr};
-        top_order_out<512>(entries, number, k, to);
+        const int here = min(number, k);  // (fewer than k: the row's last part, short and alone in its group)
+        top_order_out<512>(entries, number, here, to);
+        if (out != nullptr)
+            for (int i = here + (int)threadIdx.x; i < k; i += 512) out[job * k + i] = 0;
     }
 }
 

@@ -316,6 +316,18 @@ def test_top_logits_of_special_rows(V, k, dtype):
     check_top(more, k)
 
 
+@pytest.mark.parametrize("V,k", [(2093057, 400), (2093065, 79), (2314929, 573)], ids=str)
+def test_top_logits_of_a_short_last_part(V, k):
+    """Rows taken in parts, the last of which has fewer values than k (17, 25 and 561) and is joined by itself at first."""
+    x = values(1, V, dtype=torch.float32)
+    x[0, -1] = 100.0
+    for fill in (255, 1):  # (in memory that held anything)
+        junk = torch.full((1 << 26,), fill, dtype=torch.uint8, device="cuda")
+        del junk
+        check_top(x, k)
+    check_top(x.bfloat16(), k)
+
+
 def test_top_logits_shapes_and_strides():
     x = values(3, 4, 200)
     check_top(x, 9)
