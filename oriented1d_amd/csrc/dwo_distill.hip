@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
                 const long long v = classes[row * k + j];
                 const float f = to_float(logits[row * k + j]);
                 const bool is = v >= 0 && v < V;
-                if (v != -1 && (!is || !(f < INFINITY))) bad = 1.f;
+                if (v != -1 && f != -INFINITY && (!is || !(f < INFINITY))) bad = 1.f;
                 if (is && f != -INFINITY) t[i] = f, c[i] = (int)v;
             }
             most = fmaxf(most, t[i]);

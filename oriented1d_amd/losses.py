@@ -95,8 +95,9 @@ def distillation_of(logits, teacher_logits, teacher_classes, temperature=1.0, re
         raise RuntimeError("the teacher's logits get no gradient: detach them")
     t = teacher_logits.float()
     classes = teacher_classes
-    bad = (classes != -1) & ((classes < 0) | (classes >= logits.shape[-1]) | ~(t < float("inf")))
-    there = (classes != -1) & (t != float("-inf")) & ~bad
+    there = (classes != -1) & (t != float("-inf"))
+    bad = there & ((classes < 0) | (classes >= logits.shape[-1]) | ~(t < float("inf")))
+    there = there & ~bad
     bad, some = bad.any(-1), there.any(-1)
     counts = bad | some
     nothing = torch.where(bad, float("nan"), 0.0).to(torch.float32)

@@ -490,6 +490,18 @@ def test_distillation_special_rows():
     assert (losses.linear_distillation(x, w, b, logits, none, reduction="none") == 0).all()
 
 
+def test_distillation_of_absent_entries_of_any_class():
+    x, w, b, logits, classes = make_distill(20, 24, 50, 5, torch.float32)
+    logits[::2, 1:3] = float("-inf")
+    clean = losses.linear_distillation(x, w, b, logits, classes, reduction="none")
+    wild = classes.clone()
+    wild[::2, 1], wild[::4, 2] = 50, -7
+    wild[2, 2] = 1 << 40
+    loss = losses.linear_distillation(x, w, b, logits, wild, reduction="none")
+    assert torch.isfinite(clean).all() and torch.equal(loss, clean)
+    assert torch.equal(torch.autograd.grad(loss.sum(), x)[0], torch.autograd.grad(clean.sum(), x)[0])
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_distillation_with_classes_twice(dtype):
     """Entries of one class count each for itself: the gradient takes the sum of their p."""

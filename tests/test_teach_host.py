@@ -149,6 +149,15 @@ def test_transforms_compose_the_same_values():
     assert torch.func.vmap(lambda a, u: losses.linear_distillation(a, w, b, u, torch.full((5, 4), -1)))(x, t).isnan().all()
 
 
+def test_absent_entries_may_be_of_any_class():
+    torch.manual_seed(2)
+    own, t, c = torch.randn(4, 9), torch.randn(4, 3), torch.randint(0, 9, (4, 3))
+    t[:, 1] = float("-inf")
+    want = losses.distillation_of(own, t, c, reduction="none")
+    c[:, 1] = torch.tensor([9, -2, -1, 1 << 40])
+    assert torch.equal(losses.distillation_of(own, t, c, reduction="none"), want)
+
+
 def test_top_logits_under_transforms():
     x = torch.tensor([[1.0, 3.0, 3.0, float("nan"), -0.0, 0.0], [2.0, 2.0, 2.0, 2.0, 2.0, float("-inf")]])
     got = torch.func.vmap(lambda v: losses.top_logits(v, 5))(x)
