@@ -6,7 +6,7 @@
 //
 // A first pass makes each row's distribution, with its entries in the order of their classes, and a table that says for each run of 64 classes which
 // entries lie in it: so the product over all classes, whose epilogue leaves the statistics of l (dwo_head.hip), finds the few sums that are some
-// entry's logit among its own and leaves them too.  Backward, in pieces of the classes: the product again, its sums turned into up T q; a pass over the
+// entry's logit among its own and leaves them too.  (Where most runs have several entries it leaves all its sums instead.)  Backward, in pieces of the classes: the product again, its sums turned into up T q; a pass over the
 // entries then puts up T (q - p) in their places, computed from the logits left by the forward pass in fp32 and rounded once.
 #include "dwo_head.h"
 
@@ -15,6 +15,7 @@ namespace dwo {
 typedef int mma_i4 __attribute__((ext_vector_type(4)));
 
 constexpr int kDistillMost = 1024;  // entries of a row
+constexpr int kNowhere = 1 << 30;   // an absent entry's class is this and its place: no two are the same
 constexpr int kRun = 64;            // classes of a word of the table, no fewer than a wave's columns in any tile
 // A run's word: the first entry's place in the run, its place among the row's entries, and how many there are
 __device__ __forceinline__ unsigned run_word(int place, int start, int count) { return (unsigned)place | (unsigned)start << 6 | (unsigned)count << 16; }
@@ -43,11 +44,11 @@ struct Kept {
 // ------------------------------------------------------------------------------------------------- the teacher's entries
 // G lanes a row, N entries a lane (j = lane + G i).  An entry's place in the order of classes is the number of those in front of it; entries of one
 // class, which are rare, stay in their order.  (8192 rows of 64 entries, 65536 classes: 14 us, 33 MB of them the table; each row's words are written as
-// zeros, and those of its runs again.)
+// zeros, and those of its runs again.  Of many entries their comparisons bound it, two instructions for each pair.)
 template <typename T, int G, int N>
 __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restrict__ logits, const long long *__restrict__ classes, Kept kept,
                                                               unsigned *__restrict__ table, long rows, long V, int k, long pitch, float per) {
-    constexpr int ROWS = 256 / G, NOWHERE = 0x7fffffff;
+    constexpr int ROWS = 256 / G;
     constexpr int PITCH = G * N + 4;  // (rows of a wave on different banks)
     __shared__ __attribute__((aligned(16))) int lds[ROWS][PITCH];
     const int lane = threadIdx.x % G;
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int j = lane + G * i;
-            t[i] = -INFINITY, c[i] = NOWHERE;
+            t[i] = -INFINITY, c[i] = kNowhere + j;
             if (real && j < k) {
                 const long long v = classes[row * k + j];
                 const float f = to_float(logits[row * k + j]);
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
             most = fmaxf(most, t[i]);
             mine[j] = c[i];
         }
-        if (real)
+        if (real && table != nullptr)
             for (long b = lane; b < pitch / 4; b += G) reinterpret_cast<mma_u4 *>(table + row * pitch)[b] = mma_u4{0u, 0u, 0u, 0u};
         const bool any_bad = join(bad, [](float a, float b) { return fmaxf(a, b); }) != 0.f;
         most = join(most, [](float a, float b) { return fmaxf(a, b); });
@@ -92,18 +93,20 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
         const float part = some && !any_bad ? 1.f / sum : 0.f;
         if (real && lane == 0) kept.state[row] = any_bad ? ROW_BAD : some ? 0 : ROW_OUT;
         __syncthreads();  // (the classes are in LDS)
-        int rank[N] = {}, same[N] = {};
-        for (int j = 0; j < k; j += 4) {  // (behind the last entry there is none)
+        int rank[N] = {}, ranks = 0;
+        for (int j = 0; j < k; j += 4) {  // (what is behind the last entry is above all)
             const mma_i4 other = *reinterpret_cast<const mma_i4 *>(mine + j);
 #pragma unroll
             for (int h = 0; h < 4; h++)
 #pragma unroll
-                for (int i = 0; i < N; i++) rank[i] += other[h] < c[i] ? 1 : 0, same[i] += other[h] == c[i] ? 1 : 0;
+                for (int i = 0; i < N; i++) rank[i] += other[h] < c[i] ? 1 : 0;
         }
-        int most_same = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) most_same = max(most_same, lane + G * i < k ? same[i] : 0);
-        if (__any(most_same > 1))
+        for (int i = 0; i < N; i++) ranks += lane + G * i < k ? rank[i] : 0;
+#pragma unroll
+        for (int off = 1; off < G; off <<= 1) ranks += __shfl_xor(ranks, off, 64);
+        // (0 .. k - 1 unless two are the same)
+        if (__any(ranks != k * (k - 1) / 2))
             for (int j = 0; j < k; j++) {
                 const int other = mine[j];
 #pragma unroll
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const T *__restric
                 const int at = rank[i], run = c[i] / kRun;
                 kept.classes[row * k + at] = c[i];
                 kept.p[row * k + at] = t[i] * part;
-                if (c[i] != NOWHERE && (at == 0 || mine[at - 1] / kRun != run)) {
+                if (table != nullptr && c[i] < kNowhere && (at == 0 || mine[at - 1] / kRun != run)) {
                     int count = 1;
                     while (at + count < k && mine[at + count] / kRun == run) count++;
                     table[row * pitch + run] = run_word(c[i] % kRun, at, count);
@@ -140,6 +143,7 @@ static int launch_entries(const void *logits, const long long *classes, const Ke
     else if (k <= 16) go(distill_entries_kernel<T, 16, 1>, 16);
     else if (k <= 32) go(distill_entries_kernel<T, 32, 1>, 32);
     else if (k <= 64) go(distill_entries_kernel<T, 64, 1>, 64);
+    else if (k <= 128) go(distill_entries_kernel<T, 64, 2>, 64);
     else if (k <= 256) go(distill_entries_kernel<T, 64, 4>, 64);
     else go(distill_entries_kernel<T, 64, 16>, 64);
     return status();
@@ -154,12 +158,13 @@ struct DistillStatsEpi {
     const int *classes;
     int k;
     float *at;     // [M][k]
+    float *all;    // or all logits, [M][up4(V)], and no table
     float2 *part;  // [classes / (16 NF)][M]: largest logit, sum of exponentials of those / T below it
     float scale;   // log2(e) / T
     static constexpr int kRow = 4;  // the words of the 256 classes around the tile
     __device__ __forceinline__ unsigned row(const Product &, long m, long n0, int i) const {
         const long b = n0 / (4 * kRun) * 4 + i;
-        return b < pitch ? table[m * pitch + b] : 0u;
+        return table != nullptr && b < pitch ? table[m * pitch + b] : 0u;
     }
     template <int NF>
     __device__ __forceinline__ RowClasses<NF> begin(const Product &p, long n0) const {
@@ -191,6 +196,12 @@ struct DistillStatsEpi {
         for (int i = 0; i < NF; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) v[i][r] += l.bias[i][r], most = fmaxf(most, v[i][r]);
+        if (all != nullptr && m < p.M)
+#pragma unroll
+            for (int i = 0; i < NF; i++) {
+                const long n = class_of(n0, i, 0), wide = (p.N + 3) / 4 * 4;
+                if (n < wide) *reinterpret_cast<mma_f4 *>(all + m * wide + n) = v[i];
+            }
         const unsigned word = rows[n0 / kRun % 4];
         if (m < p.M && word != 0) {
             const int lane_class = (int)class_of(n0, 0, 0), start = run_start(word), count = run_count(word);
@@ -224,8 +235,8 @@ struct DistillStatsEpi {
 // parts: 64 threads a row 7.9 us, 16 of them 11.6; 8192 rows of 1024 parts, 67 MB, 17 either way: memory.)
 template <int R, int K>
 __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__restrict__ part, Kept kept, float *__restrict__ loss,
-                                                            float *__restrict__ mean, float *__restrict__ count, float2 *__restrict__ block, long M,
-                                                            int parts, int entries, float T) {
+                                                            float *__restrict__ mean, float *__restrict__ count, float2 *__restrict__ block,
+                                                            const float *__restrict__ all, long wide, long M, int parts, int entries, float T) {
     constexpr int FOUR = R == 16 ? 4 : 1, W = K / FOUR;
     __shared__ float most_of[W][R + 1], sum_of[W][R + 1];
     __shared__ float2 rows[R];
@@ -276,7 +287,14 @@ __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__rest
         if (state == 0)
             for (int j = k; j < entries; j += K) {
                 const float p = kept.p[m * entries + j];
-                if (p > 0.f) value = __builtin_fmaf(p, logf(p) - (kept.at[m * entries + j] - lse) * per, value);
+                float l = 0.f;
+                if (all != nullptr) {
+                    const int c = kept.classes[m * entries + j];
+                    if (c < kNowhere) kept.at[m * entries + j] = l = all[m * wide + c];
+                } else if (p > 0.f) {
+                    l = kept.at[m * entries + j];
+                }
+                if (p > 0.f) value = __builtin_fmaf(p, logf(p) - (l - lse) * per, value);
             }
         if constexpr (FOUR > 1) value = over_lanes(value, total_of);
         sum_of[w][r] = value;
@@ -376,6 +394,11 @@ struct DistillSizes : HeadSizes {
 // (T and 1 / T, their squares, and logits times either stay numbers of fp32 by far)
 static bool temperature_ok(float T) { return T >= 1e-4f && T <= 1e4f; }
 
+// Entries that are many of few classes: all logits are left, up to 256 MB of them, and the join takes those of the entries (forward, us, by the table of
+// runs and this way: 4212 x 568 x 86, k = 81 in fp16 66, 33; 8192 x 512 x 4000, k = 200 in bf16 142, 106; 32768 x 256 x 150 in fp16 with k = 10 37, 32, 8 33,
+// 30, 6 29.8, 28.7, but 5 28.3, 28.6; 8192 x 256 x 1000 with k = 32 31.8, 32.3)
+static bool dense_entries(const DistillSizes &s) { return s.V <= 24 * (long)s.k && s.rows * s.V <= 1L << 26; }
+
 static int distill_forward(const DistillSizes &s, const void *x, const void *w, const void *b, const void *logits, const long long *classes, float T,
                            float *keep, float *loss, float *count, bool mean, Arena &ws, hipStream_t st) {
     Staging stage;
@@ -385,27 +408,35 @@ static int distill_forward(const DistillSizes &s, const void *x, const void *w, 
     const Product p = make_product(ox, ow, s.rows, s.V, s.C, 0);
     const int width = wave_columns(tile_for(p.M, p.N, p.steps));
     const int parts = (int)((s.V + width - 1) / width);
-    // (rows of a workgroup as in head_forward)
-    const bool few = s.rows <= 128, narrow = !few && parts <= 16;
+    // (rows of a workgroup as in head_forward; few of many parts share them among more threads)
+    const bool few = s.rows <= 128 && parts <= 256, narrow = !few && parts <= 16 && s.k <= 16;
     const int group = few || narrow ? 64 : 16;
     const int blocks = few ? 1 : (int)std::min((s.rows + group - 1) / group, 1L << 20);
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
-    unsigned *table = (unsigned *)ws.take((size_t)s.rows * run_pitch(s.V) * sizeof(unsigned));
+    const bool dense = dense_entries(s);
+    const long wide = (s.V + 3) / 4 * 4;
+    unsigned *table = dense ? nullptr : (unsigned *)ws.take((size_t)s.rows * run_pitch(s.V) * sizeof(unsigned));
+    float *all = dense ? (float *)ws.take((size_t)s.rows * wide * sizeof(float)) : nullptr;
     float2 *block = mean && blocks > 1 ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;
     if (ws.dry()) return 0;
     const Kept kept(keep, s.rows, s.k);
     const float per = 1.f / T;
     auto *const entries = s.teacher == DWO_F32 ? launch_entries<float> : s.teacher == DWO_BF16 ? launch_entries<bf16_t> : launch_entries<f16_t>;
     if ((e = entries(logits, classes, kept, table, s.rows, s.V, s.k, per, st))) return e;
-    const DistillStatsEpi epi{{b, s.dtype}, table, run_pitch(s.V), kept.classes, s.k, kept.at, part, 1.44269504f * per};
+    const DistillStatsEpi epi{{b, s.dtype}, table, run_pitch(s.V), kept.classes, s.k, kept.at, all, part, 1.44269504f * per};
     if ((e = launch_product<false, false, false>(p, s.dtype, epi, st))) return e;
     const bool long_rows = !few && !narrow && parts >= 128;
     auto *const join = few ? distill_join_kernel<64, 16> : narrow ? distill_join_kernel<64, 4> : long_rows ? distill_join_kernel<16, 64> : distill_join_kernel<16, 16>;
-    join<<<dim3((unsigned)blocks), dim3(few || long_rows ? 1024 : 256), 0, st>>>(part, kept, mean ? nullptr : loss, mean ? loss : nullptr, count, block, s.rows, parts,
-                                                                    s.k, T);
+    join<<<dim3((unsigned)blocks), dim3(few || long_rows ? 1024 : 256), 0, st>>>(part, kept, mean ? nullptr : loss, mean ? loss : nullptr, count, block, all, wide, s.rows,
+                                                                                 parts, s.k, T);
     if (block != nullptr) head_mean_kernel<<<dim3(1), dim3(1024), 0, st>>>(block, blocks, loss, count);
     return status();
 }
+
+// Few rows and a large weight: dx has one tile and long sums, dw many tiles and short ones, and a tile that suits both takes longer than two launches (us of
+// both passes together, and apart: fp32 17 x 296 x 47541 333, 244, 128 x 512 x 30000 315, 276; bf16 1 x 512 x 65536 167, 144, 64 rows 154, 153; but
+// fp32 30 x 1024 x 10000 155, 162, 300 x 512 x 30000 402, 414)
+static bool products_apart(const DistillSizes &s) { return s.rows <= 128 && s.V * s.C >= 12L << 20; }
 
 static int distill_backward(const DistillSizes &s, const float *up, const void *x, const void *w, const void *b, const float *keep, float T,
                             const float *count, void *dx, void *dw, void *db, int grad, Arena &ws, hipStream_t st) {
@@ -435,7 +466,7 @@ static int distill_backward(const DistillSizes &s, const float *up, const void *
         epi.factor = T / (half && mean ? kHalfScale : 1.f);
         return epi;
     };
-    return head_pieces(s, ox, ow, g, dx, dw, db, grad, make, shared, ws, st);
+    return head_pieces(s, ox, ow, g, dx, dw, db, grad, make, shared, ws, st, products_apart(s));
 }
 
 }  // namespace dwo

@@ -111,10 +111,10 @@ struct HeadSizes {
 };
 
 // dx, dw and db from the logits' gradients G, made in pieces of the classes: make(from, n, w, g) leaves those of n classes in operand g, and
-// shared(epilogue) is what the products that read it give it back.
+// shared(epilogue) is what the products that read it give it back.  Both in one launch, or apart: each is then split and in tiles as suits it alone.
 template <class Make, class Shared>
 int head_pieces(const HeadSizes &s, const Operand &ox, const Operand &ow, const Operand &g, void *dx, void *dw, void *db, int grad, Make &&make,
-                Shared &&shared, Arena &ws, hipStream_t st) {
+                Shared &&shared, Arena &ws, hipStream_t st, bool apart = false) {
     const long piece = s.piece();
     // dx is summed over the pieces in fp32
     const bool many = piece < s.V;
@@ -136,6 +136,11 @@ int head_pieces(const HeadSizes &s, const Operand &ox, const Operand &ow, const 
             PlainEpi epi = shared(plain_epilogue({last ? dx : (void *)sum, s.C, 0, last ? s.dtype : (int)OUT_F32}));
             epi.before = from > 0 ? sum : nullptr;
             group.add(false, gp, wp, s.rows, s.C, n, epi);
+            if (apart) {
+                if ((e = group.launch(s.dtype, ws, st))) return e;
+                if (ws.used > peak) peak = ws.used;
+                ws.used = held, group = ProductGroup{};
+            }
         }
         if (dw != nullptr) {
             PlainEpi epi = shared(plain_epilogue({(char *)dw + (size_t)from * s.C * grad_size, s.C, 0, grad}));

@@ -427,6 +427,15 @@ def test_linear_distillation(shape, dtype, T, absent, reduction):
     assert torch.equal(again, loss)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(500, 40, 86, 81), (150, 33, 2401, 100), (150, 33, 2400, 100), (700, 24, 193, 128), (9, 20, 7, 129), (3, 640, 20001, 5),
+                                   (17, 600, 21000, 12), (100, 24, 9000, 70), (128, 100, 16388, 3)], ids=str)
+def test_distillation_of_many_entries_and_of_few_rows(shape, dtype, reduction):
+    """Entries that are many of few classes, and few rows of many classes, to either side of where they go another way."""
+    test_linear_distillation(shape, dtype, 1.5, True, reduction)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows,C,V,k", [(20000, 32, 8003, 20), (1601, 520, 2041, 64), (25003, 100, 603, 9)], ids=str)
 def test_distillation_in_large_tiles_and_pieces(rows, C, V, k, dtype):
