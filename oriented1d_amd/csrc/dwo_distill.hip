@@ -6,8 +6,9 @@
 //
 // A first pass makes each row's distribution, with its entries in the order of their classes, and a table that says for each run of 64 classes which
 // entries lie in it: so the product over all classes, whose epilogue leaves the statistics of l (dwo_head.hip), finds the few sums that are some
-// entry's logit among its own and leaves them too.  (Where most runs have several entries it leaves all its sums instead.)  Backward, in pieces of the classes: the product again, its sums turned into up T q; a pass over the
-// entries then puts up T (q - p) in their places, computed from the logits left by the forward pass in fp32 and rounded once.
+// entry's logit among its own and leaves them too.  (Where most runs have several entries it leaves all its sums instead.)  Backward, in
+// pieces of the classes: the product again, its sums turned into up T q; a pass over the entries then puts up T (q - p) in their places, computed from
+// the logits left by the forward pass in fp32 and rounded once.
 #include "dwo_head.h"
 
 namespace dwo {

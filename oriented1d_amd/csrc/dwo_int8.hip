@@ -155,24 +155,28 @@ struct Columns8 {
         }
     }
 };
-// N neighbours (a multiple of four) of row m, those below D
+// N neighbours (four or eight) of row m, those below D: in pieces of 16, 8 or 4 bytes, as the rows' distance allows
 template <int N>
 __device__ __forceinline__ void out_row(const Out &o, long m, long n, long D, const mma_f4 (&v)[N / 4]) {
-    const bool wide = o.pitch % 8 == 0 && ((uintptr_t)o.p & 15) == 0 && n + N <= D;
-    if (wide && o.type == OUT_F32) {
+    const bool whole = n + N <= D, aligned = ((uintptr_t)o.p & 15) == 0;
+    if (whole && aligned && o.type == OUT_F32 && o.pitch % 4 == 0) {
         mma_f4 *to = reinterpret_cast<mma_f4 *>(reinterpret_cast<float *>(o.p) + (size_t)m * o.pitch + n);
 #pragma unroll
         for (int i = 0; i < N / 4; i++) to[i] = v[i];
-    } else if (wide) {
+    } else if (whole && aligned && o.type != OUT_F32 && o.pitch % 2 == 0) {
         uint16_t *to = reinterpret_cast<uint16_t *>(o.p) + (size_t)m * o.pitch + n;
         unsigned w[N / 2];
 #pragma unroll
         for (int i = 0; i < N / 2; i++) w[i] = pack16(o.type, v[i / 2][2 * (i % 2)], v[i / 2][2 * (i % 2) + 1]);
-        if constexpr (N == 4) {
-            *reinterpret_cast<mma_u2 *>(to) = mma_u2{w[0], w[1]};
-        } else {
+        if (N == 8 && o.pitch % 8 == 0) {
 #pragma unroll
             for (int i = 0; i < N / 8; i++) reinterpret_cast<mma_u4 *>(to)[i] = mma_u4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        } else if (o.pitch % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < N / 4; i++) reinterpret_cast<mma_u2 *>(to)[i] = mma_u2{w[2 * i], w[2 * i + 1]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) reinterpret_cast<unsigned *>(to)[i] = w[i];
         }
     } else {
 #pragma unroll
