@@ -107,6 +107,9 @@ __device__ __forceinline__ unsigned top_bisect(unsigned lo, unsigned hi, int k, 
     return lo;
 }
 __device__ __forceinline__ int top_enough(int k) { return k + k / 4 + 8; }
+// of those that are gathered: what is sorted is a power of two
+__device__ __forceinline__ int top_enough_entries(int k) { return min(top_enough(k), k > 1 ? 1 << (32 - __builtin_clz(k - 1)) : 1); }
+__device__ __forceinline__ int top_refined(int k) { return max(256, k + k / 2); }
 
 // ------------------------------------------------------------------------------------------------- short rows
 // Rows of up to G E values, G lanes each and k up to G: place = lane + G e; the lanes are the units.  The 64 / G rows of a wave go through the same
@@ -240,6 +243,19 @@ __device__ __forceinline__ void top_order_out(u64 *entries, int n, int want, con
             for (int j = part; j < n; j += share) rank += entries[j] > own ? 1 : 0;
         for (int off = 1; off < share; off *= 2) rank += __shfl_xor(rank, off, 64);
         if (i < n && part == 0 && rank < want) out.put(rank, own);
+        return;
+    }
+    if (THREADS == 128 && size == 256) {
+        const int i = (int)threadIdx.x, k = i + THREADS;
+        const u64 own[2] = {entries[i], k < n ? entries[k] : 0};  // (more than 128 are there)
+        int rank[2] = {};
+#pragma unroll 4
+        for (int j = 0; j < n; j++) {
+            const u64 other = entries[j];
+            rank[0] += other > own[0] ? 1 : 0, rank[1] += other > own[1] ? 1 : 0;
+        }
+        if (rank[0] < want) out.put(rank[0], own[0]);
+        if (k < n && rank[1] < want) out.put(rank[1], own[1]);
         return;
     }
     for (int i = n + (int)threadIdx.x; i < size; i += THREADS) entries[i] = 0;
@@ -412,6 +428,25 @@ __global__ __launch_bounds__(THREADS, THREADS < 512 ? 4 : sizeof(T) == 4 ? 6 : 8
             least_last = bound, most_last = hi > ((unsigned)kTopInf<T> ^ 0x80000000u) ? 0xffffffffu : hi;
         }
         int n = number;
+        if (!hard && n > top_refined(want)) {
+            // few units for so many: the bound lets many through, and the k-th largest is looked for among them
+            const unsigned last = top_bisect<T>(least_last, most_last, want, top_enough_entries(want), [&](unsigned v) {
+                unsigned c = 0;
+                for (int i = (int)threadIdx.x; i < n; i += THREADS) c += (unsigned)(entries[i] >> 32) >= v ? 1u : 0u;
+                return sum(lanes_join<64>(c, Total{}));
+            });
+            __syncthreads();
+            if (threadIdx.x == 0) number = 0;
+            // (what stays goes to places that have been read)
+            for (int first = 0; first < n; first += THREADS) {
+                const int i = first + (int)threadIdx.x;
+                const u64 entry = i < n ? entries[i] : 0;
+                __syncthreads();
+                if (i < n && (unsigned)(entry >> 32) >= last) entries[atomicAdd(&number, 1)] = entry;
+            }
+            __syncthreads();
+            n = number;
+        }
         if (hard) {
             // (rare: all values again from memory, each time)
             auto visit = [&](auto &&f) {
