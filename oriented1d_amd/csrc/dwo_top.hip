@@ -329,7 +329,7 @@ constexpr int kTopEntries = THREADS >= 512 ? 4096 : 2048;
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, THREADS < 512 ? 4 : sizeof(T) == 4 ? 6 : 8) void top_kernel(const T *__restrict__ x, T *__restrict__ values, long long *__restrict__ places,
                                                       u64 *__restrict__ out, long rows, long V, int k, int parts, long length) {
-    constexpr int WAVES = THREADS / 64, UNITS = kTopUnits, CAP = kTopEntries<THREADS>;  // (k is at most twice THREADS)
+    constexpr int WAVES = THREADS / 64, UNITS = kTopUnits, CAP = kTopEntries<THREADS>;  // (k is at most four times THREADS, as units are)
     constexpr unsigned NONE = (unsigned)(-kTopInf<T>) ^ 0x80000000u;
     __shared__ u64 entries[CAP];
     __shared__ uint16_t hot[THREADS * UNITS];
@@ -543,10 +543,13 @@ struct TopPlan {
     }
     // lanes of a row, or 0
     int lanes() const { return V <= 256 && k <= 16 ? 16 : V <= 512 && k <= 32 ? 32 : V <= 1024 && k <= 64 ? 64 : 0; }
-    bool small() const { return V <= 8192 && k <= 256; }
+    // Workgroups of 128 threads, more of which a CU has, of no more values than are theirs to sort while others wait (bf16, us, and by 512 threads: 8192 rows of
+    // 4000 values, k = 200 88, 161, k = 300 115, 203; 2000 x 1500, k = 200 30, 48, but 16 rows 21.8, 16.8; 2000 x 4000, k = 400 74, 61; 8192 x 8000, k = 400
+    // 243, 217)
+    bool small() const { return V <= 8192 && (k <= 128 || (k <= 256 && rows > 512) || (k <= 512 && V <= 4096 && rows > 4096)); }
     // parts of a row: where rows are few, no fewer than 4096 and 8 k values each
     int parts() const {
-        if (lanes() != 0 || small()) return 1;
+        if (lanes() != 0 || V <= 8192) return 1;
         const long least = std::max(4096L, 8L * k), most = V / least, want = (512 + rows - 1) / rows;
         return (int)std::max(std::min(most, want), 1L);
     }

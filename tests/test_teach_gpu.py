@@ -263,7 +263,9 @@ def check_top(x, k):
 TOP = [(1, 1, 1), (3, 5, 5), (7, 64, 64), (5, 65, 1), (64, 150, 8), (9, 256, 64), (10, 257, 33), (6, 1000, 64), (6, 1000, 65), (4, 1024, 16), (3, 1025, 20),
        (3, 1025, 1024), (5, 4097, 100), (2, 16376, 256), (2, 16377, 7), (3, 16384, 64), (2, 21841, 100), (2, 65528, 64), (2, 65536, 64), (1, 65537, 64),
        (3, 131072, 1), (2, 150001, 256), (1, 600000, 1024), (2, 70000, 1000),
-       (4, 9000, 1024), (4, 5000, 900), (4, 3000, 256), (600, 8193, 3), (9, 512, 17), (5, 255, 16)]
+       (4, 9000, 1024), (4, 5000, 900), (4, 3000, 256), (600, 8193, 3), (9, 512, 17), (5, 255, 16),
+       (520, 700, 300), (520, 4096, 512), (520, 4097, 512), (520, 8191, 256), (3, 8192, 129), (520, 600, 512), (520, 513, 257), (3, 300, 300), (4100, 600, 300),
+       (4100, 1030, 512), (4100, 4096, 257)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
