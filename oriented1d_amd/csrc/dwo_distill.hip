@@ -9,6 +9,9 @@
 // entry's logit among its own and leaves them too.  (Where most runs have several entries it leaves all its sums instead.)  Backward, in
 // pieces of the classes: the product again, its sums turned into up T q; a pass over the entries then puts up T (q - p) in their places, computed from
 // the logits left by the forward pass in fp32 and rounded once.
+//
+// Of a row's statistics both numbers are kept, the largest logit m and s = sum exp((l - m) / T): q = exp((l - m) / T) / s.  One number, m + T log s,
+// would be rounded at the size of the logits, and 1 / T times that is an error of all of a row's q (logits of 64, T = 0.001: 0.4 %).
 #include "dwo_head.h"
 
 namespace dwo {
@@ -25,20 +28,23 @@ __device__ __forceinline__ int run_start(unsigned w) { return w >> 6 & 1023; }
 __device__ __forceinline__ int run_count(unsigned w) { return w >> 16; }
 static long run_pitch(long V) { return ((V + kRun - 1) / kRun + 3) / 4 * 4; }
 
-enum { ROW_OUT = -1, ROW_BAD = -2 };  // a row's state: without entries; a class that is none or a logit that is no number; 0 otherwise
+// A row's state: without entries; a class that is none or a logit that is no number; of others 0, and from the join on the bits of its largest logit
+// (0 where all are -infinity), which is never NaN, as these two are
+enum { ROW_OUT = -1, ROW_BAD = -2 };
+__device__ __forceinline__ bool row_odd(int state) { return state == ROW_OUT || state == ROW_BAD; }
 struct RowStates {
     const int *state;
-    __device__ __forceinline__ int of(long m) const { return state[m]; }
+    __device__ __forceinline__ int of(long m) const { return row_odd(state[m]) ? -1 : 0; }
 };
 // what the backward pass takes of the forward one: [M][k] each but the last two, [M]
 struct Kept {
     int *classes;  // in order, absent ones behind the others
     float *p, *at;  // and the layer's logit there (not written for absent ones)
     int *state;
-    float *lse;  // T log sum exp (l / T)
+    float *sum;  // of exp((l - the largest) / T)
     Kept(float *keep, long rows, int k) {
         const size_t all = (size_t)rows * k;
-        classes = (int *)keep, p = keep + all, at = keep + 2 * all, state = (int *)(keep + 3 * all), lse = keep + 3 * all + rows;
+        classes = (int *)keep, p = keep + all, at = keep + 2 * all, state = (int *)(keep + 3 * all), sum = keep + 3 * all + rows;
     }
 };
 
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__rest
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < W; i++) s += sum_of[i][r] * __builtin_amdgcn_exp2f((most_of[i][r] - base) * scale);
-        const float lse = base + T * logf(s);
+        const float log_sum = logf(s);
         __syncthreads();
         // sum of p (log p - log q): both logarithms are of one size where the layer follows the teacher
         float value = 0.f;
@@ -295,7 +301,7 @@ __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__rest
                 } else if (p > 0.f) {
                     l = kept.at[m * entries + j];
                 }
-                if (p > 0.f) value = __builtin_fmaf(p, logf(p) - (l - lse) * per, value);
+                if (p > 0.f) value = __builtin_fmaf(p, logf(p) - ((l - base) * per - log_sum), value);
             }
         if constexpr (FOUR > 1) value = over_lanes(value, total_of);
         sum_of[w][r] = value;
@@ -305,7 +311,8 @@ __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__rest
             for (int i = 1; i < W; i++) value += sum_of[i][r];
             value = state == ROW_OUT ? 0.f : state == ROW_BAD ? NAN : T * T * value;
             if (m < M) {
-                kept.lse[m] = lse;
+                kept.sum[m] = s;
+                if (state == 0) kept.state[m] = __float_as_int(base);
                 if (loss != nullptr) loss[m] = value;
             }
             rows[r] = make_float2(value, state != ROW_OUT ? 1.f : 0.f);
@@ -324,43 +331,41 @@ __global__ __launch_bounds__(R *K) void distill_join_kernel(const float2 *__rest
 // q times what each row's loss receives, without what all rows share (T, and a mean's up / count); in fp16 times a power of two, as dwo_head.hip has it
 struct DistillGrad {
     const int *state;
-    const float *lse, *up, *scale;  // up null: a mean; scale null: `fixed`
+    const float *sum, *up, *scale;  // up null: a mean; scale null: `fixed`
     float per, fixed;               // 1 / T
+    __device__ __forceinline__ float factor(long m) const { return (up != nullptr ? up[m] : 1.f) * (scale != nullptr ? scale[0] : fixed); }
 };
 struct DistillGradEpi {
     static constexpr bool kSums = false, kDirect = false;
     Values bias;  // of the piece
     DistillGrad d;
     Out g;  // [M][pitch]
-    struct Lane : Classes {
-        float scale;
-    };
+    using Lane = Classes;
     __device__ __forceinline__ Lane begin(const Product &p, long n) const {
         Lane l;
         l.init(bias, n, p.N);
-        l.scale = d.scale != nullptr ? d.scale[0] : d.fixed;
         return l;
     }
-    static constexpr int kRow = 3;  // the state, the log of the sum, what arrives at the loss
+    static constexpr int kRow = 2;  // the state, or largest logit; what arrives at the loss, over the sum
     __device__ __forceinline__ unsigned row(const Product &, long m, long, int k) const {
-        return k == 0 ? (unsigned)d.state[m] : k == 1 ? __float_as_uint(d.lse[m]) : __float_as_uint(d.up != nullptr ? d.up[m] : 1.f);
+        return k == 0 ? (unsigned)d.state[m] : __float_as_uint(d.factor(m) / d.sum[m]);
     }
     __device__ __forceinline__ Nothing load(const Product &, long, long) const { return {}; }
     __device__ __forceinline__ void octet(const Product &p, const Lane &l, const unsigned *rows, const Nothing &, int, long m, long n,
                                           float (&v)[8]) const {
         if (m >= p.M || n >= g.pitch) return;
         const int state = (int)rows[0];
-        const float lse = __uint_as_float(rows[1]), f = __uint_as_float(rows[2]) * l.scale;
+        const float most = __uint_as_float(rows[0]), f = __uint_as_float(rows[1]);
         if (g.plane != 0) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = prod_exp((v[e] + l.bias[e] - lse) * d.per) * f;
+            for (int e = 0; e < 8; e++) v[e] = prod_exp((v[e] + l.bias[e] - most) * d.per) * f;
         } else {
             const float scale = 1.44269504f * d.per;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f((v[e] + l.bias[e] - lse) * scale) * f;
+            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f((v[e] + l.bias[e] - most) * scale) * f;
         }
         // rows without entries, or with an entry that is none, and columns behind the last class
-        if (state < 0 || n + 8 > p.N) {
+        if (row_odd(state) || n + 8 > p.N) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = state == ROW_OUT || n + e >= p.N ? 0.f : state == ROW_BAD ? NAN : v[e];
         }
@@ -370,7 +375,6 @@ struct DistillGradEpi {
 // The same at the entries' places, from class `from` on, less their p.  Entries of one class are neighbours: the first writes for all.
 __global__ __launch_bounds__(256) void distill_places_kernel(Kept kept, DistillGrad d, Out g, long rows, int k, long from, long n) {
     const long total = rows * k;
-    const float scale = d.scale != nullptr ? d.scale[0] : d.fixed;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const int c = kept.classes[i];
         if (c < from || c >= from + n) continue;
@@ -378,11 +382,11 @@ __global__ __launch_bounds__(256) void distill_places_kernel(Kept kept, DistillG
         const long m = i / k;
         const int j = (int)(i % k), before = j > 0 ? kept.classes[i - 1] : -1, after = j + 1 < k ? kept.classes[i + 1] : -1, state = kept.state[m];
         float p = kept.p[i];
-        const float l = kept.at[i], lse = d.lse[m], f = (d.up != nullptr ? d.up[m] : 1.f) * scale;
-        if (state != 0 || before == c) continue;
+        const float l = kept.at[i], sum = d.sum[m], f = d.factor(m);
+        if (row_odd(state) || before == c) continue;
         if (after == c)
             for (int o = 1; j + o < k && kept.classes[i + o] == c; o++) p += kept.p[i + o];
-        operand_one(g, m, c - from, (prod_exp((l - lse) * d.per) - p) * f);
+        operand_one(g, m, c - from, (prod_exp((l - __int_as_float(state)) * d.per) / sum - p) * f);
     }
 }
 
@@ -453,7 +457,7 @@ static int distill_backward(const DistillSizes &s, const float *up, const void *
         head_scale_kernel<<<dim3(1), dim3(1024), 0, st>>>(up, RowStates{kept.state}, s.rows, scale);
         if ((e = status())) return e;
     }
-    const DistillGrad d{kept.state, kept.lse, mean ? nullptr : up, scale, 1.f / T, half && mean ? kHalfScale : 1.f};
+    const DistillGrad d{kept.state, kept.sum, mean ? nullptr : up, scale, 1.f / T, half && mean ? kHalfScale : 1.f};
     auto make = [&](long from, long n, const Operand &wp, const Operand &gp) {
         const DistillGradEpi epi{{b != nullptr ? (const char *)b + from * size_of(s.dtype) : nullptr, s.dtype}, d, out_of(gp, s.dtype)};
         const int status_of = launch_product<false, false, false>(make_product(ox, wp, s.rows, n, s.C, 0), s.dtype, epi, st);

@@ -560,6 +560,46 @@ def test_distillation_temperatures(T):
         assert float((g.double() - r).norm()) <= min(1.0, 1e-5 + 4e-6 * 20 / T) * float(r.norm()) + 1e-6 * T
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T", [1e-4, 1e-3, 0.05, 1.0, 8.0])
+def test_distillation_of_exact_logits_at_all_temperatures(T, dtype, reduction):
+    """Logits that fp32 holds exactly, some 64 and within a few T of each other: no error of theirs is there to be divided by T, and
+    the limits are the same at every T.
+
+    x and w are whole numbers up to 3 times powers of two, the bias is 64, and a unit of the logits is from T / 16 to T / 8, 2^-17 or more, which numbers
+    of 64 to 128 have for a step or a multiple of it.  Logits of 32 products are some 23 units apart, 3 T, seldom 20 T: what is d T below the
+    largest has an exponent that is d 2^-23 off, of its q of e^-d at most 1e-7; sums of 50 and logarithms of up to 4 are 2^-22 off.  So a loss is within (20
+    2^-23 + 2^-22 + as much for the teacher's) T^2 < 1e-5 T^2, and gradients, differences of p and q, within 1e-5 of their norm, and half a step more
+    where they are rounded to 16 bits (held in two halves before)."""
+    rows, C, V, k = 40, 32, 50, 6
+    gen = torch.Generator("cuda").manual_seed(7)
+    unit = 2.0 ** (math.floor(math.log2(T)) - 3)
+    shares = 2.0 ** (math.floor(math.log2(unit)) // 2)
+
+    def whole(*shape):
+        return torch.randint(-3, 4, shape, generator=gen, device="cuda").float()
+
+    x, w = (whole(rows, C) * shares).to(dtype).requires_grad_(), (whole(V, C) * (unit / shares)).to(dtype).requires_grad_()
+    b = torch.full((V,), 64.0, device="cuda", dtype=dtype).requires_grad_()
+    ref = leaves64(x, w, b)
+    own = F.linear(*ref)
+    assert torch.equal(own.detach().float().double(), own.detach()) and torch.equal(F.linear(ref[0], ref[1]).detach() / unit % 1, torch.zeros_like(own))
+    classes = torch.rand(rows, V, generator=gen, device="cuda").argsort(1)[:, :k]
+    logits = whole(rows, k) * T
+    loss = losses.linear_distillation(x, w, b, logits, classes, temperature=T, reduction=reduction)
+    want = distill64(*ref, logits, classes, T, reduction)
+    assert ((loss.double() - want).abs() <= 1e-5 * T * T + 2.0 ** -23 * want.abs()).all()
+    # (gradients of size 1 in fp16 as well)
+    up = torch.full_like(loss, 1.0 / T)
+    got = torch.autograd.grad(loss, [x, w, b], up)
+    r = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    for g, t, name in zip(got, torch.autograd.grad(want, ref, up.double()), ["dx", "dw", "db"]):
+        floor = 2.0 ** -25 * math.sqrt(t.numel()) if dtype == torch.float16 else 0.0
+        off = float((g.double() - t).norm())
+        assert off <= (r + 1e-5) * float(t.norm()) + floor, "%s: %.3g of its norm" % (name, off / float(t.norm()))
+
+
 def test_distillation_types_and_autocast():
     x, w, b, logits, classes = make_distill(66, 64, 144, 7, torch.float32)
     for other in DTYPES:
