@@ -24,12 +24,13 @@ __device__ __forceinline__ int top_order(unsigned bits) {
     const int sign = bits & TOP ? -1 : 0;
     return ((int)(bits & (TOP - 1)) ^ sign) - sign;
 }
-// the same with what is no number above everything, as a number without a sign: the bisections' order
+// the same with what is no number above everything, one key for all of them, as a number without a sign: the bisections' order
 template <typename T>
-__device__ __forceinline__ unsigned top_key(unsigned bits) {
-    const int s = top_order<T>(bits);
+__device__ __forceinline__ unsigned order_key(int s) {
     return s > kTopInf<T> || s < -kTopInf<T> ? 0xffffffffu : (unsigned)s ^ 0x80000000u;
 }
+template <typename T>
+__device__ __forceinline__ unsigned top_key(unsigned bits) { return order_key<T>(top_order<T>(bits)); }
 // the value of a key; of zeros and of what is no number it is in memory
 template <typename T>
 __device__ __forceinline__ T key_value(unsigned key) {
@@ -373,14 +374,14 @@ __global__ __launch_bounds__(THREADS, THREADS < 512 ? 4 : sizeof(T) == 4 ? 6 : 8
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 high = max(high, range[u].high()), low = min(low, range[u].low());
-                own[u] = (unsigned)range[u].high() ^ 0x80000000u;
+                own[u] = order_key<T>(range[u].high());  // (never below -infinity)
             }
             // (what is no number and has no sign is above the infinities there too; with a sign it is below everything, and its unit may be missed)
             const bool odd = low < -kTopInf<T>;
             unsigned bottom = 0xffffffffu;  // of units with a piece
 #pragma unroll
             for (int u = 0; u < UNITS; u++) bottom = min(bottom, (int)threadIdx.x + u * THREADS < q ? own[u] : 0xffffffffu);
-            const unsigned top = lanes_join<64>(max((unsigned)high ^ 0x80000000u, edge_key), Larger{});
+            const unsigned top = lanes_join<64>(max(order_key<T>(high), edge_key), Larger{});
             bottom = lanes_join<64>(bottom, Smaller{});
             __syncthreads();  // (what the last row left is read)
             turn ^= 1;

@@ -318,6 +318,27 @@ def test_top_logits_of_special_rows(V, k, dtype):
     check_top(more, k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("V,k", [(1000, 70), (1100, 4), (5003, 64), (8193, 300), (65536, 4), (65536, 600), (80001, 30)], ids=str)
+def test_top_logits_of_numbers_that_are_none_in_several_ways(V, k, dtype):
+    """NaN of different bits are one value: the lowest classes, whichever bits they have."""
+    x = values(6, V, dtype=dtype)
+    bits = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    low = {torch.float32: 0x7fc00000, torch.bfloat16: 0x7fc0, torch.float16: 0x7e00}[dtype]
+    smallest = {torch.float32: 0x7f800001, torch.bfloat16: 0x7f81, torch.float16: 0x7c01}[dtype]
+    far = torch.arange(V - 8 * min(2 * k + 20, V // 16), V, 8, device="cuda")
+    bits[0, :4], bits[0, far] = low, low + 1
+    bits[1, :k], bits[1, far] = smallest, low + 3
+    # in every unit, the first by one bit and the others by another
+    bits[2, ::2], bits[2, :k // 8 * 8 + 8] = low + 1, low
+    bits[3, :], bits[3, V // 2:] = low, low + 1
+    bits[4, far], bits[4, 1], bits[4, 2] = low + 2, smallest, low + 5
+    bits[5, V - k - 3:V - 3], bits[5, V - 3:] = low + 1, low
+    x[5, 7] = float("inf")
+    assert x.isnan().any(1).all()
+    check_top(x, k)
+
+
 @pytest.mark.parametrize("V,k", [(2093057, 400), (2093065, 79), (2314929, 573)], ids=str)
 def test_top_logits_of_a_short_last_part(V, k):
     """Rows taken in parts, the last of which has fewer values than k (17, 25 and 561) and is joined by itself at first."""
