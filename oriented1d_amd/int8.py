@@ -15,26 +15,40 @@ from . import _lib, fused
 from .checkpoint8 import activation_code, require_ordinary
 
 
-class QuantizedRows(NamedTuple):
-    """Rows in 8-bit integers: ``codes`` int8, rows filled up with zeros to a multiple of sixteen, and ``scales`` fp32, what a step of each row's
-    codes stands for."""
+class _CodesAndScales(NamedTuple):
     codes: torch.Tensor
     scales: torch.Tensor
+
+
+class QuantizedRows(_CodesAndScales):
+    """Rows in 8-bit integers: ``codes`` int8, rows filled up with zeros to a multiple of sixteen, and ``scales`` fp32, what a step of each row's
+    codes stands for.  A tuple of these two.  ``channels`` is how many of a row's codes are values, or None where it is not known: zeros behind them and
+    codes of zero look alike, and a layer checks its input's channels by it."""
+    channels: Optional[int] = None
+
+    def __new__(cls, codes, scales, channels=None):
+        self = super().__new__(cls, codes, scales)
+        self.channels = channels
+        return self
 
 
 def quantize_rows(x):
     """``x`` [..., C] in 8-bit integers, without its history: codes [..., C'] (C' the next multiple of sixteen) and scales [...].  A row with an
     infinity or NaN has codes of zero and a scale that is NaN."""
     require_ordinary("quantize_rows", x)
-    return QuantizedRows(*_lib.host(x.get_device()).int8_rows(x))
+    return QuantizedRows(*_lib.host(x.get_device()).int8_rows(x), x.shape[-1])
 
 
 def linear_int8(x, weight, bias=None, activation=None):
     """``act(F.linear(x, W, bias))`` for ``x`` [..., C], W the rows that ``weight``, the ``quantize_rows`` of a [D, C] matrix, holds, and x's rows held the
     same way; ``activation``: None, "gelu" (exact) or "silu".  The result has x's type and is rounded once.  A row or output channel that holds an
-    infinity or NaN is NaN.  Under autocast x and bias are converted as for ``F.linear``."""
+    infinity or NaN is NaN.  Under autocast x and bias are converted as for ``F.linear``.  C has to be ``weight.channels``; where that is None (codes
+    and scales that were put together by hand) only its next multiple of sixteen is compared."""
     code = -1 if activation is None else activation_code(activation)
     require_ordinary("linear_int8", x, weight.codes, weight.scales, bias)
+    channels = getattr(weight, "channels", None)
+    if channels is not None and x.shape[-1:] != (channels,):
+        raise RuntimeError("x must have the %d channels that the weight's rows were made of, and has the shape %s" % (channels, tuple(x.shape)))
     dtype = fused._autocast(x)
     return _lib.host(x.get_device()).int8_linear(x if dtype is None else x.to(dtype), weight.codes, weight.scales, bias, code)
 
@@ -44,6 +58,8 @@ class LinearInt8(nn.Module):
 
     def __init__(self, weight: QuantizedRows, in_features: int, bias: Optional[torch.Tensor] = None):
         super().__init__()
+        if weight.codes.dim() != 2 or weight.codes.shape[1] != -(-in_features // 16) * 16 or getattr(weight, "channels", None) not in (None, in_features):
+            raise ValueError("the weight's rows must be those of a matrix of %d columns" % in_features)
         self.in_features, self.out_features = in_features, weight.codes.shape[0]
         self.register_buffer("codes", weight.codes)
         self.register_buffer("scales", weight.scales)
@@ -65,7 +81,7 @@ class LinearInt8(nn.Module):
         return "%d, %d, bias=%r" % (self.in_features, self.out_features, self.bias is not None)
 
     def forward(self, x, activation=None):
-        return linear_int8(x, QuantizedRows(self.codes, self.scales), self.bias, activation)
+        return linear_int8(x, QuantizedRows(self.codes, self.scales, self.in_features), self.bias, activation)
 
 
 def quantize_network(network):

@@ -240,6 +240,23 @@ def test_linear_int8_refusals():
         int8.linear_int8(x, w, activation="relu")
 
 
+def test_linear_int8_refuses_other_channels():
+    """Codes are filled up to whole sixteen: an x with some more or fewer channels would meet zeros there, and have another largest magnitude."""
+    layer = nn.Linear(40, 24).cuda()
+    held, mine = int8.quantize_rows(layer.weight), int8.LinearInt8.of(layer)
+    assert held.channels == 40
+    x = values(4, 40)
+    with torch.no_grad():
+        want = int8.linear_int8(x, held, layer.bias)
+        assert torch.equal(mine(x), want)
+        for C in (33, 39, 41, 48, 49):
+            for call in (mine, lambda v: int8.linear_int8(v, held)):
+                with pytest.raises(RuntimeError, match="40 channels"):
+                    call(values(4, C))
+        # codes and scales by themselves say nothing of it
+        assert torch.equal(int8.linear_int8(x, int8.QuantizedRows(*held), layer.bias), want)
+
+
 # ---------------------------------------------------------------------------------------------------- top logits
 def top64(x, k):
     v, c = torch.sort(x.cpu(), dim=-1, descending=True, stable=True)

@@ -1,6 +1,8 @@
 """The operators between a teacher and its student without a GPU: status codes of the C entry points before any GPU work, workspace sizes, what the
 Python entry points refuse, and what they compose under transforms."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -110,6 +112,24 @@ def test_python_refusals():
         net(torch.zeros(1, 3, 32, 32), torch.zeros(1, dtype=torch.long), teacher=(t, c))
     with pytest.raises(RuntimeError, match="no gradient"):  # (where the loss is composed as well)
         losses.distillation_of(torch.randn(4, 16), t.clone().requires_grad_(), c)
+
+
+def test_layers_in_8_bits_check_their_channels():
+    held = int8.QuantizedRows(torch.zeros(24, 48, dtype=torch.int8), torch.ones(24), 40)
+    layer = int8.LinearInt8(int8.QuantizedRows(*held), 40)
+    for x in (torch.zeros(4, 41), torch.zeros(4, 33), torch.zeros(2, 48), torch.zeros(2, 3, 39), torch.zeros(40, 1), torch.zeros(())):
+        for call in (layer, lambda v: int8.linear_int8(v, held)):
+            with pytest.raises(RuntimeError, match="40 channels"):
+                call(x)
+    for weight, channels in ((held, 41), (held, 16), (int8.QuantizedRows(*held), 49), (int8.QuantizedRows(held.codes[0], held.scales), 40)):
+        with pytest.raises(ValueError, match="columns"):
+            int8.LinearInt8(weight, channels)
+    # a tuple of codes and scales, whose copies know their channels
+    codes, scales = held
+    assert codes is held.codes and scales is held.scales and len(held) == 2 and held._fields == ("codes", "scales")
+    for other in (copy.copy(held), copy.deepcopy(held), pickle.loads(pickle.dumps(held))):
+        assert isinstance(other, int8.QuantizedRows) and other.channels == 40 and torch.equal(other.codes, codes)
+    assert int8.QuantizedRows(codes, scales).channels is None and copy.deepcopy(layer).in_features == 40
 
 
 def plain(logits, t, c, T):
