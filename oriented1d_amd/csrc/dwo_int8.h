@@ -21,9 +21,10 @@ struct Mma<i8_t> {
     }
 };
 
-__device__ __forceinline__ bool near_one(float v) {  // 2^-60 .. 2^60; zero is
+// 2^-59 .. 2^61; zero is.  Of two such numbers the product over 127, 2^-125 or more, has all its bits, as products with whole numbers have then
+__device__ __forceinline__ bool near_one(float v) {
     const unsigned e = __float_as_uint(v) >> 23 & 0xff;
-    return e - 67u <= 120u || v == 0.f;
+    return e - 68u <= 119u || v == 0.f;
 }
 constexpr float kWholes = 12582912.f;  // 1.5 2^23: a sum with it is rounded to a whole number, ties to even, whose low byte is the sum's
 

@@ -221,6 +221,25 @@ def test_linear_int8_scales_of_all_sizes():
     assert y[:, [2, 4]].isnan().all() and ((y[:, [0, 1, 3]].double() - want[:, [0, 1, 3]]).abs() <= 1e-6 * want[:, [0, 1, 3]].abs()).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+def test_linear_int8_is_the_same_where_a_step_is_almost_none(dtype):
+    """Magnitudes and scales around 2^-60: what a whole number stands for is near 2^-127, where fp32 has a bit less, and the results above that."""
+    w = values(800, 200, dtype=dtype)
+    held = int8.quantize_rows(w)
+    x = values(2100, 200, dtype=dtype)
+    for e, f in ((-61, -60), (-60, -60), (-60, -61), (-59, -60), (-59, -59), (-62, -58)):
+        # every row's largest is 1.0 .. 2.0 times 2^e, every scale 1.0 .. 2.0 times 2^f
+        a = x * (torch.rand(2100, 1, device="cuda").add(1.0) * 2.0 ** e).to(dtype) / x.abs().amax(1, keepdim=True)
+        scales = torch.rand(800, device="cuda").add(1.0) * 2.0 ** f
+        weight = int8.QuantizedRows(held.codes, scales)
+        y = int8.linear_int8(a, weight)
+        q, most = codes64(a)
+        want = (q @ held.codes[:, :200].double().t()) * (most / 127) * scales.double()
+        assert ((y.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 3e-7) * want.abs() + 2.0 ** -127).all()
+        for n in (1, 16, 17, 200, 1900):
+            assert torch.equal(int8.linear_int8(a[:n], weight), y[:n]), (e, f, n)
+
+
 def test_linear_int8_refusals():
     x, w = values(4, 40), int8.quantize_rows(values(24, 40))
     with pytest.raises(RuntimeError, match="no gradients"):
