@@ -86,10 +86,16 @@ def _temperature(value):
     return value
 
 
+def _reduction(value):
+    if value not in ("mean", "none"):
+        raise ValueError("reduction must be 'mean' or 'none'")
+
+
 def distillation_of(logits, teacher_logits, teacher_classes, temperature=1.0, reduction="mean"):
     """``linear_distillation`` of a classifier's own ``logits`` [..., V], from PyTorch ops: for any leading dimensions and none."""
     if teacher_logits.shape != teacher_classes.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_classes.dtype != torch.int64:
         raise RuntimeError("teacher_classes must be int64, one class for every teacher logit, and both have entries for every row of x")
+    _reduction(reduction)
     temperature = _temperature(temperature)
     if torch.is_grad_enabled() and teacher_logits.requires_grad:
         raise RuntimeError("the teacher's logits get no gradient: detach them")
@@ -130,8 +136,7 @@ def linear_distillation(x, weight, bias, teacher_logits, teacher_classes, *, tem
     gradients of their own; teacher's logits that require one are refused.  k is at most 1024, the temperature from 1e-4 to 1e4.  Under autocast x
     and parameters are converted as for ``F.linear``.  Calls under compilation, tracing or torch.func transforms compose the same values from
     PyTorch ops; gradients of gradients are refused.  The loss and what goes into 16-bit products are computed and held as for ``linear_cross_entropy``."""
-    if reduction not in ("mean", "none"):
-        raise ValueError("reduction must be 'mean' or 'none'")
+    _reduction(reduction)
     temperature = _temperature(temperature)
     if not ordinary(x, weight, bias, teacher_logits, teacher_classes):
         return distillation_of(fused.linear_as(x, weight, bias), teacher_logits, teacher_classes, temperature, reduction)

@@ -169,6 +169,13 @@ def test_transforms_compose_the_same_values():
     assert torch.func.vmap(lambda a, u: losses.linear_distillation(a, w, b, u, torch.full((5, 4), -1)))(x, t).isnan().all()
 
 
+def test_the_composed_loss_refuses_other_reductions():
+    own, t, c = torch.randn(4, 9), torch.randn(4, 3), torch.randint(0, 9, (4, 3))
+    for reduction in ("sum", "batchmean", None):
+        with pytest.raises(ValueError, match="reduction"):
+            losses.distillation_of(own, t, c, reduction=reduction)
+
+
 def test_absent_entries_may_be_of_any_class():
     torch.manual_seed(2)
     own, t, c = torch.randn(4, 9), torch.randn(4, 3), torch.randint(0, 9, (4, 3))
