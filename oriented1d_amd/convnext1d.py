@@ -371,6 +371,8 @@ class ConvNeXt1D(nn.Module):
 
     def top_logits(self, x, k):
         """The ``k`` largest logits of each of the images x and their classes, without gradients: what a student learns from."""
+        if self.out_stages:
+            raise ValueError("a network of stage outputs has no classes")
         with torch.no_grad():
             return losses.top_logits(self(x), k)
 

@@ -132,6 +132,13 @@ def test_layers_in_8_bits_check_their_channels():
     assert int8.QuantizedRows(codes, scales).channels is None and copy.deepcopy(layer).in_features == 40
 
 
+def test_networks_of_stage_outputs_have_no_top_logits():
+    net = ConvNeXt1D(depths=(1, 1, 1, 1), dims=(16, 24, 32, 40), out_stages=True)
+    for call in (lambda x: net.top_logits(x, 3), lambda x: net.distill(x, (torch.zeros(1, 3), torch.zeros(1, 3, dtype=torch.long)))):
+        with pytest.raises(ValueError, match="classes"):
+            call(torch.zeros(1, 3, 32, 32))
+
+
 def plain(logits, t, c, T):
     """Row by row, over the entries that are there."""
     out = []
