@@ -402,7 +402,8 @@ static bool temperature_ok(float T) { return T >= 1e-4f && T <= 1e4f; }
 // Entries that are many of few classes: all logits are left, up to 256 MB of them, and the join takes those of the entries (forward, us, by the table of
 // runs and this way: 4212 x 568 x 86, k = 81 in fp16 66, 33; 8192 x 512 x 4000, k = 200 in bf16 142, 106; 32768 x 256 x 150 in fp16 with k = 10 37, 32, 8 33,
 // 30, 6 29.8, 28.7, but 5 28.3, 28.6; 8192 x 256 x 1000 with k = 32 31.8, 32.3)
-static bool dense_entries(const DistillSizes &s) { return s.V <= 24 * (long)s.k && s.rows * s.V <= 1L << 26; }
+static long logits_pitch(long V) { return (V + 3) / 4 * 4; }
+static bool dense_entries(const DistillSizes &s) { return s.V <= 24 * (long)s.k && s.rows * logits_pitch(s.V) <= 1L << 26; }
 
 static int distill_forward(const DistillSizes &s, const void *x, const void *w, const void *b, const void *logits, const long long *classes, float T,
                            float *keep, float *loss, float *count, bool mean, Arena &ws, hipStream_t st) {
@@ -419,7 +420,7 @@ static int distill_forward(const DistillSizes &s, const void *x, const void *w, 
     const int blocks = few ? 1 : (int)std::min((s.rows + group - 1) / group, 1L << 20);
     float2 *part = (float2 *)ws.take((size_t)parts * s.rows * sizeof(float2));
     const bool dense = dense_entries(s);
-    const long wide = (s.V + 3) / 4 * 4;
+    const long wide = logits_pitch(s.V);
     unsigned *table = dense ? nullptr : (unsigned *)ws.take((size_t)s.rows * run_pitch(s.V) * sizeof(unsigned));
     float *all = dense ? (float *)ws.take((size_t)s.rows * wide * sizeof(float)) : nullptr;
     float2 *block = mean && blocks > 1 ? (float2 *)ws.take((size_t)blocks * sizeof(float2)) : nullptr;

@@ -43,6 +43,19 @@ def test_workspace_sizes():
     assert L.dwo_distill_workspace_bytes(8192, 1024, 65536, 64, 1, BF16) < 3 * (1 << 28) + 8192 * 1024 * 4
 
 
+def test_all_logits_are_kept_up_to_256_megabytes():
+    """Of few classes for each entry; their rows are of whole sixteen bytes.  Beside them 8 bytes a row and tile of classes."""
+    L = lib()
+    for V in (5, 9, 13, 4, 16, 31):
+        for k in (1, 8):
+            pitch = -(-V // 4) * 4
+            for rows in ((1 << 26) // V, (1 << 26) // pitch):  # (more than that, or as much)
+                # (where they are not kept, a word for each 64 classes, of which a row has whole sixteen bytes as well)
+                words = 0 if V <= 24 * k and rows * pitch <= 1 << 26 else rows * 16
+                held = (1 << 28 if words == 0 else words) + rows * 8 * (2 if V > 16 else 1)
+                assert L.dwo_distill_workspace_bytes(rows, 8, V, k, 0, BF16) <= held + (1 << 23), (V, k, rows)
+
+
 def test_status_codes():
     L = lib()
 
