@@ -360,6 +360,7 @@ struct DistillGradEpi {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = prod_exp((v[e] + l.bias[e] - most) * d.per) * f;
         } else {
+            // (rounded to 16 bits next, by 2^-8 or 2^-11 of itself: the multiple's rounding, 2^-24 of the difference, is 2^-18 at q of e^-64)
             const float scale = 1.44269504f * d.per;
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f((v[e] + l.bias[e] - most) * scale) * f;

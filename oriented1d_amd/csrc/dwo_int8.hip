@@ -296,7 +296,7 @@ struct WeightRows {
 
 // Tiles of 64 rows, 32 columns a wave, two steps ahead, two workgroups of eight waves a CU (25088 x 384 -> 1536 with GELU: 54 us, in twice as many of four,
 // which make the codes of the same rows twice, 56; 25088 x 96 -> 384 16.3 and 19.9; 64 columns, eight waves a CU: 70; steps further ahead no faster, 32 rows
-// 73: each reads the weight once more)
+// 73: each reads the weight once more.  The case's 392 tiles are in one round on 512 places: 136 CUs have two workgroups and 120 have one)
 constexpr int kTileRows = 4, kTileColumns = 2, kTileAhead = 2, kTileWaves = 8, kTilePerCu = 2;
 
 // 16 MF rows of x, taken to codes on the way into LDS, times the weight's columns, which come from the caches straight to registers, two steps ahead: a
@@ -414,7 +414,8 @@ struct Int8Sizes {
     bool ok() const { return rows >= 1 && rows <= 1L << 30 && C >= 1 && C <= 65536 && D >= 1 && D <= 65536 && known(dtype); }
 };
 // Up to sixteen rows of codes that fit LDS, and a weight whose reading does not take over (bf16, us, as rows of codes and tiles: 1 x 1024 -> 4096 6.8,
-// 9.9; 16 x 1024 -> 4096 6.8, 9.9; 1 x 4096 -> 1024 7.7, 12.8; up to 64 rows, whose codes every workgroup makes again, 32 x 768 -> 2048 10.7, 9.5; of 32 and 64 MB 16 x 1024 -> 32768 16.7, 12.4; 1 x 4096 -> 16384 18.6, 17.4)
+// 9.9; 16 x 1024 -> 4096 6.8, 9.9; 1 x 4096 -> 1024 7.7, 12.8; beyond sixteen rows, whose codes every workgroup would make again, 32 x 768 -> 2048 10.7, 9.5; weights of 32 and 64 MB 16 x 1024 -> 32768 16.7,
+// 12.4; 1 x 4096 -> 16384 18.6, 17.4)
 static bool few_rows(const Int8Sizes &s) {
     return s.rows <= 16 && s.C <= 4096 && s.rows * s.C <= 16384 && s.D * code_pitch(s.C) <= 1L << 24;
 }

@@ -3,8 +3,9 @@
 // A row is read once for the largest values of its units, a few neighbouring pieces each.  The k-th largest of these is no more than the row's k-th
 // largest; it is found by bisection, and need not be met exactly.  Only units that reach it can hold one of the k: little more than k of two thousand.
 // They are read again, what reaches the bound is gathered, usually less than 3/2 k, and each entry's place among the others is the number in front of
-// it.  Where too many are gathered (rows of few distinct values) the k-th largest itself is found by bisection over all values, and among those equal to it
-// the last place that still counts (8192 rows of 65536 zeros, bf16: 2.9 ms; 0.2 of any values).
+// it.  Where too many are gathered (rows of few distinct values, or of fewer than k finite ones among -infinity) the k-th largest itself is found by bisection
+// over all values, and among those equal to it the last place that still counts (8192 rows of 65536, k = 64, bf16: zeros 2.9 ms, 32 finite values among
+// -infinity 5.0, a NaN with a sign in each 6.3, in fp32 6.2, 16 and 13; 0.2 and 0.37 of any values).
 #include <algorithm>
 
 #include "dwo_product.h"

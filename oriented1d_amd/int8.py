@@ -2,9 +2,10 @@
 
 A row x with largest magnitude a is held as whole numbers ``q = round(127 x / a)``, ties to even, times ``a / 127``.  A layer's weight is held so
 once, row by row (``quantize_rows``); ``linear_int8`` takes the rows of its input the same way, call by call, sums the products of whole numbers
-exactly and scales the sums.  Half the bytes of 16-bit weights, and twice their products' rate.
+exactly and scales the sums.  Weights take half the bytes of 16-bit ones; activations cross memory in their own type.
 
-CUDA tensors of type float32, bfloat16 and float16.  There are no gradients: calls that would need them are refused.
+CUDA tensors of type float32, bfloat16 and float16.  There are no gradients: calls that would need them are refused, as are calls under compilation,
+tracing and torch.func transforms.
 """
 from typing import NamedTuple, Optional
 
@@ -87,7 +88,11 @@ class LinearInt8(nn.Module):
 def quantize_network(network):
     """Puts a ``LinearInt8`` in the place of every wide layer of a network of ``convnext1d``: the pointwise layers of its plain blocks and its
     classifier.  (The stem, the operators, the norms and gated blocks stay as they are.)  The network is then for inference alone; returned.
-    Where one of these layers is a subclass of its own, or has hooks, which would be lost, the call is refused and changes nothing."""
+    Where one of these layers is a subclass of its own, or has hooks, which would be lost, the call is refused and changes nothing.
+
+    A network of fp32 becomes faster, one of 16-bit type slower, since its own blocks keep what lies between the two layers on the chip: the
+    ConvNeXt-T-1D takes 16800 images a second in fp32 at a batch of 128 where it took 8300, and 775 where 483 by themselves; in bfloat16 28200 where 38200, and
+    1010 where 1460.  What a 16-bit network gains is the memory of its weights."""
     from .convnext1d import Block, ConvNeXt1D
 
     found = []
